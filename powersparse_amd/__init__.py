@@ -20,6 +20,10 @@ __all__ = [
     "Stream", "Event", "HostCsr", "set_device", "device_count", "device_props", "synchronize",
     "synth", "read_mtx", "read_binary", "write_binary", "generate_sigbit", "workset_count",
     "dense_input", "GROUP_SIZE", "spmm_launch", "sddmm_launch",
+    "DeviceArray", "EmbeddingLookup", "EmbeddingGrad", "embedding_grad_workspace_bytes",
+    "ExpertSort", "expert_sort_workspace_bytes", "ExpertDispatch", "ExpertDispatchGrad",
+    "ExpertCombine", "ExpertCombineGrad", "GradientList", "GradNorm", "ClipGrads",
+    "ClipGradNorm",
 ]
 
 
@@ -622,3 +626,11 @@ def sddmm_launch(worksets, residue_offset, rows, cols, N, lhs, rhs, outputs, str
                                             _ptr(residue_offset), rows, cols, N, _ptr(lhs),
                                             _ptr(rhs), _out_array(outputs, len(worksets)),
                                             int(task_chunk), _ptr(stream)))
+
+
+# ------------------------------------------------------------ row operators
+
+from .rows import (DeviceArray, EmbeddingLookup, EmbeddingGrad,  # noqa: E402
+                   embedding_grad_workspace_bytes, ExpertSort, expert_sort_workspace_bytes,
+                   ExpertDispatch, ExpertDispatchGrad, ExpertCombine, ExpertCombineGrad,
+                   GradientList, GradNorm, ClipGrads, ClipGradNorm)

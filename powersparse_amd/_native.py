@@ -1,6 +1,7 @@
 """ctypes bindings of the two in-tree shared libraries.
 
-lib/libpowersparse_hip.so     HIP kernels + C ABI        (include/powersparse_hip.h)
+lib/libpowersparse_hip.so     HIP kernels + C ABI        (include/powersparse_hip.h,
+                              include/powersparse_rows.h)
 lib/libpowersparse.so         C++17 host API, C facade   (include/powersparse.h)
 lib/libpowersparse_bench.so   the CSV benchmark harness (include/powersparse_bench.h),
                               loaded on demand (bench())
@@ -91,6 +92,48 @@ class HubBlock(ctypes.Structure):
         ("stored", c_void_p),
     ]
 
+
+class Rows(ctypes.Structure):
+    """ps_rows: a row-major matrix in device memory."""
+
+    _fields_ = [("data", c_void_p), ("rows", ctypes.c_longlong), ("cols", ctypes.c_longlong),
+                ("ld", ctypes.c_longlong), ("dtype", ctypes.c_int)]
+
+
+class Ids(ctypes.Structure):
+    """ps_ids: ids in device memory."""
+
+    _fields_ = [("data", c_void_p), ("count", ctypes.c_longlong), ("type", ctypes.c_int)]
+
+
+# The row operators (include/powersparse_rows.h), in libpowersparse_hip.so.
+_rows_p = ctypes.POINTER(Rows)
+_ids_p = ctypes.POINTER(Ids)
+ROWS_API = [
+    ("ps_embedding_lookup", ctypes.c_int, [_rows_p, _ids_p, ctypes.c_float, _rows_p, c_void_p]),
+    ("ps_embedding_grad_workspace_bytes", ctypes.c_size_t,
+     [ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong]),
+    ("ps_embedding_grad", ctypes.c_int,
+     [_ids_p, _rows_p, ctypes.c_float, ctypes.c_longlong, ctypes.c_int, _rows_p, c_void_p,
+      ctypes.c_size_t, c_void_p]),
+    ("ps_expert_sort_workspace_bytes", ctypes.c_size_t, [ctypes.c_longlong, ctypes.c_int]),
+    ("ps_expert_sort", ctypes.c_int,
+     [_ids_p, ctypes.c_int, c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_size_t, c_void_p]),
+    ("ps_expert_dispatch", ctypes.c_int, [_rows_p, c_void_p, ctypes.c_int, _rows_p, c_void_p]),
+    ("ps_expert_combine", ctypes.c_int,
+     [_rows_p, c_void_p, c_void_p, ctypes.c_int, _rows_p, c_void_p]),
+    ("ps_expert_combine_grad", ctypes.c_int,
+     [_rows_p, _rows_p, c_void_p, c_void_p, ctypes.c_int, _rows_p, c_void_p, c_void_p]),
+    ("ps_grad_list_create", ctypes.c_int,
+     [ctypes.c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(ctypes.c_longlong), c_int_p,
+      ctypes.POINTER(c_void_p), c_int_p, ctypes.POINTER(c_void_p)]),
+    ("ps_grad_list_destroy", None, [c_void_p]),
+    ("ps_grad_norm", ctypes.c_int, [c_void_p, ctypes.c_float, c_void_p, c_void_p]),
+    ("ps_clip_grads", ctypes.c_int,
+     [c_void_p, ctypes.c_float, ctypes.c_float, c_void_p, c_void_p]),
+    ("ps_clip_grad_norm", ctypes.c_int,
+     [c_void_p, ctypes.c_float, ctypes.c_float, c_void_p, c_void_p]),
+]
 
 # (name, restype, argtypes) of every exported entry point. Tests check that
 # each symbol declared in include/*.h is exported.
@@ -386,6 +429,7 @@ def libs():
                     "`make -C powersparse_amd`")
         hip = ctypes.CDLL(HIP_LIB_PATH, mode=ctypes.RTLD_GLOBAL)
         _bind(hip, HIP_API)
+        _bind(hip, ROWS_API)
         host = ctypes.CDLL(HOST_LIB_PATH, mode=ctypes.RTLD_GLOBAL)
         _bind(host, HOST_API)
         _hip, _host = hip, host

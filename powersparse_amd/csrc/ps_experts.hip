@@ -1,0 +1,215 @@
+// Tokens sorted by expert and back: the sort of the slots, the copies into
+// expert order, the weighted sums back, and their gradients.
+//
+// With P the slots x tokens matrix that has a one where a slot is a token's,
+// the dispatch is xs = P x, the combination y = P^T diag(w) ys, and their
+// gradients dx = P^T dxs, dys = diag(w) P dy and dw = the dots of dy's and ys's
+// rows at P's nonzeros: products by a sparse matrix whose k entries per token
+// are the positions the sort gives. They are walked token by token, so a token's
+// row is read or written once and the k rows of its slots are each touched once.
+//
+// All are bound by memory traffic: a slot's row is read or written in whole
+// 16-byte pieces, and the positions (4 bytes a slot) hide behind it.
+#include "ps_id_sort.hpp"
+#include "ps_rows.hpp"
+
+namespace ps {
+namespace {
+
+struct ExpertSink {
+  static constexpr bool kStarts = true;
+  int *order, *position, *offsets;
+  uint32_t experts;
+  __device__ __forceinline__ void put(uint32_t pos, uint32_t key, uint32_t slot) const {
+    order[pos] = int(slot);
+    position[slot] = key < experts ? int(pos) : -1;
+  }
+  __device__ __forceinline__ void bin_start(uint32_t bin, uint32_t start) const {
+    offsets[bin] = int(start);
+  }
+};
+
+template <typename T, int N>
+__global__ __launch_bounds__(kRowThreads) void dispatch_kernel(Mat<const T> x,
+                                                               const int* __restrict__ position,
+                                                               int top_k, Mat<T> xs, Pieces p,
+                                                               Items items_of) {
+  const auto [first, items] = items_of.of_block(kRowThreads);
+  if (threadIdx.x >= items) return;
+  const Item it = ItemBase(first, p).at(threadIdx.x, p);
+  const int c = p.begin(it.piece);
+  using V = typename PieceOf<T, N>::type;
+  const V v = *reinterpret_cast<const V*>(x.at(it.row, c));
+  const int* pos = position + it.row * top_k;
+  for (int k = 0; k < top_k; ++k) {
+    const int q = pos[k];
+    if (q >= 0 && q < xs.rows) *reinterpret_cast<V*>(xs.at(q, c)) = v;
+  }
+}
+
+template <typename T, int N>
+__global__ __launch_bounds__(kRowThreads) void combine_kernel(Mat<const T> ys,
+                                                              const int* __restrict__ position,
+                                                              const float* __restrict__ weights,
+                                                              int top_k, Mat<T> y, Pieces p,
+                                                              Items items_of) {
+  const auto [first, items] = items_of.of_block(kRowThreads);
+  if (threadIdx.x >= items) return;
+  const Item it = ItemBase(first, p).at(threadIdx.x, p);
+  const int c = p.begin(it.piece);
+  const long long s = it.row * top_k;
+  Floats<N> acc = 0.f;
+  for (int k = 0; k < top_k; ++k) {
+    const int q = position[s + k];
+    if (q < 0 || q >= ys.rows) continue;
+    const float w = weights ? weights[s + k] : 1.f;
+    acc += w * load_piece<N>(ys.at(q, c));
+  }
+  store_piece<N>(y.at(it.row, c), acc);
+}
+
+// One workgroup per token.
+template <typename T, int N>
+__global__ __launch_bounds__(kRowThreads) void combine_grad_kernel(
+    Mat<const T> dy, Mat<const T> ys, const int* __restrict__ position,
+    const float* __restrict__ weights, int top_k, Mat<T> dys, float* __restrict__ dweights,
+    Pieces p, Items tokens) {
+  __shared__ float part[kRowThreads / kWave];
+  const long long t = (long long)tokens.of_block(1).first;
+  for (int k = 0; k < top_k; ++k) {
+    const long long s = t * top_k + k;
+    const int q = position[s];
+    const bool valid = q >= 0 && q < ys.rows;
+    float dot = 0.f;
+    if (valid) {
+      const float w = weights[s];
+      for (int i = threadIdx.x; i < int(p.per_row.d); i += kRowThreads) {
+        const int c = p.begin(i);
+        const int seen = i * N - c;  // elements that the piece before has added
+        const Floats<N> g = load_piece<N>(dy.at(t, c));
+        const Floats<N> v = load_piece<N>(ys.at(q, c));
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (e >= seen) dot += g[e] * v[e];
+        store_piece<N>(dys.at(q, c), w * g);
+      }
+    }
+#pragma unroll
+    for (int d = kWave / 2; d; d >>= 1) dot += __shfl_xor(dot, d, kWave);
+    __syncthreads();
+    if (lane_id() == 0) part[threadIdx.x / kWave] = dot;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float sum = 0.f;
+      for (int w = 0; w < kRowThreads / kWave; ++w) sum += part[w];
+      dweights[s] = sum;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace ps
+
+extern "C" {
+
+size_t ps_expert_sort_workspace_bytes(long long slots, int experts) {
+  if (slots < 0 || slots > (1LL << 30) || experts < 1 || experts > 1024) return 0;
+  return ps::id_sort_table_bytes(slots, experts + 1) + 16;
+}
+
+int ps_expert_sort(const ps_ids* ids, int experts, int* order, int* position, int* offsets,
+                   void* workspace, size_t workspace_bytes, ps_stream_t stream) {
+  PS_CHECK_IDS(ids);
+  PS_CHECK_ARG(experts >= 1 && experts <= 1024, "ps_expert_sort: 1 to 1024 experts");
+  PS_CHECK_ARG(offsets && (!ids->count || (order && position)), "ps_expert_sort: null output");
+  PS_CHECK_ARG(workspace && ps::aligned16(workspace) &&
+                   workspace_bytes >= ps_expert_sort_workspace_bytes(ids->count, experts),
+               "ps_expert_sort: workspace too small or misaligned");
+  const ps::ExpertSink sink{order, position, offsets, uint32_t(experts)};
+  ps::Digit dg{0, 1, experts + 1};
+  while ((1 << dg.bits) < dg.bins) ++dg.bits;
+  const uint32_t n = uint32_t(ids->count);
+  const hipStream_t st = ps::to_hip(stream);
+  if (ids->type == PS_I64)
+    return ps::id_sort_pass(
+        ps::IdSource<long long>{static_cast<const long long*>(ids->data), experts, -1}, sink, n,
+        dg, workspace, ps::ClearOnTheWay{}, st);
+  return ps::id_sort_pass(ps::IdSource<int>{static_cast<const int*>(ids->data), experts, -1}, sink,
+                          n, dg, workspace, ps::ClearOnTheWay{}, st);
+}
+
+int ps_expert_dispatch(const ps_rows* x, const int* position, int top_k, const ps_rows* xs,
+                       ps_stream_t stream) {
+  PS_CHECK_ROWS(x);
+  PS_CHECK_ROWS(xs);
+  PS_CHECK_ARG(x->dtype == xs->dtype && x->cols == xs->cols,
+               "ps_expert_dispatch: x and xs differ in type or width");
+  PS_CHECK_ARG(top_k >= 1 && top_k <= 1024, "ps_expert_dispatch: 1 to 1024 slots per token");
+  PS_CHECK_ARG(position || !x->rows, "ps_expert_dispatch: null positions");
+  PS_CHECK_ARG(!ps::overlap(x, xs), "ps_expert_dispatch: x and xs overlap");
+  if (!x->rows || !xs->rows) return PS_OK;
+  return ps::with_dtype(x->dtype, [&](auto t) {
+    using T = decltype(t);
+    return ps::with_width<sizeof(T)>(x->cols, [&](auto n) {
+      const ps::Pieces p(x->cols, n);
+      const unsigned long long items = (unsigned long long)x->rows * p.per_row.d;
+      return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
+        ps::dispatch_kernel<T, n><<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
+            ps::mat<const T>(x), position, top_k, ps::mat<T>(xs), p, part);
+      });
+    });
+  });
+}
+
+int ps_expert_combine(const ps_rows* ys, const int* position, const float* weights, int top_k,
+                      const ps_rows* y, ps_stream_t stream) {
+  PS_CHECK_ROWS(ys);
+  PS_CHECK_ROWS(y);
+  PS_CHECK_ARG(ys->dtype == y->dtype && ys->cols == y->cols,
+               "ps_expert_combine: ys and y differ in type or width");
+  PS_CHECK_ARG(top_k >= 1 && top_k <= 1024, "ps_expert_combine: 1 to 1024 slots per token");
+  PS_CHECK_ARG(position || !y->rows, "ps_expert_combine: null positions");
+  PS_CHECK_ARG(!ps::overlap(ys, y), "ps_expert_combine: ys and y overlap");
+  if (!y->rows) return PS_OK;
+  return ps::with_dtype(y->dtype, [&](auto t) {
+    using T = decltype(t);
+    return ps::with_width<sizeof(T)>(y->cols, [&](auto n) {
+      const ps::Pieces p(y->cols, n);
+      const unsigned long long items = (unsigned long long)y->rows * p.per_row.d;
+      return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
+        ps::combine_kernel<T, n><<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
+            ps::mat<const T>(ys), position, weights, top_k, ps::mat<T>(y), p, part);
+      });
+    });
+  });
+}
+
+int ps_expert_combine_grad(const ps_rows* dy, const ps_rows* ys, const int* position,
+                           const float* weights, int top_k, const ps_rows* dys, float* dweights,
+                           ps_stream_t stream) {
+  PS_CHECK_ROWS(dy);
+  PS_CHECK_ROWS(ys);
+  PS_CHECK_ROWS(dys);
+  PS_CHECK_ARG(dy->dtype == ys->dtype && dy->dtype == dys->dtype && dy->cols == ys->cols &&
+                   dy->cols == dys->cols && ys->rows == dys->rows,
+               "ps_expert_combine_grad: dy, ys and dys differ in type, width or rows");
+  PS_CHECK_ARG(top_k >= 1 && top_k <= 1024, "ps_expert_combine_grad: 1 to 1024 slots per token");
+  PS_CHECK_ARG((position && weights && dweights) || !dy->rows,
+               "ps_expert_combine_grad: null positions or weights");
+  PS_CHECK_ARG(!ps::overlap(dy, dys) && !ps::overlap(ys, dys),
+               "ps_expert_combine_grad: dys overlaps an input");
+  if (!dy->rows) return PS_OK;
+  return ps::with_dtype(dy->dtype, [&](auto t) {
+    using T = decltype(t);
+    return ps::with_width<sizeof(T)>(dy->cols, [&](auto n) {
+      const ps::Pieces p(dy->cols, n);
+      return ps::launch_items(dy->rows, 1, [&](uint32_t blocks, ps::Items part) {
+        ps::combine_grad_kernel<T, n><<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
+            ps::mat<const T>(dy), ps::mat<const T>(ys), position, weights, top_k,
+            ps::mat<T>(dys), dweights, p, part);
+      });
+    });
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,290 @@
+// The norm over many gradient tensors, and clipping by it.
+//
+// The tensors are cut into chunks; a fixed number of workgroups walks them and
+// each adds its chunks' squares in 64 bits: FP32 squares overflow from 1.8e19
+// and vanish below 1e-23, and 64-bit sums hide every rounding order. One launch
+// leaves a sum per workgroup, and the next launch's workgroups each add those
+// (at most kBlocks, from the L2) before they scale their chunks: no atomics, so
+// the same bits every time, and no launch between the two.
+//
+// Bound by memory: every gradient is read once for the norm and, where it
+// changes, once more to be scaled. The second pass walks the chunks backwards,
+// so what the first one read last is still in the last-level cache.
+#include <algorithm>
+#include <vector>
+
+#include "ps_rows.hpp"
+
+namespace ps {
+
+struct GradTensor {
+  const void* data;
+  void* out;
+  long long count;
+  int dtype, out_dtype;
+};
+struct GradChunk {
+  uint32_t tensor, index;  // elements [index * chunk, ...) of the tensor
+};
+
+namespace {
+
+constexpr int kClipThreads = 256;
+constexpr uint32_t kBlocks = 2048;
+constexpr int kStep = 2048;  // chunks are multiples of this many elements
+
+struct Grads {
+  const GradTensor* tensors;
+  const GradChunk* chunks;
+  uint32_t chunk_count, chunk;
+  bool in_place;
+};
+
+// Sum over the workgroup, in every thread.
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[kClipThreads / kWave];
+#pragma unroll
+  for (int d = kWave / 2; d; d >>= 1) v += __shfl_xor(v, d, kWave);
+  __syncthreads();
+  if (lane_id() == 0) part[threadIdx.x / kWave] = v;
+  __syncthreads();
+  v = 0;
+  for (int w = 0; w < kClipThreads / kWave; ++w) v += part[w];
+  return v;
+}
+
+template <typename T>
+__device__ double square_sum(const T* p, uint32_t count) {
+  constexpr int N = 16 / sizeof(T);
+  double s = 0;
+  uint32_t i = threadIdx.x * N;
+  for (; i + N <= count; i += kClipThreads * N) {
+    const Floats<N> v = load_piece<N>(p + i);
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += double(v[e]) * double(v[e]);
+  }
+  for (; i < count; ++i) s += double(float(p[i])) * double(float(p[i]));
+  return s;
+}
+
+__global__ __launch_bounds__(kClipThreads) void norm_kernel(Grads g, double* __restrict__ sums) {
+  double s = 0;
+  for (uint32_t q = blockIdx.x; q < g.chunk_count; q += gridDim.x) {
+    const GradChunk ch = g.chunks[q];
+    const GradTensor t = g.tensors[ch.tensor];
+    const long long from = (long long)ch.index * g.chunk;
+    const uint32_t count = uint32_t(min((long long)g.chunk, t.count - from));
+    if (t.dtype == PS_F32)
+      s += square_sum(static_cast<const f32*>(t.data) + from, count);
+    else if (t.dtype == PS_F16)
+      s += square_sum(static_cast<const f16*>(t.data) + from, count);
+    else
+      s += square_sum(static_cast<const bf16*>(t.data) + from, count);
+  }
+  s = block_sum(s);
+  if (threadIdx.x == 0) sums[blockIdx.x] = s;
+}
+
+// The norm from the workgroups' sums, in every thread.
+__device__ __forceinline__ double norm_of(const double* sums, uint32_t count, double grad_scale) {
+  double s = 0;
+  for (uint32_t i = threadIdx.x; i < count; i += kClipThreads) s += sums[i];
+  return sqrt(block_sum(s)) * fabs(grad_scale);
+}
+
+__global__ __launch_bounds__(kClipThreads) void norm_join_kernel(const double* __restrict__ sums,
+                                                                 uint32_t count, double grad_scale,
+                                                                 float* __restrict__ norm) {
+  const double v = norm_of(sums, count, grad_scale);
+  if (threadIdx.x == 0) *norm = float(v);
+}
+
+template <typename T, typename O>
+__device__ void scale_chunk(const T* p, O* out, uint32_t count, float c) {
+  constexpr int N = 16 / (sizeof(T) < sizeof(O) ? sizeof(T) : sizeof(O));
+  uint32_t i = threadIdx.x * N;
+  for (; i + N <= count; i += kClipThreads * N) store_piece<N>(out + i, c * load_piece<N>(p + i));
+  for (; i < count; ++i) out[i] = O(c * float(p[i]));
+}
+
+template <typename T>
+__device__ void scale_to(const GradTensor& t, long long from, uint32_t count, float c) {
+  const T* p = static_cast<const T*>(t.data) + from;
+  if (t.out_dtype == PS_F32)
+    scale_chunk(p, static_cast<f32*>(t.out) + from, count, c);
+  else if (t.out_dtype == PS_F16)
+    scale_chunk(p, static_cast<f16*>(t.out) + from, count, c);
+  else
+    scale_chunk(p, static_cast<bf16*>(t.out) + from, count, c);
+}
+
+// sums: the norm kernel's, or null with *norm given.
+__global__ __launch_bounds__(kClipThreads) void clip_kernel(Grads g,
+                                                            const double* __restrict__ sums,
+                                                            uint32_t sum_count, double max_norm,
+                                                            double grad_scale,
+                                                            float* __restrict__ norm) {
+  double v;
+  if (sums) {
+    v = norm_of(sums, sum_count, grad_scale);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = float(v);
+  } else {
+    v = double(*norm);
+  }
+  const double ratio = max_norm / (v + 1e-6);
+  const float c = float((ratio > 1.0 ? 1.0 : ratio) * grad_scale);  // a NaN ratio stays
+  if (g.in_place && c == 1.f) return;
+  for (uint32_t q = blockIdx.x; q < g.chunk_count; q += gridDim.x) {
+    const GradChunk ch = g.chunks[g.chunk_count - 1 - q];
+    const GradTensor t = g.tensors[ch.tensor];
+    const long long from = (long long)ch.index * g.chunk;
+    const uint32_t count = uint32_t(min((long long)g.chunk, t.count - from));
+    if (t.dtype == PS_F32)
+      scale_to<f32>(t, from, count, c);
+    else if (t.dtype == PS_F16)
+      scale_to<f16>(t, from, count, c);
+    else
+      scale_to<bf16>(t, from, count, c);
+  }
+}
+
+}  // namespace
+}  // namespace ps
+
+struct ps_grad_list {
+  void* tables = nullptr;  // tensors, chunks, the workgroups' sums
+  ps::Grads grads{};
+  double* sums = nullptr;
+  uint32_t blocks = 0;
+};
+
+namespace ps {
+namespace {
+
+int launch_norm(const ps_grad_list& l, hipStream_t stream) {
+  if (!l.blocks) return PS_OK;
+  norm_kernel<<<l.blocks, kClipThreads, 0, stream>>>(l.grads, l.sums);
+  PS_LAUNCHED();
+  return PS_OK;
+}
+
+}  // namespace
+}  // namespace ps
+
+extern "C" {
+
+int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
+                        const int* dtypes, void* const* out, const int* out_dtypes,
+                        ps_grad_list** list) {
+  PS_CHECK_ARG(list, "ps_grad_list_create: null output");
+  *list = nullptr;
+  PS_CHECK_ARG(tensors >= 0 && tensors <= (1 << 24), "ps_grad_list_create: bad tensor count");
+  PS_CHECK_ARG(!tensors || (data && counts && dtypes && !out == !out_dtypes),
+               "ps_grad_list_create: null array");
+  try {
+    std::vector<ps::GradTensor> table;
+    long long total = 0;
+    for (int i = 0; i < tensors; ++i) {
+      const std::string name = "ps_grad_list_create: tensor " + std::to_string(i);
+      const int out_dtype = out ? out_dtypes[i] : dtypes[i];
+      PS_CHECK_ARG(ps::dtype_valid(dtypes[i]) && ps::dtype_valid(out_dtype),
+                   name + ": unknown element type");
+      PS_CHECK_ARG(counts[i] >= 0 && counts[i] <= (1LL << 44) && total <= (1LL << 44),
+                   name + ": bad count");
+      if (!counts[i]) continue;
+      void* const to = out ? out[i] : data[i];
+      PS_CHECK_ARG(data[i] && to, name + ": null data");
+      const size_t size = ps::dtype_size(dtypes[i]), out_size = ps::dtype_size(out_dtype);
+      PS_CHECK_ARG(reinterpret_cast<uintptr_t>(data[i]) % size == 0 &&
+                       reinterpret_cast<uintptr_t>(to) % out_size == 0,
+                   name + ": misaligned data");
+      PS_CHECK_ARG((to == data[i] && out_dtype == dtypes[i]) ||
+                       !ps::overlap(data[i], size_t(counts[i]) * size, to,
+                                    size_t(counts[i]) * out_size),
+                   name + ": overlaps its output");
+      table.push_back({data[i], to, counts[i], dtypes[i], out_dtype});
+      total += counts[i];
+    }
+    // about four chunks a workgroup, so that none has much more than another
+    long long chunk = total / (4LL * ps::kBlocks) / ps::kStep * ps::kStep;
+    chunk = std::min<long long>(std::max<long long>(chunk, ps::kStep), 32 * ps::kStep);
+    std::vector<ps::GradChunk> chunks;
+    bool in_place = true;
+    for (size_t i = 0; i < table.size(); ++i) {
+      in_place = in_place && table[i].out == table[i].data;
+      const long long n = (table[i].count + chunk - 1) / chunk;
+      PS_CHECK_ARG(n + (long long)chunks.size() < (1LL << 31), "ps_grad_list_create: too large");
+      for (long long q = 0; q < n; ++q) chunks.push_back({uint32_t(i), uint32_t(q)});
+    }
+    const size_t table_bytes = (table.size() * sizeof(ps::GradTensor) + 255) & ~size_t(255);
+    const size_t chunk_bytes = (chunks.size() * sizeof(ps::GradChunk) + 255) & ~size_t(255);
+    void* base = nullptr;
+    PS_HIP(ps::dev_malloc(&base, table_bytes + chunk_bytes + ps::kBlocks * sizeof(double)));
+    char* const at = static_cast<char*>(base);
+    int rc = PS_OK;
+    if (!table.empty())
+      rc = ps_memcpy_htod(at, table.data(), table.size() * sizeof(ps::GradTensor));
+    if (rc == PS_OK && !chunks.empty())
+      rc = ps_memcpy_htod(at + table_bytes, chunks.data(), chunks.size() * sizeof(ps::GradChunk));
+    ps_grad_list* l = rc == PS_OK ? new (std::nothrow) ps_grad_list : nullptr;
+    if (!l) {
+      ps::dev_free(base);
+      return rc != PS_OK ? rc : ps::fail(PS_ERR_RUNTIME, "ps_grad_list_create: out of memory");
+    }
+    l->tables = base;
+    l->grads.tensors = reinterpret_cast<const ps::GradTensor*>(at);
+    l->grads.chunks = reinterpret_cast<const ps::GradChunk*>(at + table_bytes);
+    l->grads.chunk_count = uint32_t(chunks.size());
+    l->grads.chunk = uint32_t(chunk);
+    l->grads.in_place = in_place;
+    l->sums = reinterpret_cast<double*>(at + table_bytes + chunk_bytes);
+    l->blocks = std::min(uint32_t(chunks.size()), ps::kBlocks);
+    *list = l;
+    return PS_OK;
+  } catch (const std::exception& e) {
+    return ps::fail(PS_ERR_RUNTIME, std::string("ps_grad_list_create: ") + e.what());
+  }
+}
+
+void ps_grad_list_destroy(ps_grad_list* list) {
+  if (!list) return;
+  ps::dev_free(list->tables);
+  delete list;
+}
+
+int ps_grad_norm(ps_grad_list* list, float grad_scale, float* norm, ps_stream_t stream) {
+  PS_CHECK_ARG(list && norm, "ps_grad_norm: null argument");
+  const hipStream_t st = ps::to_hip(stream);
+  const int rc = ps::launch_norm(*list, st);
+  if (rc != PS_OK) return rc;
+  ps::norm_join_kernel<<<1, ps::kClipThreads, 0, st>>>(list->sums, list->blocks,
+                                                       double(grad_scale), norm);
+  PS_LAUNCHED();
+  return PS_OK;
+}
+
+int ps_clip_grads(ps_grad_list* list, float max_norm, float grad_scale, const float* norm,
+                  ps_stream_t stream) {
+  PS_CHECK_ARG(list && norm, "ps_clip_grads: null argument");
+  PS_CHECK_ARG(max_norm >= 0.f, "ps_clip_grads: the bound is not a number from 0 up");
+  if (!list->blocks) return PS_OK;
+  ps::clip_kernel<<<list->blocks, ps::kClipThreads, 0, ps::to_hip(stream)>>>(
+      list->grads, nullptr, 0, double(max_norm), double(grad_scale), const_cast<float*>(norm));
+  PS_LAUNCHED();
+  return PS_OK;
+}
+
+int ps_clip_grad_norm(ps_grad_list* list, float max_norm, float grad_scale, float* norm,
+                      ps_stream_t stream) {
+  PS_CHECK_ARG(list && norm, "ps_clip_grad_norm: null argument");
+  PS_CHECK_ARG(max_norm >= 0.f, "ps_clip_grad_norm: the bound is not a number from 0 up");
+  const hipStream_t st = ps::to_hip(stream);
+  const int rc = ps::launch_norm(*list, st);
+  if (rc != PS_OK) return rc;
+  ps::clip_kernel<<<std::max(list->blocks, 1u), ps::kClipThreads, 0, st>>>(
+      list->grads, list->sums, list->blocks, double(max_norm), double(grad_scale), norm);
+  PS_LAUNCHED();
+  return PS_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,213 @@
+// Shared parts of the row operators (powersparse_rows.h): element types,
+// 16-byte row accesses, the item -> (row, column) map and argument checks.
+//
+// A row of `cols` elements is moved in pieces of N (16 bytes of the narrower
+// type). An item is one piece of one row; items are numbered row by row and
+// dealt to threads in order, so a wave's accesses are contiguous for every
+// width. The last piece of a row ends with the row and overlaps the one before
+// it when N does not divide cols: both write the same values there, and no row
+// needs element-sized accesses. Only rows shorter than N take pieces of one
+// element. Pieces are aligned to their element only, which global memory
+// accesses of any width allow.
+#pragma once
+
+#include "powersparse_rows.h"
+#include "ps_common.hpp"
+
+namespace ps {
+
+using f32 = float;
+using f16 = _Float16;
+using bf16 = __bf16;
+
+template <typename T, int N>
+struct PieceOf {
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+template <int N>
+using Floats = typename PieceOf<float, N>::type;
+
+template <int N, typename T>
+__device__ __forceinline__ Floats<N> load_piece(const T* p) {
+  if constexpr (N == 1) {
+    Floats<1> f;
+    f[0] = float(*p);
+    return f;
+  } else {
+    const auto v = *reinterpret_cast<const typename PieceOf<T, N>::type*>(p);
+    return __builtin_convertvector(v, Floats<N>);
+  }
+}
+
+template <int N, typename T>
+__device__ __forceinline__ void store_piece(T* p, const Floats<N>& f) {
+  if constexpr (N == 1) {
+    *p = T(f[0]);
+  } else {
+    *reinterpret_cast<typename PieceOf<T, N>::type*>(p) =
+        __builtin_convertvector(f, typename PieceOf<T, N>::type);
+  }
+}
+
+// A matrix as the kernels read it.
+template <typename T>
+struct Mat {
+  T* data;
+  long long rows, ld;
+  __device__ __forceinline__ T* at(long long r, int c) const { return data + r * ld + c; }
+};
+
+// x / d and x % d for x < 2^31, d >= 1, by a multiplication (Granlund and
+// Montgomery 1994): m = ceil(2^(32 + s) / d) - 2^32 with 2^(s-1) < d <= 2^s.
+struct FastDiv {
+  uint32_t d, m, s;
+  explicit FastDiv(uint32_t divisor) : d(divisor), m(0), s(0) {
+    while ((uint64_t(1) << s) < d) ++s;
+    m = uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t x) const {
+    const uint32_t t = __umulhi(x, m);
+    return uint32_t((uint64_t(t) + x) >> s);
+  }
+};
+
+// Pieces per row and where piece q begins.
+struct Pieces {
+  int cols, width;  // width: elements per piece
+  FastDiv per_row;
+  Pieces(long long cols_, int width_)
+      : cols(int(cols_)), width(width_), per_row(uint32_t((cols_ + width_ - 1) / width_)) {}
+  __device__ __forceinline__ int begin(int q) const { return min(q * width, cols - width); }
+};
+
+constexpr int kRowThreads = 256;
+
+// A launch's share of an operator's items (a launch holds fewer than 2^32
+// threads).
+struct Items {
+  unsigned long long begin, end;
+  struct Block {
+    unsigned long long first;  // this workgroup's first item
+    unsigned long long count;  // items from there to the share's end
+  };
+  __device__ __forceinline__ Block of_block(uint32_t per_block) const {
+    const unsigned long long f = begin + (unsigned long long)blockIdx.x * per_block;
+    return {f, end - f};
+  }
+};
+
+// Item `j` of this workgroup, counted from the workgroup's first item `first`
+// (64-bit: items may exceed 2^32), as (row, piece).
+struct Item {
+  long long row;
+  int piece;
+};
+struct ItemBase {
+  long long row;
+  uint32_t rest;
+  __device__ __forceinline__ ItemBase(unsigned long long first, const Pieces& p)
+      : row((long long)(first / p.per_row.d)), rest(uint32_t(first % p.per_row.d)) {}
+  __device__ __forceinline__ Item at(uint32_t j, const Pieces& p) const {
+    const uint32_t t = rest + j;
+    const uint32_t r = p.per_row.div(t);
+    return {row + r, int(t - r * p.per_row.d)};
+  }
+};
+
+__device__ __forceinline__ long long load_id(const int* ids, long long i) { return ids[i]; }
+__device__ __forceinline__ long long load_id(const long long* ids, long long i) { return ids[i]; }
+
+// --------------------------------------------------------------- host side
+
+inline size_t dtype_size(int dtype) { return dtype == PS_F32 ? 4 : 2; }
+inline bool dtype_valid(int dtype) { return dtype >= PS_F32 && dtype <= PS_BF16; }
+
+// Empty string, or what is wrong with a matrix.
+inline std::string rows_error(const ps_rows* m, const char* name) {
+  const std::string n = name;
+  if (!m) return n + " is null";
+  if (!dtype_valid(m->dtype)) return n + ": unknown element type";
+  if (m->rows < 0 || m->cols < 1 || m->cols > (1 << 24)) return n + ": bad shape";
+  if (m->ld < m->cols) return n + ": row stride shorter than a row";
+  if (m->rows && m->ld > (1LL << 48) / m->rows) return n + ": too large";
+  if (m->rows && !m->data) return n + ": null data";
+  if (reinterpret_cast<uintptr_t>(m->data) % dtype_size(m->dtype)) return n + ": misaligned data";
+  return "";
+}
+inline std::string ids_error(const ps_ids* ids) {
+  if (!ids) return "ids is null";
+  if (ids->type != PS_I32 && ids->type != PS_I64) return "ids: unknown id type";
+  if (ids->count < 0 || ids->count > (1LL << 30)) return "ids: bad count";
+  if (ids->count && !ids->data) return "ids: null data";
+  if (reinterpret_cast<uintptr_t>(ids->data) % (ids->type == PS_I64 ? 8 : 4))
+    return "ids: misaligned data";
+  return "";
+}
+#define PS_CHECK_ROWS(m)                                          \
+  do {                                                            \
+    const std::string ps_error_ = ps::rows_error(m, #m);          \
+    if (!ps_error_.empty()) return ps::fail(PS_ERR_INVALID, ps_error_); \
+  } while (0)
+#define PS_CHECK_IDS(ids)                                         \
+  do {                                                            \
+    const std::string ps_error_ = ps::ids_error(ids);             \
+    if (!ps_error_.empty()) return ps::fail(PS_ERR_INVALID, ps_error_); \
+  } while (0)
+
+inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+inline size_t rows_bytes(const ps_rows* m) {
+  return m->rows ? (size_t(m->rows - 1) * size_t(m->ld) + size_t(m->cols)) * dtype_size(m->dtype)
+                 : 0;
+}
+// Column ranges of one wider matrix share its memory range and no element.
+inline bool overlap(const ps_rows* a, const ps_rows* b) {
+  if (!overlap(a->data, rows_bytes(a), b->data, rows_bytes(b))) return false;
+  const size_t pitch = size_t(a->ld) * dtype_size(a->dtype);
+  if (pitch != size_t(b->ld) * dtype_size(b->dtype)) return true;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a->data), y = reinterpret_cast<uintptr_t>(b->data);
+  const size_t apart = x <= y ? (y - x) % pitch : (pitch - (x - y) % pitch) % pitch;
+  return apart < size_t(a->cols) * dtype_size(a->dtype) ||
+         apart + size_t(b->cols) * dtype_size(b->dtype) > pitch;
+}
+
+template <typename T>
+inline Mat<T> mat(const ps_rows* m) {
+  return {static_cast<T*>(m->data), m->rows, m->ld};
+}
+
+// Calls f(T{}) with the element type of `dtype`.
+template <typename F>
+inline int with_dtype(int dtype, F&& f) {
+  if (dtype == PS_F32) return f(f32{});
+  if (dtype == PS_F16) return f(f16{});
+  return f(bf16{});
+}
+
+// Calls f(N) with the elements per piece of rows of `cols` elements, the
+// narrower of whose types has `size` bytes, as a constant.
+template <int kSize, typename F>
+inline int with_width(long long cols, F&& f) {
+  constexpr int N = 16 / kSize;
+  if (cols >= N) return f(std::integral_constant<int, N>{});
+  return f(std::integral_constant<int, 1>{});
+}
+
+// Launches f(workgroups, Items) over `items` items, `per_block` for each
+// workgroup of up to 1024 threads.
+template <typename F>
+inline int launch_items(unsigned long long items, uint32_t per_block, F&& f) {
+  constexpr unsigned long long kBlocks = 1u << 21;
+  for (unsigned long long at = 0; at < items; at += kBlocks * per_block) {
+    const unsigned long long left = items - at;
+    const unsigned long long blocks = (left + per_block - 1) / per_block;
+    f(uint32_t(blocks < kBlocks ? blocks : kBlocks),
+      Items{at, blocks < kBlocks ? items : at + kBlocks * per_block});
+    PS_LAUNCHED();
+  }
+  return PS_OK;
+}
+
+}  // namespace ps

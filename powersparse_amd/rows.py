@@ -1,0 +1,296 @@
+"""Row operators on the device: embedding lookup and its gradient, tokens sorted by expert
+and back with their gradients, and the norm and clipping of many gradient tensors
+(include/powersparse_rows.h).
+
+Arrays are DeviceArray (a DeviceBuffer or raw pointer with a shape and a type) or any
+tensor object with data_ptr, shape, stride, dtype and is_cuda, such as torch's. Matrices
+are row-major with any row stride; element types are float32, float16 and bfloat16. Every
+call checks shapes, types and sizes on the host, enqueues its kernels on `stream` (an ops
+Stream, a raw handle, None: the null stream) and returns without synchronising: arrays and
+workspaces must stay alive until the stream has passed the call. Wrong arguments raise
+ValueError.
+"""
+import ctypes
+
+from . import _native
+from ._native import Ids, Rows
+
+_DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+_ID_TYPES = {"int32": 0, "int64": 1}
+_BYTES = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "int64": 8, "uint8": 1}
+
+
+class DeviceArray:
+    """A one- or two-dimensional array in device memory: `data` (DeviceBuffer, another
+    object with a `ptr`, or a device address), `shape`, `dtype` ("float32", "float16",
+    "bfloat16", "int32", "int64", "uint8"), `ld` the row stride in elements (default:
+    contiguous) and `offset` where it begins, in elements."""
+
+    def __init__(self, data, shape, dtype="float32", ld=None, offset=0):
+        if dtype not in _BYTES:
+            raise ValueError(f"dtype must be one of {sorted(_BYTES)}")
+        shape = (shape,) if isinstance(shape, int) else tuple(int(s) for s in shape)
+        if len(shape) not in (1, 2) or min(shape) < 0 or offset < 0:
+            raise ValueError("a DeviceArray has one or two dimensions")
+        self.shape, self.dtype, self.data = shape, dtype, data
+        self.ld = int(ld) if ld is not None else shape[-1]
+        if len(shape) == 1 and self.ld != shape[0] or self.ld < shape[-1]:
+            raise ValueError("row stride shorter than a row")
+        size = _BYTES[dtype]
+        elements = 0 if 0 in shape else (self.ld * (shape[0] - 1) + shape[1] if len(shape) == 2
+                                         else shape[0])
+        nbytes = getattr(data, "nbytes", None)
+        if nbytes is not None and (offset + elements) * size > nbytes:
+            raise ValueError("the buffer is too small for the array")
+        base = data.ptr if hasattr(data, "ptr") else int(data or 0)
+        self.ptr = (base or 0) + offset * size
+
+
+_tensor_dtypes = {}  # a tensor library's dtype object -> its name
+
+
+def _described(x, name):
+    """(address, shape, row stride or None for a vector, dtype name) of an array."""
+    if isinstance(x, DeviceArray):
+        return x.ptr, x.shape, x.ld if len(x.shape) == 2 else None, x.dtype
+    try:
+        dtype = _tensor_dtypes.get(x.dtype)
+        if dtype is None:
+            dtype = _tensor_dtypes[x.dtype] = str(x.dtype).rsplit(".", 1)[-1]
+        on_gpu, shape, stride, ptr = x.is_cuda, x.shape, x.stride(), x.data_ptr()
+    except (AttributeError, TypeError):
+        raise ValueError(f"{name}: not a device array") from None
+    if not on_gpu:
+        raise ValueError(f"{name} is not in device memory")
+    return ptr, shape, stride, dtype
+
+
+def _rows(x, name):
+    """The ps_rows of a matrix."""
+    ptr, shape, stride, dtype = _described(x, name)
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"{name}: element type {dtype} is not float32, float16 or bfloat16")
+    if len(shape) != 2:
+        raise ValueError(f"{name} is not a matrix")
+    rows, cols = shape
+    if type(stride) is tuple:
+        if stride[1] != 1 and cols > 1 and rows:
+            raise ValueError(f"{name}: elements of a row are not contiguous")
+        stride = stride[0]
+        if rows <= 1 or cols == 0:  # the stride is not used, and may be anything
+            stride = cols
+    return Rows(ptr, rows, cols, stride, code)
+
+
+def _flat(x, name, dtypes, count=None, optional=False):
+    """Address, element count and dtype of a contiguous array of any shape."""
+    if x is None and optional:
+        return None, 0, None
+    ptr, shape, stride, dtype = _described(x, name)
+    if dtype not in dtypes:
+        raise ValueError(f"{name}: element type {dtype} is not {' or '.join(dtypes)}")
+    n = 1
+    for s in shape:
+        n *= s
+    if type(stride) is tuple:
+        want = 1
+        for s, d in zip(reversed(shape), reversed(stride)):
+            if s != 1 and d != want and n:
+                raise ValueError(f"{name} is not contiguous")
+            want *= s
+    elif stride is not None and stride != shape[1] and shape[0] > 1:
+        raise ValueError(f"{name} is not contiguous")
+    if count is not None and n != count:
+        raise ValueError(f"{name} has {n} elements where {count} are needed")
+    return ptr, n, dtype
+
+
+def _ids(x, name="ids"):
+    ptr, n, dtype = _flat(x, name, _ID_TYPES)
+    return Ids(ptr, n, _ID_TYPES[dtype])
+
+
+def _space(x, name="workspace"):
+    """Address and bytes of a workspace: a DeviceBuffer or a contiguous array."""
+    if hasattr(x, "nbytes") and hasattr(x, "ptr") and not isinstance(x, DeviceArray):
+        return x.ptr, x.nbytes
+    ptr, n, dtype = _flat(x, name, _BYTES)
+    return ptr, n * _BYTES[dtype]
+
+
+def _stream(stream):
+    if stream is None or type(stream) is int:
+        return stream
+    return stream.ptr if hasattr(stream, "ptr") else int(stream)
+
+
+def _call(status):
+    if status:
+        from . import _hip_call
+        _hip_call(status)
+
+
+# --------------------------------------------------------------- embedding
+
+def EmbeddingLookup(table, ids, out, scale=1.0, stream=None):
+    """out[i] = scale * table[ids[i]]; zeros for ids outside the table. `ids` (int32 or
+    int64, any shape) are taken in order; out has one row for each. table and out may differ
+    in type."""
+    _call(_native.hip().ps_embedding_lookup(_rows(table, "table"), _ids(ids), scale,
+                                            _rows(out, "out"), _stream(stream)))
+
+
+def embedding_grad_workspace_bytes(count, cols, table_rows):
+    """Workspace of EmbeddingGrad for `count` ids, rows of `cols` and a table of `table_rows`."""
+    n = _native.hip().ps_embedding_grad_workspace_bytes(int(count), int(cols), int(table_rows))
+    if not n:
+        raise ValueError("embedding_grad_workspace_bytes: sizes out of range")
+    return n
+
+
+def EmbeddingGrad(ids, grad_out, grad_table, workspace, scale=1.0, padding_idx=-1,
+                  accumulate=False, stream=None):
+    """grad_table[v] = scale * sum of grad_out[i] over the i with ids[i] = v, zeros for rows
+    without ids; accumulate=True adds to grad_table instead. Ids outside the table and
+    `padding_idx` take no part. The sum's order is fixed: the same bits every time."""
+    ptr, nbytes = _space(workspace)
+    _call(_native.hip().ps_embedding_grad(
+        _ids(ids), _rows(grad_out, "grad_out"), scale, padding_idx, bool(accumulate),
+        _rows(grad_table, "grad_table"), ptr, nbytes, _stream(stream)))
+
+
+# ----------------------------------------------------------------- experts
+
+def expert_sort_workspace_bytes(slots, experts):
+    """Workspace of ExpertSort for `slots` ids (tokens * top_k) and `experts` experts."""
+    n = _native.hip().ps_expert_sort_workspace_bytes(int(slots), int(experts))
+    if not n:
+        raise ValueError("expert_sort_workspace_bytes: sizes out of range (1 to 1024 experts)")
+    return n
+
+
+def ExpertSort(ids, order, position, offsets, workspace, stream=None):
+    """Stable sort of the slots of `ids` (tokens x top_k experts) by expert: `order` the slots
+    by expert, dropped ones (id outside the experts) last; `position` each slot's place in
+    `order`, -1 for dropped ones; `offsets` (experts + 1) where each expert's slots begin.
+    All int32."""
+    slots = _ids(ids)
+    at, count, _ = _flat(offsets, "offsets", ("int32",))
+    ptr, nbytes = _space(workspace)
+    _call(_native.hip().ps_expert_sort(
+        slots, count - 1, _flat(order, "order", ("int32",), slots.count)[0],
+        _flat(position, "position", ("int32",), slots.count)[0], at, ptr, nbytes,
+        _stream(stream)))
+
+
+def _top_k(position, tokens):
+    """Address of the positions and slots per token."""
+    ptr, n, _ = _flat(position, "position", ("int32",))
+    if tokens == 0:
+        return ptr, 1
+    if n == 0 or n % tokens:
+        raise ValueError(f"position: {n} slots do not divide among {tokens} tokens")
+    return ptr, n // tokens
+
+
+def ExpertDispatch(x, position, xs, stream=None):
+    """xs[position[t, k]] = x[t]: every token's row to its slots' places. Rows of xs that no
+    position names are left alone, positions outside xs are skipped."""
+    src = _rows(x, "x")
+    ptr, top_k = _top_k(position, src.rows)
+    _call(_native.hip().ps_expert_dispatch(src, ptr, top_k, _rows(xs, "xs"), _stream(stream)))
+
+
+def ExpertCombine(ys, position, weights, y, stream=None):
+    """y[t] = sum over k of weights[t, k] * ys[position[t, k]] (float32 weights; None: ones);
+    positions outside ys are skipped."""
+    out = _rows(y, "y")
+    ptr, top_k = _top_k(position, out.rows)
+    w = _flat(weights, "weights", ("float32",), out.rows * top_k, optional=True)[0]
+    _call(_native.hip().ps_expert_combine(_rows(ys, "ys"), ptr, w, top_k, out, _stream(stream)))
+
+
+def ExpertDispatchGrad(dxs, position, dx, stream=None):
+    """The gradient of ExpertDispatch: dx[t] = sum over k of dxs[position[t, k]]."""
+    ExpertCombine(dxs, position, None, dx, stream)
+
+
+def ExpertCombineGrad(dy, ys, position, weights, dys, dweights, stream=None):
+    """The gradients of ExpertCombine: dys[position[t, k]] = weights[t, k] * dy[t] and
+    dweights[t, k] = <dy[t], ys[position[t, k]]>, 0 for dropped slots. Rows of dys that no
+    position names are left alone."""
+    src = _rows(dy, "dy")
+    ptr, top_k = _top_k(position, src.rows)
+    n = src.rows * top_k
+    _call(_native.hip().ps_expert_combine_grad(
+        src, _rows(ys, "ys"), ptr, _flat(weights, "weights", ("float32",), n)[0], top_k,
+        _rows(dys, "dys"), _flat(dweights, "dweights", ("float32",), n)[0], _stream(stream)))
+
+
+# --------------------------------------------------------------- gradients
+
+class GradientList:
+    """The gradient tensors of a model (contiguous arrays of any shape and of float32,
+    float16 or bfloat16) and where their clipped values go: `outs`, one of the same size for
+    each, or None for in place. Made once while the tensors stay where they are; calls on
+    one list must not overlap. Keeps the tensors alive."""
+
+    def __init__(self, grads, outs=None):
+        self._h = None
+        self._keep = (list(grads), list(outs) if outs is not None else None)
+        grads, outs = self._keep
+        if outs is not None and len(outs) != len(grads):
+            raise ValueError("outs: one for each gradient")
+        n = len(grads)
+        src = [_flat(g, f"gradient {i}", _DTYPES) for i, g in enumerate(grads)]
+        data = (ctypes.c_void_p * max(n, 1))(*[p for p, _, _ in src])
+        counts = (ctypes.c_longlong * max(n, 1))(*[c for _, c, _ in src])
+        types = (ctypes.c_int * max(n, 1))(*[_DTYPES[d] for _, _, d in src])
+        to = to_types = None
+        if outs is not None:
+            dst = [_flat(o, f"output {i}", _DTYPES, c) for i, (o, (_, c, _)) in
+                   enumerate(zip(outs, src))]
+            to = (ctypes.c_void_p * max(n, 1))(*[p for p, _, _ in dst])
+            to_types = (ctypes.c_int * max(n, 1))(*[_DTYPES[d] for _, _, d in dst])
+        h = ctypes.c_void_p()
+        _call(_native.hip().ps_grad_list_create(n, data, counts, types, to, to_types,
+                                                ctypes.byref(h)))
+        self._h = h.value
+
+    @property
+    def handle(self):
+        if not self._h:
+            raise ValueError("the gradient list is closed")
+        return self._h
+
+    def close(self):
+        if self._h:
+            _native.hip().ps_grad_list_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def GradNorm(grads, norm, grad_scale=1.0, stream=None):
+    """norm (one float32 on the device) = the 2-norm of grad_scale * g over a GradientList."""
+    _call(_native.hip().ps_grad_norm(grads.handle, grad_scale,
+                                     _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))
+
+
+def ClipGrads(grads, max_norm, norm, grad_scale=1.0, stream=None):
+    """g * grad_scale * min(1, max_norm / (norm + 1e-6)) with a given norm, e.g. one that the
+    ranks of a job have put together."""
+    _call(_native.hip().ps_clip_grads(grads.handle, max_norm, grad_scale,
+                                      _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))
+
+
+def ClipGradNorm(grads, max_norm, norm, grad_scale=1.0, stream=None):
+    """GradNorm and ClipGrads in one call: norm receives the norm before clipping."""
+    _call(_native.hip().ps_clip_grad_norm(grads.handle, max_norm, grad_scale,
+                                          _flat(norm, "norm", ("float32",), 1)[0],
+                                          _stream(stream)))

@@ -1,0 +1,183 @@
+"""What the row operators refuse, on the host and before any device call: shapes,
+types, strides, alignments, sizes, workspaces and overlaps, through Python and
+through the C ABI. The addresses are never followed."""
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+
+import powersparse_amd as ps
+from powersparse_amd import _native
+from powersparse_amd._native import Ids, Rows
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+A, B, C, D = (k << 32 for k in (1, 2, 3, 4))  # addresses far from each other
+
+
+def mat(at, rows, cols, dtype="float32", **more):
+    return ps.DeviceArray(at, (rows, cols), dtype, **more)
+
+
+def vec(at, n, dtype):
+    return ps.DeviceArray(at, n, dtype)
+
+
+def refused(text, f, *args, **kwargs):
+    with pytest.raises(ValueError, match=text):
+        f(*args, **kwargs)
+
+
+def test_every_declared_symbol_is_exported_and_bound():
+    text = open(os.path.join(ROOT, "include", "powersparse_rows.h")).read()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    names = sorted(set(re.findall(r"^\s*[A-Za-z_][\w\s\*]*?\b(ps_\w+)\s*\(", text, re.M)))
+    _native.libs()
+    out = subprocess.run(["nm", "-D", "--defined-only", _native.HIP_LIB_PATH],
+                         capture_output=True, text=True, check=True).stdout
+    exported = {line.split()[-1] for line in out.splitlines() if line.strip()}
+    assert len(names) >= 12 and not [n for n in names if n not in exported]
+    assert set(names) == {n for n, _, _ in _native.ROWS_API}
+
+
+def test_device_array():
+    refused("dtype", ps.DeviceArray, A, 4, "float64")
+    refused("one or two dimensions", ps.DeviceArray, A, (2, 2, 2))
+    refused("one or two dimensions", ps.DeviceArray, A, (-1,))
+    refused("row stride", ps.DeviceArray, A, (2, 8), ld=7)
+    refused("row stride", ps.DeviceArray, A, 8, ld=9)
+
+    class Buffer:
+        ptr, nbytes = A, 64
+
+    refused("too small", ps.DeviceArray, Buffer(), 17)
+    refused("too small", ps.DeviceArray, Buffer(), (2, 4), ld=13)
+    assert ps.DeviceArray(Buffer(), (2, 4), ld=12).ptr == A
+    assert ps.DeviceArray(Buffer(), 8, "float16", offset=24).ptr == A + 48
+    refused("too small", ps.DeviceArray, Buffer(), 8, "float16", offset=25)
+
+
+def test_tensors_on_the_host_are_refused():
+    host = torch.zeros((4, 4))
+    ids = torch.zeros(4, dtype=torch.int64)
+    refused("table is not in device memory", ps.EmbeddingLookup, host, ids, host)
+    refused("ids is not in device memory", ps.EmbeddingLookup, mat(A, 4, 4), ids, mat(B, 4, 4))
+    refused("not a device array", ps.EmbeddingLookup, [1.0], ids, host)
+    refused("gradient 0 is not in device memory", ps.GradientList, [host])
+    refused("workspace is not in device memory", ps.EmbeddingGrad, vec(C, 4, "int32"),
+            mat(A, 4, 4), mat(B, 4, 4), torch.zeros(1 << 20, dtype=torch.uint8))
+
+
+def test_lookup():
+    def call(table=None, ids=None, out=None):
+        ps.EmbeddingLookup(table or mat(A, 9, 8), ids or vec(B, 4, "int64"), out or mat(C, 4, 8))
+
+    refused("out is not ids x table columns", call, out=mat(C, 5, 8))
+    refused("out is not ids x table columns", call, out=mat(C, 4, 9))
+    refused("overlap", call, out=mat(A + 64, 4, 8))
+    refused("overlap", call, table=mat(A, 9, 8, ld=32), out=mat(A + 16, 4, 8, ld=32))
+    refused("element type int32", call, table=mat(A, 9, 8, "int32"))
+    refused("ids: element type float32", call, ids=vec(B, 4, "float32"))
+    refused("not a matrix", call, out=vec(C, 32, "float32"))
+    refused("misaligned", call, table=mat(A + 2, 9, 8))
+    refused("misaligned", call, ids=vec(B + 4, 4, "int64"))
+    refused("null data", call, table=mat(0, 9, 8))
+    refused("null data", call, ids=vec(0, 4, "int64"))
+    refused("bad shape", call, table=mat(A, 9, 0), out=mat(C, 4, 0))
+
+
+def test_lookup_grad():
+    work = vec(D, ps.embedding_grad_workspace_bytes(40, 8, 9), "uint8")
+
+    def call(ids=None, dy=None, grad=None, work=work):
+        ps.EmbeddingGrad(ids or vec(B, 40, "int32"), dy or mat(A, 40, 8), grad or mat(C, 9, 8),
+                         work)
+
+    refused("grad_out is not ids x grad columns", call, dy=mat(A, 41, 8))
+    refused("grad_out is not ids x grad columns", call, grad=mat(C, 9, 7))
+    refused("overlap", call, grad=mat(A, 9, 8))
+    refused("workspace too small", call, work=vec(D, work.shape[0] - 1, "uint8"))
+    refused("workspace too small or misaligned", call, work=vec(D + 8, 1 << 20, "uint8"))
+    refused("workspace too small", call, work=vec(0, work.shape[0], "uint8"))
+    refused("out of range", ps.embedding_grad_workspace_bytes, -1, 8, 9)
+    refused("out of range", ps.embedding_grad_workspace_bytes, 8, 0, 9)
+    refused("out of range", ps.embedding_grad_workspace_bytes, 8, 8, 1 << 31)
+
+
+def test_expert_sort():
+    work = vec(D, ps.expert_sort_workspace_bytes(40, 5), "uint8")
+
+    def call(ids=None, order=None, position=None, offsets=None, work=work):
+        ps.ExpertSort(ids or mat(A, 20, 2, "int64"), order or vec(B, 40, "int32"),
+                      position or mat(B + 4096, 20, 2, "int32"), offsets or vec(C, 6, "int32"),
+                      work)
+
+    refused("1 to 1024 experts", call, offsets=vec(C, 1, "int32"))
+    refused("1 to 1024 experts", call, offsets=vec(C, 1026, "int32"))
+    refused("order has 39 elements where 40", call, order=vec(B, 39, "int32"))
+    refused("position has 42 elements", call, position=mat(B, 21, 2, "int32"))
+    refused("offsets: element type int64", call, offsets=vec(C, 6, "int64"))
+    refused("ids is not contiguous", call, ids=mat(A, 20, 2, "int64", ld=3))
+    refused("workspace too small", call, work=vec(D, work.shape[0] - 1, "uint8"))
+    refused("null output", call, order=vec(0, 40, "int32"))
+    refused("1 to 1024 experts", ps.expert_sort_workspace_bytes, 40, 1025)
+
+
+def test_dispatch_and_combine():
+    x, xs, at = mat(A, 20, 8), mat(B, 40, 8), mat(C, 20, 2, "int32")
+    w = mat(C + 4096, 20, 2)
+    refused("41 slots do not divide among 20", ps.ExpertDispatch, x, vec(C, 41, "int32"), xs)
+    refused("differ in type or width", ps.ExpertDispatch, x, at, mat(B, 40, 8, "float16"))
+    refused("differ in type or width", ps.ExpertDispatch, x, at, mat(B, 40, 9))
+    refused("overlap", ps.ExpertDispatch, x, at, mat(A + 32, 40, 8))
+    refused("null positions", ps.ExpertDispatch, x, mat(0, 20, 2, "int32"), xs)
+    refused("1 to 1024 slots", ps.ExpertDispatch, x, mat(C, 20, 1025, "int32"), xs)
+    refused("weights has 41 elements", ps.ExpertCombine, xs, at, vec(D, 41, "float32"), x)
+    refused("weights: element type float16", ps.ExpertCombine, xs, at, mat(D, 20, 2, "float16"), x)
+    refused("differ in type or width", ps.ExpertCombine, mat(B, 40, 7), at, w, x)
+    refused("overlap", ps.ExpertCombine, mat(A, 40, 8), at, w, x)
+    refused("overlap", ps.ExpertDispatchGrad, mat(A, 40, 8), at, x)
+    dw = mat(D, 20, 2)
+    refused("differ in type, width or rows", ps.ExpertCombineGrad, x, xs, at, w, mat(D, 39, 8), dw)
+    refused("overlaps an input", ps.ExpertCombineGrad, x, xs, at, w, xs, dw)
+    refused("dweights has 20 elements", ps.ExpertCombineGrad, x, xs, at, w, mat(D, 40, 8),
+            mat(D, 20, 1))
+
+
+def test_column_ranges_of_one_matrix_that_overlap():
+    """x and xs in the rows of one buffer, some columns in common."""
+    for off in (1, 7, 25, 31, 33):
+        refused("overlap", ps.ExpertDispatch, mat(A, 20, 8, ld=32), mat(C, 20, 1, "int32"),
+                mat(A + 4 * off, 20, 8, ld=32))
+
+
+def test_gradient_list():
+    g = vec(A, 100, "float32")
+    refused("outs: one for each", ps.GradientList, [g], [])
+    refused("output 0 has 99 elements", ps.GradientList, [g], [vec(B, 99, "float32")])
+    refused("gradient 0: element type int32", ps.GradientList, [vec(A, 4, "int32")])
+    refused("tensor 0: null data", ps.GradientList, [vec(0, 4, "float32")])
+    refused("tensor 1: misaligned", ps.GradientList, [g, vec(B + 2, 4, "float32")])
+    refused("overlaps its output", ps.GradientList, [g], [vec(A + 4, 100, "float32")])
+    refused("overlaps its output", ps.GradientList, [g], [vec(A, 100, "float16")])
+    hip = _native.hip()
+    assert hip.ps_grad_norm(None, 1.0, A, None) == _native.PS_ERR_INVALID
+    assert hip.ps_clip_grads(None, 1.0, 1.0, A, None) == _native.PS_ERR_INVALID
+    assert hip.ps_clip_grad_norm(None, 1.0, 1.0, A, None) == _native.PS_ERR_INVALID
+    hip.ps_grad_list_destroy(None)
+
+
+def test_c_abi():
+    """What Python cannot pass."""
+    hip = _native.hip()
+    ok, ids = Rows(A, 4, 8, 8, 0), Ids(B, 4, 0)
+    out = Rows(C, 4, 8, 8, 0)
+    bad = [(None, ids, out), (ok, None, out), (ok, ids, None), (Rows(A, 4, 8, 8, 3), ids, out),
+           (Rows(A, 4, 8, 8, -1), ids, out), (Rows(A, -1, 8, 8, 0), ids, out),
+           (Rows(A, 4, 8, 7, 0), ids, out), (Rows(A, 1 << 40, 8, 1 << 20, 0), ids, out),
+           (Rows(A, 4, (1 << 24) + 1, 1 << 25, 0), ids, out), (ok, Ids(B, 4, 2), out),
+           (ok, Ids(B, -1, 0), out), (ok, Ids(B, (1 << 30) + 1, 0), out)]
+    for t, i, o in bad:
+        assert hip.ps_embedding_lookup(t, i, 1.0, o, None) == _native.PS_ERR_INVALID
+        assert _native.hip().ps_last_error()
