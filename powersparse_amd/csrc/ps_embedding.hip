@@ -6,15 +6,15 @@
 // The gradient is the transposed product. Atomic additions would make its bits
 // depend on their order and serialise on popular rows, so the ids are sorted
 // (stably, ps_id_sort.hpp) and the gradient rows are sums over runs of equal
-// ids. The sorted list is cut into chunks of kChunk entries, each one thread's
-// per piece of the width:
+// ids. The sorted list is cut into chunks, each one thread's per piece of the
+// width:
 //  - a run belongs to the chunk it starts in when it ends before the next
 //    chunk's end: one thread adds all of it and writes the row;
 //  - a longer run is cut at the chunks' borders, every part is kept as a row of
 //    32-bit partial sums, and a second launch adds the parts in order.
-// So partial sums cost traffic only for runs of more than kChunk entries, and
-// no row waits for one thread to walk a popular id's whole run. Rows without
-// ids are cleared by the same launch, from flags the sort sets.
+// So partial sums cost traffic only for runs longer than a chunk, and no row
+// waits for one thread to walk a popular id's whole run. Rows without ids are
+// cleared by the same launch, from flags the sort sets.
 #include <algorithm>
 
 #include "ps_id_sort.hpp"
@@ -38,7 +38,16 @@ __global__ __launch_bounds__(kRowThreads) void lookup_kernel(Mat<const T> table,
   store_piece<N>(out.at(it.row, c), v);
 }
 
-constexpr uint32_t kChunk = 16;
+// Entries per chunk: the fewest, from 16 to 256, that leave at most kRunThreads
+// threads for the chunks (four waves a SIMD): longer chunks mean fewer partial
+// sums, shorter ones more loads in flight.
+constexpr unsigned long long kRunThreads = 1u << 18;
+uint32_t chunk_size(long long n, long long cols) {
+  uint32_t c = 16;
+  while (c < 256 && (unsigned long long)(n / c) * ((unsigned long long)(cols + 7) / 8) > kRunThreads)
+    c *= 2;
+  return c;
+}
 
 struct FlagSink {
   static constexpr bool kStarts = false;
@@ -58,7 +67,7 @@ struct FlagSink {
 // row 2q, its last run's in row 2q + 1, ld floats apart.
 struct Runs {
   const uint32_t *keys, *at;
-  uint32_t n, rows;
+  uint32_t n, rows, chunk;  // chunk: entries of a chunk
   float* partial;
   long long ld;
   uint32_t *long_count, *long_list;  // the chunks in which long runs start
@@ -78,47 +87,102 @@ __device__ __forceinline__ void write_grad(const Mat<G>& grad, uint32_t row, int
   }
 }
 
+// One chunk's runs, for one piece of the width. Rows are loaded kAhead at a
+// time and one batch ahead of the additions, ids two batches ahead: a row's
+// address waits for its id, and a wait for loads also waits for the stores
+// issued before them, so the next rows are under way before a finished run is
+// written.
 template <typename T, typename G, int N>
 __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& grad, float scale,
                          bool accumulate, uint32_t chunk, int piece, const Pieces& p) {
+  constexpr int kAhead = 4;
+  using V = typename PieceOf<T, N>::type;
+  constexpr uint32_t kNone = 0xFFFFFFFFu;  // no key
   const int c = p.begin(piece);
   const int seen = piece * N - c;
-  const uint32_t b = chunk * kChunk, e = min(b + kChunk, r.n);
-  uint32_t i = b;
-  if (b > 0 && r.keys[b - 1] == r.keys[b]) {  // a run that starts in a chunk before
-    const uint32_t k = r.keys[b];
-    const bool is_long = k < r.rows && ((b > kChunk && r.keys[b - kChunk - 1] == k) ||
-                                        (b + kChunk < r.n && r.keys[b + kChunk] == k));
-    Floats<N> sum = 0.f;
-    for (; i < e && r.keys[i] == k; ++i)
-      if (is_long) sum += load_piece<N>(dy.at(r.at[i], c));
-    if (is_long) store_piece<N>(r.partial + (2ull * chunk) * r.ld + c, sum);
-  }
-  while (i < e) {
-    const uint32_t k = r.keys[i];
-    if (k >= r.rows) break;  // only ids that take no part follow
-    // the run ends with the chunk, or within the next one, or is long
-    const uint32_t next = min(e + kChunk, r.n);
-    Floats<N> sum = 0.f;
-    for (; i < e && r.keys[i] == k; ++i) sum += load_piece<N>(dy.at(r.at[i], c));
-    if (i == e && e < r.n && r.keys[e] == k) {
-      if (next < r.n && r.keys[next] == k) {
-        store_piece<N>(r.partial + (2ull * chunk + 1) * r.ld + c, sum);
-        if (piece == 0) r.long_list[atomicAdd(r.long_count, 1u)] = chunk;
-        break;
-      }
-      for (; i < next && r.keys[i] == k; ++i) sum += load_piece<N>(dy.at(r.at[i], c));
+  const uint32_t size = r.chunk, b = chunk * size, e = min(b + size, r.n);
+  const uint32_t next = min(e + size, r.n);
+  uint32_t id[2][kAhead], at[2][kAhead];  // of the batches after the loaded one
+  const auto load_ids = [&](uint32_t i, int s) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const uint32_t q = min(i + j, r.n - 1);
+      id[s][j] = r.keys[q];
+      at[s][j] = r.at[q];
     }
-    write_grad<G, N>(grad, k, c, seen, sum, scale, accumulate);
+  };
+  load_ids(b, 0);
+  load_ids(b + kAhead, 1);
+  const uint32_t first = r.keys[b], last = r.keys[e - 1];
+  // The first run may start in a chunk before: then it is that chunk's, or long.
+  const bool continued = b > 0 && r.keys[b - 1] == first;
+  const bool head_long = continued && ((b > size && r.keys[b - size - 1] == first) ||
+                                       (e < r.n && r.keys[e] == first));
+  // The last run may go on: then it is long, or this chunk's to the end.
+  const bool own_tail = e < r.n && r.keys[e] == last && last < r.rows &&
+                        !(continued && first == last);
+  const bool tail_long = own_tail && next < r.n && r.keys[next] == last;
+  const uint32_t end = own_tail && !tail_long ? next : e;
+
+  uint32_t key[2][kAhead];
+  V row[2][kAhead];
+  const auto load_rows = [&](uint32_t i, int s) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const bool mine = i + j < e || (i + j < end && id[s][j] == last);
+      key[s][j] = mine && id[s][j] < r.rows ? id[s][j] : kNone;
+      const bool wanted = key[s][j] != kNone && !(continued && !head_long && key[s][j] == first);
+      row[s][j] = wanted ? *reinterpret_cast<const V*>(dy.at(at[s][j], c)) : V(T(0.f));
+    }
+  };
+  uint32_t current = kNone;
+  bool in_head = false;
+  Floats<N> sum = 0.f;
+  const auto finish = [&] {
+    if (current >= r.rows) return;  // nothing yet
+    if (!in_head)
+      write_grad<G, N>(grad, current, c, seen, sum, scale, accumulate);
+    else if (head_long)
+      store_piece<N>(r.partial + (2ull * chunk) * r.ld + c, sum);
+  };
+  load_rows(b, 0);
+  for (uint32_t i = b; i < end; i += 2 * kAhead) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint32_t here = i + s * kAhead;
+      load_ids(here + 2 * kAhead, s);
+      load_rows(here + kAhead, s ^ 1);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (key[s][j] == kNone) continue;
+        if (key[s][j] != current) {
+          finish();
+          in_head = continued && key[s][j] == first;
+          current = key[s][j];
+          sum = 0.f;
+        }
+        sum += __builtin_convertvector(row[s][j], Floats<N>);
+      }
+    }
+    if (i + 2 * kAhead >= e && key[0][0] == kNone) break;  // the run has ended
+  }
+  if (tail_long) {
+    store_piece<N>(r.partial + (2ull * chunk + 1) * r.ld + c, sum);
+    if (piece == 0) r.long_list[atomicAdd(r.long_count, 1u)] = chunk;
+  } else {
+    finish();
   }
 }
 
 // Workgroups [0, run_blocks) add runs, the rest clear the rows without ids.
+// Cleared rows are not read again soon: non-temporal stores, and 16 KB a
+// workgroup.
+constexpr uint32_t kClearItems = 4;  // per thread
 template <typename T, typename G, int N>
 __global__ __launch_bounds__(kRowThreads) void grad_runs_kernel(
     Runs r, Mat<const T> dy, Mat<G> grad, float scale, bool accumulate, Pieces p,
     uint32_t run_blocks, unsigned long long run_items, const uint8_t* __restrict__ flags,
-    uint32_t rows_per_block) {
+    Items clear_items) {
   if (blockIdx.x < run_blocks) {
     const unsigned long long first = (unsigned long long)blockIdx.x * kRowThreads;
     if (first + threadIdx.x >= run_items) return;
@@ -126,32 +190,75 @@ __global__ __launch_bounds__(kRowThreads) void grad_runs_kernel(
     sum_runs<T, G, N>(r, dy, grad, scale, accumulate, uint32_t(it.row), it.piece, p);
     return;
   }
-  const long long row0 = (long long)(blockIdx.x - run_blocks) * rows_per_block;
-  const uint32_t count = uint32_t(min((long long)rows_per_block, grad.rows - row0));
-  const uint32_t items = count * p.per_row.d;
-  for (uint32_t j = threadIdx.x; j < items; j += kRowThreads) {
-    const uint32_t q = p.per_row.div(j);
-    if (!flags[row0 + q])
-      store_piece<N>(grad.at(row0 + q, p.begin(int(j - q * p.per_row.d))), Floats<N>(0.f));
+  const unsigned long long first =
+      clear_items.begin +
+      (unsigned long long)(blockIdx.x - run_blocks) * (kRowThreads * kClearItems);
+  const unsigned long long left = clear_items.end - first;
+  const ItemBase base(first, p);
+  Item it[kClearItems];
+  uint8_t used[kClearItems];
+#pragma unroll
+  for (uint32_t u = 0; u < kClearItems; ++u) {
+    const uint32_t j = u * kRowThreads + threadIdx.x;
+    it[u] = base.at(j, p);
+    used[u] = j < left ? flags[it[u].row] : 1;
   }
+  using V = typename PieceOf<G, N>::type;
+#pragma unroll
+  for (uint32_t u = 0; u < kClearItems; ++u)
+    if (!used[u])
+      __builtin_nontemporal_store(
+          V(G(0.f)), reinterpret_cast<V*>(grad.at(it[u].row, p.begin(it[u].piece))));
 }
 
 // Adds the parts of the long runs: the last part of the chunk a run starts in,
-// then the first parts of the chunks it reaches.
+// then the first parts of the chunks it reaches. A workgroup takes one run and
+// kJoinPieces pieces of the width, its thread groups each a share of the parts
+// in order, and the shares are added by halves.
+constexpr int kJoinThreads = 1024;
+constexpr int kJoinPieces = 16;
+constexpr int kJoinGroups = kJoinThreads / kJoinPieces;
+
 template <typename G, int N>
-__global__ __launch_bounds__(kRowThreads) void grad_join_kernel(Runs r, Mat<G> grad, float scale,
-                                                                bool accumulate, Pieces p) {
-  const uint32_t count = *r.long_count;
-  for (uint32_t l = blockIdx.x; l < count; l += gridDim.x) {
-    const uint32_t chunk = r.long_list[l];
-    const uint32_t k = r.keys[min((chunk + 1) * kChunk, r.n) - 1];
-    for (int piece = threadIdx.x; piece < int(p.per_row.d); piece += kRowThreads) {
-      const int c = p.begin(piece);
-      Floats<N> sum = load_piece<N>(r.partial + (2ull * chunk + 1) * r.ld + c);
-      for (uint32_t q = chunk + 1; q * kChunk < r.n && r.keys[q * kChunk] == k; ++q)
-        sum += load_piece<N>(r.partial + (2ull * q) * r.ld + c);
-      write_grad<G, N>(grad, k, c, piece * N - c, sum, scale, accumulate);
+__global__ __launch_bounds__(kJoinThreads) void grad_join_kernel(Runs r, Mat<G> grad, float scale,
+                                                                 bool accumulate, Pieces p) {
+  __shared__ float part[kJoinGroups / 2][kJoinPieces * N];
+  const uint32_t tiles = (p.per_row.d + kJoinPieces - 1) / kJoinPieces;
+  const unsigned long long work = (unsigned long long)*r.long_count * tiles;
+  const int group = threadIdx.x / kJoinPieces, lane = threadIdx.x % kJoinPieces;
+  for (unsigned long long l = blockIdx.x; l < work; l += gridDim.x) {
+    const uint32_t chunk = r.long_list[l / tiles];
+    const int piece = int(l % tiles) * kJoinPieces + lane;
+    const uint32_t k = r.keys[(chunk + 1) * r.chunk - 1];
+    uint32_t reached = 0;  // chunks after this one that begin inside the run
+    for (int found = kJoinThreads; found == kJoinThreads; reached += found) {
+      const unsigned long long q = (unsigned long long)(chunk + 1 + reached + threadIdx.x) * r.chunk;
+      found = __syncthreads_count(q < r.n && r.keys[q] == k);
     }
+    const uint32_t share = (reached + kJoinGroups - 1) / kJoinGroups;
+    const uint32_t from = min(group * share, reached), to = min(from + share, reached);
+    const bool on = piece < int(p.per_row.d);
+    const int c = on ? p.begin(piece) : 0;
+    Floats<N> sum = 0.f;
+    if (on) {
+      if (group == 0) sum = load_piece<N>(r.partial + (2ull * chunk + 1) * r.ld + c);
+      const float* at = r.partial + 2ull * (chunk + 1) * r.ld + c;
+#pragma unroll 8
+      for (uint32_t q = from; q < to; ++q) sum += load_piece<N>(at + 2ull * q * r.ld);
+    }
+    int half = kJoinGroups / 2;
+    while (half && half * share >= reached) half /= 2;  // groups without a share
+    for (; half; half /= 2) {
+      if (group >= half && group < 2 * half)
+#pragma unroll
+        for (int e = 0; e < N; ++e) part[group - half][lane * N + e] = sum[e];
+      __syncthreads();
+      if (group < half)
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += part[group][lane * N + e];
+      __syncthreads();
+    }
+    if (group == 0 && on) write_grad<G, N>(grad, k, c, piece * N - c, sum, scale, accumulate);
   }
 }
 
@@ -186,13 +293,19 @@ GradSpace grad_space(long long n, long long cols, long long rows) {
   s.table = take(id_sort_table_bytes(n, 1 << bits));
   s.cleared_bytes = (size_t(rows) + 16 + 15) & ~size_t(15);  // the long runs' count, the flags
   s.cleared = take(s.cleared_bytes);
-  const size_t chunks = size_t((n + kChunk - 1) / kChunk);
+  const size_t chunk = chunk_size(n, cols);
+  const size_t chunks = (size_t(n) + chunk - 1) / chunk;
   s.long_list = take(chunks * 4);
   s.ld = (cols + 7) & ~7LL;
   s.partial = take(2 * chunks * size_t(s.ld) * 4);
   s.total = at;
   return s;
 }
+
+// The one workgroup that sorts a tile clears this many 16-byte words on the way
+// (64 KB); more are cleared by a launch of their own.
+constexpr size_t kTileClears = 4096;
+__global__ void clear_kernel(ClearOnTheWay clear) { clear_share(clear); }
 
 // Sorts the ids; returns which of the two buffers holds the result.
 template <typename I>
@@ -201,7 +314,20 @@ int sort_ids(const I* ids, uint32_t n, long long rows, long long padding, char* 
   int bits = 0;
   const int passes = digit_passes(rows, &bits);
   const auto buffer = [&](size_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
-  ClearOnTheWay clear{reinterpret_cast<uint4*>(ws + s.cleared), s.cleared_bytes / 16};
+  ClearOnTheWay clear{reinterpret_cast<uint4*>(ws + s.cleared),
+                      flags ? s.cleared_bytes / 16 : 1};
+  if (n <= kIdTile) {
+    if (clear.count > kTileClears) {
+      clear_kernel<<<unsigned(std::min<size_t>((clear.count + 255) / 256, 1024)), 256, 0, stream>>>(
+          clear);
+      PS_LAUNCHED();
+      clear = {};
+    }
+    *result = 0;
+    return id_sort_tile(IdSource<I>{ids, rows, padding},
+                        FlagSink{buffer(s.keys[0]), buffer(s.at[0]), flags, uint32_t(rows)}, n,
+                        Digit{0, bits, 1 << bits}, passes, clear, stream);
+  }
   for (int k = 0; k < passes; ++k) {
     const Digit dg{k * bits, bits, 1 << bits};
     const int to = k & 1;
@@ -237,7 +363,7 @@ int ps_embedding_lookup(const ps_rows* table, const ps_ids* ids, float scale, co
     return ps::with_dtype(out->dtype, [&](auto o) {
       using T = decltype(t);
       using O = decltype(o);
-      return ps::with_width<(sizeof(T) < sizeof(O) ? sizeof(T) : sizeof(O))>(
+      return ps::with_width<(sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O))>(
           out->cols, [&](auto n) {
             const ps::Pieces p(out->cols, n);
             const unsigned long long items = (unsigned long long)out->rows * p.per_row.d;
@@ -298,38 +424,46 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
   r.ld = s.ld;
   r.long_count = reinterpret_cast<uint32_t*>(ws + s.cleared);
   r.long_list = reinterpret_cast<uint32_t*>(ws + s.long_list);
-  const uint32_t chunks = (n + ps::kChunk - 1) / ps::kChunk;
+  r.chunk = ps::chunk_size(ids->count, grad->cols);
+  const uint32_t chunks = (n + r.chunk - 1) / r.chunk;
   return ps::with_dtype(grad_out->dtype, [&](auto t) {
     return ps::with_dtype(grad->dtype, [&](auto g) {
       using T = decltype(t);
       using G = decltype(g);
-      return ps::with_width<(sizeof(T) < sizeof(G) ? sizeof(T) : sizeof(G))>(
+      return ps::with_width<(sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G))>(
           grad->cols, [&](auto w) {
             const ps::Pieces p(grad->cols, w);
             const unsigned long long items = (unsigned long long)chunks * p.per_row.d;
             const unsigned long long run_blocks =
                 (items + ps::kRowThreads - 1) / ps::kRowThreads;
-            // 64 KB and more a clearing workgroup, at most 2^20 of them
-            unsigned long long per_block =
-                std::max<unsigned long long>(1, 65536 / (size_t(grad->cols) * sizeof(G)));
-            per_block = std::max<unsigned long long>(per_block, (grad->rows >> 20) + 1);
-            const unsigned long long clear_blocks =
-                flags ? (grad->rows + per_block - 1) / per_block : 0;
-            PS_CHECK_ARG(run_blocks + clear_blocks < (1u << 24) &&
-                             per_block * p.per_row.d < (1u << 31),
-                         "ps_embedding_grad: too many elements for one launch");
-            if (run_blocks + clear_blocks) {
+            // The first launch takes the runs and as many rows to clear as
+            // fit beside them, the others more rows.
+            const unsigned long long clears =
+                flags ? (unsigned long long)grad->rows * p.per_row.d : 0;
+            PS_CHECK_ARG(run_blocks < (1u << 23), "ps_embedding_grad: too many ids for one launch");
+            uint32_t runs = uint32_t(run_blocks);
+            unsigned long long done = 0;
+            do {
+              const unsigned long long per_block = ps::kRowThreads * ps::kClearItems;
+              const unsigned long long blocks =
+                  std::min<unsigned long long>((clears - done + per_block - 1) / per_block, 1u << 23);
+              if (!(runs + blocks)) break;
+              const unsigned long long end = std::min(clears, done + blocks * per_block);
               ps::grad_runs_kernel<T, G, w>
-                  <<<uint32_t(run_blocks + clear_blocks), ps::kRowThreads, 0, st>>>(
+                  <<<uint32_t(runs + blocks), ps::kRowThreads, 0, st>>>(
                       r, ps::mat<const T>(grad_out), ps::mat<G>(grad), scale, accumulate != 0, p,
-                      uint32_t(run_blocks), items, flags, uint32_t(per_block));
+                      runs, items, flags, ps::Items{done, end});
               PS_LAUNCHED();
-            }
-            // a long run takes more than kChunk ids
-            if (n > ps::kChunk + 1) {
+              runs = 0;
+              done = end;
+            } while (done < clears);
+            // a long run holds more than a chunk
+            if (n > r.chunk + 1) {
+              const uint32_t tiles = (p.per_row.d + ps::kJoinPieces - 1) / ps::kJoinPieces;
+              const unsigned long long most = (unsigned long long)chunks * tiles;
               ps::grad_join_kernel<G, w>
-                  <<<std::min(chunks, 2048u), ps::kRowThreads, 0, st>>>(r, ps::mat<G>(grad), scale,
-                                                                       accumulate != 0, p);
+                  <<<uint32_t(std::min(most, 512ull)), ps::kJoinThreads, 0, st>>>(
+                      r, ps::mat<G>(grad), scale, accumulate != 0, p);
               PS_LAUNCHED();
             }
             return PS_OK;

@@ -130,12 +130,13 @@ int ps_expert_sort(const ps_ids* ids, int experts, int* order, int* position, in
   while ((1 << dg.bits) < dg.bins) ++dg.bits;
   const uint32_t n = uint32_t(ids->count);
   const hipStream_t st = ps::to_hip(stream);
+  const auto sort = [&](const auto& src) {
+    if (n <= ps::kIdTile) return ps::id_sort_tile(src, sink, n, dg, 1, ps::ClearOnTheWay{}, st);
+    return ps::id_sort_pass(src, sink, n, dg, workspace, ps::ClearOnTheWay{}, st);
+  };
   if (ids->type == PS_I64)
-    return ps::id_sort_pass(
-        ps::IdSource<long long>{static_cast<const long long*>(ids->data), experts, -1}, sink, n,
-        dg, workspace, ps::ClearOnTheWay{}, st);
-  return ps::id_sort_pass(ps::IdSource<int>{static_cast<const int*>(ids->data), experts, -1}, sink,
-                          n, dg, workspace, ps::ClearOnTheWay{}, st);
+    return sort(ps::IdSource<long long>{static_cast<const long long*>(ids->data), experts, -1});
+  return sort(ps::IdSource<int>{static_cast<const int*>(ids->data), experts, -1});
 }
 
 int ps_expert_dispatch(const ps_rows* x, const int* position, int top_k, const ps_rows* xs,

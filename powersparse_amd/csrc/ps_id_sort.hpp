@@ -2,12 +2,16 @@
 // become keys below a limit (ids out of range take the limit itself, so they
 // sort last), and a pass puts the elements of one digit after another's.
 //
-// A pass over more than one tile counts every tile's digits, scans the counts
-// (digit by digit, tile by tile) and places the elements; a single tile does it
-// all in one launch. A tile is ranked wave by wave: the lanes of 64 consecutive
-// elements that hold the same digit are found with one ballot per bit, an
-// element's rank is (its digit's count in the wave's earlier steps) + (lower
-// lanes with that digit). No atomics, so equal keys keep their order.
+// A tile is ranked wave by wave: the lanes of 64 consecutive elements that hold
+// the same digit are found with one ballot per bit, an element's rank is (its
+// digit's count in the wave's earlier steps) + (lower lanes with that digit). No
+// atomics decide a place, so equal keys keep their order.
+//
+// Launches, at some 5 us each, are what a sort of this size costs. One tile
+// takes one for all digits, the elements staying in LDS. Up to kSelfTiles tiles
+// take two a digit: one counts every tile's digits, the next one's workgroups
+// each add up the counts that precede their own. More tiles take the device
+// scan between the two, as every workgroup would read the whole table.
 #pragma once
 
 #include "ps_common.hpp"
@@ -59,27 +63,31 @@ struct Digit {
   int shift, bits, bins;
 };
 
-template <typename Source>
-__device__ __forceinline__ void rank_tile(const Source& src, uint32_t n, const Digit& dg,
-                                          uint16_t* cnt, uint32_t (&key)[kIdItems],
+constexpr uint32_t kSelfTiles = 128;
+constexpr int kIdWaves = kIdThreads / kWave;
+
+// Index in the tile of item r of this thread.
+__device__ __forceinline__ uint32_t tile_item(int r) {
+  return (threadIdx.x / kWave) * (kIdItems * kWave) + r * kWave + lane_id();
+}
+
+// The waves' digit counts in cnt (bins per wave) and the items' ranks among
+// their wave's; `valid` items from the tile's start. Other waves may read cnt
+// after a barrier.
+__device__ __forceinline__ void rank_tile(const uint32_t (&key)[kIdItems], uint32_t valid,
+                                          const Digit& dg, uint16_t* cnt,
                                           uint32_t (&loc)[kIdItems]) {
-  const int w = threadIdx.x / kWave, lane = lane_id();
+  const int lane = lane_id();
   const uint32_t mask = (1u << dg.bits) - 1u;
   const uint64_t lower = (uint64_t(1) << lane) - 1u;
-  uint16_t* mine = cnt + w * dg.bins;
+  uint16_t* mine = cnt + (threadIdx.x / kWave) * dg.bins;
   for (int b = lane; b < dg.bins; b += kWave) mine[b] = 0;
-  const uint32_t base = blockIdx.x * kIdTile + w * (kIdItems * kWave) + lane;
-#pragma unroll
-  for (int r = 0; r < kIdItems; ++r) {
-    const uint32_t i = base + r * kWave;
-    key[r] = i < n ? src.key(i) : 0u;
-  }
   wave_lds_sync();
 #pragma unroll
   for (int r = 0; r < kIdItems; ++r) {
-    const bool valid = base + r * kWave < n;
+    const bool in = tile_item(r) < valid;
     const uint32_t d = (key[r] >> dg.shift) & mask;
-    uint64_t peers = __ballot(valid);
+    uint64_t peers = __ballot(in);
     for (int b = 0; b < dg.bits; ++b) {
       const bool one = (d >> b) & 1u;
       const uint64_t m = __ballot(one);
@@ -89,9 +97,43 @@ __device__ __forceinline__ void rank_tile(const Source& src, uint32_t n, const D
     loc[r] = before + uint32_t(__popcll(peers & lower));
     wave_lds_sync();
     // the highest lane of each digit advances the wave's counter
-    if (valid && (peers >> lane) == 1u) mine[d] = uint16_t(before + uint32_t(__popcll(peers)));
+    if (in && (peers >> lane) == 1u) mine[d] = uint16_t(before + uint32_t(__popcll(peers)));
     wave_lds_sync();
   }
+}
+
+// Turns bin b's counts into the waves' offsets in it; returns its total.
+__device__ __forceinline__ uint32_t wave_offsets(uint16_t* cnt, int bins, int b) {
+  uint32_t c[kIdWaves], total = 0;
+#pragma unroll
+  for (int q = 0; q < kIdWaves; ++q) c[q] = cnt[q * bins + b];
+#pragma unroll
+  for (int q = 0; q < kIdWaves; ++q) {
+    cnt[q * bins + b] = uint16_t(total);
+    total += c[q];
+  }
+  return total;
+}
+
+// In place exclusive scan of v[0 .. bins), bins <= 2 * kIdThreads; begins and
+// ends with a barrier.
+__device__ __forceinline__ void scan_bins(uint32_t* v, int bins, uint32_t* wave_sum) {
+  const int w = threadIdx.x / kWave, lane = lane_id(), b = 2 * threadIdx.x;
+  __syncthreads();
+  const uint32_t x = b < bins ? v[b] : 0u, y = b + 1 < bins ? v[b + 1] : 0u;
+  uint32_t incl = x + y;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const uint32_t t = uint32_t(__shfl_up(int(incl), d, kWave));
+    if (lane >= d) incl += t;
+  }
+  if (lane == kWave - 1) wave_sum[w] = incl;
+  __syncthreads();
+  uint32_t first = incl - x - y;
+  for (int q = 0; q < w; ++q) first += wave_sum[q];
+  if (b < bins) v[b] = first;
+  if (b + 1 < bins) v[b + 1] = first + x;
+  __syncthreads();
 }
 
 __device__ __forceinline__ void clear_share(const ClearOnTheWay& c) {
@@ -100,83 +142,135 @@ __device__ __forceinline__ void clear_share(const ClearOnTheWay& c) {
     c.data[i] = uint4{0, 0, 0, 0};
 }
 
-// Counts of every tile: table[digit * tiles + tile].
+// Where the count of (tile, bin) is in the table.
+struct TableAt {
+  size_t tile, bin;  // strides
+};
+
+// Counts of every tile.
 template <typename Source>
 __global__ __launch_bounds__(kIdThreads) void id_count_kernel(Source src, uint32_t n, Digit dg,
                                                               uint32_t* __restrict__ table,
-                                                              ClearOnTheWay clear) {
-  __shared__ uint16_t cnt[kIdThreads / kWave * kIdMaxBins];
-  clear_share(clear);
+                                                              TableAt at, ClearOnTheWay clear) {
+  __shared__ uint16_t cnt[kIdWaves * kIdMaxBins];
+  const uint32_t base = blockIdx.x * kIdTile, valid = min(n - base, kIdTile);
   uint32_t key[kIdItems], loc[kIdItems];
-  rank_tile(src, n, dg, cnt, key, loc);
+#pragma unroll
+  for (int r = 0; r < kIdItems; ++r)
+    key[r] = tile_item(r) < valid ? src.key(base + tile_item(r)) : 0u;
+  clear_share(clear);
+  rank_tile(key, valid, dg, cnt, loc);
   __syncthreads();
-  for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) {
-    uint32_t total = 0;
-    for (int q = 0; q < kIdThreads / kWave; ++q) total += cnt[q * dg.bins + b];
-    table[size_t(b) * gridDim.x + blockIdx.x] = total;
-  }
+  for (int b = threadIdx.x; b < dg.bins; b += kIdThreads)
+    table[blockIdx.x * at.tile + b * at.bin] = wave_offsets(cnt, dg.bins, b);
 }
 
-// Places a tile's elements. starts: the scanned counts, or null for a single
-// tile, whose own counts are scanned here.
-template <typename Source, typename Sink>
+// Places a tile's elements. table: the counts (kSelf), or their scan.
+template <bool kSelf, typename Source, typename Sink>
 __global__ __launch_bounds__(kIdThreads) void id_place_kernel(Source src, Sink sink, uint32_t n,
                                                               Digit dg,
-                                                              const uint32_t* __restrict__ starts,
-                                                              ClearOnTheWay clear) {
-  __shared__ uint16_t cnt[kIdThreads / kWave * kIdMaxBins];
-  __shared__ uint32_t start[kIdMaxBins + 1];
-  __shared__ uint32_t wave_sum[kIdThreads / kWave];
-  constexpr int kWaves = kIdThreads / kWave;
-  const int w = threadIdx.x / kWave, lane = lane_id();
-  clear_share(clear);
-  uint32_t key[kIdItems], loc[kIdItems];
-  rank_tile(src, n, dg, cnt, key, loc);
-  __syncthreads();
-  // counts -> the waves' offsets in their digit; thread t owns digits 2t, 2t + 1
-  uint32_t total[2] = {0, 0};
-  for (int k = 0; k < 2; ++k) {
-    const int b = 2 * int(threadIdx.x) + k;
-    if (b < dg.bins)
-      for (int q = 0; q < kWaves; ++q) {
-        const uint32_t c = cnt[q * dg.bins + b];
-        cnt[q * dg.bins + b] = uint16_t(total[k]);
-        total[k] += c;
-      }
-  }
-  uint32_t first;
-  if (starts) {
-    first = 0;
-  } else {
-    uint32_t incl = total[0] + total[1];
+                                                              const uint32_t* __restrict__ table,
+                                                              TableAt at) {
+  __shared__ uint16_t cnt[kIdWaves * kIdMaxBins];
+  __shared__ uint32_t start[kIdMaxBins], ahead[kSelf ? kIdMaxBins : 1];
+  __shared__ uint32_t wave_sum[kIdWaves];
+  const uint32_t base = blockIdx.x * kIdTile, valid = min(n - base, kIdTile);
+  uint32_t key[kIdItems], value[kIdItems], loc[kIdItems];
 #pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const uint32_t t = uint32_t(__shfl_up(int(incl), d, kWave));
-      if (lane >= d) incl += t;
-    }
-    if (lane == kWave - 1) wave_sum[w] = incl;
-    __syncthreads();
-    first = incl - (total[0] + total[1]);
-    for (int q = 0; q < w; ++q) first += wave_sum[q];
+  for (int r = 0; r < kIdItems; ++r) {
+    const bool in = tile_item(r) < valid;
+    key[r] = in ? src.key(base + tile_item(r)) : 0u;
+    value[r] = in ? src.value(base + tile_item(r)) : 0u;
   }
-  for (int k = 0; k < 2; ++k) {
-    const int b = 2 * int(threadIdx.x) + k;
-    if (b < dg.bins) {
-      const uint32_t s = starts ? starts[size_t(b) * gridDim.x + blockIdx.x] : first;
-      start[b] = s;
-      if (Sink::kStarts && blockIdx.x == 0) sink.bin_start(uint32_t(b), s);
-      first += total[k];
+  if constexpr (kSelf) {
+    // start: all tiles' counts, ahead: the earlier tiles'. The tiles are shared
+    // out among as many threads a bin as there are.
+    for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) start[b] = ahead[b] = 0;
+    __syncthreads();
+    int parts = kIdThreads;  // threads a bin
+    while (parts > 1 && parts * dg.bins > kIdThreads) parts /= 2;
+    const uint32_t tiles = gridDim.x;
+    for (int j = threadIdx.x; j < parts * dg.bins; j += kIdThreads) {
+      const int part = j / dg.bins, b = j - part * dg.bins;
+      uint32_t all = 0, before = 0;
+#pragma unroll 8
+      for (uint32_t t = part; t < tiles; t += parts) {
+        const uint32_t c = table[t * at.tile + b * at.bin];
+        all += c;
+        before += t < blockIdx.x ? c : 0u;
+      }
+      atomicAdd(&start[b], all);
+      atomicAdd(&ahead[b], before);
     }
+    scan_bins(start, dg.bins, wave_sum);
+  } else {
+    for (int b = threadIdx.x; b < dg.bins; b += kIdThreads)
+      start[b] = table[blockIdx.x * at.tile + b * at.bin];
+  }
+  rank_tile(key, valid, dg, cnt, loc);
+  __syncthreads();
+  for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) {
+    (void)wave_offsets(cnt, dg.bins, b);
+    if (Sink::kStarts && blockIdx.x == 0) sink.bin_start(uint32_t(b), start[b]);
+    if constexpr (kSelf) start[b] += ahead[b];
   }
   __syncthreads();
   const uint32_t mask = (1u << dg.bits) - 1u;
-  const uint32_t base = blockIdx.x * kIdTile + w * (kIdItems * kWave) + lane;
 #pragma unroll
   for (int r = 0; r < kIdItems; ++r) {
-    const uint32_t i = base + r * kWave;
-    if (i < n) {
+    if (tile_item(r) < valid) {
       const uint32_t d = (key[r] >> dg.shift) & mask;
-      sink.put(start[d] + cnt[w * dg.bins + d] + loc[r], key[r], src.value(i));
+      sink.put(start[d] + cnt[(threadIdx.x / kWave) * dg.bins + d] + loc[r], key[r], value[r]);
+    }
+  }
+}
+
+// All passes over one tile: `dg` is the first digit, the others follow it.
+template <typename Source, typename Sink>
+__global__ __launch_bounds__(kIdThreads) void id_sort_tile_kernel(Source src, Sink sink, uint32_t n,
+                                                                  Digit dg, int passes,
+                                                                  ClearOnTheWay clear) {
+  __shared__ uint16_t cnt[kIdWaves * kIdMaxBins];
+  __shared__ uint32_t start[kIdMaxBins];
+  __shared__ uint32_t wave_sum[kIdWaves];
+  __shared__ uint32_t keys[kIdTile], values[kIdTile];
+  uint32_t key[kIdItems], value[kIdItems], loc[kIdItems];
+#pragma unroll
+  for (int r = 0; r < kIdItems; ++r) {
+    const bool in = tile_item(r) < n;
+    key[r] = in ? src.key(tile_item(r)) : 0u;
+    value[r] = in ? src.value(tile_item(r)) : 0u;
+  }
+  clear_share(clear);  // before the last pass, whose puts may mark the cleared bytes
+  const uint32_t mask = (1u << dg.bits) - 1u;
+  for (int k = 0; k < passes; ++k, dg.shift += dg.bits) {
+    rank_tile(key, n, dg, cnt, loc);
+    __syncthreads();
+    for (int b = threadIdx.x; b < dg.bins; b += kIdThreads)
+      start[b] = wave_offsets(cnt, dg.bins, b);
+    scan_bins(start, dg.bins, wave_sum);
+    if (Sink::kStarts && k == passes - 1)
+      for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) sink.bin_start(uint32_t(b), start[b]);
+#pragma unroll
+    for (int r = 0; r < kIdItems; ++r) {
+      if (tile_item(r) < n) {
+        const uint32_t d = (key[r] >> dg.shift) & mask;
+        const uint32_t pos = start[d] + cnt[(threadIdx.x / kWave) * dg.bins + d] + loc[r];
+        if (k == passes - 1) {
+          sink.put(pos, key[r], value[r]);
+        } else {
+          keys[pos] = key[r];
+          values[pos] = value[r];
+        }
+      }
+    }
+    if (k < passes - 1) {
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < kIdItems; ++r) {
+        key[r] = tile_item(r) < n ? keys[tile_item(r)] : 0u;
+        value[r] = tile_item(r) < n ? values[tile_item(r)] : 0u;
+      }
     }
   }
 }
@@ -189,26 +283,37 @@ inline size_t id_sort_table_bytes(long long n, int bins) {
   return ((table * 4 + 255) & ~size_t(255)) + ps_scan_workspace_bytes(table);
 }
 
-// One pass: n elements of src by digit dg into sink; table holds
-// id_sort_table_bytes(n, dg.bins) bytes. `clear` is done by the first launch.
+// One pass over several tiles: n elements of src by digit dg into sink; table
+// holds id_sort_table_bytes(n, dg.bins) bytes. `clear` is done by the first
+// launch.
 template <typename Source, typename Sink>
 int id_sort_pass(const Source& src, const Sink& sink, uint32_t n, const Digit& dg, void* table,
                  const ClearOnTheWay& clear, hipStream_t stream) {
-  const uint32_t tiles = n ? (n + kIdTile - 1) / kIdTile : 1;
-  if (tiles == 1) {
-    id_place_kernel<<<1, kIdThreads, 0, stream>>>(src, sink, n, dg, nullptr, clear);
-    PS_LAUNCHED();
-    return PS_OK;
-  }
+  const uint32_t tiles = (n + kIdTile - 1) / kIdTile;
   uint32_t* counts = static_cast<uint32_t*>(table);
   const size_t entries = size_t(tiles) * size_t(dg.bins);
-  id_count_kernel<<<tiles, kIdThreads, 0, stream>>>(src, n, dg, counts, clear);
+  const bool self = tiles <= kSelfTiles;
+  const TableAt at = self ? TableAt{size_t(dg.bins), 1} : TableAt{1, tiles};
+  id_count_kernel<<<tiles, kIdThreads, 0, stream>>>(src, n, dg, counts, at, clear);
   PS_LAUNCHED();
-  const int rc = ps_exclusive_scan_u32(counts, counts, entries,
-                                       static_cast<char*>(table) + ((entries * 4 + 255) & ~size_t(255)),
-                                       reinterpret_cast<ps_stream_t>(stream));
-  if (rc != PS_OK) return rc;
-  id_place_kernel<<<tiles, kIdThreads, 0, stream>>>(src, sink, n, dg, counts, ClearOnTheWay{});
+  if (self) {
+    id_place_kernel<true><<<tiles, kIdThreads, 0, stream>>>(src, sink, n, dg, counts, at);
+  } else {
+    const int rc = ps_exclusive_scan_u32(
+        counts, counts, entries, static_cast<char*>(table) + ((entries * 4 + 255) & ~size_t(255)),
+        reinterpret_cast<ps_stream_t>(stream));
+    if (rc != PS_OK) return rc;
+    id_place_kernel<false><<<tiles, kIdThreads, 0, stream>>>(src, sink, n, dg, counts, at);
+  }
+  PS_LAUNCHED();
+  return PS_OK;
+}
+
+// The whole sort when n fits one tile.
+template <typename Source, typename Sink>
+int id_sort_tile(const Source& src, const Sink& sink, uint32_t n, const Digit& first, int passes,
+                 const ClearOnTheWay& clear, hipStream_t stream) {
+  id_sort_tile_kernel<<<1, kIdThreads, 0, stream>>>(src, sink, n, first, passes, clear);
   PS_LAUNCHED();
   return PS_OK;
 }
