@@ -47,6 +47,9 @@ __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(Mat<const T> x,
   }
 }
 
+// Rows of a token's slots under way at once.
+constexpr int kSlotsAhead = 4;
+
 template <typename T, int N>
 __global__ __launch_bounds__(kRowThreads) void combine_kernel(Mat<const T> ys,
                                                               const int* __restrict__ position,
@@ -58,12 +61,21 @@ __global__ __launch_bounds__(kRowThreads) void combine_kernel(Mat<const T> ys,
   const Item it = ItemBase(first, p).at(threadIdx.x, p);
   const int c = p.begin(it.piece);
   const long long s = it.row * top_k;
+  using V = typename PieceOf<T, N>::type;
   Floats<N> acc = 0.f;
-  for (int k = 0; k < top_k; ++k) {
-    const int q = position[s + k];
-    if (q < 0 || q >= ys.rows) continue;
-    const float w = weights ? weights[s + k] : 1.f;
-    acc += w * load_piece<N>(ys.at(q, c));
+  for (int k0 = 0; k0 < top_k; k0 += kSlotsAhead) {
+    float w[kSlotsAhead];
+    V v[kSlotsAhead];
+#pragma unroll
+    for (int j = 0; j < kSlotsAhead; ++j) {
+      const int k = min(k0 + j, top_k - 1);
+      const int q = position[s + k];
+      const bool on = k0 + j < top_k && q >= 0 && q < ys.rows;
+      w[j] = on && weights ? weights[s + k] : 1.f;
+      v[j] = on ? *reinterpret_cast<const V*>(ys.at(q, c)) : V(T(0.f));
+    }
+#pragma unroll
+    for (int j = 0; j < kSlotsAhead; ++j) acc += w[j] * __builtin_convertvector(v[j], Floats<N>);
   }
   store_piece<N>(y.at(it.row, c), acc);
 }
