@@ -23,7 +23,7 @@
 namespace ps {
 namespace {
 
-template <typename T, typename O, typename I, int N>
+template <typename T, typename O, typename I, int N, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void lookup_kernel(Mat<const T> table,
                                                              const I* __restrict__ ids,
                                                              float scale, Mat<O> out, Pieces p,
@@ -35,7 +35,7 @@ __global__ __launch_bounds__(kRowThreads) void lookup_kernel(Mat<const T> table,
   const long long id = ids[it.row];
   Floats<N> v = 0.f;
   if (id >= 0 && id < table.rows) v = scale * load_piece<N>(table.at(id, c));
-  store_piece<N>(out.at(it.row, c), v);
+  store_piece<N, kStream>(out.at(it.row, c), v);
 }
 
 // Entries per chunk: the fewest, from 16 to 256, that leave at most kRunThreads
@@ -367,15 +367,18 @@ int ps_embedding_lookup(const ps_rows* table, const ps_ids* ids, float scale, co
           out->cols, [&](auto n) {
             const ps::Pieces p(out->cols, n);
             const unsigned long long items = (unsigned long long)out->rows * p.per_row.d;
-            return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
-              if (ids->type == PS_I64)
-                ps::lookup_kernel<T, O, long long, n><<<blocks, ps::kRowThreads, 0, st>>>(
-                    ps::mat<const T>(table), static_cast<const long long*>(ids->data), scale,
-                    ps::mat<O>(out), p, part);
-              else
-                ps::lookup_kernel<T, O, int, n><<<blocks, ps::kRowThreads, 0, st>>>(
-                    ps::mat<const T>(table), static_cast<const int*>(ids->data), scale,
-                    ps::mat<O>(out), p, part);
+            return ps::with_flag(ps::streamed(out), [&](auto stream_out) {
+              return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
+                if (ids->type == PS_I64)
+                  ps::lookup_kernel<T, O, long long, n, stream_out>
+                      <<<blocks, ps::kRowThreads, 0, st>>>(
+                          ps::mat<const T>(table), static_cast<const long long*>(ids->data), scale,
+                          ps::mat<O>(out), p, part);
+                else
+                  ps::lookup_kernel<T, O, int, n, stream_out><<<blocks, ps::kRowThreads, 0, st>>>(
+                      ps::mat<const T>(table), static_cast<const int*>(ids->data), scale,
+                      ps::mat<O>(out), p, part);
+              });
             });
           });
     });

@@ -29,7 +29,7 @@ struct ExpertSink {
   }
 };
 
-template <typename T, int N>
+template <typename T, int N, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(Mat<const T> x,
                                                                const int* __restrict__ position,
                                                                int top_k, Mat<T> xs, Pieces p,
@@ -43,14 +43,19 @@ __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(Mat<const T> x,
   const int* pos = position + it.row * top_k;
   for (int k = 0; k < top_k; ++k) {
     const int q = pos[k];
-    if (q >= 0 && q < xs.rows) *reinterpret_cast<V*>(xs.at(q, c)) = v;
+    if (q < 0 || q >= xs.rows) continue;
+    V* const to = reinterpret_cast<V*>(xs.at(q, c));
+    if constexpr (kStream)
+      __builtin_nontemporal_store(v, to);
+    else
+      *to = v;
   }
 }
 
 // Rows of a token's slots under way at once.
 constexpr int kSlotsAhead = 4;
 
-template <typename T, int N>
+template <typename T, int N, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void combine_kernel(Mat<const T> ys,
                                                               const int* __restrict__ position,
                                                               const float* __restrict__ weights,
@@ -77,46 +82,92 @@ __global__ __launch_bounds__(kRowThreads) void combine_kernel(Mat<const T> ys,
 #pragma unroll
     for (int j = 0; j < kSlotsAhead; ++j) acc += w[j] * __builtin_convertvector(v[j], Floats<N>);
   }
-  store_piece<N>(y.at(it.row, c), acc);
+  store_piece<N, kStream>(y.at(it.row, c), acc);
 }
 
-// One workgroup per token.
-template <typename T, int N>
+// kLanes threads a token: the pieces of its row among them, and one dot a slot
+// summed over them.
+template <typename T, int N, int kLanes, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void combine_grad_kernel(
     Mat<const T> dy, Mat<const T> ys, const int* __restrict__ position,
     const float* __restrict__ weights, int top_k, Mat<T> dys, float* __restrict__ dweights,
     Pieces p, Items tokens) {
-  __shared__ float part[kRowThreads / kWave];
-  const long long t = (long long)tokens.of_block(1).first;
-  for (int k = 0; k < top_k; ++k) {
-    const long long s = t * top_k + k;
-    const int q = position[s];
-    const bool valid = q >= 0 && q < ys.rows;
-    float dot = 0.f;
-    if (valid) {
-      const float w = weights[s];
-      for (int i = threadIdx.x; i < int(p.per_row.d); i += kRowThreads) {
-        const int c = p.begin(i);
-        const int seen = i * N - c;  // elements that the piece before has added
-        const Floats<N> g = load_piece<N>(dy.at(t, c));
-        const Floats<N> v = load_piece<N>(ys.at(q, c));
+  constexpr int kTokens = kRowThreads / kLanes;
+  __shared__ float part[kLanes > kWave ? kSlotsAhead : 1][kRowThreads / kWave];
+  const auto [first, count] = tokens.of_block(kTokens);
+  const uint32_t mine = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  // threads without a token go along: the sums below take every lane
+  const bool on = mine < count;
+  const long long t = (long long)first + (on ? mine : 0);
+  const int pieces = int(p.per_row.d);
+  using V = typename PieceOf<T, N>::type;
+  for (int k0 = 0; k0 < top_k; k0 += kSlotsAhead) {
+    int q[kSlotsAhead];
+    float w[kSlotsAhead], dot[kSlotsAhead];
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (e >= seen) dot += g[e] * v[e];
-        store_piece<N>(dys.at(q, c), w * g);
+    for (int j = 0; j < kSlotsAhead; ++j) {
+      const long long s = t * top_k + min(k0 + j, top_k - 1);
+      q[j] = position[s];
+      w[j] = weights[s];
+      if (!on || k0 + j >= top_k || q[j] < 0 || q[j] >= ys.rows) q[j] = -1;
+      dot[j] = 0.f;
+    }
+    for (int i = lane; i < pieces; i += kLanes) {
+      const int c = p.begin(i);
+      const int seen = i * N - c;  // elements that the piece before has added
+      const Floats<N> g = load_piece<N>(dy.at(t, c));
+      V v[kSlotsAhead];
+#pragma unroll
+      for (int j = 0; j < kSlotsAhead; ++j)
+        v[j] = q[j] >= 0 ? *reinterpret_cast<const V*>(ys.at(q[j], c)) : V(T(0.f));
+#pragma unroll
+      for (int j = 0; j < kSlotsAhead; ++j) {
+        if (q[j] < 0) continue;
+        const Floats<N> f = __builtin_convertvector(v[j], Floats<N>);
+#pragma unroll
+        for (int e = 0; e < N; ++e) dot[j] += e >= seen ? g[e] * f[e] : 0.f;
+        store_piece<N, kStream>(dys.at(q[j], c), w[j] * g);
       }
     }
 #pragma unroll
-    for (int d = kWave / 2; d; d >>= 1) dot += __shfl_xor(dot, d, kWave);
-    __syncthreads();
-    if (lane_id() == 0) part[threadIdx.x / kWave] = dot;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      float sum = 0.f;
-      for (int w = 0; w < kRowThreads / kWave; ++w) sum += part[w];
-      dweights[s] = sum;
+    for (int j = 0; j < kSlotsAhead; ++j)
+#pragma unroll
+      for (int d = (kLanes < kWave ? kLanes : kWave) / 2; d; d >>= 1)
+        dot[j] += __shfl_xor(dot[j], d, kWave);
+    if constexpr (kLanes > kWave) {
+      __syncthreads();
+      if (lane_id() == 0)
+#pragma unroll
+        for (int j = 0; j < kSlotsAhead; ++j) part[j][threadIdx.x / kWave] = dot[j];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kSlotsAhead; ++j) {
+        dot[j] = 0.f;
+#pragma unroll
+        for (int u = 0; u < kRowThreads / kWave; ++u) dot[j] += part[j][u];
+      }
     }
+    if (on && lane == 0)
+#pragma unroll
+      for (int j = 0; j < kSlotsAhead; ++j)
+        if (k0 + j < top_k) dweights[t * top_k + k0 + j] = dot[j];
   }
+}
+
+// Calls f(lanes) with the threads a token's row gets: its pieces, one each up
+// to 64, or a workgroup from 256 pieces on. Gradients of the combination, us:
+// 16,384 x 4 x 2,048 BF16 134 with 64 lanes, 119 with 256; 256 x 8 x 4,096 18.3
+// and 10.1; but 32,768 x 4 x 1,024 123 and 150, 65,536 x 4 x 333 FP16 74 and
+// 187. Fewer lanes than pieces cost as well (333: 89 with 32), and so do idle
+// ones (65,536 x 4 x 64 BF16: 14.3 with 8, 17.5 with 16, 54 with 64).
+template <typename F>
+int with_lanes(const Pieces& p, F&& f) {
+  const uint32_t pieces = p.per_row.d;
+  if (pieces >= 256) return f(std::integral_constant<int, 256>{});
+  if (pieces > 32) return f(std::integral_constant<int, 64>{});
+  if (pieces > 16) return f(std::integral_constant<int, 32>{});
+  if (pieces > 8) return f(std::integral_constant<int, 16>{});
+  return f(std::integral_constant<int, 8>{});
 }
 
 }  // namespace
@@ -166,9 +217,12 @@ int ps_expert_dispatch(const ps_rows* x, const int* position, int top_k, const p
     return ps::with_width<sizeof(T)>(x->cols, [&](auto n) {
       const ps::Pieces p(x->cols, n);
       const unsigned long long items = (unsigned long long)x->rows * p.per_row.d;
-      return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
-        ps::dispatch_kernel<T, n><<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
-            ps::mat<const T>(x), position, top_k, ps::mat<T>(xs), p, part);
+      return ps::with_flag(ps::streamed(xs), [&](auto stream_out) {
+        return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
+          ps::dispatch_kernel<T, n, stream_out>
+              <<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
+                  ps::mat<const T>(x), position, top_k, ps::mat<T>(xs), p, part);
+        });
       });
     });
   });
@@ -189,9 +243,12 @@ int ps_expert_combine(const ps_rows* ys, const int* position, const float* weigh
     return ps::with_width<sizeof(T)>(y->cols, [&](auto n) {
       const ps::Pieces p(y->cols, n);
       const unsigned long long items = (unsigned long long)y->rows * p.per_row.d;
-      return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
-        ps::combine_kernel<T, n><<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
-            ps::mat<const T>(ys), position, weights, top_k, ps::mat<T>(y), p, part);
+      return ps::with_flag(ps::streamed(y), [&](auto stream_out) {
+        return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
+          ps::combine_kernel<T, n, stream_out>
+              <<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
+                  ps::mat<const T>(ys), position, weights, top_k, ps::mat<T>(y), p, part);
+        });
       });
     });
   });
@@ -216,10 +273,16 @@ int ps_expert_combine_grad(const ps_rows* dy, const ps_rows* ys, const int* posi
     using T = decltype(t);
     return ps::with_width<sizeof(T)>(dy->cols, [&](auto n) {
       const ps::Pieces p(dy->cols, n);
-      return ps::launch_items(dy->rows, 1, [&](uint32_t blocks, ps::Items part) {
-        ps::combine_grad_kernel<T, n><<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
-            ps::mat<const T>(dy), ps::mat<const T>(ys), position, weights, top_k,
-            ps::mat<T>(dys), dweights, p, part);
+      return ps::with_lanes(p, [&](auto lanes) {
+        return ps::with_flag(ps::streamed(dys), [&](auto stream_out) {
+          return ps::launch_items(
+              dy->rows, ps::kRowThreads / lanes, [&](uint32_t blocks, ps::Items part) {
+                ps::combine_grad_kernel<T, n, lanes, stream_out>
+                    <<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
+                        ps::mat<const T>(dy), ps::mat<const T>(ys), position, weights, top_k,
+                        ps::mat<T>(dys), dweights, p, part);
+              });
+        });
       });
     });
   });
