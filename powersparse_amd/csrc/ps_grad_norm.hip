@@ -24,19 +24,23 @@ struct GradTensor {
   int dtype, out_dtype;
 };
 struct GradChunk {
-  uint32_t tensor, index;  // elements [index * chunk, ...) of the tensor
+  uint32_t tensor, index;  // elements [index * kChunk, ...) of the tensor
 };
 
 namespace {
 
 constexpr int kClipThreads = 256;
 constexpr uint32_t kBlocks = 2048;
-constexpr int kStep = 2048;  // chunks are multiples of this many elements
+// Elements of a chunk. The workgroups go through the chunks side by side, so
+// small chunks keep what they touch at one time together: clipping 800 M BF16
+// elements into FP32 took 951 us with 4096, 984 with 8192, 1089 with 32,768,
+// 992 with 2048.
+constexpr long long kChunk = 4096;
 
 struct Grads {
   const GradTensor* tensors;
   const GradChunk* chunks;
-  uint32_t chunk_count, chunk;
+  uint32_t chunk_count;
   bool in_place;
 };
 
@@ -72,8 +76,8 @@ __global__ __launch_bounds__(kClipThreads) void norm_kernel(Grads g, double* __r
   for (uint32_t q = blockIdx.x; q < g.chunk_count; q += gridDim.x) {
     const GradChunk ch = g.chunks[q];
     const GradTensor t = g.tensors[ch.tensor];
-    const long long from = (long long)ch.index * g.chunk;
-    const uint32_t count = uint32_t(min((long long)g.chunk, t.count - from));
+    const long long from = (long long)ch.index * kChunk;
+    const uint32_t count = uint32_t(min(kChunk, t.count - from));
     if (t.dtype == PS_F32)
       s += square_sum(static_cast<const f32*>(t.data) + from, count);
     else if (t.dtype == PS_F16)
@@ -101,9 +105,11 @@ __global__ __launch_bounds__(kClipThreads) void norm_join_kernel(const double* _
 
 template <typename T, typename O>
 __device__ void scale_chunk(const T* p, O* out, uint32_t count, float c) {
-  constexpr int N = 16 / (sizeof(T) < sizeof(O) ? sizeof(T) : sizeof(O));
+  constexpr int N = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
   uint32_t i = threadIdx.x * N;
-  for (; i + N <= count; i += kClipThreads * N) store_piece<N>(out + i, c * load_piece<N>(p + i));
+#pragma unroll 4
+  for (; i + N <= count; i += kClipThreads * N)
+    store_piece<N>(out + i, c * load_piece<N>(p + i));
   for (; i < count; ++i) out[i] = O(c * float(p[i]));
 }
 
@@ -137,8 +143,8 @@ __global__ __launch_bounds__(kClipThreads) void clip_kernel(Grads g,
   for (uint32_t q = blockIdx.x; q < g.chunk_count; q += gridDim.x) {
     const GradChunk ch = g.chunks[g.chunk_count - 1 - q];
     const GradTensor t = g.tensors[ch.tensor];
-    const long long from = (long long)ch.index * g.chunk;
-    const uint32_t count = uint32_t(min((long long)g.chunk, t.count - from));
+    const long long from = (long long)ch.index * kChunk;
+    const uint32_t count = uint32_t(min(kChunk, t.count - from));
     if (t.dtype == PS_F32)
       scale_to<f32>(t, from, count, c);
     else if (t.dtype == PS_F16)
@@ -164,6 +170,14 @@ namespace {
 int launch_norm(const ps_grad_list& l, hipStream_t stream) {
   if (!l.blocks) return PS_OK;
   norm_kernel<<<l.blocks, kClipThreads, 0, stream>>>(l.grads, l.sums);
+  PS_LAUNCHED();
+  return PS_OK;
+}
+
+int launch_clip(const ps_grad_list& l, uint32_t blocks, const double* sums, float max_norm,
+                float grad_scale, float* norm, hipStream_t stream) {
+  clip_kernel<<<blocks, kClipThreads, 0, stream>>>(l.grads, sums, l.blocks, double(max_norm),
+                                                   double(grad_scale), norm);
   PS_LAUNCHED();
   return PS_OK;
 }
@@ -205,14 +219,11 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
       table.push_back({data[i], to, counts[i], dtypes[i], out_dtype});
       total += counts[i];
     }
-    // about four chunks a workgroup, so that none has much more than another
-    long long chunk = total / (4LL * ps::kBlocks) / ps::kStep * ps::kStep;
-    chunk = std::min<long long>(std::max<long long>(chunk, ps::kStep), 32 * ps::kStep);
     std::vector<ps::GradChunk> chunks;
     bool in_place = true;
     for (size_t i = 0; i < table.size(); ++i) {
       in_place = in_place && table[i].out == table[i].data;
-      const long long n = (table[i].count + chunk - 1) / chunk;
+      const long long n = (table[i].count + ps::kChunk - 1) / ps::kChunk;
       PS_CHECK_ARG(n + (long long)chunks.size() < (1LL << 31), "ps_grad_list_create: too large");
       for (long long q = 0; q < n; ++q) chunks.push_back({uint32_t(i), uint32_t(q)});
     }
@@ -235,7 +246,6 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
     l->grads.tensors = reinterpret_cast<const ps::GradTensor*>(at);
     l->grads.chunks = reinterpret_cast<const ps::GradChunk*>(at + table_bytes);
     l->grads.chunk_count = uint32_t(chunks.size());
-    l->grads.chunk = uint32_t(chunk);
     l->grads.in_place = in_place;
     l->sums = reinterpret_cast<double*>(at + table_bytes + chunk_bytes);
     l->blocks = std::min(uint32_t(chunks.size()), ps::kBlocks);
@@ -268,10 +278,8 @@ int ps_clip_grads(ps_grad_list* list, float max_norm, float grad_scale, const fl
   PS_CHECK_ARG(list && norm, "ps_clip_grads: null argument");
   PS_CHECK_ARG(max_norm >= 0.f, "ps_clip_grads: the bound is not a number from 0 up");
   if (!list->blocks) return PS_OK;
-  ps::clip_kernel<<<list->blocks, ps::kClipThreads, 0, ps::to_hip(stream)>>>(
-      list->grads, nullptr, 0, double(max_norm), double(grad_scale), const_cast<float*>(norm));
-  PS_LAUNCHED();
-  return PS_OK;
+  return ps::launch_clip(*list, list->blocks, nullptr, max_norm, grad_scale,
+                         const_cast<float*>(norm), ps::to_hip(stream));
 }
 
 int ps_clip_grad_norm(ps_grad_list* list, float max_norm, float grad_scale, float* norm,
@@ -281,10 +289,8 @@ int ps_clip_grad_norm(ps_grad_list* list, float max_norm, float grad_scale, floa
   const hipStream_t st = ps::to_hip(stream);
   const int rc = ps::launch_norm(*list, st);
   if (rc != PS_OK) return rc;
-  ps::clip_kernel<<<std::max(list->blocks, 1u), ps::kClipThreads, 0, st>>>(
-      list->grads, list->sums, list->blocks, double(max_norm), double(grad_scale), norm);
-  PS_LAUNCHED();
-  return PS_OK;
+  return ps::launch_clip(*list, std::max(list->blocks, 1u), list->sums, max_norm, grad_scale,
+                         norm, st);
 }
 
 }  // extern "C"
