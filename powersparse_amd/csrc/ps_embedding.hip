@@ -38,12 +38,15 @@ __global__ __launch_bounds__(kRowThreads) void lookup_kernel(Mat<const T> table,
   store_piece<N, kStream>(out.at(it.row, c), v);
 }
 
-// Entries per chunk: the fewest, from 16 to 256, that leave at most kRunThreads
-// threads for the chunks (four waves a SIMD): longer chunks mean fewer partial
-// sums, shorter ones more loads in flight.
+// Entries per chunk. Few for short lists, where latency counts (1,021 ids of 96
+// columns: 14.9 us with 4, 19.0 with 16; 32,768 of 64: 38.9 with 8, 43.7 with 4,
+// 42.2 with 16); otherwise the fewest from 16 to 256 that leave at most
+// kRunThreads threads for the chunks, four waves a SIMD: longer chunks mean fewer
+// parts of long runs, shorter ones more loads in flight.
 constexpr unsigned long long kRunThreads = 1u << 18;
 uint32_t chunk_size(long long n, long long cols) {
-  uint32_t c = 16;
+  uint32_t c = 4;
+  while (c < 16 && n / c > 4096) c *= 2;
   while (c < 256 && (unsigned long long)(n / c) * ((unsigned long long)(cols + 7) / 8) > kRunThreads)
     c *= 2;
   return c;
@@ -62,6 +65,8 @@ struct FlagSink {
   __device__ __forceinline__ void bin_start(uint32_t, uint32_t) const {}
 };
 
+constexpr uint32_t kManyChunks = 64;
+
 // The sorted ids (keys; `rows` = takes no part) and where their rows of
 // grad_out are, n of them, and the partial sums: chunk q's first run's part in
 // row 2q, its last run's in row 2q + 1, ld floats apart.
@@ -70,7 +75,11 @@ struct Runs {
   uint32_t n, rows, chunk;  // chunk: entries of a chunk
   float* partial;
   long long ld;
-  uint32_t *long_count, *long_list;  // the chunks in which long runs start
+  // The chunks in which long runs start: those that reach up to kManyChunks
+  // chunks (count 0, listed from the front) and longer ones (count 1, from the
+  // back).
+  uint32_t *long_count, *long_list;
+  uint32_t chunks;
 };
 
 template <typename G, int N>
@@ -168,7 +177,13 @@ __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& gr
   }
   if (tail_long) {
     store_piece<N>(r.partial + (2ull * chunk + 1) * r.ld + c, sum);
-    if (piece == 0) r.long_list[atomicAdd(r.long_count, 1u)] = chunk;
+    if (piece == 0) {
+      const unsigned long long far = e + (unsigned long long)kManyChunks * size;
+      if (far < r.n && r.keys[far] == last)
+        r.long_list[r.chunks - 1 - atomicAdd(r.long_count + 1, 1u)] = chunk;
+      else
+        r.long_list[atomicAdd(r.long_count, 1u)] = chunk;
+    }
   } else {
     finish();
   }
@@ -211,54 +226,79 @@ __global__ __launch_bounds__(kRowThreads) void grad_runs_kernel(
           V(G(0.f)), reinterpret_cast<V*>(grad.at(it[u].row, p.begin(it[u].piece))));
 }
 
-// Adds the parts of the long runs: the last part of the chunk a run starts in,
-// then the first parts of the chunks it reaches. A workgroup takes one run and
-// kJoinPieces pieces of the width, its thread groups each a share of the parts
-// in order, and the shares are added by halves.
-constexpr int kJoinThreads = 1024;
-constexpr int kJoinPieces = 16;
-constexpr int kJoinGroups = kJoinThreads / kJoinPieces;
+// How many of the chunks from `from` on begin inside the run of key k: every
+// round asks at as many places as there are threads.
+__device__ __forceinline__ uint32_t chunks_in_run(const Runs& r, uint32_t from, uint32_t k) {
+  uint32_t lo = 0, hi = r.chunks - from;  // the answer's bounds
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + kRowThreads - 1) / kRowThreads;
+    const uint32_t at = lo + threadIdx.x * step;
+    const uint32_t hits = __syncthreads_count(
+        at < hi && r.keys[(unsigned long long)(from + at) * r.chunk] == k);
+    if (!hits) return lo;
+    hi = min(hi, lo + hits * step);
+    lo += (hits - 1) * step + 1;
+  }
+  return lo;
+}
 
-template <typename G, int N>
-__global__ __launch_bounds__(kJoinThreads) void grad_join_kernel(Runs r, Mat<G> grad, float scale,
-                                                                 bool accumulate, Pieces p) {
-  __shared__ float part[kJoinGroups / 2][kJoinPieces * N];
-  const uint32_t tiles = (p.per_row.d + kJoinPieces - 1) / kJoinPieces;
-  const unsigned long long work = (unsigned long long)*r.long_count * tiles;
-  const int group = threadIdx.x / kJoinPieces, lane = threadIdx.x % kJoinPieces;
-  for (unsigned long long l = blockIdx.x; l < work; l += gridDim.x) {
-    const uint32_t chunk = r.long_list[l / tiles];
-    const int piece = int(l % tiles) * kJoinPieces + lane;
-    const uint32_t k = r.keys[(chunk + 1) * r.chunk - 1];
-    uint32_t reached = 0;  // chunks after this one that begin inside the run
-    for (int found = kJoinThreads; found == kJoinThreads; reached += found) {
-      const unsigned long long q = (unsigned long long)(chunk + 1 + reached + threadIdx.x) * r.chunk;
-      found = __syncthreads_count(q < r.n && r.keys[q] == k);
-    }
-    const uint32_t share = (reached + kJoinGroups - 1) / kJoinGroups;
-    const uint32_t from = min(group * share, reached), to = min(from + share, reached);
-    const bool on = piece < int(p.per_row.d);
-    const int c = on ? p.begin(piece) : 0;
-    Floats<N> sum = 0.f;
-    if (on) {
-      if (group == 0) sum = load_piece<N>(r.partial + (2ull * chunk + 1) * r.ld + c);
-      const float* at = r.partial + 2ull * (chunk + 1) * r.ld + c;
+// Adds the parts of the long run that starts in `chunk` for kJoinPieces pieces
+// of the width: its last part, then the first parts of the chunks it reaches.
+// The workgroup's thread groups take shares of the parts in order, and the
+// shares are added by halves.
+template <int kJoinPieces, typename G, int N>
+__device__ void join_run(const Runs& r, const Mat<G>& grad, float scale, bool accumulate,
+                         uint32_t chunk, uint32_t tile, const Pieces& p, float* part) {
+  constexpr uint32_t kGroups = kRowThreads / kJoinPieces;
+  const uint32_t group = threadIdx.x / kJoinPieces, lane = threadIdx.x % kJoinPieces;
+  const uint32_t piece = tile * kJoinPieces + lane;
+  const uint32_t k = r.keys[(chunk + 1) * r.chunk - 1];
+  const uint32_t reached = chunks_in_run(r, chunk + 1, k);
+  const uint32_t share = (reached + kGroups - 1) / kGroups;
+  const uint32_t from = min(group * share, reached), to = min(from + share, reached);
+  const bool on = piece < p.per_row.d;
+  const int c = on ? p.begin(int(piece)) : 0;
+  Floats<N> sum = 0.f;
+  if (on) {
+    if (group == 0) sum = load_piece<N>(r.partial + (2ull * chunk + 1) * r.ld + c);
+    const float* at = r.partial + 2ull * (chunk + 1) * r.ld + c;
 #pragma unroll 8
-      for (uint32_t q = from; q < to; ++q) sum += load_piece<N>(at + 2ull * q * r.ld);
-    }
-    int half = kJoinGroups / 2;
-    while (half && half * share >= reached) half /= 2;  // groups without a share
-    for (; half; half /= 2) {
-      if (group >= half && group < 2 * half)
+    for (uint32_t q = from; q < to; ++q) sum += load_piece<N>(at + 2ull * q * r.ld);
+  }
+  uint32_t half = kGroups / 2;
+  while (half && half * share >= reached) half /= 2;  // groups without a share
+  for (; half; half /= 2) {
+    if (group >= half && group < 2 * half)
 #pragma unroll
-        for (int e = 0; e < N; ++e) part[group - half][lane * N + e] = sum[e];
-      __syncthreads();
-      if (group < half)
+      for (int e = 0; e < N; ++e) part[((group - half) * kJoinPieces + lane) * N + e] = sum[e];
+    __syncthreads();
+    if (group < half)
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum[e] += part[group][lane * N + e];
-      __syncthreads();
-    }
-    if (group == 0 && on) write_grad<G, N>(grad, k, c, piece * N - c, sum, scale, accumulate);
+      for (int e = 0; e < N; ++e) sum[e] += part[(group * kJoinPieces + lane) * N + e];
+    __syncthreads();
+  }
+  if (group == 0 && on) write_grad<G, N>(grad, k, c, int(piece) * N - c, sum, scale, accumulate);
+}
+
+// Workgroups of 16 groups for runs of some parts, of 64 for those of many: 2,048
+// parts of 336 columns take 12 us so, 22 with 16 groups.
+constexpr int kFewPieces = 16, kManyPieces = 4;
+template <typename G, int N>
+__global__ __launch_bounds__(kRowThreads) void grad_join_kernel(Runs r, Mat<G> grad, float scale,
+                                                                bool accumulate, Pieces p) {
+  __shared__ float part[kRowThreads / 2 * N];
+  const uint32_t few_tiles = (p.per_row.d + kFewPieces - 1) / kFewPieces;
+  const uint32_t many_tiles = (p.per_row.d + kManyPieces - 1) / kManyPieces;
+  const unsigned long long few = (unsigned long long)r.long_count[0] * few_tiles;
+  const unsigned long long many = (unsigned long long)r.long_count[1] * many_tiles;
+  for (unsigned long long l = blockIdx.x; l < many + few; l += gridDim.x) {
+    if (l < many)
+      join_run<kManyPieces, G, N>(r, grad, scale, accumulate,
+                                  r.long_list[r.chunks - 1 - l / many_tiles],
+                                  uint32_t(l % many_tiles), p, part);
+    else
+      join_run<kFewPieces, G, N>(r, grad, scale, accumulate, r.long_list[(l - many) / few_tiles],
+                                 uint32_t((l - many) % few_tiles), p, part);
   }
 }
 
@@ -428,7 +468,7 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
   r.long_count = reinterpret_cast<uint32_t*>(ws + s.cleared);
   r.long_list = reinterpret_cast<uint32_t*>(ws + s.long_list);
   r.chunk = ps::chunk_size(ids->count, grad->cols);
-  const uint32_t chunks = (n + r.chunk - 1) / r.chunk;
+  r.chunks = (n + r.chunk - 1) / r.chunk;
   return ps::with_dtype(grad_out->dtype, [&](auto t) {
     return ps::with_dtype(grad->dtype, [&](auto g) {
       using T = decltype(t);
@@ -436,7 +476,7 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
       return ps::with_width<(sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G))>(
           grad->cols, [&](auto w) {
             const ps::Pieces p(grad->cols, w);
-            const unsigned long long items = (unsigned long long)chunks * p.per_row.d;
+            const unsigned long long items = (unsigned long long)r.chunks * p.per_row.d;
             const unsigned long long run_blocks =
                 (items + ps::kRowThreads - 1) / ps::kRowThreads;
             // The first launch takes the runs and as many rows to clear as
@@ -462,10 +502,10 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
             } while (done < clears);
             // a long run holds more than a chunk
             if (n > r.chunk + 1) {
-              const uint32_t tiles = (p.per_row.d + ps::kJoinPieces - 1) / ps::kJoinPieces;
-              const unsigned long long most = (unsigned long long)chunks * tiles;
+              const uint32_t tiles = (p.per_row.d + ps::kManyPieces - 1) / ps::kManyPieces;
+              const unsigned long long most = (unsigned long long)r.chunks * tiles;
               ps::grad_join_kernel<G, w>
-                  <<<uint32_t(std::min(most, 512ull)), ps::kJoinThreads, 0, st>>>(
+                  <<<uint32_t(std::min(most, 2048ull)), ps::kRowThreads, 0, st>>>(
                       r, ps::mat<G>(grad), scale, accumulate != 0, p);
               PS_LAUNCHED();
             }

@@ -19,7 +19,7 @@
 namespace ps {
 
 constexpr int kIdThreads = 1024;
-constexpr int kIdItems = 4;  // per thread
+constexpr int kIdItems = 4;  // per thread, at most
 constexpr uint32_t kIdTile = kIdThreads * kIdItems;
 constexpr int kIdMaxBins = 1025;  // 1024 digits, or 1024 experts and the dropped slots
 
@@ -66,16 +66,16 @@ struct Digit {
 constexpr uint32_t kSelfTiles = 128;
 constexpr int kIdWaves = kIdThreads / kWave;
 
-// Index in the tile of item r of this thread.
-__device__ __forceinline__ uint32_t tile_item(int r) {
-  return (threadIdx.x / kWave) * (kIdItems * kWave) + r * kWave + lane_id();
+// Index in the tile of item r of this thread, of `items` items a thread.
+__device__ __forceinline__ uint32_t tile_item(int r, int items) {
+  return (threadIdx.x / kWave) * (items * kWave) + r * kWave + lane_id();
 }
 
 // The waves' digit counts in cnt (bins per wave) and the items' ranks among
-// their wave's; `valid` items from the tile's start. Other waves may read cnt
+// their wave's; `valid` elements from the tile's start. Other waves may read cnt
 // after a barrier.
 __device__ __forceinline__ void rank_tile(const uint32_t (&key)[kIdItems], uint32_t valid,
-                                          const Digit& dg, uint16_t* cnt,
+                                          int items, const Digit& dg, uint16_t* cnt,
                                           uint32_t (&loc)[kIdItems]) {
   const int lane = lane_id();
   const uint32_t mask = (1u << dg.bits) - 1u;
@@ -85,7 +85,8 @@ __device__ __forceinline__ void rank_tile(const uint32_t (&key)[kIdItems], uint3
   wave_lds_sync();
 #pragma unroll
   for (int r = 0; r < kIdItems; ++r) {
-    const bool in = tile_item(r) < valid;
+    if (r >= items) break;
+    const bool in = tile_item(r, items) < valid;
     const uint32_t d = (key[r] >> dg.shift) & mask;
     uint64_t peers = __ballot(in);
     for (int b = 0; b < dg.bits; ++b) {
@@ -149,17 +150,17 @@ struct TableAt {
 
 // Counts of every tile.
 template <typename Source>
-__global__ __launch_bounds__(kIdThreads) void id_count_kernel(Source src, uint32_t n, Digit dg,
+__global__ __launch_bounds__(kIdThreads) void id_count_kernel(Source src, uint32_t n, int items, Digit dg,
                                                               uint32_t* __restrict__ table,
                                                               TableAt at, ClearOnTheWay clear) {
   __shared__ uint16_t cnt[kIdWaves * kIdMaxBins];
-  const uint32_t base = blockIdx.x * kIdTile, valid = min(n - base, kIdTile);
+  const uint32_t tile = items * kIdThreads, base = blockIdx.x * tile, valid = min(n - base, tile);
   uint32_t key[kIdItems], loc[kIdItems];
 #pragma unroll
   for (int r = 0; r < kIdItems; ++r)
-    key[r] = tile_item(r) < valid ? src.key(base + tile_item(r)) : 0u;
+    key[r] = r < items && tile_item(r, items) < valid ? src.key(base + tile_item(r, items)) : 0u;
   clear_share(clear);
-  rank_tile(key, valid, dg, cnt, loc);
+  rank_tile(key, valid, items, dg, cnt, loc);
   __syncthreads();
   for (int b = threadIdx.x; b < dg.bins; b += kIdThreads)
     table[blockIdx.x * at.tile + b * at.bin] = wave_offsets(cnt, dg.bins, b);
@@ -168,19 +169,19 @@ __global__ __launch_bounds__(kIdThreads) void id_count_kernel(Source src, uint32
 // Places a tile's elements. table: the counts (kSelf), or their scan.
 template <bool kSelf, typename Source, typename Sink>
 __global__ __launch_bounds__(kIdThreads) void id_place_kernel(Source src, Sink sink, uint32_t n,
-                                                              Digit dg,
+                                                              int items, Digit dg,
                                                               const uint32_t* __restrict__ table,
                                                               TableAt at) {
   __shared__ uint16_t cnt[kIdWaves * kIdMaxBins];
   __shared__ uint32_t start[kIdMaxBins], ahead[kSelf ? kIdMaxBins : 1];
   __shared__ uint32_t wave_sum[kIdWaves];
-  const uint32_t base = blockIdx.x * kIdTile, valid = min(n - base, kIdTile);
+  const uint32_t tile = items * kIdThreads, base = blockIdx.x * tile, valid = min(n - base, tile);
   uint32_t key[kIdItems], value[kIdItems], loc[kIdItems];
 #pragma unroll
   for (int r = 0; r < kIdItems; ++r) {
-    const bool in = tile_item(r) < valid;
-    key[r] = in ? src.key(base + tile_item(r)) : 0u;
-    value[r] = in ? src.value(base + tile_item(r)) : 0u;
+    const bool in = r < items && tile_item(r, items) < valid;
+    key[r] = in ? src.key(base + tile_item(r, items)) : 0u;
+    value[r] = in ? src.value(base + tile_item(r, items)) : 0u;
   }
   if constexpr (kSelf) {
     // start: all tiles' counts, ahead: the earlier tiles'. The tiles are shared
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(kIdThreads) void id_place_kernel(Source src, Sink s
     for (int b = threadIdx.x; b < dg.bins; b += kIdThreads)
       start[b] = table[blockIdx.x * at.tile + b * at.bin];
   }
-  rank_tile(key, valid, dg, cnt, loc);
+  rank_tile(key, valid, items, dg, cnt, loc);
   __syncthreads();
   for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) {
     (void)wave_offsets(cnt, dg.bins, b);
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(kIdThreads) void id_place_kernel(Source src, Sink s
   const uint32_t mask = (1u << dg.bits) - 1u;
 #pragma unroll
   for (int r = 0; r < kIdItems; ++r) {
-    if (tile_item(r) < valid) {
+    if (r < items && tile_item(r, items) < valid) {
       const uint32_t d = (key[r] >> dg.shift) & mask;
       sink.put(start[d] + cnt[(threadIdx.x / kWave) * dg.bins + d] + loc[r], key[r], value[r]);
     }
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(kIdThreads) void id_place_kernel(Source src, Sink s
 // All passes over one tile: `dg` is the first digit, the others follow it.
 template <typename Source, typename Sink>
 __global__ __launch_bounds__(kIdThreads) void id_sort_tile_kernel(Source src, Sink sink, uint32_t n,
-                                                                  Digit dg, int passes,
+                                                                  int items, Digit dg, int passes,
                                                                   ClearOnTheWay clear) {
   __shared__ uint16_t cnt[kIdWaves * kIdMaxBins];
   __shared__ uint32_t start[kIdMaxBins];
@@ -237,14 +238,14 @@ __global__ __launch_bounds__(kIdThreads) void id_sort_tile_kernel(Source src, Si
   uint32_t key[kIdItems], value[kIdItems], loc[kIdItems];
 #pragma unroll
   for (int r = 0; r < kIdItems; ++r) {
-    const bool in = tile_item(r) < n;
-    key[r] = in ? src.key(tile_item(r)) : 0u;
-    value[r] = in ? src.value(tile_item(r)) : 0u;
+    const bool in = r < items && tile_item(r, items) < n;
+    key[r] = in ? src.key(tile_item(r, items)) : 0u;
+    value[r] = in ? src.value(tile_item(r, items)) : 0u;
   }
   clear_share(clear);  // before the last pass, whose puts may mark the cleared bytes
   const uint32_t mask = (1u << dg.bits) - 1u;
   for (int k = 0; k < passes; ++k, dg.shift += dg.bits) {
-    rank_tile(key, n, dg, cnt, loc);
+    rank_tile(key, n, items, dg, cnt, loc);
     __syncthreads();
     for (int b = threadIdx.x; b < dg.bins; b += kIdThreads)
       start[b] = wave_offsets(cnt, dg.bins, b);
@@ -253,7 +254,7 @@ __global__ __launch_bounds__(kIdThreads) void id_sort_tile_kernel(Source src, Si
       for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) sink.bin_start(uint32_t(b), start[b]);
 #pragma unroll
     for (int r = 0; r < kIdItems; ++r) {
-      if (tile_item(r) < n) {
+      if (r < items && tile_item(r, items) < n) {
         const uint32_t d = (key[r] >> dg.shift) & mask;
         const uint32_t pos = start[d] + cnt[(threadIdx.x / kWave) * dg.bins + d] + loc[r];
         if (k == passes - 1) {
@@ -268,18 +269,27 @@ __global__ __launch_bounds__(kIdThreads) void id_sort_tile_kernel(Source src, Si
       __syncthreads();
 #pragma unroll
       for (int r = 0; r < kIdItems; ++r) {
-        key[r] = tile_item(r) < n ? keys[tile_item(r)] : 0u;
-        value[r] = tile_item(r) < n ? values[tile_item(r)] : 0u;
+        const bool in = r < items && tile_item(r, items) < n;
+        key[r] = in ? keys[tile_item(r, items)] : 0u;
+        value[r] = in ? values[tile_item(r, items)] : 0u;
       }
     }
   }
 }
 
+// Items a thread takes: the fewest that leave at most kFewTiles tiles, as every
+// item is a step of the ranking and every tile a row of counts to add up.
+constexpr uint32_t kFewTiles = 64;
+inline int id_items(long long n) {
+  int items = 1;
+  while (items < kIdItems && n > (long long)kFewTiles * kIdThreads * items) items *= 2;
+  return items;
+}
+
 // Bytes of the count table and its scan for passes over n elements.
 inline size_t id_sort_table_bytes(long long n, int bins) {
-  const size_t tiles = size_t((n + kIdTile - 1) / kIdTile);
-  if (tiles <= 1) return 0;
-  const size_t table = tiles * size_t(bins);
+  const long long tile = (long long)id_items(n) * kIdThreads;
+  const size_t table = size_t((n + tile - 1) / tile) * size_t(bins);
   return ((table * 4 + 255) & ~size_t(255)) + ps_scan_workspace_bytes(table);
 }
 
@@ -289,31 +299,33 @@ inline size_t id_sort_table_bytes(long long n, int bins) {
 template <typename Source, typename Sink>
 int id_sort_pass(const Source& src, const Sink& sink, uint32_t n, const Digit& dg, void* table,
                  const ClearOnTheWay& clear, hipStream_t stream) {
-  const uint32_t tiles = (n + kIdTile - 1) / kIdTile;
+  const int items = id_items(n);
+  const uint32_t tiles = (n + items * kIdThreads - 1) / (items * kIdThreads);
   uint32_t* counts = static_cast<uint32_t*>(table);
   const size_t entries = size_t(tiles) * size_t(dg.bins);
   const bool self = tiles <= kSelfTiles;
   const TableAt at = self ? TableAt{size_t(dg.bins), 1} : TableAt{1, tiles};
-  id_count_kernel<<<tiles, kIdThreads, 0, stream>>>(src, n, dg, counts, at, clear);
+  id_count_kernel<<<tiles, kIdThreads, 0, stream>>>(src, n, items, dg, counts, at, clear);
   PS_LAUNCHED();
   if (self) {
-    id_place_kernel<true><<<tiles, kIdThreads, 0, stream>>>(src, sink, n, dg, counts, at);
+    id_place_kernel<true><<<tiles, kIdThreads, 0, stream>>>(src, sink, n, items, dg, counts, at);
   } else {
     const int rc = ps_exclusive_scan_u32(
         counts, counts, entries, static_cast<char*>(table) + ((entries * 4 + 255) & ~size_t(255)),
         reinterpret_cast<ps_stream_t>(stream));
     if (rc != PS_OK) return rc;
-    id_place_kernel<false><<<tiles, kIdThreads, 0, stream>>>(src, sink, n, dg, counts, at);
+    id_place_kernel<false><<<tiles, kIdThreads, 0, stream>>>(src, sink, n, items, dg, counts, at);
   }
   PS_LAUNCHED();
   return PS_OK;
 }
 
-// The whole sort when n fits one tile.
+// The whole sort when n fits one tile of kIdTile elements.
 template <typename Source, typename Sink>
 int id_sort_tile(const Source& src, const Sink& sink, uint32_t n, const Digit& first, int passes,
                  const ClearOnTheWay& clear, hipStream_t stream) {
-  id_sort_tile_kernel<<<1, kIdThreads, 0, stream>>>(src, sink, n, first, passes, clear);
+  const int items = n ? int((n + kIdThreads - 1) / kIdThreads) : 1;
+  id_sort_tile_kernel<<<1, kIdThreads, 0, stream>>>(src, sink, n, items, first, passes, clear);
   PS_LAUNCHED();
   return PS_OK;
 }
