@@ -54,12 +54,11 @@ uint32_t chunk_size(long long n, long long cols) {
 
 struct FlagSink {
   static constexpr bool kStarts = false;
-  uint32_t *keys, *values;
+  uint2* pairs;
   uint8_t* flags;  // flags[row] = 1 for rows with ids (null: not wanted)
   uint32_t rows;
   __device__ __forceinline__ void put(uint32_t pos, uint32_t key, uint32_t value) const {
-    keys[pos] = key;
-    values[pos] = value;
+    pairs[pos] = uint2{key, value};
     if (flags && key < rows) flags[key] = 1;
   }
   __device__ __forceinline__ void bin_start(uint32_t, uint32_t) const {}
@@ -67,11 +66,12 @@ struct FlagSink {
 
 constexpr uint32_t kManyChunks = 64;
 
-// The sorted ids (keys; `rows` = takes no part) and where their rows of
-// grad_out are, n of them, and the partial sums: chunk q's first run's part in
-// row 2q, its last run's in row 2q + 1, ld floats apart.
+// The sorted ids (`rows` = takes no part) and where their rows of grad_out are,
+// n of them, and the partial sums: chunk q's first run's part in row 2q, its
+// last run's in row 2q + 1, ld floats apart.
 struct Runs {
-  const uint32_t *keys, *at;
+  const uint2* sorted;
+  __device__ __forceinline__ uint32_t key(unsigned long long i) const { return sorted[i].x; }
   uint32_t n, rows, chunk;  // chunk: entries of a chunk
   float* partial;
   long long ld;
@@ -116,21 +116,22 @@ __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& gr
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const uint32_t q = min(i + j, r.n - 1);
-      id[s][j] = r.keys[q];
-      at[s][j] = r.at[q];
+      const uint2 pair = r.sorted[q];
+      id[s][j] = pair.x;
+      at[s][j] = pair.y;
     }
   };
   load_ids(b, 0);
   load_ids(b + kAhead, 1);
-  const uint32_t first = r.keys[b], last = r.keys[e - 1];
+  const uint32_t first = r.key(b), last = r.key(e - 1);
   // The first run may start in a chunk before: then it is that chunk's, or long.
-  const bool continued = b > 0 && r.keys[b - 1] == first;
-  const bool head_long = continued && ((b > size && r.keys[b - size - 1] == first) ||
-                                       (e < r.n && r.keys[e] == first));
+  const bool continued = b > 0 && r.key(b - 1) == first;
+  const bool head_long = continued && ((b > size && r.key(b - size - 1) == first) ||
+                                       (e < r.n && r.key(e) == first));
   // The last run may go on: then it is long, or this chunk's to the end.
-  const bool own_tail = e < r.n && r.keys[e] == last && last < r.rows &&
+  const bool own_tail = e < r.n && r.key(e) == last && last < r.rows &&
                         !(continued && first == last);
-  const bool tail_long = own_tail && next < r.n && r.keys[next] == last;
+  const bool tail_long = own_tail && next < r.n && r.key(next) == last;
   const uint32_t end = own_tail && !tail_long ? next : e;
 
   uint32_t key[2][kAhead];
@@ -179,7 +180,7 @@ __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& gr
     store_piece<N>(r.partial + (2ull * chunk + 1) * r.ld + c, sum);
     if (piece == 0) {
       const unsigned long long far = e + (unsigned long long)kManyChunks * size;
-      if (far < r.n && r.keys[far] == last)
+      if (far < r.n && r.key(far) == last)
         r.long_list[r.chunks - 1 - atomicAdd(r.long_count + 1, 1u)] = chunk;
       else
         r.long_list[atomicAdd(r.long_count, 1u)] = chunk;
@@ -234,7 +235,7 @@ __device__ __forceinline__ uint32_t chunks_in_run(const Runs& r, uint32_t from, 
     const uint32_t step = (hi - lo + kRowThreads - 1) / kRowThreads;
     const uint32_t at = lo + threadIdx.x * step;
     const uint32_t hits = __syncthreads_count(
-        at < hi && r.keys[(unsigned long long)(from + at) * r.chunk] == k);
+        at < hi && r.key((unsigned long long)(from + at) * r.chunk) == k);
     if (!hits) return lo;
     hi = min(hi, lo + hits * step);
     lo += (hits - 1) * step + 1;
@@ -252,7 +253,7 @@ __device__ void join_run(const Runs& r, const Mat<G>& grad, float scale, bool ac
   constexpr uint32_t kGroups = kRowThreads / kJoinPieces;
   const uint32_t group = threadIdx.x / kJoinPieces, lane = threadIdx.x % kJoinPieces;
   const uint32_t piece = tile * kJoinPieces + lane;
-  const uint32_t k = r.keys[(chunk + 1) * r.chunk - 1];
+  const uint32_t k = r.key((chunk + 1) * r.chunk - 1);
   const uint32_t reached = chunks_in_run(r, chunk + 1, k);
   const uint32_t share = (reached + kGroups - 1) / kGroups;
   const uint32_t from = min(group * share, reached), to = min(from + share, reached);
@@ -304,7 +305,8 @@ __global__ __launch_bounds__(kRowThreads) void grad_join_kernel(Runs r, Mat<G> g
 
 // The workspace of the gradient.
 struct GradSpace {
-  size_t keys[2], at[2], table, cleared, cleared_bytes, long_list, partial, total;
+  size_t pairs[2], table, cleared, cleared_bytes, long_list, partial, total;
+  size_t groups_bytes, flags;  // flags: from `cleared` on
   long long ld;
 };
 
@@ -319,19 +321,19 @@ int digit_passes(long long rows, int* bits) {
 GradSpace grad_space(long long n, long long cols, long long rows) {
   GradSpace s{};
   int bits = 0;
-  digit_passes(rows, &bits);
+  const int passes = digit_passes(rows, &bits);
   size_t at = 0;
   const auto take = [&at](size_t bytes) {
     const size_t from = at;
     at += (bytes + 255) & ~size_t(255);
     return from;
   };
-  for (int k = 0; k < 2; ++k) {
-    s.keys[k] = take(size_t(n) * 4);
-    s.at[k] = take(size_t(n) * 4);
-  }
+  for (int k = 0; k < 2; ++k) s.pairs[k] = take(size_t(n) * sizeof(uint2));
   s.table = take(id_sort_table_bytes(n, 1 << bits));
-  s.cleared_bytes = (size_t(rows) + 16 + 15) & ~size_t(15);  // the long runs' count, the flags
+  // the long runs' counts, every pass's groups, the flags
+  s.groups_bytes = id_sort_group_bytes(n, 1 << bits);
+  s.flags = 16 + size_t(passes) * s.groups_bytes;
+  s.cleared_bytes = (s.flags + size_t(rows) + 15) & ~size_t(15);
   s.cleared = take(s.cleared_bytes);
   const size_t chunk = chunk_size(n, cols);
   const size_t chunks = (size_t(n) + chunk - 1) / chunk;
@@ -345,7 +347,6 @@ GradSpace grad_space(long long n, long long cols, long long rows) {
 // The one workgroup that sorts a tile clears this many 16-byte words on the way
 // (64 KB); more are cleared by a launch of their own.
 constexpr size_t kTileClears = 4096;
-__global__ void clear_kernel(ClearOnTheWay clear) { clear_share(clear); }
 
 // Sorts the ids; returns which of the two buffers holds the result.
 template <typename I>
@@ -353,33 +354,31 @@ int sort_ids(const I* ids, uint32_t n, long long rows, long long padding, char* 
              const GradSpace& s, uint8_t* flags, int* result, hipStream_t stream) {
   int bits = 0;
   const int passes = digit_passes(rows, &bits);
-  const auto buffer = [&](size_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
+  const auto pairs = [&](int k) { return reinterpret_cast<uint2*>(ws + s.pairs[k]); };
   ClearOnTheWay clear{reinterpret_cast<uint4*>(ws + s.cleared),
-                      flags ? s.cleared_bytes / 16 : 1};
+                      (flags ? s.cleared_bytes : s.flags) / 16};
+  if (s.groups_bytes || (n <= kIdTile && clear.count > kTileClears)) {
+    const int rc = id_clear(clear, stream);
+    if (rc != PS_OK) return rc;
+    clear = {};
+  }
   if (n <= kIdTile) {
-    if (clear.count > kTileClears) {
-      clear_kernel<<<unsigned(std::min<size_t>((clear.count + 255) / 256, 1024)), 256, 0, stream>>>(
-          clear);
-      PS_LAUNCHED();
-      clear = {};
-    }
     *result = 0;
     return id_sort_tile(IdSource<I>{ids, rows, padding},
-                        FlagSink{buffer(s.keys[0]), buffer(s.at[0]), flags, uint32_t(rows)}, n,
-                        Digit{0, bits, 1 << bits}, passes, clear, stream);
+                        FlagSink{pairs(0), flags, uint32_t(rows)}, n, Digit{0, bits, 1 << bits},
+                        passes, clear, stream);
   }
   for (int k = 0; k < passes; ++k) {
     const Digit dg{k * bits, bits, 1 << bits};
-    const int to = k & 1;
-    const FlagSink sink{buffer(s.keys[to]), buffer(s.at[to]), k == passes - 1 ? flags : nullptr,
-                        uint32_t(rows)};
+    const FlagSink sink{pairs(k & 1), k == passes - 1 ? flags : nullptr, uint32_t(rows)};
+    void* const groups = ws + s.cleared + 16 + size_t(k) * s.groups_bytes;
     const int rc =
-        k == 0 ? id_sort_pass(IdSource<I>{ids, rows, padding}, sink, n, dg, ws + s.table, clear,
-                              stream)
-               : id_sort_pass(PairSource{buffer(s.keys[to ^ 1]), buffer(s.at[to ^ 1])}, sink, n,
-                              dg, ws + s.table, ClearOnTheWay{}, stream);
+        k == 0 ? id_sort_pass(IdSource<I>{ids, rows, padding}, sink, n, dg, ws + s.table, groups,
+                              clear, stream)
+               : id_sort_pass(PairSource{pairs((k & 1) ^ 1)}, sink, n, dg, ws + s.table, groups,
+                              ClearOnTheWay{}, stream);
     if (rc != PS_OK) return rc;
-    *result = to;
+    *result = k & 1;
   }
   return PS_OK;
 }
@@ -448,7 +447,7 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
   if (!grad->rows || (!ids->count && accumulate)) return PS_OK;
   const hipStream_t st = ps::to_hip(stream);
   char* ws = static_cast<char*>(workspace);
-  uint8_t* flags = accumulate ? nullptr : reinterpret_cast<uint8_t*>(ws + s.cleared + 16);
+  uint8_t* flags = accumulate ? nullptr : reinterpret_cast<uint8_t*>(ws + s.cleared + s.flags);
   const uint32_t n = uint32_t(ids->count);
   int result = 0;
   const int rc =
@@ -459,8 +458,7 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
                          flags, &result, st);
   if (rc != PS_OK) return rc;
   ps::Runs r{};
-  r.keys = reinterpret_cast<const uint32_t*>(ws + s.keys[result]);
-  r.at = reinterpret_cast<const uint32_t*>(ws + s.at[result]);
+  r.sorted = reinterpret_cast<const uint2*>(ws + s.pairs[result]);
   r.n = n;
   r.rows = uint32_t(grad->rows);
   r.partial = reinterpret_cast<float*>(ws + s.partial);

@@ -177,7 +177,7 @@ extern "C" {
 
 size_t ps_expert_sort_workspace_bytes(long long slots, int experts) {
   if (slots < 0 || slots > (1LL << 30) || experts < 1 || experts > 1024) return 0;
-  return ps::id_sort_table_bytes(slots, experts + 1) + 16;
+  return ps::id_sort_group_bytes(slots, experts + 1) + ps::id_sort_table_bytes(slots, experts + 1);
 }
 
 int ps_expert_sort(const ps_ids* ids, int experts, int* order, int* position, int* offsets,
@@ -195,7 +195,14 @@ int ps_expert_sort(const ps_ids* ids, int experts, int* order, int* position, in
   const hipStream_t st = ps::to_hip(stream);
   const auto sort = [&](const auto& src) {
     if (n <= ps::kIdTile) return ps::id_sort_tile(src, sink, n, dg, 1, ps::ClearOnTheWay{}, st);
-    return ps::id_sort_pass(src, sink, n, dg, workspace, ps::ClearOnTheWay{}, st);
+    // the groups' counts, then the table
+    const size_t groups = ps::id_sort_group_bytes(n, dg.bins);
+    if (groups) {
+      const int rc = ps::id_clear({static_cast<uint4*>(workspace), groups / 16}, st);
+      if (rc != PS_OK) return rc;
+    }
+    return ps::id_sort_pass(src, sink, n, dg, static_cast<char*>(workspace) + groups, workspace,
+                            ps::ClearOnTheWay{}, st);
   };
   if (ids->type == PS_I64)
     return sort(ps::IdSource<long long>{static_cast<const long long*>(ids->data), experts, -1});

@@ -8,10 +8,11 @@
 // atomics decide a place, so equal keys keep their order.
 //
 // Launches, at some 5 us each, are what a sort of this size costs. One tile
-// takes one for all digits, the elements staying in LDS. Up to kSelfTiles tiles
-// take two a digit: one counts every tile's digits, the next one's workgroups
-// each add up the counts that precede their own. More tiles take the device
-// scan between the two, as every workgroup would read the whole table.
+// takes one for all digits, the elements staying in LDS. More tiles take two a
+// digit: one counts every tile's digits, and the next one's workgroups each add
+// up the counts that precede their own: of every tile while they are few, of
+// groups of tiles and of the tiles of one's own group beyond. The tables of
+// very many tiles go through the device scan between the two.
 #pragma once
 
 #include "ps_common.hpp"
@@ -34,22 +35,11 @@ struct IdSource {
   }
   __device__ __forceinline__ uint32_t value(uint32_t i) const { return i; }
 };
+// Sorted pairs: x the key, y the value (where the element was).
 struct PairSource {
-  const uint32_t *keys, *values;
-  __device__ __forceinline__ uint32_t key(uint32_t i) const { return keys[i]; }
-  __device__ __forceinline__ uint32_t value(uint32_t i) const { return values[i]; }
-};
-
-// Where the elements of a pass go. `bin_start` gets every digit's first
-// position (Sink::kStarts only).
-struct PairSink {
-  static constexpr bool kStarts = false;
-  uint32_t *keys, *values;
-  __device__ __forceinline__ void put(uint32_t pos, uint32_t key, uint32_t value) const {
-    keys[pos] = key;
-    values[pos] = value;
-  }
-  __device__ __forceinline__ void bin_start(uint32_t, uint32_t) const {}
+  const uint2* pairs;
+  __device__ __forceinline__ uint32_t key(uint32_t i) const { return pairs[i].x; }
+  __device__ __forceinline__ uint32_t value(uint32_t i) const { return pairs[i].y; }
 };
 
 // Bytes cleared by the sort's first launch on the way (16-byte multiple).
@@ -63,7 +53,11 @@ struct Digit {
   int shift, bits, bins;
 };
 
-constexpr uint32_t kSelfTiles = 128;
+// Tiles up to which every workgroup adds up all tiles' counts, and up to which
+// it does so by groups of kGroupTiles (a placing launch over 512 digits took
+// 11.1 us with 32 tiles so, 14.5 with 64, 9.2 with 257 in groups; the groups'
+// clearing is a launch of its own).
+constexpr uint32_t kFewTiles = 32, kGroupTiles = 32, kGroupedTiles = 1024;
 constexpr int kIdWaves = kIdThreads / kWave;
 
 // Index in the tile of item r of this thread, of `items` items a thread.
@@ -143,16 +137,18 @@ __device__ __forceinline__ void clear_share(const ClearOnTheWay& c) {
     c.data[i] = uint4{0, 0, 0, 0};
 }
 
-// Where the count of (tile, bin) is in the table.
-struct TableAt {
-  size_t tile, bin;  // strides
+// The count table: counts[tile * tile_stride + bin * bin_stride]; groups: the
+// counts of kGroupTiles tiles together, cleared before the pass, or null.
+struct IdTable {
+  uint32_t *counts, *groups;
+  size_t tile_stride, bin_stride;
 };
 
 // Counts of every tile.
 template <typename Source>
-__global__ __launch_bounds__(kIdThreads) void id_count_kernel(Source src, uint32_t n, int items, Digit dg,
-                                                              uint32_t* __restrict__ table,
-                                                              TableAt at, ClearOnTheWay clear) {
+__global__ __launch_bounds__(kIdThreads) void id_count_kernel(Source src, uint32_t n, int items,
+                                                              Digit dg, IdTable table,
+                                                              ClearOnTheWay clear) {
   __shared__ uint16_t cnt[kIdWaves * kIdMaxBins];
   const uint32_t tile = items * kIdThreads, base = blockIdx.x * tile, valid = min(n - base, tile);
   uint32_t key[kIdItems], loc[kIdItems];
@@ -162,18 +158,20 @@ __global__ __launch_bounds__(kIdThreads) void id_count_kernel(Source src, uint32
   clear_share(clear);
   rank_tile(key, valid, items, dg, cnt, loc);
   __syncthreads();
-  for (int b = threadIdx.x; b < dg.bins; b += kIdThreads)
-    table[blockIdx.x * at.tile + b * at.bin] = wave_offsets(cnt, dg.bins, b);
+  for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) {
+    const uint32_t c = wave_offsets(cnt, dg.bins, b);
+    table.counts[blockIdx.x * table.tile_stride + b * table.bin_stride] = c;
+    if (table.groups && c) atomicAdd(&table.groups[blockIdx.x / kGroupTiles * dg.bins + b], c);
+  }
 }
 
-// Places a tile's elements. table: the counts (kSelf), or their scan.
-template <bool kSelf, typename Source, typename Sink>
+// Places a tile's elements. kScanned: the counts have been scanned.
+template <bool kScanned, typename Source, typename Sink>
 __global__ __launch_bounds__(kIdThreads) void id_place_kernel(Source src, Sink sink, uint32_t n,
                                                               int items, Digit dg,
-                                                              const uint32_t* __restrict__ table,
-                                                              TableAt at) {
+                                                              IdTable table) {
   __shared__ uint16_t cnt[kIdWaves * kIdMaxBins];
-  __shared__ uint32_t start[kIdMaxBins], ahead[kSelf ? kIdMaxBins : 1];
+  __shared__ uint32_t start[kIdMaxBins], ahead[kScanned ? 1 : kIdMaxBins];
   __shared__ uint32_t wave_sum[kIdWaves];
   const uint32_t tile = items * kIdThreads, base = blockIdx.x * tile, valid = min(n - base, tile);
   uint32_t key[kIdItems], value[kIdItems], loc[kIdItems];
@@ -183,22 +181,30 @@ __global__ __launch_bounds__(kIdThreads) void id_place_kernel(Source src, Sink s
     key[r] = in ? src.key(base + tile_item(r, items)) : 0u;
     value[r] = in ? src.value(base + tile_item(r, items)) : 0u;
   }
-  if constexpr (kSelf) {
-    // start: all tiles' counts, ahead: the earlier tiles'. The tiles are shared
-    // out among as many threads a bin as there are.
+  if constexpr (!kScanned) {
+    // start: all counts of a bin, ahead: the earlier tiles'. The rows of counts
+    // are shared out among as many threads a bin as there are.
     for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) start[b] = ahead[b] = 0;
     __syncthreads();
     int parts = kIdThreads;  // threads a bin
     while (parts > 1 && parts * dg.bins > kIdThreads) parts /= 2;
-    const uint32_t tiles = gridDim.x;
+    const uint32_t* rows = table.groups ? table.groups : table.counts;
+    const uint32_t mine = table.groups ? blockIdx.x / kGroupTiles : blockIdx.x;
+    const uint32_t count =
+        table.groups ? (gridDim.x + kGroupTiles - 1) / kGroupTiles : gridDim.x;
     for (int j = threadIdx.x; j < parts * dg.bins; j += kIdThreads) {
       const int part = j / dg.bins, b = j - part * dg.bins;
       uint32_t all = 0, before = 0;
 #pragma unroll 8
-      for (uint32_t t = part; t < tiles; t += parts) {
-        const uint32_t c = table[t * at.tile + b * at.bin];
+      for (uint32_t t = part; t < count; t += parts) {
+        const uint32_t c = rows[size_t(t) * dg.bins + b];
         all += c;
-        before += t < blockIdx.x ? c : 0u;
+        before += t < mine ? c : 0u;
+      }
+      if (table.groups) {
+#pragma unroll 8
+        for (uint32_t t = mine * kGroupTiles + part; t < blockIdx.x; t += parts)
+          before += table.counts[size_t(t) * dg.bins + b];
       }
       atomicAdd(&start[b], all);
       atomicAdd(&ahead[b], before);
@@ -206,14 +212,14 @@ __global__ __launch_bounds__(kIdThreads) void id_place_kernel(Source src, Sink s
     scan_bins(start, dg.bins, wave_sum);
   } else {
     for (int b = threadIdx.x; b < dg.bins; b += kIdThreads)
-      start[b] = table[blockIdx.x * at.tile + b * at.bin];
+      start[b] = table.counts[blockIdx.x * table.tile_stride + b * table.bin_stride];
   }
   rank_tile(key, valid, items, dg, cnt, loc);
   __syncthreads();
   for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) {
     (void)wave_offsets(cnt, dg.bins, b);
     if (Sink::kStarts && blockIdx.x == 0) sink.bin_start(uint32_t(b), start[b]);
-    if constexpr (kSelf) start[b] += ahead[b];
+    if constexpr (!kScanned) start[b] += ahead[b];
   }
   __syncthreads();
   const uint32_t mask = (1u << dg.bits) - 1u;
@@ -277,45 +283,66 @@ __global__ __launch_bounds__(kIdThreads) void id_sort_tile_kernel(Source src, Si
   }
 }
 
-// Items a thread takes: the fewest that leave at most kFewTiles tiles, as every
-// item is a step of the ranking and every tile a row of counts to add up.
-constexpr uint32_t kFewTiles = 64;
-inline int id_items(long long n) {
-  int items = 1;
-  while (items < kIdItems && n > (long long)kFewTiles * kIdThreads * items) items *= 2;
-  return items;
+static __global__ void id_clear_kernel(ClearOnTheWay clear) { clear_share(clear); }
+
+// How n elements are cut. Every item of a thread is a step of the ranking,
+// every tile a row of counts: one item while the tiles are no more than the
+// compute units, then more (10^6 ids, placing: 57 us with 977 tiles of one item,
+// 25 with 245 of four).
+struct IdCut {
+  int items;
+  uint32_t tiles, groups;  // groups: 0 where they are not used
+};
+inline IdCut id_cut(long long n) {
+  IdCut c{1, 0, 0};
+  while (c.items < kIdItems && n > 256LL * kIdThreads * c.items) c.items *= 2;
+  const long long tile = (long long)c.items * kIdThreads;
+  c.tiles = uint32_t((n + tile - 1) / tile);
+  if (c.tiles > kFewTiles && c.tiles <= kGroupedTiles)
+    c.groups = (c.tiles + kGroupTiles - 1) / kGroupTiles;
+  return c;
 }
 
-// Bytes of the count table and its scan for passes over n elements.
+// The workspace of a sort's passes: the count table and its scan, from `at` on,
+// and, to be cleared before the first pass, the groups of every pass.
 inline size_t id_sort_table_bytes(long long n, int bins) {
-  const long long tile = (long long)id_items(n) * kIdThreads;
-  const size_t table = size_t((n + tile - 1) / tile) * size_t(bins);
+  const size_t table = size_t(id_cut(n).tiles) * size_t(bins);
   return ((table * 4 + 255) & ~size_t(255)) + ps_scan_workspace_bytes(table);
 }
+inline size_t id_sort_group_bytes(long long n, int bins) {
+  return (size_t(id_cut(n).groups) * size_t(bins) * 4 + 15) & ~size_t(15);
+}
 
-// One pass over several tiles: n elements of src by digit dg into sink; table
-// holds id_sort_table_bytes(n, dg.bins) bytes. `clear` is done by the first
-// launch.
+// One pass over several tiles: n elements of src by digit dg into sink. table:
+// id_sort_table_bytes(n, dg.bins) bytes, groups: id_sort_group_bytes() cleared
+// ones for this pass alone. `clear` is done by the first launch.
 template <typename Source, typename Sink>
 int id_sort_pass(const Source& src, const Sink& sink, uint32_t n, const Digit& dg, void* table,
-                 const ClearOnTheWay& clear, hipStream_t stream) {
-  const int items = id_items(n);
-  const uint32_t tiles = (n + items * kIdThreads - 1) / (items * kIdThreads);
+                 void* groups, const ClearOnTheWay& clear, hipStream_t stream) {
+  const IdCut cut = id_cut(n);
   uint32_t* counts = static_cast<uint32_t*>(table);
-  const size_t entries = size_t(tiles) * size_t(dg.bins);
-  const bool self = tiles <= kSelfTiles;
-  const TableAt at = self ? TableAt{size_t(dg.bins), 1} : TableAt{1, tiles};
-  id_count_kernel<<<tiles, kIdThreads, 0, stream>>>(src, n, items, dg, counts, at, clear);
+  const size_t entries = size_t(cut.tiles) * size_t(dg.bins);
+  const bool scanned = cut.tiles > kGroupedTiles;
+  const IdTable t{counts, cut.groups ? static_cast<uint32_t*>(groups) : nullptr,
+                  scanned ? 1 : size_t(dg.bins), scanned ? size_t(cut.tiles) : 1};
+  id_count_kernel<<<cut.tiles, kIdThreads, 0, stream>>>(src, n, cut.items, dg, t, clear);
   PS_LAUNCHED();
-  if (self) {
-    id_place_kernel<true><<<tiles, kIdThreads, 0, stream>>>(src, sink, n, items, dg, counts, at);
-  } else {
+  if (scanned) {
     const int rc = ps_exclusive_scan_u32(
         counts, counts, entries, static_cast<char*>(table) + ((entries * 4 + 255) & ~size_t(255)),
         reinterpret_cast<ps_stream_t>(stream));
     if (rc != PS_OK) return rc;
-    id_place_kernel<false><<<tiles, kIdThreads, 0, stream>>>(src, sink, n, items, dg, counts, at);
+    id_place_kernel<true><<<cut.tiles, kIdThreads, 0, stream>>>(src, sink, n, cut.items, dg, t);
+  } else {
+    id_place_kernel<false><<<cut.tiles, kIdThreads, 0, stream>>>(src, sink, n, cut.items, dg, t);
   }
+  PS_LAUNCHED();
+  return PS_OK;
+}
+
+inline int id_clear(const ClearOnTheWay& clear, hipStream_t stream) {
+  const size_t blocks = (clear.count + 255) / 256;
+  id_clear_kernel<<<unsigned(blocks < 1024 ? blocks : 1024), 256, 0, stream>>>(clear);
   PS_LAUNCHED();
   return PS_OK;
 }

@@ -181,6 +181,18 @@ def test_grad_sorts(rows, count):
     check_grad(ids, 4, rows, torch.float32, torch.float32, gen)
 
 
+# tiles added up by groups, tiles of several items a thread, the scanned table
+@pytest.mark.parametrize("count", [65536, 65537, 300001, 1048577, 4300003])
+def test_grad_long_lists(count):
+    gen = generator("long", count)
+    for rows in (5, 70001):
+        say(f"grad long list rows={rows} count={count}")
+        u = torch.rand(count, generator=gen, dtype=torch.float64)
+        ids = (rows * u * u).long()
+        ids[::97] = -1
+        check_grad(ids, 2, rows, torch.float32, torch.float32, gen)
+
+
 def test_grad_nothing():
     gen = generator("nothing")
     for ids in (torch.empty(0, dtype=torch.int64), torch.full((100,), -1), torch.full((40,), 9)):

@@ -59,6 +59,23 @@ def test_sort(experts, tokens, top_k):
         assert position.view(-1).tolist() == p
 
 
+@pytest.mark.parametrize("tokens", [8192, 8193, 150000, 540001])
+@pytest.mark.parametrize("experts", [3, 200, 1024])
+def test_sort_long_lists(experts, tokens):
+    gen = generator("long", experts, tokens)
+    say(f"sort long list experts={experts} tokens={tokens}")
+    ids = torch.randint(-1, experts + 1, (tokens, 8), generator=gen)
+    order, position, offsets = sort(ids, experts)
+    key = torch.where((ids >= 0) & (ids < experts), ids, experts).view(-1)
+    o = torch.sort(key, stable=True).indices
+    assert torch.equal(order.cpu().long(), o)
+    p = torch.empty_like(o)
+    p[o] = torch.arange(o.numel())
+    assert torch.equal(position.cpu().view(-1).long(), torch.where(key < experts, p, -1))
+    counts = torch.bincount(key, minlength=experts + 1)[:experts]
+    assert offsets.tolist() == [0] + torch.cumsum(counts, 0).tolist()
+
+
 def test_sort_all_dropped():
     ids = torch.tensor([[-1, 5], [99, -(1 << 40)]])
     order, position, offsets = sort(ids, 5)
