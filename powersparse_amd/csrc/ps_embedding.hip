@@ -96,12 +96,19 @@ __device__ __forceinline__ void write_grad(const Mat<G>& grad, uint32_t row, int
   }
 }
 
+// A value that every lane of the wave has (kUniform), in a scalar register.
+template <bool kUniform>
+__device__ __forceinline__ uint32_t uniform(uint32_t x) {
+  return kUniform ? __builtin_amdgcn_readfirstlane(x) : x;
+}
+
 // One chunk's runs, for one piece of the width. Rows are loaded kAhead at a
 // time and one batch ahead of the additions, ids two batches ahead: a row's
 // address waits for its id, and a wait for loads also waits for the stores
 // issued before them, so the next rows are under way before a finished run is
-// written.
-template <typename T, typename G, int N>
+// written. Eight rows a batch are slower (262,147 skewed ids of 333 FP16
+// columns: 86 us instead of 58).
+template <bool kUniform, typename T, typename G, int N>
 __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& grad, float scale,
                          bool accumulate, uint32_t chunk, int piece, const Pieces& p) {
   constexpr int kAhead = 4;
@@ -117,21 +124,22 @@ __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& gr
     for (int j = 0; j < kAhead; ++j) {
       const uint32_t q = min(i + j, r.n - 1);
       const uint2 pair = r.sorted[q];
-      id[s][j] = pair.x;
-      at[s][j] = pair.y;
+      id[s][j] = uniform<kUniform>(pair.x);
+      at[s][j] = uniform<kUniform>(pair.y);
     }
   };
   load_ids(b, 0);
   load_ids(b + kAhead, 1);
-  const uint32_t first = r.key(b), last = r.key(e - 1);
+  const auto key_at = [&](uint32_t i) { return uniform<kUniform>(r.key(i)); };
+  const uint32_t first = key_at(b), last = key_at(e - 1);
   // The first run may start in a chunk before: then it is that chunk's, or long.
-  const bool continued = b > 0 && r.key(b - 1) == first;
-  const bool head_long = continued && ((b > size && r.key(b - size - 1) == first) ||
-                                       (e < r.n && r.key(e) == first));
+  const bool continued = b > 0 && key_at(b - 1) == first;
+  const bool head_long = continued && ((b > size && key_at(b - size - 1) == first) ||
+                                       (e < r.n && key_at(e) == first));
   // The last run may go on: then it is long, or this chunk's to the end.
-  const bool own_tail = e < r.n && r.key(e) == last && last < r.rows &&
+  const bool own_tail = e < r.n && key_at(e) == last && last < r.rows &&
                         !(continued && first == last);
-  const bool tail_long = own_tail && next < r.n && r.key(next) == last;
+  const bool tail_long = own_tail && next < r.n && key_at(next) == last;
   const uint32_t end = own_tail && !tail_long ? next : e;
 
   uint32_t key[2][kAhead];
@@ -194,16 +202,29 @@ __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& gr
 // Cleared rows are not read again soon: non-temporal stores, and 16 KB a
 // workgroup.
 constexpr uint32_t kClearItems = 4;  // per thread
-template <typename T, typename G, int N>
+template <bool kUniform, typename T, typename G, int N>
 __global__ __launch_bounds__(kRowThreads) void grad_runs_kernel(
     Runs r, Mat<const T> dy, Mat<G> grad, float scale, bool accumulate, Pieces p,
-    uint32_t run_blocks, unsigned long long run_items, const uint8_t* __restrict__ flags,
+    uint32_t run_blocks, const uint8_t* __restrict__ flags,
     Items clear_items) {
   if (blockIdx.x < run_blocks) {
-    const unsigned long long first = (unsigned long long)blockIdx.x * kRowThreads;
-    if (first + threadIdx.x >= run_items) return;
-    const Item it = ItemBase(first, p).at(threadIdx.x, p);
-    sum_runs<T, G, N>(r, dy, grad, scale, accumulate, uint32_t(it.row), it.piece, p);
+    uint32_t chunk;
+    int piece;
+    if constexpr (kUniform) {
+      const uint32_t waves = (p.per_row.d + kWave - 1) / kWave;  // per chunk
+      const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * (kRowThreads / kWave) +
+                                                        threadIdx.x / kWave);
+      chunk = w / waves;
+      piece = int((w - chunk * waves) * kWave) + lane_id();
+      if (chunk >= r.chunks || piece >= int(p.per_row.d)) return;
+    } else {
+      const unsigned long long first = (unsigned long long)blockIdx.x * kRowThreads;
+      if (first + threadIdx.x >= (unsigned long long)r.chunks * p.per_row.d) return;
+      const Item it = ItemBase(first, p).at(threadIdx.x, p);
+      chunk = uint32_t(it.row);
+      piece = it.piece;
+    }
+    sum_runs<kUniform, T, G, N>(r, dy, grad, scale, accumulate, chunk, piece, p);
     return;
   }
   const unsigned long long first =
@@ -474,9 +495,15 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
       return ps::with_width<(sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G))>(
           grad->cols, [&](auto w) {
             const ps::Pieces p(grad->cols, w);
-            const unsigned long long items = (unsigned long long)r.chunks * p.per_row.d;
+            // Waves of one chunk each from 64 pieces on: the control flow is
+            // scalar, but lanes beyond the width idle. 32,768 ids of 4,096
+            // BF16 columns 172 -> 165 us, 65,536 of 1,024 91 -> 88; but
+            // 262,144 of 256 74 -> 82, of 64 58 -> 87.
+            const bool waves = p.per_row.d >= ps::kWave;
+            const unsigned long long pieces =
+                waves ? (p.per_row.d + ps::kWave - 1) / ps::kWave * ps::kWave : p.per_row.d;
             const unsigned long long run_blocks =
-                (items + ps::kRowThreads - 1) / ps::kRowThreads;
+                (r.chunks * pieces + ps::kRowThreads - 1) / ps::kRowThreads;
             // The first launch takes the runs and as many rows to clear as
             // fit beside them, the others more rows.
             const unsigned long long clears =
@@ -490,10 +517,11 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
                   std::min<unsigned long long>((clears - done + per_block - 1) / per_block, 1u << 23);
               if (!(runs + blocks)) break;
               const unsigned long long end = std::min(clears, done + blocks * per_block);
-              ps::grad_runs_kernel<T, G, w>
-                  <<<uint32_t(runs + blocks), ps::kRowThreads, 0, st>>>(
+              const auto kernel = waves ? ps::grad_runs_kernel<true, T, G, w>
+                                        : ps::grad_runs_kernel<false, T, G, w>;
+              kernel<<<uint32_t(runs + blocks), ps::kRowThreads, 0, st>>>(
                       r, ps::mat<const T>(grad_out), ps::mat<G>(grad), scale, accumulate != 0, p,
-                      runs, items, flags, ps::Items{done, end});
+                      runs, flags, ps::Items{done, end});
               PS_LAUNCHED();
               runs = 0;
               done = end;

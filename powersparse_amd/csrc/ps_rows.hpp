@@ -127,36 +127,35 @@ __device__ __forceinline__ long long load_id(const long long* ids, long long i) 
 inline size_t dtype_size(int dtype) { return dtype == PS_F32 ? 4 : 2; }
 inline bool dtype_valid(int dtype) { return dtype >= PS_F32 && dtype <= PS_BF16; }
 
-// Empty string, or what is wrong with a matrix.
-inline std::string rows_error(const ps_rows* m, const char* name) {
-  const std::string n = name;
-  if (!m) return n + " is null";
-  if (!dtype_valid(m->dtype)) return n + ": unknown element type";
-  if (m->rows < 0 || m->cols < 1 || m->cols > (1 << 24)) return n + ": bad shape";
-  if (m->ld < m->cols) return n + ": row stride shorter than a row";
-  if (m->rows && m->ld > (1LL << 48) / m->rows) return n + ": too large";
-  if (m->rows && !m->data) return n + ": null data";
-  if (reinterpret_cast<uintptr_t>(m->data) % dtype_size(m->dtype)) return n + ": misaligned data";
-  return "";
+// What is wrong with a matrix, or null.
+inline const char* rows_error(const ps_rows* m) {
+  if (!m) return "null matrix";
+  if (!dtype_valid(m->dtype)) return "unknown element type";
+  if (m->rows < 0 || m->cols < 1 || m->cols > (1 << 24)) return "bad shape";
+  if (m->ld < m->cols) return "row stride shorter than a row";
+  if (m->rows && m->ld > (1LL << 48) / m->rows) return "too large";
+  if (m->rows && !m->data) return "null data";
+  if (reinterpret_cast<uintptr_t>(m->data) % dtype_size(m->dtype)) return "misaligned data";
+  return nullptr;
 }
-inline std::string ids_error(const ps_ids* ids) {
-  if (!ids) return "ids is null";
-  if (ids->type != PS_I32 && ids->type != PS_I64) return "ids: unknown id type";
-  if (ids->count < 0 || ids->count > (1LL << 30)) return "ids: bad count";
-  if (ids->count && !ids->data) return "ids: null data";
+inline const char* ids_error(const ps_ids* ids) {
+  if (!ids) return "null ids";
+  if (ids->type != PS_I32 && ids->type != PS_I64) return "unknown id type";
+  if (ids->count < 0 || ids->count > (1LL << 30)) return "bad count";
+  if (ids->count && !ids->data) return "null data";
   if (reinterpret_cast<uintptr_t>(ids->data) % (ids->type == PS_I64 ? 8 : 4))
-    return "ids: misaligned data";
-  return "";
+    return "misaligned data";
+  return nullptr;
 }
-#define PS_CHECK_ROWS(m)                                          \
-  do {                                                            \
-    const std::string ps_error_ = ps::rows_error(m, #m);          \
-    if (!ps_error_.empty()) return ps::fail(PS_ERR_INVALID, ps_error_); \
+#define PS_CHECK_ROWS(m)                                                                       \
+  do {                                                                                         \
+    if (const char* ps_error_ = ps::rows_error(m))                                             \
+      return ps::fail(PS_ERR_INVALID, std::string(__func__) + ": " #m ": " + ps_error_);       \
   } while (0)
-#define PS_CHECK_IDS(ids)                                         \
-  do {                                                            \
-    const std::string ps_error_ = ps::ids_error(ids);             \
-    if (!ps_error_.empty()) return ps::fail(PS_ERR_INVALID, ps_error_); \
+#define PS_CHECK_IDS(ids)                                                                      \
+  do {                                                                                         \
+    if (const char* ps_error_ = ps::ids_error(ids))                                            \
+      return ps::fail(PS_ERR_INVALID, std::string(__func__) + ": " #ids ": " + ps_error_);     \
   } while (0)
 
 inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {

@@ -15,6 +15,18 @@ import ctypes
 from . import _native
 from ._native import Ids, Rows
 
+
+class _Library:
+    """libpowersparse_hip.so's entry points, looked up once each (loaded on first use)."""
+
+    def __getattr__(self, name):
+        f = getattr(_native.hip(), name)
+        setattr(self, name, f)
+        return f
+
+
+_hip = _Library()
+
 _DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
 _ID_TYPES = {"int32": 0, "int64": 1}
 _BYTES = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "int64": 8, "uint8": 1}
@@ -46,69 +58,87 @@ class DeviceArray:
         self.ptr = (base or 0) + offset * size
 
 
-_tensor_dtypes = {}  # a tensor library's dtype object -> its name
+# Type codes by name, and by a tensor library's dtype objects as they are met.
+_row_codes = dict(_DTYPES)
+_id_codes = dict(_ID_TYPES)
+_names = {}
+
+
+def _dtype_name(dtype):
+    name = _names.get(dtype)
+    if name is None:
+        name = _names[dtype] = str(dtype).rsplit(".", 1)[-1]
+        for names, codes in ((_DTYPES, _row_codes), (_ID_TYPES, _id_codes)):
+            if name in names:
+                codes[dtype] = names[name]
+    return name
 
 
 def _described(x, name):
-    """(address, shape, row stride or None for a vector, dtype name) of an array."""
-    if isinstance(x, DeviceArray):
-        return x.ptr, x.shape, x.ld if len(x.shape) == 2 else None, x.dtype
+    """(address, shape, strides, dtype) of an array."""
+    if type(x) is DeviceArray:
+        return x.ptr, x.shape, (x.ld, 1) if len(x.shape) == 2 else (1,), x.dtype
     try:
-        dtype = _tensor_dtypes.get(x.dtype)
-        if dtype is None:
-            dtype = _tensor_dtypes[x.dtype] = str(x.dtype).rsplit(".", 1)[-1]
-        on_gpu, shape, stride, ptr = x.is_cuda, x.shape, x.stride(), x.data_ptr()
+        if x.is_cuda:
+            return x.data_ptr(), x.shape, x.stride(), x.dtype
     except (AttributeError, TypeError):
         raise ValueError(f"{name}: not a device array") from None
-    if not on_gpu:
-        raise ValueError(f"{name} is not in device memory")
-    return ptr, shape, stride, dtype
+    raise ValueError(f"{name} is not in device memory")
+
+
+def _code(dtype, codes, name, wanted):
+    """The type code of a dtype that `codes` does not hold yet."""
+    said = _dtype_name(dtype)
+    if dtype not in codes:
+        raise ValueError(f"{name}: element type {said} is not {wanted}")
+    return codes[dtype]
 
 
 def _rows(x, name):
     """The ps_rows of a matrix."""
     ptr, shape, stride, dtype = _described(x, name)
-    code = _DTYPES.get(dtype)
+    code = _row_codes.get(dtype)
     if code is None:
-        raise ValueError(f"{name}: element type {dtype} is not float32, float16 or bfloat16")
+        code = _code(dtype, _row_codes, name, "float32, float16 or bfloat16")
     if len(shape) != 2:
         raise ValueError(f"{name} is not a matrix")
     rows, cols = shape
-    if type(stride) is tuple:
-        if stride[1] != 1 and cols > 1 and rows:
-            raise ValueError(f"{name}: elements of a row are not contiguous")
-        stride = stride[0]
-        if rows <= 1 or cols == 0:  # the stride is not used, and may be anything
-            stride = cols
-    return Rows(ptr, rows, cols, stride, code)
+    ld, step = stride
+    if step != 1 and cols > 1 and rows:
+        raise ValueError(f"{name}: elements of a row are not contiguous")
+    return Rows(ptr, rows, cols, ld if rows > 1 else cols, code)
+
+
+def _contiguous(shape, stride, name):
+    """The element count of a contiguous array of any shape."""
+    n = 1
+    for s, d in zip(reversed(shape), reversed(stride)):
+        if d != n and s > 1 and 0 not in shape:
+            raise ValueError(f"{name} is not contiguous")
+        n *= s
+    return n
 
 
 def _flat(x, name, dtypes, count=None, optional=False):
-    """Address, element count and dtype of a contiguous array of any shape."""
+    """Address, element count and dtype name of a contiguous array of any shape."""
     if x is None and optional:
         return None, 0, None
     ptr, shape, stride, dtype = _described(x, name)
-    if dtype not in dtypes:
-        raise ValueError(f"{name}: element type {dtype} is not {' or '.join(dtypes)}")
-    n = 1
-    for s in shape:
-        n *= s
-    if type(stride) is tuple:
-        want = 1
-        for s, d in zip(reversed(shape), reversed(stride)):
-            if s != 1 and d != want and n:
-                raise ValueError(f"{name} is not contiguous")
-            want *= s
-    elif stride is not None and stride != shape[1] and shape[0] > 1:
-        raise ValueError(f"{name} is not contiguous")
+    said = _dtype_name(dtype)
+    if said not in dtypes:
+        raise ValueError(f"{name}: element type {said} is not {' or '.join(dtypes)}")
+    n = _contiguous(shape, stride, name)
     if count is not None and n != count:
         raise ValueError(f"{name} has {n} elements where {count} are needed")
-    return ptr, n, dtype
+    return ptr, n, said
 
 
 def _ids(x, name="ids"):
-    ptr, n, dtype = _flat(x, name, _ID_TYPES)
-    return Ids(ptr, n, _ID_TYPES[dtype])
+    ptr, shape, stride, dtype = _described(x, name)
+    code = _id_codes.get(dtype)
+    if code is None:
+        code = _code(dtype, _id_codes, name, "int32 or int64")
+    return Ids(ptr, _contiguous(shape, stride, name), code)
 
 
 def _space(x, name="workspace"):
@@ -137,13 +167,13 @@ def EmbeddingLookup(table, ids, out, scale=1.0, stream=None):
     """out[i] = scale * table[ids[i]]; zeros for ids outside the table. `ids` (int32 or
     int64, any shape) are taken in order; out has one row for each. table and out may differ
     in type."""
-    _call(_native.hip().ps_embedding_lookup(_rows(table, "table"), _ids(ids), scale,
+    _call(_hip.ps_embedding_lookup(_rows(table, "table"), _ids(ids), scale,
                                             _rows(out, "out"), _stream(stream)))
 
 
 def embedding_grad_workspace_bytes(count, cols, table_rows):
     """Workspace of EmbeddingGrad for `count` ids, rows of `cols` and a table of `table_rows`."""
-    n = _native.hip().ps_embedding_grad_workspace_bytes(int(count), int(cols), int(table_rows))
+    n = _hip.ps_embedding_grad_workspace_bytes(int(count), int(cols), int(table_rows))
     if not n:
         raise ValueError("embedding_grad_workspace_bytes: sizes out of range")
     return n
@@ -155,7 +185,7 @@ def EmbeddingGrad(ids, grad_out, grad_table, workspace, scale=1.0, padding_idx=-
     without ids; accumulate=True adds to grad_table instead. Ids outside the table and
     `padding_idx` take no part. The sum's order is fixed: the same bits every time."""
     ptr, nbytes = _space(workspace)
-    _call(_native.hip().ps_embedding_grad(
+    _call(_hip.ps_embedding_grad(
         _ids(ids), _rows(grad_out, "grad_out"), scale, padding_idx, bool(accumulate),
         _rows(grad_table, "grad_table"), ptr, nbytes, _stream(stream)))
 
@@ -164,7 +194,7 @@ def EmbeddingGrad(ids, grad_out, grad_table, workspace, scale=1.0, padding_idx=-
 
 def expert_sort_workspace_bytes(slots, experts):
     """Workspace of ExpertSort for `slots` ids (tokens * top_k) and `experts` experts."""
-    n = _native.hip().ps_expert_sort_workspace_bytes(int(slots), int(experts))
+    n = _hip.ps_expert_sort_workspace_bytes(int(slots), int(experts))
     if not n:
         raise ValueError("expert_sort_workspace_bytes: sizes out of range (1 to 1024 experts)")
     return n
@@ -178,7 +208,7 @@ def ExpertSort(ids, order, position, offsets, workspace, stream=None):
     slots = _ids(ids)
     at, count, _ = _flat(offsets, "offsets", ("int32",))
     ptr, nbytes = _space(workspace)
-    _call(_native.hip().ps_expert_sort(
+    _call(_hip.ps_expert_sort(
         slots, count - 1, _flat(order, "order", ("int32",), slots.count)[0],
         _flat(position, "position", ("int32",), slots.count)[0], at, ptr, nbytes,
         _stream(stream)))
@@ -199,7 +229,7 @@ def ExpertDispatch(x, position, xs, stream=None):
     position names are left alone, positions outside xs are skipped."""
     src = _rows(x, "x")
     ptr, top_k = _top_k(position, src.rows)
-    _call(_native.hip().ps_expert_dispatch(src, ptr, top_k, _rows(xs, "xs"), _stream(stream)))
+    _call(_hip.ps_expert_dispatch(src, ptr, top_k, _rows(xs, "xs"), _stream(stream)))
 
 
 def ExpertCombine(ys, position, weights, y, stream=None):
@@ -208,7 +238,7 @@ def ExpertCombine(ys, position, weights, y, stream=None):
     out = _rows(y, "y")
     ptr, top_k = _top_k(position, out.rows)
     w = _flat(weights, "weights", ("float32",), out.rows * top_k, optional=True)[0]
-    _call(_native.hip().ps_expert_combine(_rows(ys, "ys"), ptr, w, top_k, out, _stream(stream)))
+    _call(_hip.ps_expert_combine(_rows(ys, "ys"), ptr, w, top_k, out, _stream(stream)))
 
 
 def ExpertDispatchGrad(dxs, position, dx, stream=None):
@@ -223,7 +253,7 @@ def ExpertCombineGrad(dy, ys, position, weights, dys, dweights, stream=None):
     src = _rows(dy, "dy")
     ptr, top_k = _top_k(position, src.rows)
     n = src.rows * top_k
-    _call(_native.hip().ps_expert_combine_grad(
+    _call(_hip.ps_expert_combine_grad(
         src, _rows(ys, "ys"), ptr, _flat(weights, "weights", ("float32",), n)[0], top_k,
         _rows(dys, "dys"), _flat(dweights, "dweights", ("float32",), n)[0], _stream(stream)))
 
@@ -254,7 +284,7 @@ class GradientList:
             to = (ctypes.c_void_p * max(n, 1))(*[p for p, _, _ in dst])
             to_types = (ctypes.c_int * max(n, 1))(*[_DTYPES[d] for _, _, d in dst])
         h = ctypes.c_void_p()
-        _call(_native.hip().ps_grad_list_create(n, data, counts, types, to, to_types,
+        _call(_hip.ps_grad_list_create(n, data, counts, types, to, to_types,
                                                 ctypes.byref(h)))
         self._h = h.value
 
@@ -266,7 +296,7 @@ class GradientList:
 
     def close(self):
         if self._h:
-            _native.hip().ps_grad_list_destroy(self._h)
+            _hip.ps_grad_list_destroy(self._h)
             self._h = None
 
     def __del__(self):
@@ -278,19 +308,19 @@ class GradientList:
 
 def GradNorm(grads, norm, grad_scale=1.0, stream=None):
     """norm (one float32 on the device) = the 2-norm of grad_scale * g over a GradientList."""
-    _call(_native.hip().ps_grad_norm(grads.handle, grad_scale,
+    _call(_hip.ps_grad_norm(grads.handle, grad_scale,
                                      _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))
 
 
 def ClipGrads(grads, max_norm, norm, grad_scale=1.0, stream=None):
     """g * grad_scale * min(1, max_norm / (norm + 1e-6)) with a given norm, e.g. one that the
     ranks of a job have put together."""
-    _call(_native.hip().ps_clip_grads(grads.handle, max_norm, grad_scale,
+    _call(_hip.ps_clip_grads(grads.handle, max_norm, grad_scale,
                                       _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))
 
 
 def ClipGradNorm(grads, max_norm, norm, grad_scale=1.0, stream=None):
     """GradNorm and ClipGrads in one call: norm receives the norm before clipping."""
-    _call(_native.hip().ps_clip_grad_norm(grads.handle, max_norm, grad_scale,
+    _call(_hip.ps_clip_grad_norm(grads.handle, max_norm, grad_scale,
                                           _flat(norm, "norm", ("float32",), 1)[0],
                                           _stream(stream)))
