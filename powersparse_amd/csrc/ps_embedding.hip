@@ -45,6 +45,7 @@ __global__ __launch_bounds__(kRowThreads) void lookup_kernel(Mat<const T> table,
 // parts of long runs, shorter ones more loads in flight.
 constexpr unsigned long long kRunThreads = 1u << 18;
 uint32_t chunk_size(long long n, long long cols) {
+  if (n <= 16) return 16;  // one chunk: no run can be long, and no join is launched
   uint32_t c = 4;
   while (c < 16 && n / c > 4096) c *= 2;
   while (c < 256 && (unsigned long long)(n / c) * ((unsigned long long)(cols + 7) / 8) > kRunThreads)
