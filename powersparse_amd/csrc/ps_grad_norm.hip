@@ -22,6 +22,7 @@ struct GradTensor {
   void* out;
   long long count;
   int dtype, out_dtype;
+  long long first_chunk;
 };
 struct GradChunk {
   uint32_t tensor, index;  // elements [index * kChunk, ...) of the tensor
@@ -43,6 +44,24 @@ struct Grads {
   uint32_t chunk_count;
   bool in_place;
 };
+
+// The chunk table: the tensor that chunk q is of, by bisection.
+__global__ __launch_bounds__(kClipThreads) void chunk_kernel(const GradTensor* __restrict__ tensors,
+                                                             uint32_t tensor_count,
+                                                             GradChunk* __restrict__ chunks,
+                                                             uint32_t chunk_count) {
+  const uint32_t q = blockIdx.x * kClipThreads + threadIdx.x;
+  if (q >= chunk_count) return;
+  uint32_t lo = 0, hi = tensor_count - 1;  // the last tensor that begins at or before q
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi + 1) / 2;
+    if (tensors[mid].first_chunk <= q)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  chunks[q] = {lo, uint32_t(q - tensors[lo].first_chunk)};
+}
 
 // Sum over the workgroup, in every thread.
 __device__ __forceinline__ double block_sum(double v) {
@@ -167,6 +186,43 @@ struct ps_grad_list {
 namespace ps {
 namespace {
 
+// What is written must be read by nobody else: the index of a tensor whose
+// output meets another tensor's data or output, or -1.
+int shared_output(const std::vector<GradTensor>& table) {
+  struct Range {
+    uintptr_t begin, end;
+    int tensor;
+  };
+  const auto range = [](const void* p, long long count, int dtype, size_t tensor) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return Range{at, at + uintptr_t(count) * dtype_size(dtype), int(tensor)};
+  };
+  std::vector<Range> outs;
+  for (size_t i = 0; i < table.size(); ++i)
+    outs.push_back(range(table[i].out, table[i].count, table[i].out_dtype, i));
+  std::sort(outs.begin(), outs.end(),
+            [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  for (size_t i = 1; i < outs.size(); ++i)
+    if (outs[i].begin < outs[i - 1].end) return outs[i].tensor;
+  for (size_t i = 0; i < table.size(); ++i) {
+    const Range d = range(table[i].data, table[i].count, table[i].dtype, i);
+    // the first output that ends behind the data's begin
+    const auto o = std::upper_bound(outs.begin(), outs.end(), d.begin,
+                                    [](uintptr_t at, const Range& r) { return at < r.end; });
+    if (o != outs.end() && o->begin < d.end && o->tensor != int(i)) return int(i);
+  }
+  return -1;
+}
+
+int build_chunks(const GradTensor* tensors, uint32_t tensor_count, GradChunk* chunks,
+                 uint32_t chunk_count) {
+  chunk_kernel<<<(chunk_count + kClipThreads - 1) / kClipThreads, kClipThreads>>>(
+      tensors, tensor_count, chunks, chunk_count);
+  PS_LAUNCHED();
+  PS_HIP(hipStreamSynchronize(nullptr));
+  return PS_OK;
+}
+
 int launch_norm(const ps_grad_list& l, hipStream_t stream) {
   if (!l.blocks) return PS_OK;
   norm_kernel<<<l.blocks, kClipThreads, 0, stream>>>(l.grads, l.sums);
@@ -197,7 +253,8 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
                "ps_grad_list_create: null array");
   try {
     std::vector<ps::GradTensor> table;
-    long long total = 0;
+    long long total = 0, chunks = 0;
+    bool in_place = true;
     for (int i = 0; i < tensors; ++i) {
       const std::string name = "ps_grad_list_create: tensor " + std::to_string(i);
       const int out_dtype = out ? out_dtypes[i] : dtypes[i];
@@ -216,39 +273,39 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
                        !ps::overlap(data[i], size_t(counts[i]) * size, to,
                                     size_t(counts[i]) * out_size),
                    name + ": overlaps its output");
-      table.push_back({data[i], to, counts[i], dtypes[i], out_dtype});
+      table.push_back({data[i], to, counts[i], dtypes[i], out_dtype, chunks});
       total += counts[i];
+      chunks += (counts[i] + ps::kChunk - 1) / ps::kChunk;
+      in_place = in_place && to == data[i];
     }
-    std::vector<ps::GradChunk> chunks;
-    bool in_place = true;
-    for (size_t i = 0; i < table.size(); ++i) {
-      in_place = in_place && table[i].out == table[i].data;
-      const long long n = (table[i].count + ps::kChunk - 1) / ps::kChunk;
-      PS_CHECK_ARG(n + (long long)chunks.size() < (1LL << 31), "ps_grad_list_create: too large");
-      for (long long q = 0; q < n; ++q) chunks.push_back({uint32_t(i), uint32_t(q)});
-    }
+    PS_CHECK_ARG(chunks < (1LL << 31), "ps_grad_list_create: too many elements");
+    PS_CHECK_ARG(ps::shared_output(table) < 0,
+                 "ps_grad_list_create: an output overlaps another tensor, or a tensor is listed twice");
     const size_t table_bytes = (table.size() * sizeof(ps::GradTensor) + 255) & ~size_t(255);
-    const size_t chunk_bytes = (chunks.size() * sizeof(ps::GradChunk) + 255) & ~size_t(255);
+    const size_t chunk_bytes = (size_t(chunks) * sizeof(ps::GradChunk) + 255) & ~size_t(255);
     void* base = nullptr;
     PS_HIP(ps::dev_malloc(&base, table_bytes + chunk_bytes + ps::kBlocks * sizeof(double)));
     char* const at = static_cast<char*>(base);
+    const auto* const tensor_table = reinterpret_cast<const ps::GradTensor*>(at);
+    auto* const chunk_table = reinterpret_cast<ps::GradChunk*>(at + table_bytes);
     int rc = PS_OK;
-    if (!table.empty())
+    if (chunks) {
       rc = ps_memcpy_htod(at, table.data(), table.size() * sizeof(ps::GradTensor));
-    if (rc == PS_OK && !chunks.empty())
-      rc = ps_memcpy_htod(at + table_bytes, chunks.data(), chunks.size() * sizeof(ps::GradChunk));
+      if (rc == PS_OK) rc = ps::build_chunks(tensor_table, uint32_t(table.size()), chunk_table,
+                                             uint32_t(chunks));
+    }
     ps_grad_list* l = rc == PS_OK ? new (std::nothrow) ps_grad_list : nullptr;
     if (!l) {
       ps::dev_free(base);
       return rc != PS_OK ? rc : ps::fail(PS_ERR_RUNTIME, "ps_grad_list_create: out of memory");
     }
     l->tables = base;
-    l->grads.tensors = reinterpret_cast<const ps::GradTensor*>(at);
-    l->grads.chunks = reinterpret_cast<const ps::GradChunk*>(at + table_bytes);
-    l->grads.chunk_count = uint32_t(chunks.size());
+    l->grads.tensors = tensor_table;
+    l->grads.chunks = chunk_table;
+    l->grads.chunk_count = uint32_t(chunks);
     l->grads.in_place = in_place;
     l->sums = reinterpret_cast<double*>(at + table_bytes + chunk_bytes);
-    l->blocks = std::min(uint32_t(chunks.size()), ps::kBlocks);
+    l->blocks = std::min(uint32_t(chunks), ps::kBlocks);
     *list = l;
     return PS_OK;
   } catch (const std::exception& e) {

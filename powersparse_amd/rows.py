@@ -260,6 +260,20 @@ def ExpertCombineGrad(dy, ys, position, weights, dys, dweights, stream=None):
 
 # --------------------------------------------------------------- gradients
 
+def _spans(arrays, what):
+    """Addresses, element counts and type codes of contiguous arrays."""
+    n = max(len(arrays), 1)
+    data, counts, types = (ctypes.c_void_p * n)(), (ctypes.c_longlong * n)(), (ctypes.c_int * n)()
+    for i, x in enumerate(arrays):
+        code = _row_codes.get(getattr(x, "dtype", None))
+        if code is not None and type(x) is not DeviceArray and x.is_cuda and x.is_contiguous():
+            data[i], counts[i], types[i] = x.data_ptr(), x.numel(), code  # some hundred at a time
+        else:
+            data[i], counts[i], said = _flat(x, f"{what} {i}", _DTYPES)
+            types[i] = _DTYPES[said]
+    return data, counts, types
+
+
 class GradientList:
     """The gradient tensors of a model (contiguous arrays of any shape and of float32,
     float16 or bfloat16) and where their clipped values go: `outs`, one of the same size for
@@ -273,19 +287,16 @@ class GradientList:
         if outs is not None and len(outs) != len(grads):
             raise ValueError("outs: one for each gradient")
         n = len(grads)
-        src = [_flat(g, f"gradient {i}", _DTYPES) for i, g in enumerate(grads)]
-        data = (ctypes.c_void_p * max(n, 1))(*[p for p, _, _ in src])
-        counts = (ctypes.c_longlong * max(n, 1))(*[c for _, c, _ in src])
-        types = (ctypes.c_int * max(n, 1))(*[_DTYPES[d] for _, _, d in src])
+        data, counts, types = _spans(grads, "gradient")
         to = to_types = None
         if outs is not None:
-            dst = [_flat(o, f"output {i}", _DTYPES, c) for i, (o, (_, c, _)) in
-                   enumerate(zip(outs, src))]
-            to = (ctypes.c_void_p * max(n, 1))(*[p for p, _, _ in dst])
-            to_types = (ctypes.c_int * max(n, 1))(*[_DTYPES[d] for _, _, d in dst])
+            to, sizes, to_types = _spans(outs, "output")
+            for i in range(n):
+                if sizes[i] != counts[i]:
+                    raise ValueError(f"output {i} has {sizes[i]} elements where {counts[i]} "
+                                     "are needed")
         h = ctypes.c_void_p()
-        _call(_hip.ps_grad_list_create(n, data, counts, types, to, to_types,
-                                                ctypes.byref(h)))
+        _call(_hip.ps_grad_list_create(n, data, counts, types, to, to_types, ctypes.byref(h)))
         self._h = h.value
 
     @property

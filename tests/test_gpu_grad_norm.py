@@ -144,6 +144,21 @@ def test_nothing():
         ps.ClipGrads(ps.GradientList(grads), 1.0, norm)
 
 
+def test_many_tensors_side_by_side():
+    """Neighbours in one buffer, in place and into another one."""
+    gen = generator("many")
+    sizes = [int(n) for n in torch.randint(0, 9000, (700,), generator=gen)]
+    whole = torch.randn(sum(sizes), generator=gen).cuda()
+    before = whole.cpu().double()
+    norm = torch.empty(1, device="cuda")
+    out = torch.empty(sum(sizes), dtype=torch.bfloat16, device="cuda")
+    ps.ClipGradNorm(ps.GradientList(whole.split(sizes), out.split(sizes)), 2.0, norm)
+    e = before * (2.0 / (float(before.square().sum().sqrt()) + 1e-6))
+    ref.close(out, e, e.abs(), 2, "into another buffer")
+    ps.ClipGradNorm(ps.GradientList(whole.split(sizes)), 2.0, norm)
+    ref.close(whole, e, e.abs(), 2, "in place")
+
+
 def test_large():
     """Several chunks a workgroup, counts beyond 2^32 elements."""
     n = (1 << 32) + 5

@@ -161,6 +161,12 @@ def test_gradient_list():
     refused("tensor 1: misaligned", ps.GradientList, [g, vec(B + 2, 4, "float32")])
     refused("overlaps its output", ps.GradientList, [g], [vec(A + 4, 100, "float32")])
     refused("overlaps its output", ps.GradientList, [g], [vec(A, 100, "float16")])
+    h = vec(A + 400, 100, "float32")
+    refused("listed twice", ps.GradientList, [g, h, g])
+    refused("listed twice", ps.GradientList, [h, vec(A + 4, 100, "float32")])
+    refused("overlaps another", ps.GradientList, [g, h], [vec(B, 100, "float32"), g])
+    refused("overlaps another", ps.GradientList, [g, h], [vec(B, 100, "float32"),
+                                                          vec(B + 396, 100, "float32")])
     hip = _native.hip()
     assert hip.ps_grad_norm(None, 1.0, A, None) == _native.PS_ERR_INVALID
     assert hip.ps_clip_grads(None, 1.0, 1.0, A, None) == _native.PS_ERR_INVALID
