@@ -54,10 +54,9 @@ struct Digit {
 };
 
 // Tiles up to which every workgroup adds up all tiles' counts, and up to which
-// it does so by groups of kGroupTiles (a placing launch over 512 digits took
-// 11.1 us with 32 tiles so, 14.5 with 64, 9.2 with 257 in groups; the groups'
-// clearing is a launch of its own).
-constexpr uint32_t kFewTiles = 32, kGroupTiles = 32, kGroupedTiles = 1024;
+// it does so by groups of kGroupTiles, whose clearing is a launch of its own
+// (262,147 ids below 50,021: 33 us as 129 tiles in groups, 28 one by one).
+constexpr uint32_t kFewTiles = 192, kGroupTiles = 32, kGroupedTiles = 1024;
 constexpr int kIdWaves = kIdThreads / kWave;
 
 // Index in the tile of item r of this thread, of `items` items a thread.
@@ -137,8 +136,12 @@ __device__ __forceinline__ void clear_share(const ClearOnTheWay& c) {
     c.data[i] = uint4{0, 0, 0, 0};
 }
 
+// Counts of a tile in the table, padded to whole 16-byte loads.
+__host__ __device__ inline uint32_t table_stride(int bins) { return uint32_t(bins + 3) & ~3u; }
+
 // The count table: counts[tile * tile_stride + bin * bin_stride]; groups: the
-// counts of kGroupTiles tiles together, cleared before the pass, or null.
+// counts of kGroupTiles tiles together (table_stride() apart), cleared before the
+// pass, or null.
 struct IdTable {
   uint32_t *counts, *groups;
   size_t tile_stride, bin_stride;
@@ -161,7 +164,35 @@ __global__ __launch_bounds__(kIdThreads) void id_count_kernel(Source src, uint32
   for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) {
     const uint32_t c = wave_offsets(cnt, dg.bins, b);
     table.counts[blockIdx.x * table.tile_stride + b * table.bin_stride] = c;
-    if (table.groups && c) atomicAdd(&table.groups[blockIdx.x / kGroupTiles * dg.bins + b], c);
+    if (table.groups && c) 
+      atomicAdd(&table.groups[blockIdx.x / kGroupTiles * table_stride(dg.bins) + b], c);
+  }
+}
+
+// Adds rows first, first + step, ... below `count` of a table to `all`, and those
+// below `mine` to `before`, for the four bins of one quad.
+__device__ __forceinline__ void add_rows(const uint32_t* table, uint32_t quads, uint32_t quad,
+                                         uint32_t first, uint32_t step, uint32_t count,
+                                         uint32_t mine, uint4& all, uint4& before) {
+  constexpr int kRows = 8;
+  const uint4* rows = reinterpret_cast<const uint4*>(table) + quad;
+  for (uint32_t t0 = first; t0 < count; t0 += kRows * step) {
+    uint4 c[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) c[u] = rows[size_t(min(t0 + u * step, count - 1)) * quads];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const uint32_t t = t0 + u * step;
+      const uint32_t in = t < count ? ~0u : 0u, early = t < mine ? in : 0u;
+      all.x += c[u].x & in;
+      all.y += c[u].y & in;
+      all.z += c[u].z & in;
+      all.w += c[u].w & in;
+      before.x += c[u].x & early;
+      before.y += c[u].y & early;
+      before.z += c[u].z & early;
+      before.w += c[u].w & early;
+    }
   }
 }
 
@@ -171,7 +202,7 @@ __global__ __launch_bounds__(kIdThreads) void id_place_kernel(Source src, Sink s
                                                               int items, Digit dg,
                                                               IdTable table) {
   __shared__ uint16_t cnt[kIdWaves * kIdMaxBins];
-  __shared__ uint32_t start[kIdMaxBins], ahead[kScanned ? 1 : kIdMaxBins];
+  __shared__ uint32_t start[kIdMaxBins + 3], ahead[kScanned ? 1 : kIdMaxBins + 3];
   __shared__ uint32_t wave_sum[kIdWaves];
   const uint32_t tile = items * kIdThreads, base = blockIdx.x * tile, valid = min(n - base, tile);
   uint32_t key[kIdItems], value[kIdItems], loc[kIdItems];
@@ -182,32 +213,38 @@ __global__ __launch_bounds__(kIdThreads) void id_place_kernel(Source src, Sink s
     value[r] = in ? src.value(base + tile_item(r, items)) : 0u;
   }
   if constexpr (!kScanned) {
-    // start: all counts of a bin, ahead: the earlier tiles'. The rows of counts
-    // are shared out among as many threads a bin as there are.
-    for (int b = threadIdx.x; b < dg.bins; b += kIdThreads) start[b] = ahead[b] = 0;
-    __syncthreads();
-    int parts = kIdThreads;  // threads a bin
-    while (parts > 1 && parts * dg.bins > kIdThreads) parts /= 2;
-    const uint32_t* rows = table.groups ? table.groups : table.counts;
-    const uint32_t mine = table.groups ? blockIdx.x / kGroupTiles : blockIdx.x;
-    const uint32_t count =
-        table.groups ? (gridDim.x + kGroupTiles - 1) / kGroupTiles : gridDim.x;
-    for (int j = threadIdx.x; j < parts * dg.bins; j += kIdThreads) {
-      const int part = j / dg.bins, b = j - part * dg.bins;
-      uint32_t all = 0, before = 0;
-#pragma unroll 8
-      for (uint32_t t = part; t < count; t += parts) {
-        const uint32_t c = rows[size_t(t) * dg.bins + b];
-        all += c;
-        before += t < mine ? c : 0u;
-      }
+    // start: all counts of a bin, ahead: the earlier tiles'. A thread adds up
+    // four bins of a share of the rows, several rows' loads under way at once:
+    // they were written under other L2s and come from far (one by one they
+    // were 6 of the 12 us that 32,768 elements took).
+    // Eight rows a thread at least, so that few bins do not meet in LDS.
+    const uint32_t quads = table_stride(dg.bins) / 4;
+    const uint32_t parts = min(kIdThreads / quads, (gridDim.x + 7) / 8);
+    const uint32_t part = threadIdx.x / quads, quad = threadIdx.x - part * quads;
+    uint4 all{}, before{};
+    if (part < parts) {
       if (table.groups) {
-#pragma unroll 8
-        for (uint32_t t = mine * kGroupTiles + part; t < blockIdx.x; t += parts)
-          before += table.counts[size_t(t) * dg.bins + b];
+        const uint32_t mine = blockIdx.x / kGroupTiles;
+        add_rows(table.groups, quads, quad, part, parts, (gridDim.x - 1) / kGroupTiles + 1, mine,
+                 all, before);
+        uint4 none{};
+        add_rows(table.counts, quads, quad, mine * kGroupTiles + part, parts, blockIdx.x,
+                 blockIdx.x, none, before);
+      } else {
+        add_rows(table.counts, quads, quad, part, parts, gridDim.x, blockIdx.x, all, before);
       }
-      atomicAdd(&start[b], all);
-      atomicAdd(&ahead[b], before);
+    }
+    for (uint32_t b = threadIdx.x; b < 4 * quads; b += kIdThreads) start[b] = ahead[b] = 0;
+    __syncthreads();
+    if (part < parts) {
+      uint32_t* const to[2] = {start + 4 * quad, ahead + 4 * quad};
+      const uint4 from[2] = {all, before};
+      for (int k = 0; k < 2; ++k) {
+        atomicAdd(to[k], from[k].x);
+        atomicAdd(to[k] + 1, from[k].y);
+        atomicAdd(to[k] + 2, from[k].z);
+        atomicAdd(to[k] + 3, from[k].w);
+      }
     }
     scan_bins(start, dg.bins, wave_sum);
   } else {
@@ -286,16 +323,15 @@ __global__ __launch_bounds__(kIdThreads) void id_sort_tile_kernel(Source src, Si
 static __global__ void id_clear_kernel(ClearOnTheWay clear) { clear_share(clear); }
 
 // How n elements are cut. Every item of a thread is a step of the ranking,
-// every tile a row of counts: one item while the tiles are no more than the
-// compute units, then more (10^6 ids, placing: 57 us with 977 tiles of one item,
-// 25 with 245 of four).
+// every tile a row of counts: as few items as leave no more than kFewTiles
+// tiles.
 struct IdCut {
   int items;
   uint32_t tiles, groups;  // groups: 0 where they are not used
 };
 inline IdCut id_cut(long long n) {
   IdCut c{1, 0, 0};
-  while (c.items < kIdItems && n > 256LL * kIdThreads * c.items) c.items *= 2;
+  while (c.items < kIdItems && n > (long long)kFewTiles * kIdThreads * c.items) c.items *= 2;
   const long long tile = (long long)c.items * kIdThreads;
   c.tiles = uint32_t((n + tile - 1) / tile);
   if (c.tiles > kFewTiles && c.tiles <= kGroupedTiles)
@@ -306,11 +342,11 @@ inline IdCut id_cut(long long n) {
 // The workspace of a sort's passes: the count table and its scan, from `at` on,
 // and, to be cleared before the first pass, the groups of every pass.
 inline size_t id_sort_table_bytes(long long n, int bins) {
-  const size_t table = size_t(id_cut(n).tiles) * size_t(bins);
+  const size_t table = size_t(id_cut(n).tiles) * table_stride(bins);
   return ((table * 4 + 255) & ~size_t(255)) + ps_scan_workspace_bytes(table);
 }
 inline size_t id_sort_group_bytes(long long n, int bins) {
-  return (size_t(id_cut(n).groups) * size_t(bins) * 4 + 15) & ~size_t(15);
+  return size_t(id_cut(n).groups) * table_stride(bins) * 4;
 }
 
 // One pass over several tiles: n elements of src by digit dg into sink. table:
@@ -324,7 +360,7 @@ int id_sort_pass(const Source& src, const Sink& sink, uint32_t n, const Digit& d
   const size_t entries = size_t(cut.tiles) * size_t(dg.bins);
   const bool scanned = cut.tiles > kGroupedTiles;
   const IdTable t{counts, cut.groups ? static_cast<uint32_t*>(groups) : nullptr,
-                  scanned ? 1 : size_t(dg.bins), scanned ? size_t(cut.tiles) : 1};
+                  scanned ? 1 : table_stride(dg.bins), scanned ? size_t(cut.tiles) : 1};
   id_count_kernel<<<cut.tiles, kIdThreads, 0, stream>>>(src, n, cut.items, dg, t, clear);
   PS_LAUNCHED();
   if (scanned) {
