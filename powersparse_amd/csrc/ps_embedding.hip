@@ -131,16 +131,20 @@ __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& gr
   };
   load_ids(b, 0);
   load_ids(b + kAhead, 1);
+  // The ids around the chunk, loaded together: they come from far, and asked
+  // for one after another they cost as much as the rows.
   const auto key_at = [&](uint32_t i) { return uniform<kUniform>(r.key(i)); };
-  const uint32_t first = key_at(b), last = key_at(e - 1);
+  const uint32_t first = id[0][0], last = key_at(e - 1);
+  const uint32_t before = key_at(max(b, 1u) - 1), far_before = key_at(max(b, size + 1) - size - 1);
+  const uint32_t behind = key_at(min(e, r.n - 1)), far_behind = key_at(min(next, r.n - 1));
   // The first run may start in a chunk before: then it is that chunk's, or long.
-  const bool continued = b > 0 && key_at(b - 1) == first;
-  const bool head_long = continued && ((b > size && key_at(b - size - 1) == first) ||
-                                       (e < r.n && key_at(e) == first));
+  const bool continued = b > 0 && before == first;
+  const bool head_long =
+      continued && ((b > size && far_before == first) || (e < r.n && behind == first));
   // The last run may go on: then it is long, or this chunk's to the end.
-  const bool own_tail = e < r.n && key_at(e) == last && last < r.rows &&
-                        !(continued && first == last);
-  const bool tail_long = own_tail && next < r.n && key_at(next) == last;
+  const bool own_tail =
+      e < r.n && behind == last && last < r.rows && !(continued && first == last);
+  const bool tail_long = own_tail && next < r.n && far_behind == last;
   const uint32_t end = own_tail && !tail_long ? next : e;
 
   uint32_t key[2][kAhead];
