@@ -138,6 +138,7 @@ __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& gr
   const uint32_t before = key_at(max(b, 1u) - 1), far_before = key_at(max(b, size + 1) - size - 1);
   const uint32_t behind = key_at(min(e, r.n - 1)), far_behind = key_at(min(next, r.n - 1));
   // The first run may start in a chunk before: then it is that chunk's, or long.
+  if (first >= r.rows) return;  // only ids that take no part
   const bool continued = b > 0 && before == first;
   const bool head_long =
       continued && ((b > size && far_before == first) || (e < r.n && behind == first));
@@ -155,7 +156,8 @@ __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& gr
       const bool mine = i + j < e || (i + j < end && id[s][j] == last);
       key[s][j] = mine && id[s][j] < r.rows ? id[s][j] : kNone;
       const bool wanted = key[s][j] != kNone && !(continued && !head_long && key[s][j] == first);
-      row[s][j] = wanted ? *reinterpret_cast<const V*>(dy.at(at[s][j], c)) : V(T(0.f));
+      // (row 0 for the others: a load without a branch around it)
+      row[s][j] = *reinterpret_cast<const V*>(dy.at(wanted ? at[s][j] : 0u, c));
     }
   };
   uint32_t current = kNone;
