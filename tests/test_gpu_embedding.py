@@ -243,7 +243,7 @@ def test_on_another_stream():
             late.add_(table)  # work before the call on its stream
         late.copy_(table)
     ps.EmbeddingLookup(late, ids, out, stream=stream.cuda_stream)
-    ps.EmbeddingGrad(ids, out, grad, work, stream=stream.cuda_stream)
+    ps.EmbeddingGrad(ids, out, grad, work, stream=stream)
     stream.synchronize()
     assert torch.equal(out, table[ids])
     exact, mag, most = ref.lookup_grad(ids, out, 1000, 1.0)
