@@ -2,13 +2,14 @@
 and back with their gradients, and the norm and clipping of many gradient tensors
 (include/powersparse_rows.h).
 
-Arrays are DeviceArray (a DeviceBuffer or raw pointer with a shape and a type) or any
-tensor object with data_ptr, shape, stride, dtype and is_cuda, such as torch's. Matrices
-are row-major with any row stride; element types are float32, float16 and bfloat16. Every
-call checks shapes, types and sizes on the host, enqueues its kernels on `stream` (a
-Stream, a tensor library's stream, a raw handle, or None: the null stream) and returns
-without synchronising: arrays and workspaces must stay alive, and be written by nothing
-else, until the stream has passed the call. Wrong arguments raise ValueError.
+Arrays are in the current device's memory: DeviceArray (a DeviceBuffer or raw pointer with
+a shape and a type) or any tensor object with data_ptr, shape, stride, dtype and is_cuda,
+such as torch's. Matrices are row-major with any row stride; element types are float32,
+float16 and bfloat16. Every call checks shapes, types and sizes on the host, enqueues its
+kernels on `stream` (a Stream, a tensor library's stream, a raw handle, or None: the null
+stream) and returns without synchronising: arrays and workspaces must stay alive, and be
+written by nothing else, until the stream has passed the call. Wrong arguments raise
+ValueError.
 """
 import ctypes
 
@@ -96,6 +97,13 @@ def _code(dtype, codes, name, wanted):
 
 def _rows(x, name):
     """The ps_rows of a matrix."""
+    try:  # a tensor as it mostly is; anything else, and what is refused, below
+        if x.is_cuda:
+            (rows, cols), (ld, step) = x.shape, x.stride()
+            if step == 1 and rows > 1:
+                return Rows(x.data_ptr(), rows, cols, ld, _row_codes[x.dtype])
+    except (AttributeError, KeyError, TypeError, ValueError):
+        pass
     ptr, shape, stride, dtype = _described(x, name)
     code = _row_codes.get(dtype)
     if code is None:
@@ -123,6 +131,13 @@ def _flat(x, name, dtypes, count=None, optional=False):
     """Address, element count and dtype name of a contiguous array of any shape."""
     if x is None and optional:
         return None, 0, None
+    try:
+        if x.is_cuda and x.is_contiguous() and _names[x.dtype] in dtypes:
+            n = x.numel()
+            if count is None or n == count:
+                return x.data_ptr(), n, _names[x.dtype]
+    except (AttributeError, KeyError, TypeError):
+        pass
     ptr, shape, stride, dtype = _described(x, name)
     said = _dtype_name(dtype)
     if said not in dtypes:
@@ -134,6 +149,11 @@ def _flat(x, name, dtypes, count=None, optional=False):
 
 
 def _ids(x, name="ids"):
+    try:
+        if x.is_cuda and x.is_contiguous():
+            return Ids(x.data_ptr(), x.numel(), _id_codes[x.dtype])
+    except (AttributeError, KeyError, TypeError):
+        pass
     ptr, shape, stride, dtype = _described(x, name)
     code = _id_codes.get(dtype)
     if code is None:
@@ -143,6 +163,11 @@ def _ids(x, name="ids"):
 
 def _space(x, name="workspace"):
     """Address and bytes of a workspace: a DeviceBuffer or a contiguous array."""
+    try:
+        if x.is_cuda and x.is_contiguous():
+            return x.data_ptr(), x.numel() * _BYTES[_names[x.dtype]]
+    except (AttributeError, KeyError, TypeError):
+        pass
     if hasattr(x, "nbytes") and hasattr(x, "ptr") and not isinstance(x, DeviceArray):
         return x.ptr, x.nbytes
     ptr, n, dtype = _flat(x, name, _BYTES)
@@ -169,8 +194,8 @@ def EmbeddingLookup(table, ids, out, scale=1.0, stream=None):
     """out[i] = scale * table[ids[i]]; zeros for ids outside the table. `ids` (int32 or
     int64, any shape) are taken in order; out has one row for each. table and out may differ
     in type."""
-    _call(_hip.ps_embedding_lookup(_rows(table, "table"), _ids(ids), scale,
-                                            _rows(out, "out"), _stream(stream)))
+    _call(_hip.ps_embedding_lookup(_rows(table, "table"), _ids(ids), scale, _rows(out, "out"),
+                                   _stream(stream)))
 
 
 def embedding_grad_workspace_bytes(count, cols, table_rows):
@@ -321,19 +346,18 @@ class GradientList:
 
 def GradNorm(grads, norm, grad_scale=1.0, stream=None):
     """norm (one float32 on the device) = the 2-norm of grad_scale * g over a GradientList."""
-    _call(_hip.ps_grad_norm(grads.handle, grad_scale,
-                                     _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))
+    _call(_hip.ps_grad_norm(grads.handle, grad_scale, _flat(norm, "norm", ("float32",), 1)[0],
+                            _stream(stream)))
 
 
 def ClipGrads(grads, max_norm, norm, grad_scale=1.0, stream=None):
     """g * grad_scale * min(1, max_norm / (norm + 1e-6)) with a given norm, e.g. one that the
     ranks of a job have put together."""
     _call(_hip.ps_clip_grads(grads.handle, max_norm, grad_scale,
-                                      _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))
+                             _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))
 
 
 def ClipGradNorm(grads, max_norm, norm, grad_scale=1.0, stream=None):
     """GradNorm and ClipGrads in one call: norm receives the norm before clipping."""
     _call(_hip.ps_clip_grad_norm(grads.handle, max_norm, grad_scale,
-                                          _flat(norm, "norm", ("float32",), 1)[0],
-                                          _stream(stream)))
+                                 _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))
