@@ -20,7 +20,8 @@
 namespace ps {
 
 constexpr int kIdThreads = 1024;
-constexpr int kIdItems = 4;  // per thread, at most
+constexpr int kIdItems = 4;  // per thread, at most (one tile of eight for 8192 ids: 33.0
+                             // us, two launches a digit: 25.4; 4096 ids 22.8 in one tile)
 constexpr uint32_t kIdTile = kIdThreads * kIdItems;
 constexpr int kIdMaxBins = 1025;  // 1024 digits, or 1024 experts and the dropped slots
 

@@ -171,7 +171,7 @@ def test_grad_types_and_widths(dy_t, grad_t, cols, accumulate):
 
 # 1, 2 and 3 passes of the sort; one tile and many
 @pytest.mark.parametrize("rows", [2, 1023, 1024, 70001, (1 << 20) + 5, 3000000])
-@pytest.mark.parametrize("count", [4095, 4096, 4097, 20011, 70001])
+@pytest.mark.parametrize("count", [4095, 4096, 4097, 8192, 8193, 20011, 70001])
 def test_grad_sorts(rows, count):
     gen = generator(rows, count)
     say(f"grad sort rows={rows} count={count}")

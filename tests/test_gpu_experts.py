@@ -42,7 +42,8 @@ def sort(ids, experts):
 
 @pytest.mark.parametrize("experts", [1, 2, 17, 64, 255, 256, 1023, 1024])
 @pytest.mark.parametrize("tokens,top_k", [(0, 2), (1, 1), (1, 8), (63, 1), (65, 3), (1024, 4),
-                                          (4097, 1), (2049, 6), (9000, 8)])
+                                          (4097, 1), (2049, 6), (1024, 8), (8193, 1),
+                                          (9000, 8)])
 def test_sort(experts, tokens, top_k):
     gen = generator(experts, tokens, top_k)
     for dist, id_t in (("uniform", torch.int64), ("one", torch.int32), ("skewed", torch.int32)):
