@@ -1,7 +1,7 @@
 // Shared parts of the row operators (powersparse_rows.h): element types,
 // 16-byte row accesses, the item -> (row, column) map and argument checks.
 //
-// A row of `cols` elements is moved in pieces of N (16 bytes of the narrower
+// A row of `cols` elements is moved in pieces of N (16 bytes of the wider
 // type). An item is one piece of one row; items are numbered row by row and
 // dealt to threads in order, so a wave's accesses are contiguous for every
 // width. The last piece of a row ends with the row and overlaps the one before
@@ -119,9 +119,6 @@ struct ItemBase {
   }
 };
 
-__device__ __forceinline__ long long load_id(const int* ids, long long i) { return ids[i]; }
-__device__ __forceinline__ long long load_id(const long long* ids, long long i) { return ids[i]; }
-
 // --------------------------------------------------------------- host side
 
 inline size_t dtype_size(int dtype) { return dtype == PS_F32 ? 4 : 2; }
@@ -169,8 +166,12 @@ inline size_t rows_bytes(const ps_rows* m) {
 // Column ranges of one wider matrix share its memory range and no element.
 inline bool overlap(const ps_rows* a, const ps_rows* b) {
   if (!overlap(a->data, rows_bytes(a), b->data, rows_bytes(b))) return false;
-  const size_t pitch = size_t(a->ld) * dtype_size(a->dtype);
-  if (pitch != size_t(b->ld) * dtype_size(b->dtype)) return true;
+  const size_t pitch_a = size_t(a->ld) * dtype_size(a->dtype);
+  const size_t pitch_b = size_t(b->ld) * dtype_size(b->dtype);
+  // a single row's stride says nothing
+  const size_t pitch = a->rows == 1 ? pitch_b : pitch_a;
+  if ((a->rows > 1 && b->rows > 1 && pitch_a != pitch_b) || (a->rows == 1 && b->rows == 1))
+    return true;
   const uintptr_t x = reinterpret_cast<uintptr_t>(a->data), y = reinterpret_cast<uintptr_t>(b->data);
   const size_t apart = x <= y ? (y - x) % pitch : (pitch - (x - y) % pitch) % pitch;
   return apart < size_t(a->cols) * dtype_size(a->dtype) ||
@@ -209,8 +210,8 @@ inline int with_flag(bool flag, F&& f) {
   return flag ? f(std::true_type{}) : f(std::false_type{});
 }
 
-// Calls f(N) with the elements per piece of rows of `cols` elements, the
-// narrower of whose types has `size` bytes, as a constant.
+// Calls f(N) with the elements per piece of rows of `cols` elements, the wider
+// of whose types has kSize bytes, as a constant.
 template <int kSize, typename F>
 inline int with_width(long long cols, F&& f) {
   constexpr int N = 16 / kSize;

@@ -186,6 +186,14 @@ def test_column_ranges_of_one_buffer():
     ps.ExpertDispatch(x, position, xs)
     before[position.view(-1).long(), 15:27] = before[:25, 3:15].repeat_interleave(2, 0)
     assert torch.equal(whole, before)
+    # a single row, whose own stride is not the buffer's
+    one = torch.tensor([[7, 30]], dtype=torch.int32, device="cuda")
+    ps.ExpertDispatch(whole[9:10, 3:15], one, xs)
+    before[[7, 30], 15:27] = before[9, 3:15]
+    assert torch.equal(whole, before)
+    ps.ExpertCombine(xs, one, None, whole[11:12, 3:15])
+    before[11, 3:15] = before[7, 15:27] + before[30, 15:27]
+    assert torch.equal(whole, before)
 
 
 def test_differences():

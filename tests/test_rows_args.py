@@ -150,6 +150,9 @@ def test_column_ranges_of_one_matrix_that_overlap():
     for off in (1, 7, 25, 31, 33):
         refused("overlap", ps.ExpertDispatch, mat(A, 20, 8, ld=32), mat(C, 20, 1, "int32"),
                 mat(A + 4 * off, 20, 8, ld=32))
+        refused("overlap", ps.ExpertDispatch, mat(A + 640, 1, 8), mat(C, 1, 1, "int32"),
+                mat(A + 4 * off, 20, 8, ld=32))
+    refused("overlap", ps.ExpertDispatch, mat(A, 1, 8), mat(C, 1, 1, "int32"), mat(A + 4, 1, 8))
 
 
 def test_gradient_list():
