@@ -52,8 +52,8 @@ uint32_t chunk_size(long long n, long long cols) {
   if (n <= 16) return 16;  // one chunk: no run can be long, and no join is launched
   uint32_t c = 4;
   while (c < 16 && n / c > 4096) c *= 2;
-  while (c < 256 && (unsigned long long)(n / c) * ((unsigned long long)(cols + 7) / 8) > kRunThreads)
-    c *= 2;
+  const unsigned long long pieces = (unsigned long long)(cols + 7) / 8;
+  while (c < 256 && (unsigned long long)(n / c) * pieces > kRunThreads) c *= 2;
   return c;
 }
 
@@ -525,8 +525,8 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
             unsigned long long done = 0;
             do {
               const unsigned long long per_block = ps::kRowThreads * ps::kClearItems;
-              const unsigned long long blocks =
-                  std::min<unsigned long long>((clears - done + per_block - 1) / per_block, 1u << 23);
+              const unsigned long long blocks = std::min<unsigned long long>(
+                  (clears - done + per_block - 1) / per_block, 1u << 23);
               if (!(runs + blocks)) break;
               const unsigned long long end = std::min(clears, done + blocks * per_block);
               const auto kernel = waves ? ps::grad_runs_kernel<true, T, G, w>

@@ -282,7 +282,8 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
     }
     PS_CHECK_ARG(chunks < (1LL << 31), "ps_grad_list_create: too many elements");
     PS_CHECK_ARG(ps::shared_output(table) < 0,
-                 "ps_grad_list_create: an output overlaps another tensor, or a tensor is listed twice");
+                 "ps_grad_list_create: an output overlaps another tensor, or a tensor is "
+                 "listed twice");
     const size_t table_bytes = (table.size() * sizeof(ps::GradTensor) + 255) & ~size_t(255);
     const size_t chunk_bytes = (size_t(chunks) * sizeof(ps::GradChunk) + 255) & ~size_t(255);
     void* base = nullptr;

@@ -172,7 +172,8 @@ inline bool overlap(const ps_rows* a, const ps_rows* b) {
   const size_t pitch = a->rows == 1 ? pitch_b : pitch_a;
   if ((a->rows > 1 && b->rows > 1 && pitch_a != pitch_b) || (a->rows == 1 && b->rows == 1))
     return true;
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a->data), y = reinterpret_cast<uintptr_t>(b->data);
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a->data);
+  const uintptr_t y = reinterpret_cast<uintptr_t>(b->data);
   const size_t apart = x <= y ? (y - x) % pitch : (pitch - (x - y) % pitch) % pitch;
   return apart < size_t(a->cols) * dtype_size(a->dtype) ||
          apart + size_t(b->cols) * dtype_size(b->dtype) > pitch;

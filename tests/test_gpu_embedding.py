@@ -40,7 +40,8 @@ def generator(*key):
 def test_lookup(table_t, out_t, cols):
     gen = generator(table_t, out_t, cols)
     for count, rows, pad, offset, id_t in ((1, 1, 0, 0, torch.int64), (5, 3, 1, 1, torch.int32),
-                                           (300, 77, 0, 3, torch.int64), (1030, 50, 5, 0, torch.int32)):
+                                           (300, 77, 0, 3, torch.int64),
+                                           (1030, 50, 5, 0, torch.int32)):
         say(f"lookup {table_t}->{out_t} cols={cols} count={count} rows={rows} pad={pad}")
         table, _ = values(gen, rows, cols, F[table_t], pad, offset)
         ids = torch.randint(-1, rows + 1, (count,), generator=gen)

@@ -16,11 +16,13 @@ def plain_logits(model, params, token, coo, n):
     table, router, out, *expert = params
     row, col, val = (torch.from_numpy(a) for a in coo)
     x = table[token.cpu()] * model.scale
-    h = torch.zeros((n, x.shape[1]), dtype=torch.float64).index_add(0, row, val.double()[:, None] * x[col])
+    h = torch.zeros((n, x.shape[1]), dtype=torch.float64)
+    h = h.index_add(0, row, val.double()[:, None] * x[col])
     top = (h @ router).topk(model.top_k, dim=1)
     w = torch.softmax(top.values, dim=1)
     each = torch.stack([torch.relu(h @ e) for e in expert], 1)  # nodes x experts x width
-    y = (w[..., None] * torch.gather(each, 1, top.indices[..., None].expand(-1, -1, h.shape[1]))).sum(1)
+    chosen = torch.gather(each, 1, top.indices[..., None].expand(-1, -1, h.shape[1]))
+    y = (w[..., None] * chosen).sum(1)
     return y @ out + h @ out
 
 
