@@ -8,7 +8,9 @@
  * checks its arguments on the host, enqueues its kernels on `stream` and
  * returns; nothing here synchronises, allocates (ps_grad_list_create aside) or
  * keeps anything between calls. Workspaces are the caller's, of the stated
- * size, aligned to 16 bytes, not shared by calls that may overlap.
+ * size or more, aligned to 16 bytes, not shared by calls that may overlap. The
+ * stated sizes grow with every argument, so a workspace for the largest call
+ * does for smaller ones.
  *
  * Data may hold any value: ids and positions out of range are dropped where
  * the text says so and never followed. Sums run in 32 bits in a fixed order (the

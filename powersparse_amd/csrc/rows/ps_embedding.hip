@@ -351,10 +351,15 @@ int digit_passes(long long rows, int* bits) {
   return passes;
 }
 
-GradSpace grad_space(long long n, long long cols, long long rows) {
+// What the parts of the workspace take.
+struct GradSizes {
+  size_t table, groups;  // groups: of one pass
+  int passes;
+  size_t chunks, partial;  // partial: floats
+};
+
+GradSpace grad_layout(long long n, long long rows, const GradSizes& z) {
   GradSpace s{};
-  int bits = 0;
-  const int passes = digit_passes(rows, &bits);
   size_t at = 0;
   const auto take = [&at](size_t bytes) {
     const size_t from = at;
@@ -362,19 +367,56 @@ GradSpace grad_space(long long n, long long cols, long long rows) {
     return from;
   };
   for (int k = 0; k < 2; ++k) s.pairs[k] = take(size_t(n) * sizeof(uint2));
-  s.table = take(id_sort_table_bytes(n, 1 << bits));
+  s.table = take(z.table);
   // the long runs' counts, every pass's groups, the flags
-  s.groups_bytes = id_sort_group_bytes(n, 1 << bits);
-  s.flags = 16 + size_t(passes) * s.groups_bytes;
+  s.groups_bytes = z.groups;
+  s.flags = 16 + size_t(z.passes) * z.groups;
   s.cleared_bytes = (s.flags + size_t(rows) + 15) & ~size_t(15);
   s.cleared = take(s.cleared_bytes);
-  const size_t chunk = chunk_size(n, cols);
-  const size_t chunks = (size_t(n) + chunk - 1) / chunk;
-  s.long_list = take(chunks * 4);
-  s.ld = (cols + 7) & ~7LL;
-  s.partial = take(2 * chunks * size_t(s.ld) * 4);
+  s.long_list = take(z.chunks * 4);
+  s.partial = take(z.partial * 4);
   s.total = at;
   return s;
+}
+
+long long partial_ld(long long cols) { return (cols + 7) & ~7LL; }
+
+// The workspace of one call.
+GradSpace grad_space(long long n, long long cols, long long rows) {
+  int bits = 0;
+  const int passes = digit_passes(rows, &bits);
+  const IdCut cut = id_cut(n);
+  const size_t chunk = chunk_size(n, cols), chunks = (size_t(n) + chunk - 1) / chunk;
+  const long long ld = partial_ld(cols);
+  GradSpace s = grad_layout(n, rows,
+                            {id_sort_table_bytes(cut, 1 << bits), id_sort_group_bytes(cut, 1 << bits),
+                             passes, chunks, 2 * chunks * size_t(ld)});
+  s.ld = ld;
+  return s;
+}
+
+// The bytes that callers are asked for: no less than grad_space() of any call of
+// as many ids, columns and rows or fewer, though longer chunks, wider tiles and
+// shorter digits make some larger calls need less. Each part is bounded by what
+// grows with all three:
+//  - bins: 2^bits up to 1023 rows, which take one digit, and 1024 beyond;
+//  - chunks: ceil(n / 4) while chunk_size() starts from 4, no more than 4097 where
+//    it starts from 8, ceil(n / 16) beyond;
+//  - chunks * ld: a chunk is the shortest one (bounded above), 256 entries, or
+//    leaves chunks * ld / 8 <= kRunThreads, one partly filled chunk aside.
+size_t grad_space_most(long long n, long long cols, long long rows) {
+  int bits = 0;
+  const int passes = digit_passes(rows, &bits);
+  const int bins = passes > 1 ? 1024 : 1 << bits;
+  const IdCut cut = id_cut_most(n);
+  const auto chunks_of = [n](long long chunk) { return size_t((n + chunk - 1) / chunk); };
+  const size_t chunks = std::max(std::min<size_t>(chunks_of(4), 4097), chunks_of(16));
+  const size_t ld = size_t(partial_ld(cols));
+  const size_t partial =
+      std::min(chunks * ld, std::max(8 * size_t(kRunThreads) + ld, chunks_of(256) * ld));
+  return grad_layout(n, rows, {id_sort_table_bytes(cut, bins), id_sort_group_bytes(cut, bins),
+                               passes, chunks, 2 * partial})
+      .total;
 }
 
 // The one workgroup that sorts a tile clears this many 16-byte words on the way
@@ -463,7 +505,7 @@ size_t ps_embedding_grad_workspace_bytes(long long count, long long cols, long l
   if (count < 0 || count > (1LL << 30) || cols < 1 || cols > (1 << 24) || table_rows < 0 ||
       table_rows > (1LL << 31) - 2)
     return 0;
-  return ps::grad_space(count, cols, table_rows).total;
+  return ps::grad_space_most(count, cols, table_rows);
 }
 
 int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
@@ -476,9 +518,10 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
                "ps_embedding_grad: grad_out is not ids x grad columns");
   PS_CHECK_ARG(grad->rows <= (1LL << 31) - 2, "ps_embedding_grad: too many rows");
   PS_CHECK_ARG(!ps::overlap(grad_out, grad), "ps_embedding_grad: grad_out and grad overlap");
-  const ps::GradSpace s = ps::grad_space(ids->count, grad->cols, grad->rows);
-  PS_CHECK_ARG(workspace && ps::aligned16(workspace) && workspace_bytes >= s.total,
+  PS_CHECK_ARG(workspace && ps::aligned16(workspace) &&
+                   workspace_bytes >= ps::grad_space_most(ids->count, grad->cols, grad->rows),
                "ps_embedding_grad: workspace too small or misaligned");
+  const ps::GradSpace s = ps::grad_space(ids->count, grad->cols, grad->rows);
   if (!grad->rows || (!ids->count && accumulate)) return PS_OK;
   const hipStream_t st = ps::to_hip(stream);
   char* ws = static_cast<char*>(workspace);

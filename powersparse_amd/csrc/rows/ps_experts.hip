@@ -183,7 +183,8 @@ extern "C" {
 
 size_t ps_expert_sort_workspace_bytes(long long slots, int experts) {
   if (slots < 0 || slots > (1LL << 30) || experts < 1 || experts > 1024) return 0;
-  return ps::id_sort_group_bytes(slots, experts + 1) + ps::id_sort_table_bytes(slots, experts + 1);
+  const ps::IdCut most = ps::id_cut_most(slots);
+  return ps::id_sort_group_bytes(most, experts + 1) + ps::id_sort_table_bytes(most, experts + 1);
 }
 
 int ps_expert_sort(const ps_ids* ids, int experts, int* order, int* position, int* offsets,
@@ -202,7 +203,7 @@ int ps_expert_sort(const ps_ids* ids, int experts, int* order, int* position, in
   const auto sort = [&](const auto& src) {
     if (n <= ps::kIdTile) return ps::id_sort_tile(src, sink, n, dg, 1, ps::ClearOnTheWay{}, st);
     // the groups' counts, then the table
-    const size_t groups = ps::id_sort_group_bytes(n, dg.bins);
+    const size_t groups = ps::id_sort_group_bytes(ps::id_cut(n), dg.bins);
     if (groups) {
       const int rc = ps::id_clear({static_cast<uint4*>(workspace), groups / 16}, st);
       if (rc != PS_OK) return rc;

@@ -339,20 +339,30 @@ inline IdCut id_cut(long long n) {
     c.groups = (c.tiles + kGroupTiles - 1) / kGroupTiles;
   return c;
 }
+// The most tiles and groups of any list of up to n elements: where the items a
+// thread double the tiles are half of the kFewTiles before, and beyond
+// kGroupedTiles there are no groups. What callers are asked for is sized by it,
+// so that a workspace for n does for fewer.
+inline IdCut id_cut_most(long long n) {
+  IdCut c = id_cut(n);
+  if (c.items > 1 && c.tiles < kFewTiles) c.tiles = kFewTiles;
+  if (c.tiles > kGroupedTiles) c.groups = kGroupedTiles / kGroupTiles;
+  return c;
+}
 
-// The workspace of a sort's passes: the count table and its scan, from `at` on,
-// and, to be cleared before the first pass, the groups of every pass.
-inline size_t id_sort_table_bytes(long long n, int bins) {
-  const size_t table = size_t(id_cut(n).tiles) * table_stride(bins);
+// The workspace of a sort's passes: the count table and its scan, and, to be
+// cleared before the first pass, the groups of every pass.
+inline size_t id_sort_table_bytes(const IdCut& cut, int bins) {
+  const size_t table = size_t(cut.tiles) * table_stride(bins);
   return ((table * 4 + 255) & ~size_t(255)) + ps_scan_workspace_bytes(table);
 }
-inline size_t id_sort_group_bytes(long long n, int bins) {
-  return size_t(id_cut(n).groups) * table_stride(bins) * 4;
+inline size_t id_sort_group_bytes(const IdCut& cut, int bins) {
+  return size_t(cut.groups) * table_stride(bins) * 4;
 }
 
 // One pass over several tiles: n elements of src by digit dg into sink. table:
-// id_sort_table_bytes(n, dg.bins) bytes, groups: id_sort_group_bytes() cleared
-// ones for this pass alone. `clear` is done by the first launch.
+// id_sort_table_bytes() of id_cut(n) and dg.bins, groups: id_sort_group_bytes()
+// cleared ones for this pass alone. `clear` is done by the first launch.
 template <typename Source, typename Sink>
 int id_sort_pass(const Source& src, const Sink& sink, uint32_t n, const Digit& dg, void* table,
                  void* groups, const ClearOnTheWay& clear, hipStream_t stream) {

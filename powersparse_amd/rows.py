@@ -199,7 +199,8 @@ def EmbeddingLookup(table, ids, out, scale=1.0, stream=None):
 
 
 def embedding_grad_workspace_bytes(count, cols, table_rows):
-    """Workspace of EmbeddingGrad for `count` ids, rows of `cols` and a table of `table_rows`."""
+    """Workspace of EmbeddingGrad for `count` ids, rows of `cols` and a table of `table_rows`,
+    or for fewer of any of them."""
     n = _hip.ps_embedding_grad_workspace_bytes(int(count), int(cols), int(table_rows))
     if not n:
         raise ValueError("embedding_grad_workspace_bytes: sizes out of range")
@@ -220,7 +221,8 @@ def EmbeddingGrad(ids, grad_out, grad_table, workspace, scale=1.0, padding_idx=-
 # ----------------------------------------------------------------- experts
 
 def expert_sort_workspace_bytes(slots, experts):
-    """Workspace of ExpertSort for `slots` ids (tokens * top_k) and `experts` experts."""
+    """Workspace of ExpertSort for `slots` ids (tokens * top_k) and `experts` experts, or for
+    fewer of either."""
     n = _hip.ps_expert_sort_workspace_bytes(int(slots), int(experts))
     if not n:
         raise ValueError("expert_sort_workspace_bytes: sizes out of range (1 to 1024 experts)")

@@ -286,3 +286,23 @@ def test_in_a_graph():
         step()
         torch.cuda.synchronize()
         assert torch.equal(replayed[0], out) and torch.equal(replayed[1], grad)
+
+
+@pytest.mark.parametrize("most,counts,cols,rows", [
+    (16392, (16384, 8191, 1), 1024, 50000),  # chunks of twice the entries
+    (196616, (196608, 65537), 8, 1024),      # tiles of twice the items, two digits
+    (196616, (196608, 196600), 8, 1023),
+    (4194400, (4194304, 800000), 1, 3000)])  # no groups of tiles any more
+def test_grad_in_a_workspace_for_more(most, counts, cols, rows):
+    gen = generator("workspace", most, rows)
+    work = torch.full((ps.embedding_grad_workspace_bytes(most, cols, rows),), 255,
+                      dtype=torch.uint8, device="cuda")
+    for count in counts:
+        say(f"grad of {count} ids in a workspace for {most}")
+        ids = torch.randint(-1, rows, (count,), generator=gen)
+        dy, _ = values(gen, count, cols, torch.float32)
+        grad = torch.full((rows, cols), float("nan"), device="cuda")
+        ps.EmbeddingGrad(ids.cuda(), dy, grad, work)
+        torch.cuda.synchronize()
+        exact, mag, times = ref.lookup_grad(ids, dy, rows, 1.0)
+        ref.close(grad, exact, mag, times + 2, "gradient")

@@ -286,3 +286,19 @@ def test_in_a_graph():
         step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(replayed, outs))
+
+
+@pytest.mark.parametrize("experts", [5, 1024])
+def test_sort_in_a_workspace_for_more(experts):
+    gen = generator("workspace", experts)
+    for most, count in ((196616, 196608), (4194400, 4194304), (4194400, 8193)):
+        say(f"sort of {count} slots in a workspace for {most}, {experts} experts")
+        work = torch.full((ps.expert_sort_workspace_bytes(most, experts),), 255,
+                          dtype=torch.uint8, device="cuda")
+        ids = torch.randint(-1, experts + 1, (count,), generator=gen)
+        order, position = (torch.empty(count, dtype=torch.int32, device="cuda") for _ in range(2))
+        offsets = torch.empty(experts + 1, dtype=torch.int32, device="cuda")
+        ps.ExpertSort(ids.cuda(), order, position, offsets, work)
+        key = torch.where((ids >= 0) & (ids < experts), ids, experts)
+        assert torch.equal(order.cpu().long(), torch.sort(key, stable=True).indices)
+        assert int(offsets[-1]) == int((key < experts).sum())

@@ -190,3 +190,35 @@ def test_c_abi():
     for t, i, o in bad:
         assert hip.ps_embedding_lookup(t, i, 1.0, o, None) == _native.PS_ERR_INVALID
         assert _native.hip().ps_last_error()
+
+
+# where the sorts' tiles and digits and the gradient's chunks change
+COUNTS = sorted({n + d for n in [1, 16, 1024, 4096, 65536, 1 << 30] +
+                 [4 * 4096 << k for k in range(8)] + [192 * 1024 << k for k in range(4)] +
+                 [1024 * 4096] for d in (-8, -1, 0, 1, 8) if 0 <= n + d <= 1 << 30})
+COLS = [1, 4, 7, 8, 9, 64, 336, 1023, 1024, 4096, 8191, 1 << 20, 1 << 24]
+ROWS = sorted({r + d for r in (0, 2, 511, 1023, 1 << 17, 1 << 20, 1 << 25, (1 << 31) - 3)
+               for d in (0, 1)})
+EXPERTS = [1, 2, 3, 4, 63, 64, 511, 1023, 1024]
+
+
+def never_less(size, *axes):
+    """size() never shrinks along any axis: neighbours on the grid are enough."""
+    def walk(fixed, rest):
+        if rest:
+            for v in rest[0]:
+                yield from walk(fixed + (v,), rest[1:])
+        else:
+            yield fixed
+    for place, axis in enumerate(axes):
+        others = axes[:place] + axes[place + 1:]
+        for fixed in walk((), others):
+            sizes = [size(*fixed[:place], v, *fixed[place:]) for v in axis]
+            for k in range(1, len(axis)):
+                assert sizes[k] >= sizes[k - 1], (place, fixed, axis[k - 1:k + 1],
+                                                  sizes[k - 1:k + 1])
+
+
+def test_a_workspace_for_the_largest_call_does_for_smaller_ones():
+    never_less(ps.embedding_grad_workspace_bytes, COUNTS, COLS, ROWS)
+    never_less(ps.expert_sort_workspace_bytes, COUNTS, EXPERTS)
