@@ -10,7 +10,8 @@
  * keeps anything between calls. Workspaces are the caller's, of the stated
  * size or more, aligned to 16 bytes, not shared by calls that may overlap. The
  * stated sizes grow with every argument, so a workspace for the largest call
- * does for smaller ones.
+ * does for smaller ones. What a call writes (outputs, workspace) shares no byte
+ * with anything else it is given; PS_ERR_INVALID otherwise.
  *
  * Data may hold any value: ids and positions out of range are dropped where
  * the text says so and never followed. Sums run in 32 bits in a fixed order (the

@@ -472,7 +472,8 @@ int ps_embedding_lookup(const ps_rows* table, const ps_ids* ids, float scale, co
   PS_CHECK_ROWS(out);
   PS_CHECK_ARG(table->cols == out->cols && out->rows == ids->count,
                "ps_embedding_lookup: out is not ids x table columns");
-  PS_CHECK_ARG(!ps::overlap(table, out), "ps_embedding_lookup: table and out overlap");
+  PS_CHECK_ARG(!ps::overlap(ps::region(out), {ps::region(table), ps::region(ids)}),
+               "ps_embedding_lookup: out overlaps an input");
   if (!ids->count) return PS_OK;
   const hipStream_t st = ps::to_hip(stream);
   return ps::with_dtype(table->dtype, [&](auto t) {
@@ -517,11 +518,15 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
   PS_CHECK_ARG(grad_out->cols == grad->cols && grad_out->rows == ids->count,
                "ps_embedding_grad: grad_out is not ids x grad columns");
   PS_CHECK_ARG(grad->rows <= (1LL << 31) - 2, "ps_embedding_grad: too many rows");
-  PS_CHECK_ARG(!ps::overlap(grad_out, grad), "ps_embedding_grad: grad_out and grad overlap");
   PS_CHECK_ARG(workspace && ps::aligned16(workspace) &&
                    workspace_bytes >= ps::grad_space_most(ids->count, grad->cols, grad->rows),
                "ps_embedding_grad: workspace too small or misaligned");
   const ps::GradSpace s = ps::grad_space(ids->count, grad->cols, grad->rows);
+  const ps::Region read[] = {ps::region(ids), ps::region(grad_out)};
+  PS_CHECK_ARG(!ps::overlap(ps::region(grad), {read[0], read[1]}),
+               "ps_embedding_grad: grad overlaps an input");
+  PS_CHECK_ARG(!ps::overlap(ps::region(workspace, s.total), {read[0], read[1], ps::region(grad)}),
+               "ps_embedding_grad: the workspace overlaps another argument");
   if (!grad->rows || (!ids->count && accumulate)) return PS_OK;
   const hipStream_t st = ps::to_hip(stream);
   char* ws = static_cast<char*>(workspace);

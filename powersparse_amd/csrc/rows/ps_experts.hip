@@ -160,6 +160,16 @@ __global__ __launch_bounds__(kRowThreads) void combine_grad_kernel(
   }
 }
 
+// The sort's workspace: the groups' counts, then the table.
+size_t sort_bytes(const IdCut& cut, int experts) {
+  return id_sort_group_bytes(cut, experts + 1) + id_sort_table_bytes(cut, experts + 1);
+}
+
+// What a value of four bytes for each slot of the tokens of m takes.
+Region slots(const void* p, const ps_rows* m, int top_k) {
+  return region(p, size_t(m->rows) * size_t(top_k) * 4);
+}
+
 // Calls f(lanes) with the threads a token's row gets: its pieces, one each up
 // to 64, or a workgroup from 256 pieces on. Gradients of the combination, us:
 // 16,384 x 4 x 2,048 BF16 134 with 64 lanes, 119 with 256; 256 x 8 x 4,096 18.3
@@ -183,8 +193,7 @@ extern "C" {
 
 size_t ps_expert_sort_workspace_bytes(long long slots, int experts) {
   if (slots < 0 || slots > (1LL << 30) || experts < 1 || experts > 1024) return 0;
-  const ps::IdCut most = ps::id_cut_most(slots);
-  return ps::id_sort_group_bytes(most, experts + 1) + ps::id_sort_table_bytes(most, experts + 1);
+  return ps::sort_bytes(ps::id_cut_most(slots), experts);
 }
 
 int ps_expert_sort(const ps_ids* ids, int experts, int* order, int* position, int* offsets,
@@ -195,6 +204,16 @@ int ps_expert_sort(const ps_ids* ids, int experts, int* order, int* position, in
   PS_CHECK_ARG(workspace && ps::aligned16(workspace) &&
                    workspace_bytes >= ps_expert_sort_workspace_bytes(ids->count, experts),
                "ps_expert_sort: workspace too small or misaligned");
+  const size_t slots = size_t(ids->count) * sizeof(int);
+  const ps::Region in = ps::region(ids);
+  const ps::Region to[] = {
+      ps::region(order, slots), ps::region(position, slots),
+      ps::region(offsets, (size_t(experts) + 1) * sizeof(int)),
+      ps::region(workspace, ps::sort_bytes(ps::id_cut(ids->count), experts))};
+  PS_CHECK_ARG(!ps::overlap(to[0], {in, to[1], to[2], to[3]}) &&
+                   !ps::overlap(to[1], {in, to[2], to[3]}) && !ps::overlap(to[2], {in, to[3]}) &&
+                   !ps::overlap(to[3], in),
+               "ps_expert_sort: ids, outputs and workspace overlap");
   const ps::ExpertSink sink{order, position, offsets, uint32_t(experts)};
   ps::Digit dg{0, 1, experts + 1};
   while ((1 << dg.bits) < dg.bins) ++dg.bits;
@@ -224,7 +243,8 @@ int ps_expert_dispatch(const ps_rows* x, const int* position, int top_k, const p
                "ps_expert_dispatch: x and xs differ in type or width");
   PS_CHECK_ARG(top_k >= 1 && top_k <= 1024, "ps_expert_dispatch: 1 to 1024 slots per token");
   PS_CHECK_ARG(position || !x->rows, "ps_expert_dispatch: null positions");
-  PS_CHECK_ARG(!ps::overlap(x, xs), "ps_expert_dispatch: x and xs overlap");
+  PS_CHECK_ARG(!ps::overlap(ps::region(xs), {ps::region(x), ps::slots(position, x, top_k)}),
+               "ps_expert_dispatch: xs overlaps an input");
   if (!x->rows || !xs->rows) return PS_OK;
   return ps::with_dtype(x->dtype, [&](auto t) {
     using T = decltype(t);
@@ -250,7 +270,9 @@ int ps_expert_combine(const ps_rows* ys, const int* position, const float* weigh
                "ps_expert_combine: ys and y differ in type or width");
   PS_CHECK_ARG(top_k >= 1 && top_k <= 1024, "ps_expert_combine: 1 to 1024 slots per token");
   PS_CHECK_ARG(position || !y->rows, "ps_expert_combine: null positions");
-  PS_CHECK_ARG(!ps::overlap(ys, y), "ps_expert_combine: ys and y overlap");
+  PS_CHECK_ARG(!ps::overlap(ps::region(y), {ps::region(ys), ps::slots(position, y, top_k),
+                                            ps::slots(weights, y, top_k)}),
+               "ps_expert_combine: y overlaps an input");
   if (!y->rows) return PS_OK;
   return ps::with_dtype(y->dtype, [&](auto t) {
     using T = decltype(t);
@@ -280,8 +302,13 @@ int ps_expert_combine_grad(const ps_rows* dy, const ps_rows* ys, const int* posi
   PS_CHECK_ARG(top_k >= 1 && top_k <= 1024, "ps_expert_combine_grad: 1 to 1024 slots per token");
   PS_CHECK_ARG((position && weights && dweights) || !dy->rows,
                "ps_expert_combine_grad: null positions or weights");
-  PS_CHECK_ARG(!ps::overlap(dy, dys) && !ps::overlap(ys, dys),
+  const ps::Region in[] = {ps::region(dy), ps::region(ys), ps::slots(position, dy, top_k),
+                           ps::slots(weights, dy, top_k)};
+  PS_CHECK_ARG(!ps::overlap(ps::region(dys), {in[0], in[1], in[2], in[3]}),
                "ps_expert_combine_grad: dys overlaps an input");
+  PS_CHECK_ARG(!ps::overlap(ps::slots(dweights, dy, top_k),
+                            {in[0], in[1], in[2], in[3], ps::region(dys)}),
+               "ps_expert_combine_grad: dweights overlaps another argument");
   if (!dy->rows) return PS_OK;
   return ps::with_dtype(dy->dtype, [&](auto t) {
     using T = decltype(t);

@@ -272,8 +272,8 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
                        reinterpret_cast<uintptr_t>(to) % out_size == 0,
                    name + ": misaligned data");
       PS_CHECK_ARG((to == data[i] && out_dtype == dtypes[i]) ||
-                       !ps::overlap(data[i], size_t(counts[i]) * size, to,
-                                    size_t(counts[i]) * out_size),
+                       !ps::overlap(ps::region(data[i], size_t(counts[i]) * size),
+                                    ps::region(to, size_t(counts[i]) * out_size)),
                    name + ": overlaps its output");
       table.push_back({data[i], to, counts[i], dtypes[i], out_dtype, chunks});
       total += counts[i];

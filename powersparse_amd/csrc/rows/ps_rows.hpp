@@ -11,6 +11,8 @@
 // accesses of any width allow.
 #pragma once
 
+#include <initializer_list>
+
 #include "powersparse_rows.h"
 #include "ps_common.hpp"
 
@@ -155,28 +157,40 @@ inline const char* ids_error(const ps_ids* ids) {
       return ps::fail(PS_ERR_INVALID, std::string(__func__) + ": " #ids ": " + ps_error_);     \
   } while (0)
 
-inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+// Device memory that a call reads or writes: rows of `bytes`, `pitch` apart.
+struct Region {
+  uintptr_t at;
+  size_t rows, bytes, pitch;
+  size_t span() const { return rows ? (rows - 1) * pitch + bytes : 0; }
+};
+inline Region region(const ps_rows* m) {
+  const size_t size = dtype_size(m->dtype);
+  return {reinterpret_cast<uintptr_t>(m->data), size_t(m->rows), size_t(m->cols) * size,
+          size_t(m->ld) * size};
 }
-inline size_t rows_bytes(const ps_rows* m) {
-  return m->rows ? (size_t(m->rows - 1) * size_t(m->ld) + size_t(m->cols)) * dtype_size(m->dtype)
-                 : 0;
+inline Region region(const void* p, size_t bytes) {
+  return {reinterpret_cast<uintptr_t>(p), p && bytes ? size_t(1) : 0, bytes, bytes};
 }
-// Column ranges of one wider matrix share its memory range and no element.
-inline bool overlap(const ps_rows* a, const ps_rows* b) {
-  if (!overlap(a->data, rows_bytes(a), b->data, rows_bytes(b))) return false;
-  const size_t pitch_a = size_t(a->ld) * dtype_size(a->dtype);
-  const size_t pitch_b = size_t(b->ld) * dtype_size(b->dtype);
+inline Region region(const ps_ids* ids) {
+  return region(ids->data, size_t(ids->count) * (ids->type == PS_I64 ? 8 : 4));
+}
+// Column ranges of one wider matrix share its memory range and no byte.
+inline bool overlap(const Region& a, const Region& b) {
+  if (!a.span() || !b.span() || a.at >= b.at + b.span() || b.at >= a.at + a.span()) return false;
   // a single row's stride says nothing
-  const size_t pitch = a->rows == 1 ? pitch_b : pitch_a;
-  if ((a->rows > 1 && b->rows > 1 && pitch_a != pitch_b) || (a->rows == 1 && b->rows == 1))
-    return true;
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a->data);
-  const uintptr_t y = reinterpret_cast<uintptr_t>(b->data);
-  const size_t apart = x <= y ? (y - x) % pitch : (pitch - (x - y) % pitch) % pitch;
-  return apart < size_t(a->cols) * dtype_size(a->dtype) ||
-         apart + size_t(b->cols) * dtype_size(b->dtype) > pitch;
+  const size_t pitch = a.rows == 1 ? b.pitch : a.pitch;
+  if ((a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) || (a.rows == 1 && b.rows == 1)) return true;
+  const size_t apart =
+      a.at <= b.at ? (b.at - a.at) % pitch : (pitch - (a.at - b.at) % pitch) % pitch;
+  return apart < a.bytes || apart + b.bytes > pitch;
+}
+// Whether something written meets anything else of the call. Places to write are
+// taken from ids, counts and positions: what changed them under a kernel would
+// send it anywhere.
+inline bool overlap(const Region& written, std::initializer_list<Region> others) {
+  for (const Region& o : others)
+    if (overlap(written, o)) return true;
+  return false;
 }
 
 template <typename T>
@@ -203,7 +217,7 @@ inline int with_dtype(int dtype, F&& f) {
 // in the last-level cache (65,536 x 4 x 333 FP16 131 -> 137), and gains for such
 // rows that would not (32,768 x 8 x 333 FP32 215 -> 208).
 constexpr size_t kStreamBytes = size_t(32) << 20;
-inline bool streamed(const ps_rows* out) { return rows_bytes(out) >= kStreamBytes; }
+inline bool streamed(const ps_rows* out) { return region(out).span() >= kStreamBytes; }
 
 // Calls f(flag) with a runtime flag as a constant.
 template <typename F>

@@ -302,3 +302,16 @@ def test_sort_in_a_workspace_for_more(experts):
         key = torch.where((ids >= 0) & (ids < experts), ids, experts)
         assert torch.equal(order.cpu().long(), torch.sort(key, stable=True).indices)
         assert int(offsets[-1]) == int((key < experts).sum())
+
+
+def test_positions_between_the_rows_of_the_output():
+    """Columns that a matrix leaves out of its buffer are nobody's: positions may be there."""
+    gen = generator("between")
+    whole = torch.zeros((20, 33), device="cuda")
+    x, xs = torch.randn((9, 24), generator=gen).cuda(), whole[:, :24]
+    position = whole.view(torch.int32)[7, 24:33]
+    position.copy_(torch.randperm(20, generator=gen)[:9].to(torch.int32))
+    where = position.long()
+    ps.ExpertDispatch(x, position, xs)
+    assert torch.equal(xs[where], x) and torch.equal(position.long(), where)
+    assert int(torch.count_nonzero(xs.any(1))) == 9

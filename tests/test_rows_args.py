@@ -222,3 +222,56 @@ def never_less(size, *axes):
 def test_a_workspace_for_the_largest_call_does_for_smaller_ones():
     never_less(ps.embedding_grad_workspace_bytes, COUNTS, COLS, ROWS)
     never_less(ps.expert_sort_workspace_bytes, COUNTS, EXPERTS)
+
+
+def test_what_is_written_overlaps_nothing_else():
+    """Kernels take the places that they write from ids and workspaces, so nothing written may
+    be anything else that the call reads or writes, by a single byte."""
+    def work_bytes(n):
+        return vec(D, n, "uint8")
+
+    table, ids, out = mat(A, 9, 8), vec(B, 40, "int64"), mat(C, 40, 8)
+    at_end = C + 40 * 8 * 4
+    refused("overlap", ps.EmbeddingLookup, table, vec(C, 40, "int64"), out)
+    refused("overlap", ps.EmbeddingLookup, table, vec(at_end - 8, 40, "int64"), out)
+    refused("overlap", ps.EmbeddingLookup, table, vec(C - 40 * 8 + 8, 40, "int64"), out)
+
+    n = ps.embedding_grad_workspace_bytes(40, 8, 9)
+    work, grad, dy = work_bytes(n), mat(A, 9, 8), mat(C, 40, 8)
+    refused("overlap", ps.EmbeddingGrad, vec(A, 40, "int64"), dy, grad, work)
+    for at in (A, B, C):  # the workspace on the gradient, the ids, the rows
+        refused("overlap", ps.EmbeddingGrad, ids, dy, grad, vec(at, n, "uint8"))
+    refused("overlap", ps.EmbeddingGrad, ids, dy, grad, vec(at_end - 16, n, "uint8"))
+
+    n = ps.expert_sort_workspace_bytes(40, 5)
+    order, position, offsets = vec(B, 40, "int32"), vec(C, 40, "int32"), vec(A + 4096, 6, "int32")
+    ids, work = vec(A, 40, "int32"), work_bytes(n)
+    whole = [ids, order, position, offsets, work]
+    for i in range(5):
+        for j in range(5):
+            if i != j:
+                moved = list(whole)
+                was = whole[i]
+                moved[i] = vec(whole[j].ptr, was.shape[0], was.dtype)
+                refused("overlap", ps.ExpertSort, *moved)
+
+    x, xs, at = mat(A, 20, 8), mat(B, 40, 8), mat(C, 20, 2, "int32")
+    w, dw = mat(C + 4096, 20, 2), mat(C + 8192, 20, 2)
+    refused("overlap", ps.ExpertDispatch, x, mat(B + 36, 20, 2, "int32"), xs)
+    refused("overlap", ps.ExpertCombine, xs, mat(A + 36, 20, 2, "int32"), w, x)
+    refused("overlap", ps.ExpertCombine, xs, at, mat(A + 36, 20, 2), x)
+    dys = mat(D, 40, 8)
+    for f, where in ((0, "position"), (1, "weights"), (2, "dweights")):
+        args = [x, xs, at, w, dys, dw]
+        args[(2, 3, 5)[f]] = mat(D + 36, 20, 2, "int32" if f == 0 else "float32")
+        refused("overlap", ps.ExpertCombineGrad, *args)
+    for taken in (A, B, C, C + 4096):  # dy, ys, positions, weights
+        refused("overlap", ps.ExpertCombineGrad, x, xs, at, w, dys, mat(taken, 20, 2))
+
+
+def test_flat_arrays_that_reach_from_between_rows_into_them():
+    """Columns 24 to 31 of a matrix's rows are not its own: positions there are refused from
+    the first column that is."""
+    for first in (23, 25, 31):
+        refused("overlap", ps.ExpertDispatch, mat(A, 8, 24),
+                mat(B + 4 * first, 8, 1, "int32"), mat(B, 20, 24, ld=32))
