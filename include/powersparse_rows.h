@@ -102,9 +102,10 @@ int ps_expert_combine_grad(const ps_rows* dy, const ps_rows* ys, const int* posi
 
 /* The gradient tensors of a model: data[i] holds counts[i] contiguous elements
  * of dtypes[i]. out (NULL: in place) and out_dtypes name where the clipped
- * gradients go; nothing that is written may overlap another tensor. Uploads a
- * table and synchronises; owns it and what the calls below work in (8 bytes for
- * 4096 elements): calls on one list must not overlap. */
+ * gradients go; nothing that is written may overlap another tensor, no norm may
+ * lie in an output, and none be written into a gradient (PS_ERR_INVALID).
+ * Uploads a table and synchronises; owns it and what the calls below work in (8
+ * bytes for 4096 elements): calls on one list must not overlap. */
 typedef struct ps_grad_list ps_grad_list;
 int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
                         const int* dtypes, void* const* out, const int* out_dtypes,

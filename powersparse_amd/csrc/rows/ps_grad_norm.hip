@@ -13,6 +13,7 @@
 // backwards, so what the first one read last may still be in the last-level
 // cache.
 #include <algorithm>
+#include <utility>
 #include <vector>
 
 #include "ps_rows.hpp"
@@ -178,11 +179,51 @@ __global__ __launch_bounds__(kClipThreads) void clip_kernel(Grads g,
 }  // namespace
 }  // namespace ps
 
+namespace ps {
+namespace {
+
+// Where a list's gradients, or its outputs, are: ranges that do not meet, in order.
+class Ranges {
+ public:
+  void add(const void* p, size_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    ranges_.push_back({at, at + bytes});
+  }
+  void close() {
+    std::sort(ranges_.begin(), ranges_.end(),
+              [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    size_t kept = 0;
+    for (const Range& r : ranges_) {
+      if (kept && r.begin <= ranges_[kept - 1].end)
+        ranges_[kept - 1].end = std::max(ranges_[kept - 1].end, r.end);
+      else
+        ranges_[kept++] = r;
+    }
+    ranges_.resize(kept);
+  }
+  bool meets(const void* p, size_t bytes) const {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const auto r = std::upper_bound(ranges_.begin(), ranges_.end(), at,
+                                    [](uintptr_t x, const Range& range) { return x < range.end; });
+    return r != ranges_.end() && r->begin < at + bytes;
+  }
+
+ private:
+  struct Range {
+    uintptr_t begin, end;
+  };
+  std::vector<Range> ranges_;
+};
+
+}  // namespace
+}  // namespace ps
+
 struct ps_grad_list {
   void* tables = nullptr;  // tensors, chunks, the workgroups' sums
   ps::Grads grads{};
   double* sums = nullptr;
   uint32_t blocks = 0;
+  ps::Ranges read, written;
 };
 
 namespace ps {
@@ -255,6 +296,7 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
                "ps_grad_list_create: null array");
   try {
     std::vector<ps::GradTensor> table;
+    ps::Ranges read, written;
     long long total = 0, chunks = 0;
     bool in_place = true;
     for (int i = 0; i < tensors; ++i) {
@@ -276,6 +318,8 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
                                     ps::region(to, size_t(counts[i]) * out_size)),
                    name + ": overlaps its output");
       table.push_back({data[i], to, counts[i], dtypes[i], out_dtype, chunks});
+      read.add(data[i], size_t(counts[i]) * size);
+      written.add(to, size_t(counts[i]) * out_size);
       total += counts[i];
       chunks += (counts[i] + ps::kChunk - 1) / ps::kChunk;
       in_place = in_place && to == data[i];
@@ -284,6 +328,8 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
     PS_CHECK_ARG(ps::shared_output(table) < 0,
                  "ps_grad_list_create: an output overlaps another tensor, or a tensor is "
                  "listed twice");
+    read.close();
+    written.close();
     const size_t table_bytes = (table.size() * sizeof(ps::GradTensor) + 255) & ~size_t(255);
     const size_t chunk_bytes = (size_t(chunks) * sizeof(ps::GradChunk) + 255) & ~size_t(255);
     void* base = nullptr;
@@ -309,6 +355,8 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
     l->grads.in_place = in_place;
     l->sums = reinterpret_cast<double*>(at + table_bytes + chunk_bytes);
     l->blocks = std::min(uint32_t(chunks), ps::kBlocks);
+    l->read = std::move(read);
+    l->written = std::move(written);
     *list = l;
     return PS_OK;
   } catch (const std::exception& e) {
@@ -324,6 +372,8 @@ void ps_grad_list_destroy(ps_grad_list* list) {
 
 int ps_grad_norm(ps_grad_list* list, float grad_scale, float* norm, ps_stream_t stream) {
   PS_CHECK_ARG(list && norm, "ps_grad_norm: null argument");
+  PS_CHECK_ARG(!list->read.meets(norm, sizeof(float)),
+               "ps_grad_norm: the norm lies in a gradient");
   const hipStream_t st = ps::to_hip(stream);
   const int rc = ps::launch_norm(*list, st);
   if (rc != PS_OK) return rc;
@@ -336,6 +386,8 @@ int ps_grad_norm(ps_grad_list* list, float grad_scale, float* norm, ps_stream_t 
 int ps_clip_grads(ps_grad_list* list, float max_norm, float grad_scale, const float* norm,
                   ps_stream_t stream) {
   PS_CHECK_ARG(list && norm, "ps_clip_grads: null argument");
+  PS_CHECK_ARG(!list->written.meets(norm, sizeof(float)),
+               "ps_clip_grads: the norm lies in an output");
   PS_CHECK_ARG(max_norm >= 0.f, "ps_clip_grads: the bound is not a number from 0 up");
   if (!list->blocks) return PS_OK;
   return ps::launch_clip(*list, list->blocks, nullptr, max_norm, grad_scale,
@@ -345,6 +397,9 @@ int ps_clip_grads(ps_grad_list* list, float max_norm, float grad_scale, const fl
 int ps_clip_grad_norm(ps_grad_list* list, float max_norm, float grad_scale, float* norm,
                       ps_stream_t stream) {
   PS_CHECK_ARG(list && norm, "ps_clip_grad_norm: null argument");
+  PS_CHECK_ARG(!list->read.meets(norm, sizeof(float)) &&
+                   !list->written.meets(norm, sizeof(float)),
+               "ps_clip_grad_norm: the norm lies in a gradient or an output");
   PS_CHECK_ARG(max_norm >= 0.f, "ps_clip_grad_norm: the bound is not a number from 0 up");
   const hipStream_t st = ps::to_hip(stream);
   const int rc = ps::launch_norm(*list, st);

@@ -201,3 +201,39 @@ def test_in_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(replayed[0], norm)
         assert all(torch.equal(a, b) for a, b in zip(replayed[1:], outs))
+
+
+def test_a_norm_in_a_gradient_is_refused():
+    """Workgroups read the gradients while one writes the norm, and read the norm while they
+    write the outputs."""
+    whole = torch.ones(3000, device="cuda")
+    grads = [whole[2000:3000], whole[:1000], whole[1000:1500]]  # two of them side by side
+    outs = [torch.ones(g.numel() * 2, device="cuda")[:g.numel()] for g in grads]
+    apart = torch.zeros(4, device="cuda")
+    for glist, in_place in ((ps.GradientList(grads), True), (ps.GradientList(grads, outs), False)):
+        for at in (0, 999, 1000, 1499, 2000, 2999):
+            with pytest.raises(ValueError, match="norm lies in"):
+                ps.GradNorm(glist, whole[at:at + 1])
+            with pytest.raises(ValueError, match="norm lies in"):
+                ps.ClipGradNorm(glist, 1.0, whole[at:at + 1])
+            if in_place:
+                with pytest.raises(ValueError, match="norm lies in"):
+                    ps.ClipGrads(glist, 1.0, whole[at:at + 1])
+            else:  # it is only read there, and the outputs are elsewhere
+                ps.ClipGrads(glist, 1.0, whole[at:at + 1])
+        if not in_place:
+            for at in (0, 999):
+                with pytest.raises(ValueError, match="norm lies in"):
+                    ps.ClipGrads(glist, 1.0, outs[0][at:at + 1])
+                with pytest.raises(ValueError, match="norm lies in"):
+                    ps.ClipGradNorm(glist, 1.0, outs[0][at:at + 1])
+        assert bool((whole == 1).all())
+        for norm in (whole[1500:1501], whole[1999:2000], apart[1:2]):  # between them, and apart
+            norm.zero_()
+            ps.GradNorm(glist, norm)
+            assert float(norm) == 50.0
+            ps.ClipGrads(glist, 100.0, norm)
+            ps.ClipGradNorm(glist, 100.0, norm)
+            assert float(norm) == 50.0
+            norm.fill_(1.0)
+    assert bool((whole == 1).all()) and all(bool((o == 1).all()) for o in outs)
