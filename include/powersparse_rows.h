@@ -123,8 +123,8 @@ int ps_grad_norm(ps_grad_list* list, float grad_scale, float* norm, ps_stream_t 
 int ps_clip_grads(ps_grad_list* list, float max_norm, float grad_scale, const float* norm,
                   ps_stream_t stream);
 
-/* ps_grad_norm and ps_clip_grads in two launches; *norm receives the norm
- * before clipping. */
+/* ps_grad_norm and ps_clip_grads in two launches, bit for bit: *norm receives the
+ * norm before clipping, and that FP32 value is clipped by. */
 int ps_clip_grad_norm(ps_grad_list* list, float max_norm, float grad_scale, float* norm,
                       ps_stream_t stream);
 

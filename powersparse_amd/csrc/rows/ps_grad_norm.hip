@@ -152,13 +152,14 @@ __global__ __launch_bounds__(kClipThreads) void clip_kernel(Grads g,
                                                             uint32_t sum_count, double max_norm,
                                                             double grad_scale,
                                                             float* __restrict__ norm) {
-  double v;
+  float n;  // in 32 bits either way, so that one call clips as two do
   if (sums) {
-    v = norm_of(sums, sum_count, grad_scale);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = float(v);
+    n = float(norm_of(sums, sum_count, grad_scale));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
   } else {
-    v = double(*norm);
+    n = *norm;
   }
+  const double v = n;
   const double ratio = max_norm / (v + 1e-6);
   const float c = float((ratio > 1.0 ? 1.0 : ratio) * grad_scale);  // a NaN ratio stays
   if (g.in_place && c == 1.f) return;

@@ -237,3 +237,31 @@ def test_a_norm_in_a_gradient_is_refused():
             assert float(norm) == 50.0
             norm.fill_(1.0)
     assert bool((whole == 1).all()) and all(bool((o == 1).all()) for o in outs)
+
+
+@pytest.mark.parametrize("norm_near", [1e-42, 1e-6, 1.0, 3.0, 1e30, 3.4028234e38, 1e40])
+def test_one_call_clips_as_two_do(norm_near):
+    """ClipGradNorm = GradNorm, then ClipGrads: the same bits, up to norms beyond FP32, where
+    both give zeros, as for an infinite one."""
+    gen = generator("two calls", norm_near)
+    n = 40000
+    g = torch.rand(n, generator=gen, dtype=torch.float64) + 0.5
+    g = (g * (norm_near / float(g.square().sum().sqrt()))).float().cuda()
+    whole = norm_of([g])
+    for dtype, ratio, scale in ((torch.float32, 3.0, 1.0), (torch.float32, 1.0000001, 0.7),
+                                (torch.bfloat16, 7.0, 0.3)):
+        max_norm = min(whole * scale / ratio, 3e38)
+        one, two = (torch.full((n,), 7.0, dtype=dtype, device="cuda") for _ in range(2))
+        norm, again = torch.empty(1, device="cuda"), torch.empty(1, device="cuda")
+        ps.ClipGradNorm(ps.GradientList([g], [one]), max_norm, norm, grad_scale=scale)
+        glist = ps.GradientList([g], [two])
+        ps.GradNorm(glist, again, grad_scale=scale)
+        ps.ClipGrads(glist, max_norm, again, grad_scale=scale)
+        assert torch.equal(norm, again) and torch.equal(one, two)
+        exact = whole * scale
+        if exact > torch.finfo(torch.float32).max:
+            assert float(norm) == math.inf and bool((one == 0).all())
+        else:
+            c = min(1.0, max_norm / (float(norm) + 1e-6)) * scale
+            e = g.cpu().double() * c
+            ref.close(one, e, e.abs() + c * 2.0 ** -149, 3, "clip")
