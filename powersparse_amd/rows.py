@@ -127,10 +127,8 @@ def _contiguous(shape, stride, name):
     return n
 
 
-def _flat(x, name, dtypes, count=None, optional=False):
+def _flat(x, name, dtypes, count=None):
     """Address, element count and dtype name of a contiguous array of any shape."""
-    if x is None and optional:
-        return None, 0, None
     try:
         if x.is_cuda and x.is_contiguous() and _names[x.dtype] in dtypes:
             n = x.numel()
@@ -243,19 +241,45 @@ def ExpertSort(ids, order, position, offsets, workspace, stream=None):
         _stream(stream)))
 
 
-def _top_k(position, tokens):
-    """Address of the positions and slots per token."""
-    ptr, n, _ = _flat(position, "position", ("int32",))
+def _slots(x, name, dtype, tokens, count=None):
+    """Address of a value per slot, `count` of them, and slots per token. The leading
+    dimensions of its shape hold the tokens, unless it has one dimension only: an array of as
+    many elements for other tokens would be read across them."""
+    try:
+        if x.is_cuda and x.is_contiguous():
+            rows, top_k = x.shape
+            if rows == tokens and _names[x.dtype] == dtype and \
+                    count in (None, rows * top_k) and rows * top_k:
+                return x.data_ptr(), top_k
+    except (AttributeError, KeyError, TypeError, ValueError):
+        pass
+    ptr, n, _ = _flat(x, name, (dtype,), count)
     if tokens == 0:
         return ptr, 1
     if n == 0 or n % tokens:
-        raise ValueError(f"position: {n} slots do not divide among {tokens} tokens")
+        raise ValueError(f"{name}: {n} slots do not divide among {tokens} tokens")
+    shape, leading = x.shape, 1
+    if len(shape) > 1:
+        for s in shape:
+            if leading >= tokens:
+                break
+            leading *= s
+        if leading != tokens:
+            raise ValueError(f"{name}: {' x '.join(str(s) for s in shape)} slots for {tokens} "
+                             "tokens")
     return ptr, n // tokens
+
+
+def _top_k(position, tokens):
+    """Address of the positions and slots per token."""
+    return _slots(position, "position", "int32", tokens)
 
 
 def ExpertDispatch(x, position, xs, stream=None):
     """xs[position[t, k]] = x[t]: every token's row to its slots' places. Rows of xs that no
-    position names are left alone, positions outside xs are skipped."""
+    position names are left alone, positions outside xs are skipped. `position` is (tokens,
+    top_k), a flat list of the same, or any shape whose leading dimensions hold the tokens;
+    weights below likewise."""
     src = _rows(x, "x")
     ptr, top_k = _top_k(position, src.rows)
     _call(_hip.ps_expert_dispatch(src, ptr, top_k, _rows(xs, "xs"), _stream(stream)))
@@ -266,7 +290,9 @@ def ExpertCombine(ys, position, weights, y, stream=None):
     positions outside ys are skipped."""
     out = _rows(y, "y")
     ptr, top_k = _top_k(position, out.rows)
-    w = _flat(weights, "weights", ("float32",), out.rows * top_k, optional=True)[0]
+    w = None
+    if weights is not None:
+        w = _slots(weights, "weights", "float32", out.rows, out.rows * top_k)[0]
     _call(_hip.ps_expert_combine(_rows(ys, "ys"), ptr, w, top_k, out, _stream(stream)))
 
 
@@ -283,8 +309,9 @@ def ExpertCombineGrad(dy, ys, position, weights, dys, dweights, stream=None):
     ptr, top_k = _top_k(position, src.rows)
     n = src.rows * top_k
     _call(_hip.ps_expert_combine_grad(
-        src, _rows(ys, "ys"), ptr, _flat(weights, "weights", ("float32",), n)[0], top_k,
-        _rows(dys, "dys"), _flat(dweights, "dweights", ("float32",), n)[0], _stream(stream)))
+        src, _rows(ys, "ys"), ptr, _slots(weights, "weights", "float32", src.rows, n)[0], top_k,
+        _rows(dys, "dys"), _slots(dweights, "dweights", "float32", src.rows, n)[0],
+        _stream(stream)))
 
 
 # --------------------------------------------------------------- gradients

@@ -275,3 +275,56 @@ def test_flat_arrays_that_reach_from_between_rows_into_them():
     for first in (23, 25, 31):
         refused("overlap", ps.ExpertDispatch, mat(A, 8, 24),
                 mat(B + 4 * first, 8, 1, "int32"), mat(B, 20, 24, ld=32))
+
+
+def test_slots_of_another_shape():
+    """(tokens, top_k) arrays of as many elements that belong to another number of tokens."""
+    x, xs = mat(A, 4, 8), mat(B, 16, 8)
+    w, dw = mat(C + 4096, 4, 4), mat(C + 8192, 4, 4)
+    for shape in ((8, 2), (2, 8), (16, 1), (1, 16)):
+        wrong = mat(C, *shape, "int32")
+        text = f"position: {shape[0]} x {shape[1]} slots for 4 tokens"
+        refused(text, ps.ExpertDispatch, x, wrong, xs)
+        refused(text, ps.ExpertCombine, xs, wrong, w, x)
+        refused(text, ps.ExpertDispatchGrad, xs, wrong, x)
+        refused(text, ps.ExpertCombineGrad, x, xs, wrong, w, mat(D, 16, 8), dw)
+    at = mat(C, 4, 4, "int32")
+    for shape in ((8, 2), (2, 8)):
+        other = mat(C + 4096, *shape)
+        text = f"weights: {shape[0]} x {shape[1]} slots for 4 tokens"
+        refused("^" + text, ps.ExpertCombine, xs, at, other, x)
+        refused("^" + text, ps.ExpertCombineGrad, x, xs, at, other, mat(D, 16, 8), dw)
+        refused("^d" + text, ps.ExpertCombineGrad, x, xs, at, w, mat(D, 16, 8), other)
+
+
+def test_slots_as_a_list_or_of_a_batch():
+    """One dimension, or any shape whose leading dimensions hold the tokens."""
+    class Slots:  # a tensor as far as its description goes
+        is_cuda, dtype = True, "int32"
+
+        def __init__(self, *shape):
+            self.shape = shape
+
+        def is_contiguous(self):
+            return True
+
+        def numel(self):
+            n = 1
+            for s in self.shape:
+                n *= s
+            return n
+
+        def stride(self):
+            return tuple(Slots(*self.shape[k + 1:]).numel() for k in range(len(self.shape)))
+
+        def data_ptr(self):
+            return C
+
+    from powersparse_amd import rows
+    for shape in ((16,), (4, 4), (2, 2, 4), (4, 1, 4), (1, 4, 4), (4, 4, 1), (4, 2, 2)):
+        assert rows._top_k(Slots(*shape), 4) == (C, 4)
+    assert rows._top_k(Slots(4), 4) == (C, 1) == rows._top_k(Slots(4, 1), 4)
+    assert rows._top_k(Slots(8, 1), 1) == (C, 8)  # one token: every shape is its
+    assert rows._top_k(Slots(0, 3), 0)[0] == C
+    for shape in ((2, 4, 2), (8, 2, 1), (0, 4), (4, 0), (15,), (3, 4)):
+        refused("position", rows._top_k, Slots(*shape), 4)
