@@ -4,9 +4,9 @@ and back with their gradients, and the norm and clipping of many gradient tensor
 
 Arrays are in the current device's memory: DeviceArray (a DeviceBuffer or raw pointer with
 a shape and a type) or any tensor object with data_ptr, shape, stride, dtype and is_cuda,
-such as torch's. Matrices are row-major with any row stride; element types are float32,
-float16 and bfloat16. Every call checks shapes, types and sizes on the host, enqueues its
-kernels on `stream` (a Stream, a tensor library's stream, a raw handle, or None: the null
+such as torch's; tensors that say they are on another device are refused. Matrices are
+row-major with any row stride; element types are float32, float16 and bfloat16. Every call
+checks shapes, types and sizes on the host, enqueues its kernels on `stream` (a Stream, a tensor library's stream, a raw handle, or None: the null
 stream) and returns without synchronising: arrays and workspaces must stay alive, and be
 written by nothing else, until the stream has passed the call. Wrong arguments raise
 ValueError.
@@ -186,12 +186,51 @@ def _call(status):
         _hip_call(status)
 
 
+def _count_devices():
+    from . import device_count
+    try:
+        return device_count()
+    except RuntimeError:  # none: every call fails at its launch
+        return 0
+
+
+def _current_device():
+    d = ctypes.c_int()
+    _call(_native.hip().ps_get_device(ctypes.byref(d)))
+    return d.value
+
+
+# Whether there are several devices (None: not known yet): calls then look where their arrays
+# are. With one device nothing is asked.
+_several = None
+
+
+def _check_devices(*arrays):
+    """Refuses tensors that say they are on another device than the current one, whose kernels
+    would follow their addresses."""
+    global _several
+    if _several is None:
+        _several = _count_devices() > 1
+    if not _several:
+        return
+    here = _current_device()
+    for x in arrays:
+        try:
+            at = x.get_device()
+        except AttributeError:
+            continue
+        if at >= 0 and at != here:
+            raise ValueError(f"an array is on device {at}, the current one is {here}")
+
+
 # --------------------------------------------------------------- embedding
 
 def EmbeddingLookup(table, ids, out, scale=1.0, stream=None):
     """out[i] = scale * table[ids[i]]; zeros for ids outside the table. `ids` (int32 or
     int64, any shape) are taken in order; out has one row for each. table and out may differ
     in type."""
+    if _several is not False:
+        _check_devices(table, ids, out)
     _call(_hip.ps_embedding_lookup(_rows(table, "table"), _ids(ids), scale, _rows(out, "out"),
                                    _stream(stream)))
 
@@ -210,6 +249,8 @@ def EmbeddingGrad(ids, grad_out, grad_table, workspace, scale=1.0, padding_idx=-
     """grad_table[v] = scale * sum of grad_out[i] over the i with ids[i] = v, zeros for rows
     without ids; accumulate=True adds to grad_table instead. Ids outside the table and
     `padding_idx` take no part. The sum's order is fixed: the same bits every time."""
+    if _several is not False:
+        _check_devices(ids, grad_out, grad_table, workspace)
     ptr, nbytes = _space(workspace)
     _call(_hip.ps_embedding_grad(
         _ids(ids), _rows(grad_out, "grad_out"), scale, padding_idx, bool(accumulate),
@@ -232,6 +273,8 @@ def ExpertSort(ids, order, position, offsets, workspace, stream=None):
     by expert, dropped ones (id outside the experts) last; `position` each slot's place in
     `order`, -1 for dropped ones; `offsets` (experts + 1) where each expert's slots begin.
     All int32."""
+    if _several is not False:
+        _check_devices(ids, order, position, offsets, workspace)
     slots = _ids(ids)
     at, count, _ = _flat(offsets, "offsets", ("int32",))
     ptr, nbytes = _space(workspace)
@@ -280,6 +323,8 @@ def ExpertDispatch(x, position, xs, stream=None):
     position names are left alone, positions outside xs are skipped. `position` is (tokens,
     top_k), a flat list of the same, or any shape whose leading dimensions hold the tokens;
     weights below likewise."""
+    if _several is not False:
+        _check_devices(x, position, xs)
     src = _rows(x, "x")
     ptr, top_k = _top_k(position, src.rows)
     _call(_hip.ps_expert_dispatch(src, ptr, top_k, _rows(xs, "xs"), _stream(stream)))
@@ -288,6 +333,8 @@ def ExpertDispatch(x, position, xs, stream=None):
 def ExpertCombine(ys, position, weights, y, stream=None):
     """y[t] = sum over k of weights[t, k] * ys[position[t, k]] (float32 weights; None: ones);
     positions outside ys are skipped."""
+    if _several is not False:
+        _check_devices(ys, position, weights, y)
     out = _rows(y, "y")
     ptr, top_k = _top_k(position, out.rows)
     w = None
@@ -305,6 +352,8 @@ def ExpertCombineGrad(dy, ys, position, weights, dys, dweights, stream=None):
     """The gradients of ExpertCombine: dys[position[t, k]] = weights[t, k] * dy[t] and
     dweights[t, k] = <dy[t], ys[position[t, k]]>, 0 for dropped slots. Rows of dys that no
     position names are left alone."""
+    if _several is not False:
+        _check_devices(dy, ys, position, weights, dys, dweights)
     src = _rows(dy, "dy")
     ptr, top_k = _top_k(position, src.rows)
     n = src.rows * top_k
@@ -342,6 +391,8 @@ class GradientList:
         grads, outs = self._keep
         if outs is not None and len(outs) != len(grads):
             raise ValueError("outs: one for each gradient")
+        if _several is not False:
+            _check_devices(*grads, *(outs or ()))
         n = len(grads)
         data, counts, types = _spans(grads, "gradient")
         to = to_types = None
@@ -354,6 +405,11 @@ class GradientList:
         h = ctypes.c_void_p()
         _call(_hip.ps_grad_list_create(n, data, counts, types, to, to_types, ctypes.byref(h)))
         self._h = h.value
+        self._device = _current_device()
+
+    def get_device(self):
+        """The device it was made on."""
+        return self._device
 
     @property
     def handle(self):
@@ -375,6 +431,8 @@ class GradientList:
 
 def GradNorm(grads, norm, grad_scale=1.0, stream=None):
     """norm (one float32 on the device) = the 2-norm of grad_scale * g over a GradientList."""
+    if _several is not False:
+        _check_devices(grads, norm)
     _call(_hip.ps_grad_norm(grads.handle, grad_scale, _flat(norm, "norm", ("float32",), 1)[0],
                             _stream(stream)))
 
@@ -382,11 +440,15 @@ def GradNorm(grads, norm, grad_scale=1.0, stream=None):
 def ClipGrads(grads, max_norm, norm, grad_scale=1.0, stream=None):
     """g * grad_scale * min(1, max_norm / (norm + 1e-6)) with a given norm, e.g. one that the
     ranks of a job have put together."""
+    if _several is not False:
+        _check_devices(grads, norm)
     _call(_hip.ps_clip_grads(grads.handle, max_norm, grad_scale,
                              _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))
 
 
 def ClipGradNorm(grads, max_norm, norm, grad_scale=1.0, stream=None):
     """GradNorm and ClipGrads in one call: norm receives the norm before clipping."""
+    if _several is not False:
+        _check_devices(grads, norm)
     _call(_hip.ps_clip_grad_norm(grads.handle, max_norm, grad_scale,
                                  _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))

@@ -328,3 +328,84 @@ def test_slots_as_a_list_or_of_a_batch():
     assert rows._top_k(Slots(0, 3), 0)[0] == C
     for shape in ((2, 4, 2), (8, 2, 1), (0, 4), (4, 0), (15,), (3, 4)):
         refused("position", rows._top_k, Slots(*shape), 4)
+
+
+def test_tensors_of_another_device(monkeypatch):
+    """Where there are several devices, every tensor's is compared with the current one."""
+    from powersparse_amd import rows
+
+    class Tensor:
+        is_cuda = True
+
+        def __init__(self, at, shape, dtype="float32", device=0):
+            self.shape, self.dtype, self.at, self.device = tuple(shape), dtype, at, device
+
+        def get_device(self):
+            return self.device
+
+        def is_contiguous(self):
+            return True
+
+        def numel(self):
+            n = 1
+            for s in self.shape:
+                n *= s
+            return n
+
+        def stride(self):
+            return tuple(Tensor(0, self.shape[k + 1:]).numel() for k in range(len(self.shape)))
+
+        def data_ptr(self):
+            return self.at
+
+    class List:
+        handle, device = 1 << 40, 0
+
+        def get_device(self):
+            return self.device
+
+    called = []
+    monkeypatch.setattr(rows, "_several", None)
+    monkeypatch.setattr(rows, "_count_devices", lambda: 2)
+    monkeypatch.setattr(rows, "_current_device", lambda: 0)
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: called.append(name) or 0
+
+    monkeypatch.setattr(rows, "_hip", Library())
+    table, out, dw = Tensor(A, (4, 8)), Tensor(B, (4, 8)), Tensor(B + 4096, (4, 1))
+    ids, at = Tensor(C, (4,), "int32"), Tensor(C + 4096, (4, 1), "int32")
+    off, w, work = Tensor(C + 8192, (6,), "int32"), Tensor(D, (4, 1)), Tensor(D + 4096, (99,), "uint8")
+    norm, glist = Tensor(A + 4096, (1,)), List()
+    calls = [(ps.EmbeddingLookup, (table, ids, out)), (ps.EmbeddingGrad, (ids, table, out, work)),
+             (ps.ExpertSort, (ids, Tensor(A, (4,), "int32"), at, off, work)),
+             (ps.ExpertDispatch, (table, at, out)), (ps.ExpertCombine, (table, at, w, out)),
+             (ps.ExpertDispatchGrad, (table, at, out)),
+             (ps.ExpertCombineGrad, (table, out, at, w, Tensor(D + (1 << 20), (4, 8)), dw)),
+             (ps.GradNorm, (glist, norm)), (ps.ClipGrads, (glist, 1.0, norm)),
+             (ps.ClipGradNorm, (glist, 1.0, norm))]
+    for f, args in calls:
+        f(*args)  # all on the current device
+        assert len(called) == 1
+        called.clear()
+        for x in args:
+            if isinstance(x, (Tensor, List)):
+                x.device = 1
+                refused("on device 1, the current one is 0", f, *args)
+                x.device = 0
+    for x in (table, out):
+        x.device = 1
+        refused("on device 1, the current one is 0", ps.GradientList, [table], [out])
+        x.device = 0
+    assert not called
+    # arrays that name no device are taken as they are
+    ps.EmbeddingLookup(mat(A, 4, 8), vec(C, 4, "int32"), mat(B, 4, 8))
+    assert called == ["ps_embedding_lookup"]
+    assert rows._several is True
+    # one device: found out once, and never asked again
+    monkeypatch.setattr(rows, "_several", None)
+    monkeypatch.setattr(rows, "_count_devices", lambda: 1)
+    table.device = 1
+    ps.EmbeddingLookup(table, ids, out)
+    assert rows._several is False
