@@ -6,10 +6,10 @@ Arrays are in the current device's memory: DeviceArray (a DeviceBuffer or raw po
 a shape and a type) or any tensor object with data_ptr, shape, stride, dtype and is_cuda,
 such as torch's; tensors that say they are on another device are refused. Matrices are
 row-major with any row stride; element types are float32, float16 and bfloat16. Every call
-checks shapes, types and sizes on the host, enqueues its kernels on `stream` (a Stream, a tensor library's stream, a raw handle, or None: the null
-stream) and returns without synchronising: arrays and workspaces must stay alive, and be
-written by nothing else, until the stream has passed the call. Wrong arguments raise
-ValueError.
+checks shapes, types and sizes on the host, enqueues its kernels on `stream` (a Stream, a
+tensor library's stream, a raw handle, or None: the null stream) and returns without
+synchronising: arrays and workspaces must stay alive, and be written by nothing else, until
+the stream has passed the call. Wrong arguments raise ValueError.
 """
 import ctypes
 
@@ -180,6 +180,15 @@ def _stream(stream):
     return int(getattr(stream, "cuda_stream", stream))
 
 
+def _fit(n, most):
+    """n within [-1, most], so that ctypes, which keeps the low bits of larger numbers, hands
+    over one that is as far out of range."""
+    return max(-1, min(int(n), most))
+
+
+_INT, _LONG = (1 << 31) - 1, (1 << 63) - 1
+
+
 def _call(status):
     if status:
         from . import _hip_call
@@ -238,7 +247,8 @@ def EmbeddingLookup(table, ids, out, scale=1.0, stream=None):
 def embedding_grad_workspace_bytes(count, cols, table_rows):
     """Workspace of EmbeddingGrad for `count` ids, rows of `cols` and a table of `table_rows`,
     or for fewer of any of them."""
-    n = _hip.ps_embedding_grad_workspace_bytes(int(count), int(cols), int(table_rows))
+    n = _hip.ps_embedding_grad_workspace_bytes(_fit(count, _LONG), _fit(cols, _LONG),
+                                                _fit(table_rows, _LONG))
     if not n:
         raise ValueError("embedding_grad_workspace_bytes: sizes out of range")
     return n
@@ -253,7 +263,7 @@ def EmbeddingGrad(ids, grad_out, grad_table, workspace, scale=1.0, padding_idx=-
         _check_devices(ids, grad_out, grad_table, workspace)
     ptr, nbytes = _space(workspace)
     _call(_hip.ps_embedding_grad(
-        _ids(ids), _rows(grad_out, "grad_out"), scale, padding_idx, bool(accumulate),
+        _ids(ids), _rows(grad_out, "grad_out"), scale, _fit(padding_idx, _LONG), bool(accumulate),
         _rows(grad_table, "grad_table"), ptr, nbytes, _stream(stream)))
 
 
@@ -262,7 +272,7 @@ def EmbeddingGrad(ids, grad_out, grad_table, workspace, scale=1.0, padding_idx=-
 def expert_sort_workspace_bytes(slots, experts):
     """Workspace of ExpertSort for `slots` ids (tokens * top_k) and `experts` experts, or for
     fewer of either."""
-    n = _hip.ps_expert_sort_workspace_bytes(int(slots), int(experts))
+    n = _hip.ps_expert_sort_workspace_bytes(_fit(slots, _LONG), _fit(experts, _INT))
     if not n:
         raise ValueError("expert_sort_workspace_bytes: sizes out of range (1 to 1024 experts)")
     return n
@@ -279,7 +289,7 @@ def ExpertSort(ids, order, position, offsets, workspace, stream=None):
     at, count, _ = _flat(offsets, "offsets", ("int32",))
     ptr, nbytes = _space(workspace)
     _call(_hip.ps_expert_sort(
-        slots, count - 1, _flat(order, "order", ("int32",), slots.count)[0],
+        slots, _fit(count - 1, _INT), _flat(order, "order", ("int32",), slots.count)[0],
         _flat(position, "position", ("int32",), slots.count)[0], at, ptr, nbytes,
         _stream(stream)))
 
@@ -291,8 +301,8 @@ def _slots(x, name, dtype, tokens, count=None):
     try:
         if x.is_cuda and x.is_contiguous():
             rows, top_k = x.shape
-            if rows == tokens and _names[x.dtype] == dtype and \
-                    count in (None, rows * top_k) and rows * top_k:
+            if rows == tokens and 0 < top_k <= _INT and rows and \
+                    count in (None, rows * top_k) and _names[x.dtype] == dtype:
                 return x.data_ptr(), top_k
     except (AttributeError, KeyError, TypeError, ValueError):
         pass
@@ -310,7 +320,7 @@ def _slots(x, name, dtype, tokens, count=None):
         if leading != tokens:
             raise ValueError(f"{name}: {' x '.join(str(s) for s in shape)} slots for {tokens} "
                              "tokens")
-    return ptr, n // tokens
+    return ptr, _fit(n // tokens, _INT)
 
 
 def _top_k(position, tokens):

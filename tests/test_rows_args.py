@@ -1,6 +1,7 @@
 """What the row operators refuse, on the host and before any device call: shapes,
 types, strides, alignments, sizes, workspaces and overlaps, through Python and
 through the C ABI. The addresses are never followed."""
+import ctypes
 import os
 import re
 import subprocess
@@ -376,7 +377,8 @@ def test_tensors_of_another_device(monkeypatch):
     monkeypatch.setattr(rows, "_hip", Library())
     table, out, dw = Tensor(A, (4, 8)), Tensor(B, (4, 8)), Tensor(B + 4096, (4, 1))
     ids, at = Tensor(C, (4,), "int32"), Tensor(C + 4096, (4, 1), "int32")
-    off, w, work = Tensor(C + 8192, (6,), "int32"), Tensor(D, (4, 1)), Tensor(D + 4096, (99,), "uint8")
+    off, w = Tensor(C + 8192, (6,), "int32"), Tensor(D, (4, 1))
+    work = Tensor(D + 4096, (99,), "uint8")
     norm, glist = Tensor(A + 4096, (1,)), List()
     calls = [(ps.EmbeddingLookup, (table, ids, out)), (ps.EmbeddingGrad, (ids, table, out, work)),
              (ps.ExpertSort, (ids, Tensor(A, (4,), "int32"), at, off, work)),
@@ -409,3 +411,35 @@ def test_tensors_of_another_device(monkeypatch):
     table.device = 1
     ps.EmbeddingLookup(table, ids, out)
     assert rows._several is False
+
+
+def test_sizes_beyond_the_c_types():
+    """ctypes keeps the low bits of larger numbers: 2^32 + 8 experts would be 8."""
+    for experts in ((1 << 32) + 8, -(1 << 32) + 8, (1 << 31)):
+        refused("out of range", ps.expert_sort_workspace_bytes, 40, experts)
+    for n in ((1 << 64) + 8, -(1 << 64) + 8):
+        refused("out of range", ps.expert_sort_workspace_bytes, n, 8)
+        for sizes in ((n, 8, 9), (8, n, 9), (8, 8, n)):
+            refused("out of range", ps.embedding_grad_workspace_bytes, *sizes)
+    many = (1 << 32) + 2
+    refused("1 to 1024 slots", ps.ExpertDispatch, mat(A, 1, 8), vec(1 << 40, many, "int32"),
+            mat(B, 4, 8))
+    refused("1 to 1024 experts", ps.ExpertSort, vec(A, 4, "int32"), vec(B, 4, "int32"),
+            vec(C, 4, "int32"), vec(1 << 40, many, "int32"), vec(D, 1 << 20, "uint8"))
+
+
+def test_padding_beyond_64_bits(monkeypatch):
+    """No id is such a number: it is passed on as one that no row has."""
+    from powersparse_amd import rows
+    passed = []
+
+    class Library:
+        def ps_embedding_grad(self, *args):
+            passed.append(ctypes.c_longlong(args[3]).value)
+            return 0
+
+    monkeypatch.setattr(rows, "_hip", Library())
+    for padding in ((1 << 64) + 3, (1 << 63) + 3, 3, 0, -1, -(1 << 63), -(1 << 64) + 3):
+        ps.EmbeddingGrad(vec(B, 40, "int32"), mat(A, 40, 8), mat(C, 9, 8),
+                         vec(D, 1 << 20, "uint8"), padding_idx=padding)
+        assert passed.pop() == padding if 0 <= padding < 9 else not 0 <= passed.pop() < 9
