@@ -385,13 +385,13 @@ long long partial_ld(long long cols) { return (cols + 7) & ~7LL; }
 GradSpace grad_space(long long n, long long cols, long long rows) {
   int bits = 0;
   const int passes = digit_passes(rows, &bits);
+  const int bins = 1 << bits;
   const IdCut cut = id_cut(n);
   const size_t chunk = chunk_size(n, cols), chunks = (size_t(n) + chunk - 1) / chunk;
-  const long long ld = partial_ld(cols);
-  GradSpace s = grad_layout(n, rows,
-                            {id_sort_table_bytes(cut, 1 << bits), id_sort_group_bytes(cut, 1 << bits),
-                             passes, chunks, 2 * chunks * size_t(ld)});
-  s.ld = ld;
+  const size_t ld = size_t(partial_ld(cols));
+  GradSpace s = grad_layout(n, rows, {id_sort_table_bytes(cut, bins), id_sort_group_bytes(cut, bins),
+                                      passes, chunks, 2 * chunks * ld});
+  s.ld = (long long)ld;
   return s;
 }
 
@@ -484,7 +484,7 @@ int ps_embedding_lookup(const ps_rows* table, const ps_ids* ids, float scale, co
           out->cols, [&](auto n) {
             const ps::Pieces p(out->cols, n);
             const unsigned long long items = (unsigned long long)out->rows * p.per_row.d;
-            return ps::with_flag(ps::streamed(out), [&](auto stream_out) {
+            return ps::with_flag(ps::streamed(out, out->rows), [&](auto stream_out) {
               return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
                 if (ids->type == PS_I64)
                   ps::lookup_kernel<T, O, long long, n, stream_out>

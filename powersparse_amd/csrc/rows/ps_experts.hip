@@ -251,7 +251,7 @@ int ps_expert_dispatch(const ps_rows* x, const int* position, int top_k, const p
     return ps::with_width<sizeof(T)>(x->cols, [&](auto n) {
       const ps::Pieces p(x->cols, n);
       const unsigned long long items = (unsigned long long)x->rows * p.per_row.d;
-      return ps::with_flag(ps::streamed(xs), [&](auto stream_out) {
+      return ps::with_flag(ps::streamed(xs, x->rows * top_k), [&](auto stream_out) {
         return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
           ps::dispatch_kernel<T, n, stream_out>
               <<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
@@ -279,7 +279,7 @@ int ps_expert_combine(const ps_rows* ys, const int* position, const float* weigh
     return ps::with_width<sizeof(T)>(y->cols, [&](auto n) {
       const ps::Pieces p(y->cols, n);
       const unsigned long long items = (unsigned long long)y->rows * p.per_row.d;
-      return ps::with_flag(ps::streamed(y), [&](auto stream_out) {
+      return ps::with_flag(ps::streamed(y, y->rows), [&](auto stream_out) {
         return ps::launch_items(items, ps::kRowThreads, [&](uint32_t blocks, ps::Items part) {
           ps::combine_kernel<T, n, stream_out>
               <<<blocks, ps::kRowThreads, 0, ps::to_hip(stream)>>>(
@@ -315,7 +315,7 @@ int ps_expert_combine_grad(const ps_rows* dy, const ps_rows* ys, const int* posi
     return ps::with_width<sizeof(T)>(dy->cols, [&](auto n) {
       const ps::Pieces p(dy->cols, n);
       return ps::with_lanes(p, [&](auto lanes) {
-        return ps::with_flag(ps::streamed(dys), [&](auto stream_out) {
+        return ps::with_flag(ps::streamed(dys, dy->rows * top_k), [&](auto stream_out) {
           return ps::launch_items(
               dy->rows, ps::kRowThreads / lanes, [&](uint32_t blocks, ps::Items part) {
                 ps::combine_grad_kernel<T, n, lanes, stream_out>

@@ -214,10 +214,16 @@ inline int with_dtype(int dtype, F&& f) {
 // 350); 16 MB 7.2 -> 7.1 (12.7 -> 13.7). Sort, dispatch and combination of 16,384
 // tokens x 4 x 512 BF16 59 -> 43, x 8 x 4,096 506 -> 459, their gradients 56 ->
 // 52 and 689 -> 664. It loses for scattered rows that share lines and would stay
-// in the last-level cache (65,536 x 4 x 333 FP16 131 -> 137), and gains for such
-// rows that would not (32,768 x 8 x 333 FP32 215 -> 208).
+// in the last-level cache (65,536 x 4 x 333 FP16 131 -> 137; lookups into 33 of 96
+// FP32 columns, 40 MB 23 -> 31), and gains for such rows that would not (32,768 x 8
+// x 333 FP32 215 -> 208; 33 of 40 columns, 264 MB 161 -> 136).
 constexpr size_t kStreamBytes = size_t(32) << 20;
-inline bool streamed(const ps_rows* out) { return region(out).span() >= kStreamBytes; }
+// What counts is what a call writes: `written` rows of out at most, without the
+// gaps between them.
+inline bool streamed(const ps_rows* out, long long written) {
+  const long long rows = written < out->rows ? written : out->rows;
+  return size_t(rows) * size_t(out->cols) * dtype_size(out->dtype) >= kStreamBytes;
+}
 
 // Calls f(flag) with a runtime flag as a constant.
 template <typename F>
