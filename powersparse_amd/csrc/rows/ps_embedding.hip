@@ -389,8 +389,9 @@ GradSpace grad_space(long long n, long long cols, long long rows) {
   const IdCut cut = id_cut(n);
   const size_t chunk = chunk_size(n, cols), chunks = (size_t(n) + chunk - 1) / chunk;
   const size_t ld = size_t(partial_ld(cols));
-  GradSpace s = grad_layout(n, rows, {id_sort_table_bytes(cut, bins), id_sort_group_bytes(cut, bins),
-                                      passes, chunks, 2 * chunks * ld});
+  GradSpace s =
+      grad_layout(n, rows, {id_sort_table_bytes(cut, bins), id_sort_group_bytes(cut, bins), passes,
+                            chunks, 2 * chunks * ld});
   s.ld = (long long)ld;
   return s;
 }
