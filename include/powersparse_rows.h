@@ -110,6 +110,8 @@ typedef struct ps_grad_list ps_grad_list;
 int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
                         const int* dtypes, void* const* out, const int* out_dtypes,
                         ps_grad_list** list);
+/* Waits for nothing and may come during a capture, and while calls on the list
+ * are under way: its memory goes back when the next list is made. */
 void ps_grad_list_destroy(ps_grad_list* list);
 
 /* *norm (device) = sqrt(sum of (grad_scale * g)^2 over every element), summed

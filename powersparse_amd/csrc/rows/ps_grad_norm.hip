@@ -13,6 +13,7 @@
 // backwards, so what the first one read last may still be in the last-level
 // cache.
 #include <algorithm>
+#include <mutex>
 #include <utility>
 #include <vector>
 
@@ -225,6 +226,7 @@ struct ps_grad_list {
   double* sums = nullptr;
   uint32_t blocks = 0;
   ps::Ranges read, written;
+  ps_grad_list* retired = nullptr;  // the next destroyed list
 };
 
 namespace ps {
@@ -256,6 +258,27 @@ int shared_output(const std::vector<GradTensor>& table) {
     if (o != outs.end() && o->begin < d.end && o->tensor != int(i)) return int(i);
   }
   return -1;
+}
+
+// Destroyed lists, whose memory goes back when the next list is made, which waits
+// for the device anyway: freeing waits for it and is refused while any stream is
+// captured (the capture is lost), and a list may go at any time, from a garbage
+// collector too.
+std::mutex g_retired_mu;
+ps_grad_list* g_retired = nullptr;
+
+void free_retired() {
+  ps_grad_list* list;
+  {
+    std::lock_guard<std::mutex> lock(g_retired_mu);
+    list = std::exchange(g_retired, nullptr);
+  }
+  while (list) {
+    ps_grad_list* const next = list->retired;
+    dev_free(list->tables);
+    delete list;
+    list = next;
+  }
 }
 
 int build_chunks(const GradTensor* tensors, uint32_t tensor_count, GradChunk* chunks,
@@ -333,6 +356,7 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
     written.close();
     const size_t table_bytes = (table.size() * sizeof(ps::GradTensor) + 255) & ~size_t(255);
     const size_t chunk_bytes = (size_t(chunks) * sizeof(ps::GradChunk) + 255) & ~size_t(255);
+    ps::free_retired();
     void* base = nullptr;
     PS_HIP(ps::dev_malloc(&base, table_bytes + chunk_bytes + ps::kBlocks * sizeof(double)));
     char* const at = static_cast<char*>(base);
@@ -367,8 +391,8 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
 
 void ps_grad_list_destroy(ps_grad_list* list) {
   if (!list) return;
-  ps::dev_free(list->tables);
-  delete list;
+  std::lock_guard<std::mutex> lock(ps::g_retired_mu);
+  list->retired = std::exchange(ps::g_retired, list);
 }
 
 int ps_grad_norm(ps_grad_list* list, float grad_scale, float* norm, ps_stream_t stream) {

@@ -265,3 +265,46 @@ def test_one_call_clips_as_two_do(norm_near):
             c = min(1.0, max_norm / (float(norm) + 1e-6)) * scale
             e = g.cpu().double() * c
             ref.close(one, e, e.abs() + c * 2.0 ** -149, 3, "clip")
+
+
+def test_a_list_that_goes_during_a_capture():
+    """Its memory is given back without harm to the graph being captured."""
+    g = torch.full((5000,), 2.0, device="cuda")
+    kept, gone = ps.GradientList([g]), ps.GradientList([torch.ones(100, device="cuda")])
+    norm = torch.empty(1, device="cuda")
+    ps.GradNorm(kept, norm)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ps.GradNorm(kept, norm, stream=torch.cuda.current_stream())
+        gone.close()
+        norm.add_(1.0)
+    for value in (1.0, 3.0, 0.5):
+        g.fill_(value)
+        norm.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert abs(float(norm) - (value * math.sqrt(5000) + 1)) <= 1e-4 * float(norm)
+
+
+def test_the_memory_of_lists_goes_back():
+    g = torch.empty(1 << 28, dtype=torch.bfloat16, device="cuda")  # lists of half a megabyte
+    ps.GradientList([g]).close()
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    for _ in range(200):
+        ps.GradientList([g]).close()
+    assert before - torch.cuda.mem_get_info()[0] < 20 << 20
+
+
+def test_a_list_that_goes_while_it_works():
+    g = torch.full((1 << 27,), 2.0, device="cuda")
+    norm = torch.empty(1, device="cuda")
+    for _ in range(3):
+        glist = ps.GradientList([g])
+        for _ in range(20):
+            ps.GradNorm(glist, norm)
+        glist.close()
+        with pytest.raises(ValueError, match="closed"):
+            ps.GradNorm(glist, norm)
+    assert abs(float(norm) - 2 * 2 ** 13.5) <= 2 * ref.U32 * 2 * 2 ** 13.5
