@@ -25,6 +25,13 @@
       VALUUtilization` pass) the share of time the VALUs issue and the share of
       active lanes per VALU instruction of the sparse launch; means over the
       operator's calls.
+
+  python -m powersparse_amd.perf rows [--passes 8]
+  python -m powersparse_amd.perf rows-summarize --trace KT.db --fetch F.db --write W.db
+      The same for the row operators: every listed workload of
+      perf/operators.py between two calibration copies, and per workload and
+      kernel the launches of a pass, their median time and traffic. The trace
+      and each counter come from a run of their own, all of as many passes.
 """
 import argparse
 import collections
@@ -536,6 +543,91 @@ def summarize(args):
             json.dump(result, fh, indent=1)
 
 
+# The row operators' kernels, as plain or mangled names hold them.
+ROW_KERNEL = re.compile(r"(?:^|\W|\d)(id_sort_tile|id_count|id_place|id_clear|lookup|grad_runs|"
+                        r"grad_join|dispatch|combine_grad|combine|norm_join|norm|clip)_kernel")
+
+
+def row_cases():
+    """perf/operators.py as a module that makes the framework's calls."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "perf",
+                        "operators.py")
+    spec = importlib.util.spec_from_file_location("row_operators", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.own = True
+    return module
+
+
+def rows_workload(args):
+    import torch
+
+    import powersparse_amd as ps
+
+    ps.set_device(0)
+    src, dst = ps.DeviceBuffer(CALIB_BYTES), ps.DeviceBuffer(CALIB_BYTES)
+    ps.fill_random(src, CALIB_BYTES // 4, 7, 0.0, 1.0)
+
+    def mark():
+        torch.cuda.synchronize()
+        copy_f32(dst, src, CALIB_BYTES // 4)
+        ps.synchronize()
+
+    module = row_cases()
+    for case in module.listed():
+        states = [module.prepare(case, k) for k in range(2)]  # inputs change from pass to pass
+        for state in states:
+            module.run(state)
+        mark()
+        for i in range(args.passes):
+            module.run(states[i % 2])
+        mark()
+        print(f"{case['name']}: {args.passes} passes", flush=True)
+        del states
+        torch.cuda.empty_cache()
+
+
+def row_passes(dispatches):
+    """[{kernel: [value of each launch]}] of every workload: what lies between its two
+    calibration copies."""
+    out, inside = [], False
+    for name, _, value in dispatches:
+        if name.endswith("copy_f32_kernel"):
+            inside = not inside
+            if inside:
+                out.append(collections.OrderedDict())
+        elif inside and ROW_KERNEL.search(name):
+            out[-1].setdefault(ROW_KERNEL.search(name).group(1), []).append(value)
+    return out
+
+
+def rows_summarize(args):
+    def median(values):
+        return sorted(values)[len(values) // 2]
+
+    names = [case["name"] for case in row_cases().listed()]
+    fetch, write = read_counters(args.fetch, "FETCH_SIZE"), read_counters(args.write, "WRITE_SIZE")
+    kf, kw = calibration(fetch), calibration(write)
+    parts = [row_passes(d) for d in (read_dispatches(args.trace), fetch, write)]
+    if any(len(p) != len(names) for p in parts):
+        raise SystemExit(f"{[len(p) for p in parts]} workloads where {len(names)} were run")
+    print(f"Calibration (1 GiB ps::copy_f32_kernel): FETCH x{kf:.4f}, WRITE x{kw:.4f}\n\n"
+          "| workload | kernel | launches a pass | us a launch | read MB | written MB | TB/s |\n"
+          "|---|---|---|---|---|---|---|")
+    for name, times, reads, writes in zip(names, *parts):
+        for kernel, us in times.items():
+            r = median(reads[kernel]) * 1024 * kf / 1e6
+            w = median(writes[kernel]) * 1024 * kw / 1e6
+            # small launches do not move enough for a rate to say anything
+            rate = f"{(r + w) / median(us):.2f}" if r + w > 10 else ""
+            print(f"| {name} | {kernel} | {len(us) / args.passes:g} | {median(us):.1f} | {r:.1f} | "
+                  f"{w:.1f} | {rate} |")
+            name = ""
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(prog="python -m powersparse_amd.perf")
     sub = ap.add_subparsers(dest="cmd", required=True)
@@ -554,6 +646,13 @@ def main(argv=None):
     ks.add_argument("--trace", required=True)
     ks.add_argument("--fetch", required=True)
     ks.add_argument("--write", required=True)
+    r = sub.add_parser("rows")
+    r.add_argument("--passes", type=int, default=8)
+    rs = sub.add_parser("rows-summarize")
+    rs.add_argument("--trace", required=True)
+    rs.add_argument("--fetch", required=True)
+    rs.add_argument("--write", required=True)
+    rs.add_argument("--passes", type=int, default=8)
     s = sub.add_parser("summarize")
     s.add_argument("--trace", required=True)
     s.add_argument("--fetch")
@@ -571,6 +670,10 @@ def main(argv=None):
         classes(args)
     elif args.cmd == "classes-summarize":
         classes_summarize(args)
+    elif args.cmd == "rows":
+        rows_workload(args)
+    elif args.cmd == "rows-summarize":
+        rows_summarize(args)
     else:
         summarize(args)
     return 0

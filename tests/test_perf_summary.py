@@ -246,3 +246,42 @@ def test_sources_digest_follows_code_not_comments(tmp_path):
     assert tree("/* a kernel */\n__global__ void k(float* p) {\n\n    p[0] = 1.f;\n}\n") == base
     assert tree("__global__ void k(float* p) {\n  p[0] = 2.f;  // one\n}\n") != base
     assert perf.code_text("a; // b\n/* c\n d */ e  f;\n") == "a;\ne f;"
+
+
+def test_row_operators_summary(tmp_path, monkeypatch, capsys):
+    """Plain and mangled kernel names, warm-up passes outside the copies, launches a pass."""
+    class Cases:
+        @staticmethod
+        def listed():
+            return [{"name": "first"}, {"name": "second"}]
+
+    monkeypatch.setattr(perf, "row_cases", lambda: Cases)
+    lookup = "_ZN2ps12_GLOBAL__N_113lookup_kernelIDF16bDF16bxLi8ELb1EEEvNS_3MatE"
+    count = "void ps::id_count_kernel<ps::IdSource<int> >(ps::IdSource<int>, unsigned int)"
+    grad = "void ps::(anonymous namespace)::combine_grad_kernel<float, 4, 64, false>(ps::Mat)"
+
+    def run(copy, values):
+        a, b, c = values
+        return ([(lookup, 64, 1e9), (COPY, 1 << 20, copy)] + [(lookup, 64, a), (FILL, 9, 5e9)] * 2 +
+                [(COPY, 1 << 20, copy), (count, 64, 1e9), (grad, 64, 1e9), (COPY, 1 << 20, copy)] +
+                [(count, 64, b), (count, 64, b), (grad, 64, c)] * 2 + [(COPY, 1 << 20, copy)])
+
+    trace = tmp_path / "kt.db"
+    con = sqlite3.connect(trace)
+    con.execute("create table kernels (name text, grid_x integer, grid_y integer, "
+                "grid_z integer, duration real)")
+    con.executemany("insert into kernels values (?, ?, 1, 1, ?)", run(1e5, (8e3, 2e3, 4e3)))
+    con.commit()
+    con.close()
+    fetch = counter_db(tmp_path / "f.db", "FETCH_SIZE", run(2 * (1 << 30) / KIB, (62500, 10, 20)))
+    write = counter_db(tmp_path / "w.db", "WRITE_SIZE", run((1 << 30) / KIB, (31250, 0, 31250)))
+    args = ["--trace", str(trace), "--fetch", fetch, "--write", write, "--passes", "2"]
+    perf.main(["rows-summarize"] + args)
+    out = capsys.readouterr().out
+    assert "FETCH x0.5000, WRITE x1.0000" in out
+    assert "| first | lookup | 1 | 8.0 | 32.0 | 32.0 | 8.00 |" in out
+    assert "| second | id_count | 2 | 2.0 | 0.0 | 0.0 |  |" in out
+    assert "|  | combine_grad | 1 | 4.0 | 0.0 | 32.0 | 8.00 |" in out
+    monkeypatch.setattr(Cases, "listed", staticmethod(lambda: [{"name": "only"}]))
+    with pytest.raises(SystemExit):
+        perf.main(["rows-summarize"] + args)
