@@ -6,16 +6,18 @@
  *
  * Same library, status codes and streams as powersparse_hip.h: every call
  * checks its arguments on the host, enqueues its kernels on `stream` and
- * returns; nothing here synchronises, allocates (ps_grad_list_create aside) or
- * keeps anything between calls. Workspaces are the caller's, of the stated
+ * returns; nothing but ps_grad_list_create synchronises or allocates, and nothing
+ * is kept between calls. Workspaces are the caller's, of the stated
  * size or more, aligned to 16 bytes, not shared by calls that may overlap. The
  * stated sizes grow with every argument, so a workspace for the largest call
  * does for smaller ones. What a call writes (outputs, workspace) shares no byte
- * with anything else it is given; PS_ERR_INVALID otherwise.
+ * with anything else it is given, clipping in place aside; PS_ERR_INVALID
+ * otherwise.
  *
  * Data may hold any value: ids and positions out of range are dropped where
- * the text says so and never followed. Sums run in 32 bits in a fixed order (the
- * same bits every time); results are rounded once, to nearest even.
+ * the text says so and never followed. Arithmetic runs in 32 bits (norms in
+ * 64), sums in an order that the call's sizes and ids fix (the same bits every
+ * time), and what it gives is rounded to the output's type, to nearest even.
  */
 #ifndef POWERSPARSE_ROWS_H
 #define POWERSPARSE_ROWS_H
@@ -59,11 +61,13 @@ typedef struct ps_ids {
 int ps_embedding_lookup(const ps_rows* table, const ps_ids* ids, float scale, const ps_rows* out,
                         ps_stream_t stream);
 
-/* grad[v, :] = scale * (sum of grad_out[i, :] over the i with ids[i] = v, in
- * the order of i), zeros for rows without ids; with accumulate != 0 the sum is
- * added to grad and other rows are left alone. Ids outside [0, grad->rows) and
- * those equal to padding_idx (negative: none) take no part. At most 2^30 ids,
- * 2^31 - 2 rows. */
+/* grad[v, :] = scale * (sum of grad_out[i, :] over the i with ids[i] = v), zeros
+ * for rows without ids; with accumulate != 0 the sum is added to grad and other
+ * rows are left alone. Ids outside [0, grad->rows) and those equal to padding_idx
+ * (negative: none) take no part. At most 2^30 ids, 2^31 - 2 rows. A row's terms
+ * are added in the order of i, in parts where there are many: where these are cut
+ * follows from the count, the width and the other ids, so the same row's last
+ * bits may differ in a batch of another size. */
 size_t ps_embedding_grad_workspace_bytes(long long count, long long cols, long long table_rows);
 int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
                       long long padding_idx, int accumulate, const ps_rows* grad, void* workspace,

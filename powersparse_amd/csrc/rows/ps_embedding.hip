@@ -11,7 +11,10 @@
 //  - a run belongs to the chunk it starts in when it ends before the next
 //    chunk's end: one thread adds all of it and writes the row;
 //  - a longer run is cut at the chunks' borders, every part is kept as a row of
-//    32-bit partial sums, and a second launch adds the parts in order.
+//    32-bit partial sums, and a second launch adds the parts: shares of them in
+//    order, the shares by halves.
+// The order is fixed by the sizes, the ids and the place of a run among the
+// sorted ones.
 // So partial sums cost traffic only for runs longer than a chunk, and no row
 // waits for one thread to walk a popular id's whole run. Rows without ids are
 // cleared by the same launch, from flags the sort sets.
@@ -42,11 +45,15 @@ __global__ __launch_bounds__(kRowThreads) void lookup_kernel(Mat<const T> table,
   store_piece<N, kStream>(out.at(it.row, c), v);
 }
 
-// Entries per chunk. Few for short lists, where latency counts (1,021 ids of 96
-// columns: 14.9 us with 4, 19.0 with 16; 32,768 of 64: 38.9 with 8, 43.7 with 4,
-// 42.2 with 16); otherwise the fewest from 16 to 256 that leave at most
-// kRunThreads threads for the chunks, four waves a SIMD: longer chunks mean fewer
-// parts of long runs, shorter ones more loads in flight.
+// Entries per chunk: shorter ones mean more loads in flight, longer ones fewer
+// parts of long runs. 4 to 16 while no more than 4096 chunks result, as latency
+// counts there (FP32, with 4, 8 and 16: 1,021 ids of 96 columns 14.7, 16.2 and
+// 18.7 us, 8,192 of 64 24.5, 26.1 and 28.5, 32,768 of 64 30.5, 30.8 and 33.2, drawn
+// by 1/rank 31.9, 28.4 and 28.7; 65,536 of 64, which take 16, 38, 33.9 and 35.3).
+// Then doubled, up to 256, while the chunks hold more than kRunThreads threads,
+// four waves a SIMD, at a thread for 8 columns. That is what rows of 16 bits
+// take; FP32 rows have twice the threads, rows narrower than a piece one an
+// element, and beyond 256 entries the threads grow with the list.
 constexpr unsigned long long kRunThreads = 1u << 18;
 uint32_t chunk_size(long long n, long long cols) {
   if (n <= 16) return 16;  // one chunk: no run can be long, and no join is launched

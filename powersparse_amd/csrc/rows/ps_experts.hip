@@ -55,7 +55,10 @@ __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(Mat<const T> x,
   }
 }
 
-// Rows of a token's slots under way at once.
+// Rows of a token's slots under way at once. Combination, with one and with four,
+// us: 4 x 8 x 2,048 BF16 4.2 and 3.9, 256 x 8 x 4,096 4.8 and 4.5, 16,384 x 8 x
+// 4,096 222.6 and 220.3; places left empty cost: 16,384 x 2 x 333 FP32 13.3 and
+// 13.9, 30,011 x 3 x 333 28.3 and 28.9.
 constexpr int kSlotsAhead = 4;
 
 // y = sum of weighted slots, one piece of a token a thread, in the order of k.
