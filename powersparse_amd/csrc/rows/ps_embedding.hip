@@ -108,19 +108,14 @@ __device__ __forceinline__ void write_grad(const Mat<G>& grad, uint32_t row, int
   }
 }
 
-// A value that every lane of the wave has (kUniform), in a scalar register.
-template <bool kUniform>
-__device__ __forceinline__ uint32_t uniform(uint32_t x) {
-  return kUniform ? __builtin_amdgcn_readfirstlane(x) : x;
-}
-
 // One chunk's runs, for one piece of the width. Rows are loaded kAhead at a
 // time and one batch ahead of the additions, ids two batches ahead: a row's
 // address waits for its id, and a wait for loads also waits for the stores
 // issued before them, so the next rows are under way before a finished run is
-// written. Eight rows a batch are slower (262,147 skewed ids of 333 FP16
-// columns: 86 us instead of 58).
-template <bool kUniform, typename T, typename G, int N>
+// written. Eight rows a batch are slower (calls of 262,147 skewed ids of 333 FP16
+// columns 83.4 us instead of 80.0, 32,768 of 4,096 BF16 98.7 instead of 93.1, 1,021
+// of 96 FP32 16.9 instead of 14.4).
+template <typename T, typename G, int N>
 __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& grad, float scale,
                          bool accumulate, uint32_t chunk, int piece, const Pieces& p) {
   constexpr int kAhead = 4;
@@ -136,18 +131,17 @@ __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& gr
     for (int j = 0; j < kAhead; ++j) {
       const uint32_t q = min(i + j, r.n - 1);
       const uint2 pair = r.sorted[q];
-      id[s][j] = uniform<kUniform>(pair.x);
-      at[s][j] = uniform<kUniform>(pair.y);
+      id[s][j] = pair.x;
+      at[s][j] = pair.y;
     }
   };
   load_ids(b, 0);
   load_ids(b + kAhead, 1);
   // The ids around the chunk, loaded together: they come from far, and asked
   // for one after another they cost as much as the rows.
-  const auto key_at = [&](uint32_t i) { return uniform<kUniform>(r.key(i)); };
-  const uint32_t first = id[0][0], last = key_at(e - 1);
-  const uint32_t before = key_at(max(b, 1u) - 1), far_before = key_at(max(b, size + 1) - size - 1);
-  const uint32_t behind = key_at(min(e, r.n - 1)), far_behind = key_at(min(next, r.n - 1));
+  const uint32_t first = id[0][0], last = r.key(e - 1);
+  const uint32_t before = r.key(max(b, 1u) - 1), far_before = r.key(max(b, size + 1) - size - 1);
+  const uint32_t behind = r.key(min(e, r.n - 1)), far_behind = r.key(min(next, r.n - 1));
   if (first >= r.rows) return;  // only ids that take no part
   // The first run may start in a chunk before: then it is that chunk's, or long.
   const bool continued = b > 0 && before == first;
@@ -222,28 +216,15 @@ __device__ void sum_runs(const Runs& r, const Mat<const T>& dy, const Mat<G>& gr
 // workgroup (64 KB ones took 10% longer). Bound by memory: 32,768 BF16 rows into
 // 131,072 x 4,096 FP32, 2.41 GB in 402 us, 6.0 TB/s.
 constexpr uint32_t kClearItems = 4;  // per thread
-template <bool kUniform, typename T, typename G, int N>
+template <typename T, typename G, int N>
 __global__ __launch_bounds__(kRowThreads) void grad_runs_kernel(
     Runs r, Mat<const T> dy, Mat<G> grad, float scale, bool accumulate, Pieces p,
     uint32_t run_blocks, const uint8_t* __restrict__ flags, Items clear_items) {
   if (blockIdx.x < run_blocks) {
-    uint32_t chunk;
-    int piece;
-    if constexpr (kUniform) {
-      const uint32_t waves = (p.per_row.d + kWave - 1) / kWave;  // per chunk
-      const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * (kRowThreads / kWave) +
-                                                        threadIdx.x / kWave);
-      chunk = w / waves;
-      piece = int((w - chunk * waves) * kWave) + lane_id();
-      if (chunk >= r.chunks || piece >= int(p.per_row.d)) return;
-    } else {
-      const unsigned long long first = (unsigned long long)blockIdx.x * kRowThreads;
-      if (first + threadIdx.x >= (unsigned long long)r.chunks * p.per_row.d) return;
-      const Item it = ItemBase(first, p).at(threadIdx.x, p);
-      chunk = uint32_t(it.row);
-      piece = it.piece;
-    }
-    sum_runs<kUniform, T, G, N>(r, dy, grad, scale, accumulate, chunk, piece, p);
+    const unsigned long long first = (unsigned long long)blockIdx.x * kRowThreads;
+    if (first + threadIdx.x >= (unsigned long long)r.chunks * p.per_row.d) return;
+    const Item it = ItemBase(first, p).at(threadIdx.x, p);
+    sum_runs<T, G, N>(r, dy, grad, scale, accumulate, uint32_t(it.row), it.piece, p);
     return;
   }
   const unsigned long long first =
@@ -428,9 +409,10 @@ size_t grad_space_most(long long n, long long cols, long long rows) {
 }
 
 // The one workgroup that sorts a tile clears this many 16-byte words on the way
-// (256 KB); more are cleared by a launch of their own (100 ids: 14.0 us on the
-// way, 16.5 by a launch for 112,000 rows, 15.1 and 15.9 for 250,000, 18.3 and 17.2
-// for 500,000).
+// (256 KB); more are cleared by a launch of their own (100 ids of 8 FP16 columns,
+// on the way and by a launch: 15.0 and 14.9 us for 10,007 rows, 15.7 and 15.7 for
+// 112,000, 16.4 and 16.0 for 250,000, 19.4 and 17.5 for 500,000; 4,000 ids 24.6 and
+// 25.9 for 112,000, 25.8 and 26.2 for 250,000, 29.3 and 28.2 for 500,000).
 constexpr size_t kTileClears = 16384;
 
 // Sorts the ids; returns which of the two buffers holds the result.
@@ -565,15 +547,9 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
       return ps::with_width<(sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G))>(
           grad->cols, [&](auto w) {
             const ps::Pieces p(grad->cols, w);
-            // Waves of one chunk each from 64 pieces on: the control flow is
-            // scalar, but lanes beyond the width idle. 32,768 ids of 4,096
-            // BF16 columns 172 -> 165 us, 65,536 of 1,024 91 -> 88; but
-            // 262,144 of 256 74 -> 82, of 64 58 -> 87.
-            const bool waves = p.per_row.d >= ps::kWave;
-            const unsigned long long pieces =
-                waves ? (p.per_row.d + ps::kWave - 1) / ps::kWave * ps::kWave : p.per_row.d;
             const unsigned long long run_blocks =
-                (r.chunks * pieces + ps::kRowThreads - 1) / ps::kRowThreads;
+                ((unsigned long long)r.chunks * p.per_row.d + ps::kRowThreads - 1) /
+                ps::kRowThreads;
             // The first launch takes the runs and as many rows to clear as
             // fit beside them, the others more rows.
             const unsigned long long clears =
@@ -587,11 +563,10 @@ int ps_embedding_grad(const ps_ids* ids, const ps_rows* grad_out, float scale,
                   (clears - done + per_block - 1) / per_block, 1u << 23);
               if (!(runs + blocks)) break;
               const unsigned long long end = std::min(clears, done + blocks * per_block);
-              const auto kernel = waves ? ps::grad_runs_kernel<true, T, G, w>
-                                        : ps::grad_runs_kernel<false, T, G, w>;
-              kernel<<<uint32_t(runs + blocks), ps::kRowThreads, 0, st>>>(
-                  r, ps::mat<const T>(grad_out), ps::mat<G>(grad), scale, accumulate != 0, p, runs,
-                  flags, ps::Items{done, end});
+              ps::grad_runs_kernel<T, G, w>
+                  <<<uint32_t(runs + blocks), ps::kRowThreads, 0, st>>>(
+                      r, ps::mat<const T>(grad_out), ps::mat<G>(grad), scale, accumulate != 0, p,
+                      runs, flags, ps::Items{done, end});
               PS_LAUNCHED();
               runs = 0;
               done = end;

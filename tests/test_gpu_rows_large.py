@@ -1,7 +1,6 @@
 """The row operators where their kernels change with the size: outputs stored with
-the non-temporal hint (32 MB and more), long chunks of the lookup's gradient in
-both its forms, more workgroups than one launch takes, tables of almost 2^31
-rows. The plain forms run on the device, in 64 bits."""
+the non-temporal hint (32 MB and more), long chunks of the lookup's gradient, more
+workgroups than one launch takes, tables of almost 2^31 rows. The plain forms run on the device, in 64 bits."""
 import zlib
 
 import pytest
@@ -116,8 +115,7 @@ def test_experts_of_large_outputs(dtype, cols):
         untouched(dys, whole)
 
 
-# Chunks of 64, 128 and 256 entries: a wave a chunk (4096 columns) and threads side by
-# side (333 columns of 16 bits).
+# Chunks of 64, 128 and 256 entries, of many pieces each (4096 columns) and of few.
 @pytest.mark.parametrize("chunk,count,cols,dy_t,grad_t", [
     (64, 20000, 4096, "bf16", "f32"), (128, 40000, 4093, "f32", "f32"),
     (256, 100000, 4096, "bf16", "bf16"), (64, 262147, 333, "f16", "f16"),
