@@ -1,18 +1,19 @@
 /*
- * powersparse_rows.h — row operators whose sparse matrix follows from ids:
- * embedding lookup and its gradient, tokens sorted by expert and back with
- * their gradients, and the norm and clipping of many gradient tensors.
- * No reference counterpart.
+ * powersparse_rows.h — the row operators of a model that trains on graphs:
+ * those whose sparse matrix follows from ids (embedding lookup and its gradient,
+ * tokens sorted by expert and back with their gradients), the router that
+ * chooses the ids, layer norm, and the end of a step (the norm and clipping of
+ * many gradient tensors, AdamW). No reference counterpart.
  *
  * Same library, status codes and streams as powersparse_hip.h: every call
  * checks its arguments on the host, enqueues its kernels on `stream` and
- * returns; nothing but ps_grad_list_create synchronises or allocates, and nothing
- * is kept between calls. Workspaces are the caller's, of the stated
+ * returns; nothing but making a list of tensors synchronises or allocates, and
+ * nothing is kept between calls. Workspaces are the caller's, of the stated
  * size or more, aligned to 16 bytes, not shared by calls that may overlap. The
  * stated sizes grow with every argument, so a workspace for the largest call
  * does for smaller ones. What a call writes (outputs, workspace) shares no byte
- * with anything else it is given, clipping in place aside; PS_ERR_INVALID
- * otherwise.
+ * with anything else it is given, clipping in place and what AdamW updates aside;
+ * PS_ERR_INVALID otherwise.
  *
  * Data may hold any value: ids and positions out of range are dropped where
  * the text says so and never followed. Arithmetic runs in 32 bits (norms in
@@ -35,6 +36,8 @@ extern "C" {
 #define PS_F32 0
 #define PS_F16 1
 #define PS_BF16 2
+/* Of optimizer states only: 8 bits, FP8 as OCP defines it, by blocks (below). */
+#define PS_E4M3 3
 
 /* Id types. */
 #define PS_I32 0
@@ -104,6 +107,53 @@ int ps_expert_combine_grad(const ps_rows* dy, const ps_rows* ys, const int* posi
                            const float* weights, int top_k, const ps_rows* dys, float* dweights,
                            ps_stream_t stream);
 
+/* The router. With p the softmax of a token's row of logits (tokens x experts):
+ * ids[t * top_k + k], k = 0 .. top_k - 1, are the experts of its largest logits in
+ * descending order, equal ones by ascending expert (a NaN counts as the largest, and
+ * makes the token's weights NaN); weights, of the same places, their p, or with
+ * normalize != 0 p divided by the sum over the chosen ones. An expert whose logit
+ * is -inf is barred: never chosen. Places left over have id -1 and weight 0. mask
+ * (NULL: none): a byte for each token, 0 where it is padding; such tokens, and those
+ * with all experts barred, take no part and have no experts.
+ * counts (experts + 1 values): how often each expert was chosen, and last the tokens
+ * that take part; loss (one value) = experts * sum over e of f_e * P_e, f_e the
+ * choices' share that is e's and P_e the mean of p over those tokens: 1 where all
+ * is balanced, 0 without tokens. Both NULL: not wanted, nor the workspace then.
+ * 1 to 1024 experts, top_k up to as many, at most 2^30 slots. */
+size_t ps_expert_route_workspace_bytes(long long tokens, int experts);
+int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsigned char* mask,
+                    int* ids, float* weights, int* counts, float* loss, void* workspace,
+                    size_t workspace_bytes, ps_stream_t stream);
+
+/* dlogits = the gradient of sum(dweights * weights) + *dloss * loss by the logits,
+ * the choices as they are: ids and counts are what ps_expert_route gave (counts may
+ * be summed over the ranks of a job: the gradient is of the loss over all their
+ * tokens then). dweights NULL: zeros; dloss (device) NULL: no loss, and counts may
+ * be NULL too. A token whose first id is negative gets zeros. */
+int ps_expert_route_grad(const ps_rows* logits, int top_k, int normalize, const int* ids,
+                         const float* dweights, const int* counts, const float* dloss,
+                         const ps_rows* dlogits, ps_stream_t stream);
+
+/* y[r, :] = (x[r, :] - mean) * rstd * weight + bias with mean the row's mean and
+ * rstd = 1 / sqrt(mean of (x - mean)^2 + eps). weight and bias hold one row of
+ * x->cols elements, of any type; NULL: ones and zeros. mean and rstd, a value for
+ * each row, are for the gradient (NULL: not wanted). x and y may differ in type.
+ * eps is a number from 0 up; with 0 a row of one value gives NaN. */
+int ps_layer_norm(const ps_rows* x, const ps_rows* weight, const ps_rows* bias, float eps,
+                  const ps_rows* y, float* mean, float* rstd, ps_stream_t stream);
+
+/* Its gradients, with xh = (x - mean) * rstd and g = dy * weight:
+ * dx = rstd * (g - (mean of g) - xh * (mean of g * xh)), dweight = sum over the
+ * rows of dy * xh, dbias = sum over the rows of dy. weight NULL: ones; dweight and
+ * dbias, one row each, NULL: not wanted; accumulate != 0: the sums are added to
+ * them. dx has x's type; dy, weight, dweight and dbias may have others. Where the
+ * rows' sums are cut follows from the sizes. */
+size_t ps_layer_norm_grad_workspace_bytes(long long rows, long long cols);
+int ps_layer_norm_grad(const ps_rows* dy, const ps_rows* x, const ps_rows* weight,
+                       const float* mean, const float* rstd, int accumulate, const ps_rows* dx,
+                       const ps_rows* dweight, const ps_rows* dbias, void* workspace,
+                       size_t workspace_bytes, ps_stream_t stream);
+
 /* The gradient tensors of a model: data[i] holds counts[i] contiguous elements
  * of dtypes[i]. out (NULL: in place) and out_dtypes name where the clipped
  * gradients go; nothing that is written may overlap another tensor, no norm may
@@ -133,6 +183,57 @@ int ps_clip_grads(ps_grad_list* list, float max_norm, float grad_scale, const fl
  * norm before clipping, and that FP32 value is clipped by. */
 int ps_clip_grad_norm(ps_grad_list* list, float max_norm, float grad_scale, float* norm,
                       ps_stream_t stream);
+
+/* A parameter of `count` contiguous elements, its gradient (only read) and its
+ * moments, which a step updates in place. Moments of PS_F32 begin with zeros.
+ * Those of PS_E4M3 are codes, a byte an element, and scales, a pair of floats for
+ * every 256 elements (the last of them may be fewer): exp_avg = code * pair[0],
+ * the square root of exp_avg_sq = code * pair[1]; they too begin with zeros. copy
+ * (NULL: none) receives the new parameter rounded to copy_dtype. */
+typedef struct ps_adamw_tensor {
+  void* param;
+  const void* grad;
+  void *exp_avg, *exp_avg_sq;
+  float* scales;
+  void* copy;
+  long long count;
+  int param_dtype, grad_dtype, copy_dtype;
+  float weight_decay;
+} ps_adamw_tensor;
+
+/* Nothing that a step writes may overlap another argument of the list's
+ * (PS_ERR_INVALID). state_dtype: PS_F32 or PS_E4M3, of all moments. Uploads a table
+ * and synchronises; owns it. Steps of one list must not overlap. */
+typedef struct ps_adamw_list ps_adamw_list;
+int ps_adamw_list_create(int tensors, const ps_adamw_tensor* list, int state_dtype,
+                         ps_adamw_list** out);
+/* As ps_grad_list_destroy. */
+void ps_adamw_list_destroy(ps_adamw_list* list);
+
+/* step: the number of this update, from 1. device_lr, device_step and norm (device,
+ * one value each): NULL, or read when the step runs, lr and step ignored then (a
+ * device step below 1 counts as 1); none may lie in what the step writes. */
+typedef struct ps_adamw_options {
+  double lr, beta1, beta2, eps;
+  long long step;
+  const float* device_lr;
+  const int* device_step;
+  const float* norm;
+  float max_norm, grad_scale;
+} ps_adamw_options;
+
+/* With g = c * grad, c = grad_scale, or with a norm (of grad_scale * grad, as
+ * ps_grad_norm gives it) grad_scale * min(1, max_norm / (*norm + 1e-6)):
+ * exp_avg = beta1 * exp_avg + (1 - beta1) * g,
+ * exp_avg_sq = beta2 * exp_avg_sq + (1 - beta2) * g^2,
+ * param -= lr * (weight_decay * param + (exp_avg / (1 - beta1^step)) /
+ * (sqrt(exp_avg_sq / (1 - beta2^step)) + eps)). A norm that is not finite: nothing
+ * changes. The parameter moves by the moments before they are rounded to 8 bits;
+ * there they go to either neighbouring code, by a rule of step and place that
+ * keeps their mean over the steps, and a second moment that is not zero stays so.
+ * A gradient that is not finite makes its element's moments NaN, in 8 bits perhaps
+ * its block's. */
+int ps_adamw_step(ps_adamw_list* list, const ps_adamw_options* options, ps_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -633,4 +633,7 @@ def sddmm_launch(worksets, residue_offset, rows, cols, N, lhs, rhs, outputs, str
 from .rows import (DeviceArray, EmbeddingLookup, EmbeddingGrad,  # noqa: E402
                    embedding_grad_workspace_bytes, ExpertSort, expert_sort_workspace_bytes,
                    ExpertDispatch, ExpertDispatchGrad, ExpertCombine, ExpertCombineGrad,
-                   GradientList, GradNorm, ClipGrads, ClipGradNorm)
+                   ExpertRoute, ExpertRouteGrad, expert_route_workspace_bytes,
+                   LayerNorm, LayerNormGrad, layer_norm_grad_workspace_bytes,
+                   GradientList, GradNorm, ClipGrads, ClipGradNorm,
+                   AdamWList, AdamWStep, STATE_BLOCK, state_blocks)

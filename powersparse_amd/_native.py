@@ -106,6 +106,25 @@ class Ids(ctypes.Structure):
     _fields_ = [("data", c_void_p), ("count", ctypes.c_longlong), ("type", ctypes.c_int)]
 
 
+class AdamWTensor(ctypes.Structure):
+    """ps_adamw_tensor: a parameter with its gradient and moments."""
+
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("exp_avg", c_void_p),
+                ("exp_avg_sq", c_void_p), ("scales", c_void_p), ("copy", c_void_p),
+                ("count", ctypes.c_longlong), ("param_dtype", ctypes.c_int),
+                ("grad_dtype", ctypes.c_int), ("copy_dtype", ctypes.c_int),
+                ("weight_decay", ctypes.c_float)]
+
+
+class AdamWOptions(ctypes.Structure):
+    """ps_adamw_options: what a step is given."""
+
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("step", ctypes.c_longlong), ("device_lr", c_void_p),
+                ("device_step", c_void_p), ("norm", c_void_p), ("max_norm", ctypes.c_float),
+                ("grad_scale", ctypes.c_float)]
+
+
 # The row operators (include/powersparse_rows.h), in libpowersparse_hip.so.
 _rows_p = ctypes.POINTER(Rows)
 _ids_p = ctypes.POINTER(Ids)
@@ -124,6 +143,20 @@ ROWS_API = [
      [_rows_p, c_void_p, c_void_p, ctypes.c_int, _rows_p, c_void_p]),
     ("ps_expert_combine_grad", ctypes.c_int,
      [_rows_p, _rows_p, c_void_p, c_void_p, ctypes.c_int, _rows_p, c_void_p, c_void_p]),
+    ("ps_expert_route_workspace_bytes", ctypes.c_size_t, [ctypes.c_longlong, ctypes.c_int]),
+    ("ps_expert_route", ctypes.c_int,
+     [_rows_p, ctypes.c_int, ctypes.c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+      c_void_p, ctypes.c_size_t, c_void_p]),
+    ("ps_expert_route_grad", ctypes.c_int,
+     [_rows_p, ctypes.c_int, ctypes.c_int, c_void_p, c_void_p, c_void_p, c_void_p, _rows_p,
+      c_void_p]),
+    ("ps_layer_norm", ctypes.c_int,
+     [_rows_p, _rows_p, _rows_p, ctypes.c_float, _rows_p, c_void_p, c_void_p, c_void_p]),
+    ("ps_layer_norm_grad_workspace_bytes", ctypes.c_size_t,
+     [ctypes.c_longlong, ctypes.c_longlong]),
+    ("ps_layer_norm_grad", ctypes.c_int,
+     [_rows_p, _rows_p, _rows_p, c_void_p, c_void_p, ctypes.c_int, _rows_p, _rows_p, _rows_p,
+      c_void_p, ctypes.c_size_t, c_void_p]),
     ("ps_grad_list_create", ctypes.c_int,
      [ctypes.c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(ctypes.c_longlong), c_int_p,
       ctypes.POINTER(c_void_p), c_int_p, ctypes.POINTER(c_void_p)]),
@@ -133,6 +166,10 @@ ROWS_API = [
      [c_void_p, ctypes.c_float, ctypes.c_float, c_void_p, c_void_p]),
     ("ps_clip_grad_norm", ctypes.c_int,
      [c_void_p, ctypes.c_float, ctypes.c_float, c_void_p, c_void_p]),
+    ("ps_adamw_list_create", ctypes.c_int,
+     [ctypes.c_int, ctypes.POINTER(AdamWTensor), ctypes.c_int, ctypes.POINTER(c_void_p)]),
+    ("ps_adamw_list_destroy", None, [c_void_p]),
+    ("ps_adamw_step", ctypes.c_int, [c_void_p, ctypes.POINTER(AdamWOptions), c_void_p]),
 ]
 
 # (name, restype, argtypes) of every exported entry point. Tests check that

@@ -1,0 +1,421 @@
+// AdamW over many tensors in one launch, with the moments in 32 bits or in 8.
+//
+// In 8 bits a moment is kept by blocks of 256 elements of a tensor: an E4M3 code
+// for each, and one FP32 scale, the block's largest magnitude / 448, E4M3's
+// largest value. Of the second moment the square root is kept, which halves the
+// range of exponents that the codes have to span.
+//
+// A moment changes little in a step: by a part in 1000 with beta2 = 0.999, where
+// two neighbouring codes are a part in 8 to 16 apart. Rounding to nearest would
+// keep every code where it is for good. So the upper of two codes is taken where
+// the fraction of the step between them is 1 - u or more, with u the fraction of
+// a Weyl sequence, (i * a + t * b) / 2^32 mod 1 for element i in step t: b / 2^32
+// is the golden ratio's fraction, so an element's u is spread evenly over the
+// steps (Weyl's equidistribution), and its code goes up as often as its moment
+// gains a step of the grid; a / 2^32 (the square root of two's fraction) spreads
+// it over the elements. A second moment that is not zero never becomes zero: the
+// step divides by it.
+#include <cmath>
+
+#include "ps_tensor_list.hpp"
+
+namespace ps {
+
+struct AdamTensor {
+  void* param;
+  const void* grad;
+  void *exp_avg, *exp_avg_sq;
+  float* scales;  // a pair for each block
+  void* copy;
+  long long count, first_chunk;
+  float decay;
+  int param_dtype, grad_dtype, copy_dtype;
+};
+
+namespace {
+
+constexpr uint32_t kAdamBlocks = 2048;
+constexpr int kStateBlock = 256;
+constexpr uint32_t kByElement = 0x6A09E667u, kByStep = 0x9E3779B9u;
+
+struct Adam {
+  const AdamTensor* tensors;
+  const Chunk* chunks;
+  uint32_t chunk_count;
+};
+
+// What a call is given; the device's values instead where a pointer is not null.
+struct AdamCall {
+  float beta1, one_beta1, beta2, one_beta2, eps, lr;
+  double log_beta1, log_beta2;  // 0 beta: -infinity
+  long long step;
+  const float* device_lr;
+  const int* device_step;
+  const float* norm;
+  double max_norm, grad_scale;
+};
+// The same as an element needs it.
+struct AdamStep {
+  float beta1, one_beta1, beta2, one_beta2, eps, lr;
+  float grad_scale, by_mean, by_root;  // 1 / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
+  uint32_t weyl;
+};
+
+// False: the norm is not finite, nothing is to change.
+__device__ __forceinline__ bool make_step(const AdamCall& c, AdamStep* s) {
+  double scale = c.grad_scale;
+  if (c.norm) {
+    const double n = *c.norm;
+    if (!(fabs(n) < INFINITY)) return false;
+    const double ratio = c.max_norm / (n + 1e-6);
+    if (ratio < 1.0) scale *= ratio;
+  }
+  const long long t = c.device_step ? max(*c.device_step, 1) : c.step;
+  *s = {c.beta1, c.one_beta1, c.beta2, c.one_beta2, c.eps, c.device_lr ? *c.device_lr : c.lr,
+        float(scale), float(-1.0 / expm1(double(t) * c.log_beta1)),
+        float(1.0 / sqrt(-expm1(double(t) * c.log_beta2))), uint32_t(t) * kByStep};
+  return true;
+}
+
+// m and v after the gradient g.
+__device__ __forceinline__ void advance(const AdamStep& s, float g, float* m, float* v) {
+  g *= s.grad_scale;
+  *m = fmaf(s.beta1, *m, s.one_beta1 * g);
+  *v = fmaf(s.beta2, *v, s.one_beta2 * g * g);
+}
+// The parameter after a step by m and the root of v. The reciprocal is the
+// hardware's, off by a unit in the last place: of the update, which is smaller
+// than the parameter it is rounded into.
+__device__ __forceinline__ float updated(const AdamStep& s, float decay, float p, float m,
+                                         float root) {
+  const float up = m * s.by_mean * __builtin_amdgcn_rcpf(fmaf(root, s.by_root, s.eps));
+  return fmaf(-s.lr, fmaf(decay, p, up), p);
+}
+
+template <int N>
+__device__ __forceinline__ void store_copy(const AdamTensor& t, long long i, const Floats<N>& f) {
+  if (!t.copy) return;
+  if (t.copy_dtype == PS_F32)
+    store_piece<N>(static_cast<f32*>(t.copy) + i, f);
+  else if (t.copy_dtype == PS_F16)
+    store_piece<N>(static_cast<f16*>(t.copy) + i, f);
+  else
+    store_piece<N>(static_cast<bf16*>(t.copy) + i, f);
+}
+
+// N elements at i of a tensor with moments in 32 bits.
+template <int N, typename P, typename G>
+__device__ __forceinline__ void step_f32(const AdamTensor& t, const AdamStep& s, long long i) {
+  P* const param = static_cast<P*>(t.param) + i;
+  float* const exp_avg = static_cast<float*>(t.exp_avg) + i;
+  float* const exp_avg_sq = static_cast<float*>(t.exp_avg_sq) + i;
+  Floats<N> p = load_piece<N>(param), m = load_piece<N>(exp_avg), v = load_piece<N>(exp_avg_sq);
+  const Floats<N> g = load_piece<N>(static_cast<const G*>(t.grad) + i);
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    float me = m[e], ve = v[e];
+    advance(s, g[e], &me, &ve);
+    p[e] = updated(s, t.decay, p[e], me, __builtin_amdgcn_sqrtf(ve));
+    m[e] = me;
+    v[e] = ve;
+  }
+  store_piece<N>(param, p);
+  store_piece<N>(exp_avg, m);
+  store_piece<N>(exp_avg_sq, v);
+  store_copy<N>(t, i, p);
+}
+
+template <typename P, typename G>
+__device__ void chunk_f32(const AdamTensor& t, const AdamStep& s, long long from, uint32_t count) {
+  constexpr int N = 4;
+  uint32_t i = threadIdx.x * N;
+  for (; i + N <= count; i += kListThreads * N) step_f32<N, P, G>(t, s, from + i);
+  for (; i < count; ++i) step_f32<1, P, G>(t, s, from + i);
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int d = kWave / 2; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
+  return v;
+}
+
+// The magnitude `a` (up to 448) on the grid of E4M3, rounded by u (32 bits). The
+// grid has 20 bits of an FP32 significand less; below 2^-6 its steps stay 2^-9, as
+// those of FP32 numbers from 2^-6 to 2^-5 with as many bits less do.
+__device__ __forceinline__ float on_grid(float a, uint32_t u) {
+  const float low = a < 0x1p-6f ? 0x1p-6f : 0.f;
+  const uint32_t b = (__float_as_uint(a + low) + (u >> 12)) & 0xFFF00000u;
+  const float f = __uint_as_float(b) - low;
+  return f > 448.f ? 448.f : f;  // (a NaN stays one)
+}
+
+// N elements of four at i, zeros behind them.
+template <typename T>
+__device__ __forceinline__ Floats<4> load_some(const T* p, int n) {
+  if (n >= 4) return load_piece<4>(p);
+  Floats<4> f = 0.f;
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    if (e < n) f[e] = float(p[e]);
+  return f;
+}
+template <typename T>
+__device__ __forceinline__ void store_some(T* p, const Floats<4>& f, int n) {
+  if (n >= 4) return store_piece<4>(p, f);
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    if (e < n) p[e] = T(f[e]);
+}
+using Codes = PieceOf<uint8_t, 4>::type;
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int n) {
+  if (n >= 4) return __builtin_bit_cast(uint32_t, *reinterpret_cast<const Codes*>(p));
+  uint32_t v = 0;
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    if (e < n) v |= uint32_t(p[e]) << 8 * e;
+  return v;
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, uint32_t v, int n) {
+  if (n >= 4) {
+    *reinterpret_cast<Codes*>(p) = __builtin_bit_cast(Codes, v);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    if (e < n) p[e] = uint8_t(v >> 8 * e);
+}
+__device__ __forceinline__ Floats<4> from_codes(uint32_t v) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(int(v), false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(int(v), true);
+  return Floats<4>{lo[0], lo[1], hi[0], hi[1]};
+}
+__device__ __forceinline__ uint32_t to_codes(const Floats<4>& f) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+  return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], lo, true));
+}
+
+// A block of a tensor with moments in 8 bits: a wave, four elements a lane.
+template <typename P, typename G>
+__device__ void block_f8(const AdamTensor& t, const AdamStep& s, long long from) {
+  const long long i = from + lane_id() * 4;
+  const int n = int(max(0LL, min(4LL, t.count - i)));
+  P* const param = static_cast<P*>(t.param) + i;
+  uint8_t* const exp_avg = static_cast<uint8_t*>(t.exp_avg) + i;
+  uint8_t* const exp_avg_sq = static_cast<uint8_t*>(t.exp_avg_sq) + i;
+  float* const scales = t.scales + from / kStateBlock * 2;
+  Floats<4> p = load_some(param, n);
+  const Floats<4> g = load_some(static_cast<const G*>(t.grad) + i, n);
+  Floats<4> m = from_codes(load_codes(exp_avg, n)) * scales[0];
+  Floats<4> r = from_codes(load_codes(exp_avg_sq, n)) * scales[1];
+  float m_most = 0.f, r_most = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float me = m[e], ve = r[e] * r[e];
+    advance(s, g[e], &me, &ve);
+    const float root = __builtin_amdgcn_sqrtf(ve);
+    p[e] = updated(s, t.decay, p[e], me, root);
+    m[e] = me;
+    r[e] = root;
+    m_most = fmaxf(m_most, fabsf(me));
+    r_most = fmaxf(r_most, root);
+  }
+  m_most = wave_max(m_most);
+  r_most = wave_max(r_most);
+  const float m_scale = fmaxf(m_most / 448.f, 0x1p-126f), r_scale = fmaxf(r_most / 448.f, 0x1p-126f);
+  const float by_m = 1.f / m_scale, by_r = 1.f / r_scale;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t u = uint32_t(i + e) * kByElement + s.weyl;
+    m[e] = copysignf(on_grid(fabsf(m[e]) * by_m, u), m[e]);
+    const float code = on_grid(r[e] * by_r, u);
+    r[e] = r[e] > 0.f ? fmaxf(code, 0x1p-9f) : code;
+  }
+  store_some(param, p, n);
+  store_codes(exp_avg, to_codes(m), n);
+  store_codes(exp_avg_sq, to_codes(r), n);
+  if (t.copy) {
+    if (t.copy_dtype == PS_F32)
+      store_some(static_cast<f32*>(t.copy) + i, p, n);
+    else if (t.copy_dtype == PS_F16)
+      store_some(static_cast<f16*>(t.copy) + i, p, n);
+    else
+      store_some(static_cast<bf16*>(t.copy) + i, p, n);
+  }
+  if (lane_id() == 0) {
+    scales[0] = m_scale;
+    scales[1] = r_scale;
+  }
+}
+
+template <typename P, typename G>
+__device__ void chunk_f8(const AdamTensor& t, const AdamStep& s, long long from, uint32_t count) {
+  for (uint32_t i = threadIdx.x / kWave * kStateBlock; i < count;
+       i += kListThreads / kWave * kStateBlock)
+    block_f8<P, G>(t, s, from + i);
+}
+
+template <bool k8, typename P, typename G>
+__device__ __forceinline__ void chunk_of(const AdamTensor& t, const AdamStep& s, long long from,
+                                         uint32_t count) {
+  if constexpr (k8)
+    chunk_f8<P, G>(t, s, from, count);
+  else
+    chunk_f32<P, G>(t, s, from, count);
+}
+template <bool k8, typename P>
+__device__ __forceinline__ void chunk_of(const AdamTensor& t, const AdamStep& s, long long from,
+                                         uint32_t count) {
+  if (t.grad_dtype == PS_F32)
+    chunk_of<k8, P, f32>(t, s, from, count);
+  else if (t.grad_dtype == PS_F16)
+    chunk_of<k8, P, f16>(t, s, from, count);
+  else
+    chunk_of<k8, P, bf16>(t, s, from, count);
+}
+
+template <bool k8>
+__global__ __launch_bounds__(kListThreads) void adamw_kernel(Adam a, AdamCall call) {
+  AdamStep s;
+  if (!make_step(call, &s)) return;
+  for (uint32_t q = blockIdx.x; q < a.chunk_count; q += gridDim.x) {
+    const Chunk ch = a.chunks[q];
+    const AdamTensor t = a.tensors[ch.tensor];
+    const long long from = (long long)ch.index * kChunk;
+    const uint32_t count = uint32_t(min(kChunk, t.count - from));
+    if (t.param_dtype == PS_F32)
+      chunk_of<k8, f32>(t, s, from, count);
+    else if (t.param_dtype == PS_F16)
+      chunk_of<k8, f16>(t, s, from, count);
+    else
+      chunk_of<k8, bf16>(t, s, from, count);
+  }
+}
+
+static_assert(kChunk % kStateBlock == 0, "a block lies in one chunk");
+
+}  // namespace
+}  // namespace ps
+
+// Its tables: tensors, chunks.
+struct ps_adamw_list : ps::TensorTables {
+  ps::Adam adam{};
+  bool in_8_bits = false;
+  ps::Ranges written;
+};
+
+extern "C" {
+
+int ps_adamw_list_create(int tensors, const ps_adamw_tensor* list, int state_dtype,
+                         ps_adamw_list** out) {
+  PS_CHECK_ARG(out, "ps_adamw_list_create: null output");
+  *out = nullptr;
+  PS_CHECK_ARG(tensors >= 0 && tensors <= (1 << 24), "ps_adamw_list_create: bad tensor count");
+  PS_CHECK_ARG(!tensors || list, "ps_adamw_list_create: null array");
+  PS_CHECK_ARG(state_dtype == PS_F32 || state_dtype == PS_E4M3,
+               "ps_adamw_list_create: states are of PS_F32 or PS_E4M3");
+  const bool in_8_bits = state_dtype == PS_E4M3;
+  try {
+    std::vector<ps::AdamTensor> table;
+    ps::Ranges written;
+    long long total = 0, chunks = 0;
+    for (int i = 0; i < tensors; ++i) {
+      const ps_adamw_tensor& t = list[i];
+      const std::string name = "ps_adamw_list_create: tensor " + std::to_string(i);
+      PS_CHECK_ARG(ps::dtype_valid(t.param_dtype) && ps::dtype_valid(t.grad_dtype) &&
+                       (!t.copy || ps::dtype_valid(t.copy_dtype)),
+                   name + ": unknown element type");
+      PS_CHECK_ARG(t.count >= 0 && t.count <= (1LL << 44) && total <= (1LL << 44),
+                   name + ": bad count");
+      PS_CHECK_ARG(std::isfinite(t.weight_decay), name + ": weight decay is not a number");
+      if (!t.count) continue;
+      PS_CHECK_ARG(t.param && t.grad && t.exp_avg && t.exp_avg_sq && (!in_8_bits || t.scales),
+                   name + ": null data");
+      const size_t state = in_8_bits ? 1 : 4, n = size_t(t.count);
+      const size_t blocks = (n + ps::kStateBlock - 1) / ps::kStateBlock;
+      const auto misaligned = [](const void* p, size_t size) {
+        return reinterpret_cast<uintptr_t>(p) % size != 0;
+      };
+      PS_CHECK_ARG(!misaligned(t.param, ps::dtype_size(t.param_dtype)) &&
+                       !misaligned(t.grad, ps::dtype_size(t.grad_dtype)) &&
+                       !misaligned(t.exp_avg, state) && !misaligned(t.exp_avg_sq, state) &&
+                       !(in_8_bits && misaligned(t.scales, 4)) &&
+                       !(t.copy && misaligned(t.copy, ps::dtype_size(t.copy_dtype))),
+                   name + ": misaligned data");
+      written.add(t.param, n * ps::dtype_size(t.param_dtype));
+      written.add(t.exp_avg, n * state);
+      written.add(t.exp_avg_sq, n * state);
+      if (in_8_bits) written.add(t.scales, blocks * 2 * sizeof(float));
+      if (t.copy) written.add(t.copy, n * ps::dtype_size(t.copy_dtype));
+      table.push_back({t.param, t.grad, t.exp_avg, t.exp_avg_sq, in_8_bits ? t.scales : nullptr,
+                       t.copy, t.count, chunks, t.weight_decay, t.param_dtype, t.grad_dtype,
+                       t.copy_dtype});
+      total += t.count;
+      chunks += (t.count + ps::kChunk - 1) / ps::kChunk;
+    }
+    PS_CHECK_ARG(chunks < (1LL << 31), "ps_adamw_list_create: too many elements");
+    PS_CHECK_ARG(written.close(),
+                 "ps_adamw_list_create: parameters, states, scales or copies overlap, or a tensor "
+                 "is listed twice");
+    for (const ps::AdamTensor& t : table)
+      PS_CHECK_ARG(!written.meets(t.grad, size_t(t.count) * ps::dtype_size(t.grad_dtype)),
+                   "ps_adamw_list_create: a gradient overlaps what the step writes");
+    std::unique_ptr<ps_adamw_list> l(new ps_adamw_list);
+    ps::ListTables<ps::AdamTensor> tables;
+    const int rc = ps::make_list_tables(table, uint32_t(chunks), 0, &l->tables, &tables);
+    if (rc != PS_OK) return rc;
+    l->adam = {tables.tensors, tables.chunks, uint32_t(chunks)};
+    l->in_8_bits = in_8_bits;
+    l->written = std::move(written);
+    *out = l.release();
+    return PS_OK;
+  } catch (const std::exception& e) {
+    return ps::fail(PS_ERR_RUNTIME, std::string("ps_adamw_list_create: ") + e.what());
+  }
+}
+
+void ps_adamw_list_destroy(ps_adamw_list* list) {
+  if (list) ps::g_retired_lists.retire(list);
+}
+
+int ps_adamw_step(ps_adamw_list* list, const ps_adamw_options* o, ps_stream_t stream) {
+  PS_CHECK_ARG(list && o, "ps_adamw_step: null argument");
+  PS_CHECK_ARG(o->beta1 >= 0 && o->beta1 < 1 && o->beta2 >= 0 && o->beta2 < 1,
+               "ps_adamw_step: betas are from 0 up to below 1");
+  PS_CHECK_ARG(o->eps >= 0, "ps_adamw_step: eps is not a number from 0 up");
+  PS_CHECK_ARG(o->device_lr || std::isfinite(o->lr), "ps_adamw_step: the rate is not a number");
+  PS_CHECK_ARG(o->device_step || o->step >= 1, "ps_adamw_step: steps are counted from 1");
+  PS_CHECK_ARG(!o->norm || o->max_norm >= 0.f,
+               "ps_adamw_step: the bound is not a number from 0 up");
+  PS_CHECK_ARG(ps::aligned4(o->device_lr) && ps::aligned4(o->device_step) && ps::aligned4(o->norm),
+               "ps_adamw_step: misaligned rate, step or norm");
+  for (const void* p : {static_cast<const void*>(o->device_lr),
+                        static_cast<const void*>(o->device_step),
+                        static_cast<const void*>(o->norm)})
+    PS_CHECK_ARG(!p || !list->written.meets(p, 4),
+                 "ps_adamw_step: the rate, step or norm lies in what the step writes");
+  if (!list->adam.chunk_count) return PS_OK;
+  const ps::AdamCall call{float(o->beta1),
+                          float(1.0 - o->beta1),
+                          float(o->beta2),
+                          float(1.0 - o->beta2),
+                          float(o->eps),
+                          float(o->lr),
+                          std::log(o->beta1),
+                          std::log(o->beta2),
+                          o->step,
+                          o->device_lr,
+                          o->device_step,
+                          o->norm,
+                          double(o->max_norm),
+                          double(o->grad_scale)};
+  const uint32_t blocks = std::min(list->adam.chunk_count, ps::kAdamBlocks);
+  const hipStream_t st = ps::to_hip(stream);
+  if (list->in_8_bits)
+    ps::adamw_kernel<true><<<blocks, ps::kListThreads, 0, st>>>(list->adam, call);
+  else
+    ps::adamw_kernel<false><<<blocks, ps::kListThreads, 0, st>>>(list->adam, call);
+  PS_LAUNCHED();
+  return PS_OK;
+}
+
+}  // extern "C"

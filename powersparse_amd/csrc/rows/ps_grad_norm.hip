@@ -12,12 +12,7 @@
 // us, 5.3 TB/s, then 4.9 GB in 957 us, 5.1 TB/s; in place 888 us in all. The
 // second pass walks the chunks backwards, so what the first one read last may
 // still be in the last-level cache.
-#include <algorithm>
-#include <mutex>
-#include <utility>
-#include <vector>
-
-#include "ps_rows.hpp"
+#include "ps_tensor_list.hpp"
 
 namespace ps {
 
@@ -28,44 +23,17 @@ struct GradTensor {
   int dtype, out_dtype;
   long long first_chunk;
 };
-struct GradChunk {
-  uint32_t tensor, index;  // elements [index * kChunk, ...) of the tensor
-};
-
 namespace {
 
-constexpr int kClipThreads = 256;
+constexpr int kClipThreads = kListThreads;
 constexpr uint32_t kBlocks = 2048;
-// Elements of a chunk. The workgroups go through the chunks side by side, so
-// small chunks keep what they touch at one time together: clipping 800 M BF16
-// elements into FP32 took 951 us with 4096, 984 with 8192, 1089 with 32,768,
-// 992 with 2048.
-constexpr long long kChunk = 4096;
 
 struct Grads {
   const GradTensor* tensors;
-  const GradChunk* chunks;
+  const Chunk* chunks;
   uint32_t chunk_count;
   bool in_place;
 };
-
-// The chunk table: the tensor that chunk q is of, by bisection.
-__global__ __launch_bounds__(kClipThreads) void chunk_kernel(const GradTensor* __restrict__ tensors,
-                                                             uint32_t tensor_count,
-                                                             GradChunk* __restrict__ chunks,
-                                                             uint32_t chunk_count) {
-  const uint32_t q = blockIdx.x * kClipThreads + threadIdx.x;
-  if (q >= chunk_count) return;
-  uint32_t lo = 0, hi = tensor_count - 1;  // the last tensor that begins at or before q
-  while (lo < hi) {
-    const uint32_t mid = (lo + hi + 1) / 2;
-    if (tensors[mid].first_chunk <= q)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  chunks[q] = {lo, uint32_t(q - tensors[lo].first_chunk)};
-}
 
 // Sum over the workgroup, in every thread.
 __device__ __forceinline__ double block_sum(double v) {
@@ -97,7 +65,7 @@ __device__ double square_sum(const T* p, uint32_t count) {
 __global__ __launch_bounds__(kClipThreads) void norm_kernel(Grads g, double* __restrict__ sums) {
   double s = 0;
   for (uint32_t q = blockIdx.x; q < g.chunk_count; q += gridDim.x) {
-    const GradChunk ch = g.chunks[q];
+    const Chunk ch = g.chunks[q];
     const GradTensor t = g.tensors[ch.tensor];
     const long long from = (long long)ch.index * kChunk;
     const uint32_t count = uint32_t(min(kChunk, t.count - from));
@@ -165,7 +133,7 @@ __global__ __launch_bounds__(kClipThreads) void clip_kernel(Grads g,
   const float c = float((ratio > 1.0 ? 1.0 : ratio) * grad_scale);  // a NaN ratio stays
   if (g.in_place && c == 1.f) return;
   for (uint32_t q = blockIdx.x; q < g.chunk_count; q += gridDim.x) {
-    const GradChunk ch = g.chunks[g.chunk_count - 1 - q];
+    const Chunk ch = g.chunks[g.chunk_count - 1 - q];
     const GradTensor t = g.tensors[ch.tensor];
     const long long from = (long long)ch.index * kChunk;
     const uint32_t count = uint32_t(min(kChunk, t.count - from));
@@ -181,52 +149,12 @@ __global__ __launch_bounds__(kClipThreads) void clip_kernel(Grads g,
 }  // namespace
 }  // namespace ps
 
-namespace ps {
-namespace {
-
-// Where a list's gradients, or its outputs, are: ranges that do not meet, in order.
-class Ranges {
- public:
-  void add(const void* p, size_t bytes) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-    ranges_.push_back({at, at + bytes});
-  }
-  void close() {
-    std::sort(ranges_.begin(), ranges_.end(),
-              [](const Range& a, const Range& b) { return a.begin < b.begin; });
-    size_t kept = 0;
-    for (const Range& r : ranges_) {
-      if (kept && r.begin <= ranges_[kept - 1].end)
-        ranges_[kept - 1].end = std::max(ranges_[kept - 1].end, r.end);
-      else
-        ranges_[kept++] = r;
-    }
-    ranges_.resize(kept);
-  }
-  bool meets(const void* p, size_t bytes) const {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-    const auto r = std::upper_bound(ranges_.begin(), ranges_.end(), at,
-                                    [](uintptr_t x, const Range& range) { return x < range.end; });
-    return r != ranges_.end() && r->begin < at + bytes;
-  }
-
- private:
-  struct Range {
-    uintptr_t begin, end;
-  };
-  std::vector<Range> ranges_;
-};
-
-}  // namespace
-}  // namespace ps
-
-struct ps_grad_list {
-  void* tables = nullptr;  // tensors, chunks, the workgroups' sums
+// Its tables: tensors, chunks, the workgroups' sums.
+struct ps_grad_list : ps::TensorTables {
   ps::Grads grads{};
   double* sums = nullptr;
   uint32_t blocks = 0;
   ps::Ranges read, written;
-  ps_grad_list* retired = nullptr;  // the next destroyed list
 };
 
 namespace ps {
@@ -258,36 +186,6 @@ int shared_output(const std::vector<GradTensor>& table) {
     if (o != outs.end() && o->begin < d.end && o->tensor != int(i)) return int(i);
   }
   return -1;
-}
-
-// Destroyed lists, whose memory goes back when the next list is made, which waits
-// for the device anyway: freeing waits for it and is refused while any stream is
-// captured (the capture is lost), and a list may go at any time, from a garbage
-// collector too.
-std::mutex g_retired_mu;
-ps_grad_list* g_retired = nullptr;
-
-void free_retired() {
-  ps_grad_list* list;
-  {
-    std::lock_guard<std::mutex> lock(g_retired_mu);
-    list = std::exchange(g_retired, nullptr);
-  }
-  while (list) {
-    ps_grad_list* const next = list->retired;
-    dev_free(list->tables);
-    delete list;
-    list = next;
-  }
-}
-
-int build_chunks(const GradTensor* tensors, uint32_t tensor_count, GradChunk* chunks,
-                 uint32_t chunk_count) {
-  chunk_kernel<<<(chunk_count + kClipThreads - 1) / kClipThreads, kClipThreads>>>(
-      tensors, tensor_count, chunks, chunk_count);
-  PS_LAUNCHED();
-  PS_HIP(hipStreamSynchronize(nullptr));
-  return PS_OK;
 }
 
 int launch_norm(const ps_grad_list& l, hipStream_t stream) {
@@ -354,35 +252,20 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
                  "listed twice");
     read.close();
     written.close();
-    const size_t table_bytes = (table.size() * sizeof(ps::GradTensor) + 255) & ~size_t(255);
-    const size_t chunk_bytes = (size_t(chunks) * sizeof(ps::GradChunk) + 255) & ~size_t(255);
-    ps::free_retired();
-    void* base = nullptr;
-    PS_HIP(ps::dev_malloc(&base, table_bytes + chunk_bytes + ps::kBlocks * sizeof(double)));
-    char* const at = static_cast<char*>(base);
-    const auto* const tensor_table = reinterpret_cast<const ps::GradTensor*>(at);
-    auto* const chunk_table = reinterpret_cast<ps::GradChunk*>(at + table_bytes);
-    int rc = PS_OK;
-    if (chunks) {
-      rc = ps_memcpy_htod(at, table.data(), table.size() * sizeof(ps::GradTensor));
-      if (rc == PS_OK) rc = ps::build_chunks(tensor_table, uint32_t(table.size()), chunk_table,
-                                             uint32_t(chunks));
-    }
-    ps_grad_list* l = rc == PS_OK ? new (std::nothrow) ps_grad_list : nullptr;
-    if (!l) {
-      ps::dev_free(base);
-      return rc != PS_OK ? rc : ps::fail(PS_ERR_RUNTIME, "ps_grad_list_create: out of memory");
-    }
-    l->tables = base;
-    l->grads.tensors = tensor_table;
-    l->grads.chunks = chunk_table;
+    std::unique_ptr<ps_grad_list> l(new ps_grad_list);
+    ps::ListTables<ps::GradTensor> tables;
+    const int rc = ps::make_list_tables(table, uint32_t(chunks), ps::kBlocks * sizeof(double),
+                                        &l->tables, &tables);
+    if (rc != PS_OK) return rc;
+    l->grads.tensors = tables.tensors;
+    l->grads.chunks = tables.chunks;
     l->grads.chunk_count = uint32_t(chunks);
     l->grads.in_place = in_place;
-    l->sums = reinterpret_cast<double*>(at + table_bytes + chunk_bytes);
+    l->sums = static_cast<double*>(tables.more);
     l->blocks = std::min(uint32_t(chunks), ps::kBlocks);
     l->read = std::move(read);
     l->written = std::move(written);
-    *list = l;
+    *list = l.release();
     return PS_OK;
   } catch (const std::exception& e) {
     return ps::fail(PS_ERR_RUNTIME, std::string("ps_grad_list_create: ") + e.what());
@@ -390,9 +273,7 @@ int ps_grad_list_create(int tensors, void* const* data, const long long* counts,
 }
 
 void ps_grad_list_destroy(ps_grad_list* list) {
-  if (!list) return;
-  std::lock_guard<std::mutex> lock(ps::g_retired_mu);
-  list->retired = std::exchange(ps::g_retired, list);
+  if (list) ps::g_retired_lists.retire(list);
 }
 
 int ps_grad_norm(ps_grad_list* list, float grad_scale, float* norm, ps_stream_t stream) {

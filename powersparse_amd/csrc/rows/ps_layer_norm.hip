@@ -1,0 +1,325 @@
+// Layer norm of rows, and its gradients.
+//
+// A row's mean is taken first and its squared deviations from it second: sums of
+// squares alone would cancel where the mean is large against the deviations.
+#include "ps_rows.hpp"
+
+namespace ps {
+namespace {
+
+// A weight or bias vector of any type; null: all `otherwise`.
+struct Vec {
+  const void* data;
+  int dtype;
+  float otherwise;
+  template <int N>
+  __device__ __forceinline__ Floats<N> at(int c) const {
+    if (!data) return Floats<N>(otherwise);
+    if (dtype == PS_F32) return load_piece<N>(static_cast<const f32*>(data) + c);
+    if (dtype == PS_F16) return load_piece<N>(static_cast<const f16*>(data) + c);
+    return load_piece<N>(static_cast<const bf16*>(data) + c);
+  }
+};
+
+constexpr int kWideThreads = 1024;
+
+// Sum over the workgroup, in every thread.
+template <int kThreads>
+__device__ __forceinline__ float block_sum(float v) {
+  __shared__ float part[kThreads / kWave];
+#pragma unroll
+  for (int d = kWave / 2; d; d >>= 1) v += __shfl_xor(v, d, kWave);
+  __syncthreads();
+  if (lane_id() == 0) part[threadIdx.x / kWave] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int w = 0; w < kThreads / kWave; ++w) v += part[w];
+  return v;
+}
+
+// The elements of piece q that the piece before has not counted.
+template <int N, typename F>
+__device__ __forceinline__ void each_new(const Pieces& p, int q, F&& f) {
+  const int seen = q * N - p.begin(q);
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (e >= seen) f(e);
+}
+
+// Rows of any width: a workgroup a row, which is read three times.
+template <typename T, typename O, int N>
+__global__ __launch_bounds__(kWideThreads) void norm_wide_kernel(Mat<const T> x, Vec weight,
+                                                                 Vec bias, float eps, Mat<O> y,
+                                                                 float* __restrict__ mean_out,
+                                                                 float* __restrict__ rstd_out,
+                                                                 Pieces p) {
+  const int pieces = int(p.per_row.d);
+  for (long long r = blockIdx.x; r < x.rows; r += gridDim.x) {
+    float s = 0.f;
+    for (int q = threadIdx.x; q < pieces; q += kWideThreads) {
+      const Floats<N> v = load_piece<N>(x.at(r, p.begin(q)));
+      each_new<N>(p, q, [&](int e) { s += v[e]; });
+    }
+    const float mean = block_sum<kWideThreads>(s) / float(p.cols);
+    s = 0.f;
+    for (int q = threadIdx.x; q < pieces; q += kWideThreads) {
+      const Floats<N> v = load_piece<N>(x.at(r, p.begin(q))) - mean;
+      each_new<N>(p, q, [&](int e) { s += v[e] * v[e]; });
+    }
+    const float rstd = 1.f / sqrtf(block_sum<kWideThreads>(s) / float(p.cols) + eps);
+    for (int q = threadIdx.x; q < pieces; q += kWideThreads) {
+      const int c = p.begin(q);
+      const Floats<N> v = (load_piece<N>(x.at(r, c)) - mean) * rstd;
+      store_piece<N>(y.at(r, c), v * weight.at<N>(c) + bias.at<N>(c));
+    }
+    if (threadIdx.x == 0) {
+      if (mean_out) mean_out[r] = mean;
+      if (rstd_out) rstd_out[r] = rstd;
+    }
+  }
+}
+
+// dx of rows of any width: a workgroup a row, which is read twice.
+template <typename T, typename O, int N>
+__global__ __launch_bounds__(kWideThreads) void grad_wide_kernel(Mat<const O> dy, Mat<const T> x,
+                                                                 Vec weight,
+                                                                 const float* __restrict__ mean_in,
+                                                                 const float* __restrict__ rstd_in,
+                                                                 Mat<T> dx, Pieces p) {
+  const int pieces = int(p.per_row.d);
+  for (long long r = blockIdx.x; r < x.rows; r += gridDim.x) {
+    const float mean = mean_in[r], rstd = rstd_in[r];
+    float s = 0.f, sx = 0.f;
+    for (int q = threadIdx.x; q < pieces; q += kWideThreads) {
+      const int c = p.begin(q);
+      const Floats<N> g = load_piece<N>(dy.at(r, c)) * weight.at<N>(c);
+      const Floats<N> xh = (load_piece<N>(x.at(r, c)) - mean) * rstd;
+      each_new<N>(p, q, [&](int e) {
+        s += g[e];
+        sx += g[e] * xh[e];
+      });
+    }
+    s = block_sum<kWideThreads>(s) / float(p.cols);
+    sx = block_sum<kWideThreads>(sx) / float(p.cols);
+    for (int q = threadIdx.x; q < pieces; q += kWideThreads) {
+      const int c = p.begin(q);
+      const Floats<N> g = load_piece<N>(dy.at(r, c)) * weight.at<N>(c);
+      const Floats<N> xh = (load_piece<N>(x.at(r, c)) - mean) * rstd;
+      store_piece<N>(dx.at(r, c), rstd * (g - s - xh * sx));
+    }
+  }
+}
+
+// Parts of the sums over the rows: one piece of every row of a range a thread.
+// parts holds for each range dweight's sums and then dbias's.
+template <typename T, typename O, int N>
+__global__ __launch_bounds__(kRowThreads) void grad_columns_kernel(
+    Mat<const O> dy, Mat<const T> x, const float* __restrict__ mean_in,
+    const float* __restrict__ rstd_in, float* __restrict__ parts, Pieces p) {
+  const int q = blockIdx.x * kRowThreads + threadIdx.x;
+  if (q >= int(p.per_row.d)) return;
+  const int c = p.begin(q);
+  Floats<N> dw = 0.f, db = 0.f;
+  for (long long r = blockIdx.y; r < x.rows; r += gridDim.y) {
+    const Floats<N> g = load_piece<N>(dy.at(r, c));
+    dw += g * ((load_piece<N>(x.at(r, c)) - mean_in[r]) * rstd_in[r]);
+    db += g;
+  }
+  float* const to = parts + size_t(blockIdx.y) * 2 * p.cols + c;
+  each_new<N>(p, q, [&](int e) {
+    to[e] = dw[e];
+    to[p.cols + e] = db[e];
+  });
+}
+
+// Where the sums over the rows go; null data: not wanted.
+struct VecOut {
+  void* data;
+  int dtype;
+  __device__ __forceinline__ void put(int c, float v, bool add) const {
+    if (dtype == PS_F32)
+      put_as(static_cast<f32*>(data) + c, v, add);
+    else if (dtype == PS_F16)
+      put_as(static_cast<f16*>(data) + c, v, add);
+    else
+      put_as(static_cast<bf16*>(data) + c, v, add);
+  }
+  template <typename T>
+  static __device__ __forceinline__ void put_as(T* p, float v, bool add) {
+    *p = T(add ? float(*p) + v : v);
+  }
+};
+
+// The parts added up: 32 columns a workgroup, eight threads each. The columns of
+// dweight first, then dbias's.
+constexpr int kJoinCols = 32, kJoinLanes = kRowThreads / kJoinCols;
+__global__ __launch_bounds__(kRowThreads) void grad_join_kernel(const float* __restrict__ parts,
+                                                                int part_count, int cols,
+                                                                VecOut dweight, VecOut dbias,
+                                                                bool add) {
+  __shared__ float sums[kJoinLanes][kJoinCols];
+  const int lane = threadIdx.x / kJoinCols, i = threadIdx.x % kJoinCols;
+  const long long c = (long long)blockIdx.x * kJoinCols + i;
+  float s = 0.f;
+  if (c < 2LL * cols)
+    for (int k = lane; k < part_count; k += kJoinLanes) s += parts[size_t(k) * 2 * cols + c];
+  sums[lane][i] = s;
+  __syncthreads();
+  if (lane || c >= 2LL * cols) return;
+  for (int k = 1; k < kJoinLanes; ++k) s += sums[k][i];
+  const VecOut& to = c < cols ? dweight : dbias;
+  if (to.data) to.put(int(c < cols ? c : c - cols), s, add);
+}
+
+// ----------------------------------------------------------------- host side
+
+// Ranges of rows that the sums over them are cut into: enough to fill the
+// device, and no more than some 32 MB of parts.
+constexpr long long kParts = 1024, kFewParts = 16, kPartCells = 1 << 22;
+long long part_count(long long rows, long long cols) {
+  long long n = kPartCells / cols;
+  n = n < kFewParts ? kFewParts : n > kParts ? kParts : n;
+  return n < rows ? n : rows;
+}
+
+Vec vec(const ps_rows* m, float otherwise) {
+  return m ? Vec{m->data, m->dtype, otherwise} : Vec{nullptr, PS_F32, otherwise};
+}
+VecOut vec_out(const ps_rows* m) { return m ? VecOut{m->data, m->dtype} : VecOut{nullptr, PS_F32}; }
+Region vec_region(const ps_rows* m) { return m ? region(m) : region(nullptr, 0); }
+Region per_row(const float* p, const ps_rows* m) {
+  return region(p, size_t(m->rows) * sizeof(float));
+}
+
+uint32_t wide_blocks(long long rows) { return uint32_t(rows < 4096 ? rows : 4096); }
+
+}  // namespace
+}  // namespace ps
+
+#define PS_CHECK_VECTOR(m, cols_)                                                           \
+  do {                                                                                      \
+    if (m) {                                                                                \
+      PS_CHECK_ROWS(m);                                                                     \
+      PS_CHECK_ARG(m->rows == 1 && m->cols == (cols_),                                      \
+                   std::string(__func__) + ": " #m " is not one row of x's columns");       \
+    }                                                                                       \
+  } while (0)
+
+extern "C" {
+
+int ps_layer_norm(const ps_rows* x, const ps_rows* weight, const ps_rows* bias, float eps,
+                  const ps_rows* y, float* mean, float* rstd, ps_stream_t stream) {
+  PS_CHECK_ROWS(x);
+  PS_CHECK_ROWS(y);
+  PS_CHECK_ARG(x->rows == y->rows && x->cols == y->cols,
+               "ps_layer_norm: x and y differ in shape");
+  PS_CHECK_VECTOR(weight, x->cols);
+  PS_CHECK_VECTOR(bias, x->cols);
+  PS_CHECK_ARG(eps >= 0.f, "ps_layer_norm: eps is not a number from 0 up");
+  PS_CHECK_ARG(ps::aligned4(mean) && ps::aligned4(rstd),
+               "ps_layer_norm: misaligned mean or rstd");
+  const ps::Region in[] = {ps::region(x), ps::vec_region(weight), ps::vec_region(bias)};
+  const ps::Region to[] = {ps::region(y), ps::per_row(mean, x), ps::per_row(rstd, x)};
+  PS_CHECK_ARG(!ps::overlap(to[0], {in[0], in[1], in[2], to[1], to[2]}) &&
+                   !ps::overlap(to[1], {in[0], in[1], in[2], to[2]}) &&
+                   !ps::overlap(to[2], {in[0], in[1], in[2]}),
+               "ps_layer_norm: an output overlaps another argument");
+  if (!x->rows) return PS_OK;
+  return ps::with_dtype(x->dtype, [&](auto t) {
+    return ps::with_dtype(y->dtype, [&](auto o) {
+      using T = decltype(t);
+      using O = decltype(o);
+      constexpr int kSize = sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O);
+      return ps::with_width<kSize>(x->cols, [&](auto n) {
+        const ps::Pieces p(x->cols, n);
+        ps::norm_wide_kernel<T, O, n>
+            <<<ps::wide_blocks(x->rows), ps::kWideThreads, 0, ps::to_hip(stream)>>>(
+                ps::mat<const T>(x), ps::vec(weight, 1.f), ps::vec(bias, 0.f), eps, ps::mat<O>(y),
+                mean, rstd, p);
+        PS_LAUNCHED();
+        return int(PS_OK);
+      });
+    });
+  });
+}
+
+size_t ps_layer_norm_grad_workspace_bytes(long long rows, long long cols) {
+  if (rows < 0 || rows > (1LL << 48) || cols < 1 || cols > (1 << 24)) return 0;
+  // part_count's parts, or more where it rounds down
+  const long long most = ps::kParts * cols < ps::kPartCells ? ps::kParts * cols : ps::kPartCells;
+  const long long cells = most > ps::kFewParts * cols ? most : ps::kFewParts * cols;
+  const long long all = rows < (1 << 24) && rows * cols < cells ? rows * cols : cells;
+  return size_t(all < 2 ? 2 : all) * 2 * sizeof(float);
+}
+
+int ps_layer_norm_grad(const ps_rows* dy, const ps_rows* x, const ps_rows* weight,
+                       const float* mean, const float* rstd, int accumulate, const ps_rows* dx,
+                       const ps_rows* dweight, const ps_rows* dbias, void* workspace,
+                       size_t workspace_bytes, ps_stream_t stream) {
+  PS_CHECK_ROWS(dy);
+  PS_CHECK_ROWS(x);
+  PS_CHECK_ROWS(dx);
+  PS_CHECK_ARG(dy->rows == x->rows && dy->cols == x->cols && dx->rows == x->rows &&
+                   dx->cols == x->cols && dx->dtype == x->dtype,
+               "ps_layer_norm_grad: dy, x and dx differ in shape, or dx and x in type");
+  PS_CHECK_VECTOR(weight, x->cols);
+  PS_CHECK_VECTOR(dweight, x->cols);
+  PS_CHECK_VECTOR(dbias, x->cols);
+  PS_CHECK_ARG((mean && rstd) || !x->rows, "ps_layer_norm_grad: null mean or rstd");
+  PS_CHECK_ARG(ps::aligned4(mean) && ps::aligned4(rstd),
+               "ps_layer_norm_grad: misaligned mean or rstd");
+  const size_t need = ps_layer_norm_grad_workspace_bytes(x->rows, x->cols);
+  const bool sums = dweight || dbias;
+  PS_CHECK_ARG(!sums || (workspace && ps::aligned16(workspace) && workspace_bytes >= need),
+               "ps_layer_norm_grad: workspace too small or misaligned");
+  const ps::Region in[] = {ps::region(dy), ps::region(x), ps::vec_region(weight),
+                           ps::per_row(mean, x), ps::per_row(rstd, x)};
+  const ps::Region to[] = {ps::region(dx), ps::vec_region(dweight), ps::vec_region(dbias),
+                           ps::region(sums ? workspace : nullptr, need)};
+  for (int i = 0; i < 4; ++i) {
+    PS_CHECK_ARG(!ps::overlap(to[i], {in[0], in[1], in[2], in[3], in[4]}),
+                 "ps_layer_norm_grad: an output or the workspace overlaps an input");
+    for (int k = 0; k < i; ++k)
+      PS_CHECK_ARG(!ps::overlap(to[i], to[k]),
+                   "ps_layer_norm_grad: outputs and workspace overlap");
+  }
+  const hipStream_t st = ps::to_hip(stream);
+  float* const parts = static_cast<float*>(workspace);
+  const uint32_t part_count = uint32_t(ps::part_count(x->rows, x->cols));
+  if (x->rows) {
+    const int rc = ps::with_dtype(x->dtype, [&](auto t) {
+      return ps::with_dtype(dy->dtype, [&](auto o) {
+        using T = decltype(t);
+        using O = decltype(o);
+        constexpr int kSize = sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O);
+        return ps::with_width<kSize>(x->cols, [&](auto n) {
+          const ps::Pieces p(x->cols, n);
+          ps::grad_wide_kernel<T, O, n>
+              <<<ps::wide_blocks(x->rows), ps::kWideThreads, 0, st>>>(
+                  ps::mat<const O>(dy), ps::mat<const T>(x), ps::vec(weight, 1.f), mean, rstd,
+                  ps::mat<T>(dx), p);
+          PS_LAUNCHED();
+          if (sums) {
+            const dim3 grid((p.per_row.d + ps::kRowThreads - 1) / ps::kRowThreads, part_count);
+            ps::grad_columns_kernel<T, O, n><<<grid, ps::kRowThreads, 0, st>>>(
+                ps::mat<const O>(dy), ps::mat<const T>(x), mean, rstd, parts, p);
+            PS_LAUNCHED();
+          }
+          return int(PS_OK);
+        });
+      });
+    });
+    if (rc != PS_OK) return rc;
+  }
+  if (sums) {
+    const uint32_t blocks = uint32_t((2 * x->cols + ps::kJoinCols - 1) / ps::kJoinCols);
+    ps::grad_join_kernel<<<blocks, ps::kRowThreads, 0, st>>>(
+        parts, int(part_count), int(x->cols), ps::vec_out(dweight), ps::vec_out(dbias),
+        accumulate != 0);
+    PS_LAUNCHED();
+  }
+  return PS_OK;
+}
+
+}  // extern "C"

@@ -157,6 +157,8 @@ inline const char* ids_error(const ps_ids* ids) {
       return ps::fail(PS_ERR_INVALID, std::string(__func__) + ": " #ids ": " + ps_error_);     \
   } while (0)
 
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
 // Device memory that a call reads or writes: rows of `bytes`, `pitch` apart.
 struct Region {
   uintptr_t at;

@@ -1,6 +1,6 @@
 """Row operators on the device: embedding lookup and its gradient, tokens sorted by expert
-and back with their gradients, and the norm and clipping of many gradient tensors
-(include/powersparse_rows.h).
+and back with their gradients, the router that chooses them, layer norm and its gradients, the
+norm and clipping of many gradient tensors, and AdamW (include/powersparse_rows.h).
 
 Arrays are in the current device's memory: DeviceArray (a DeviceBuffer or raw pointer with
 a shape and a type) or any tensor object with data_ptr, shape, stride, dtype and is_cuda,
@@ -14,7 +14,7 @@ the stream has passed the call. Wrong arguments raise ValueError.
 import ctypes
 
 from . import _native
-from ._native import Ids, Rows
+from ._native import AdamWOptions, AdamWTensor, Ids, Rows
 
 
 class _Library:
@@ -373,6 +373,119 @@ def ExpertCombineGrad(dy, ys, position, weights, dys, dweights, stream=None):
         _stream(stream)))
 
 
+def expert_route_workspace_bytes(tokens, experts):
+    """Workspace of ExpertRoute for `tokens` tokens and `experts` experts, or for fewer of
+    either."""
+    n = _hip.ps_expert_route_workspace_bytes(_fit(tokens, _LONG), _fit(experts, _INT))
+    if not n:
+        raise ValueError("expert_route_workspace_bytes: sizes out of range (1 to 1024 experts)")
+    return n
+
+
+def ExpertRoute(logits, ids, weights, counts=None, loss=None, workspace=None, mask=None,
+                normalize=True, stream=None):
+    """The top_k experts of every token by its row of logits (tokens x experts), in descending
+    order, equal ones by ascending expert: `ids` (tokens x top_k, int32) and their `weights`
+    (float32), the softmax's probabilities, with normalize=True divided by their sum. Experts
+    of logit -inf are never chosen; places left over have id -1 and weight 0. `mask` (bool or
+    uint8, one a token): 0 for padding, which takes no part.
+
+    `counts` (experts + 1, int32) receives how often each expert was chosen and, last, the
+    tokens that take part; `loss` (one float32) the balance loss, experts * sum of f_e * P_e with
+    f_e the share of the choices that is e's and P_e its mean probability. None: not wanted, and
+    no workspace either."""
+    if _several is not False:
+        _check_devices(logits, ids, weights, counts, loss, workspace, mask)
+    src = _rows(logits, "logits")
+    at, top_k = _slots(ids, "ids", "int32", src.rows)
+    out = _slots(weights, "weights", "float32", src.rows, src.rows * top_k)[0]
+    ptr, nbytes = (None, 0) if workspace is None else _space(workspace)
+    _call(_hip.ps_expert_route(
+        src, top_k, bool(normalize),
+        None if mask is None else _flat(mask, "mask", ("bool", "uint8"), src.rows)[0], at, out,
+        None if counts is None else _flat(counts, "counts", ("int32",), src.cols + 1)[0],
+        None if loss is None else _flat(loss, "loss", ("float32",), 1)[0], ptr, nbytes,
+        _stream(stream)))
+
+
+def ExpertRouteGrad(logits, ids, dweights, counts, dloss, dlogits, normalize=True, stream=None):
+    """dlogits (of the logits' type) = the gradient of sum(dweights * weights) + dloss * loss of
+    an ExpertRoute that gave `ids` and `counts`; dweights or dloss (one float32 on the device)
+    None: without it. Counts summed over the ranks of a job give the gradient of the loss over
+    all their tokens."""
+    if _several is not False:
+        _check_devices(logits, ids, dweights, counts, dloss, dlogits)
+    src = _rows(logits, "logits")
+    at, top_k = _slots(ids, "ids", "int32", src.rows)
+    dw = None
+    if dweights is not None:
+        dw = _slots(dweights, "dweights", "float32", src.rows, src.rows * top_k)[0]
+    _call(_hip.ps_expert_route_grad(
+        src, top_k, bool(normalize), at, dw,
+        None if counts is None else _flat(counts, "counts", ("int32",), src.cols + 1)[0],
+        None if dloss is None else _flat(dloss, "dloss", ("float32",), 1)[0],
+        _rows(dlogits, "dlogits"), _stream(stream)))
+
+
+# -------------------------------------------------------------- layer norm
+
+def _vector(x, name):
+    """The ps_rows of a contiguous vector, one row; None for None."""
+    if x is None:
+        return None
+    try:
+        if x.is_cuda and x.is_contiguous():
+            cols, = x.shape
+            return Rows(x.data_ptr(), 1, cols, cols, _row_codes[x.dtype])
+    except (AttributeError, KeyError, TypeError, ValueError):
+        pass
+    if len(_described(x, name)[1]) != 1:
+        raise ValueError(f"{name} is not a vector")
+    ptr, n, said = _flat(x, name, _DTYPES)
+    return Rows(ptr, 1, n, n, _DTYPES[said])
+
+
+def _per_row(x, name, rows):
+    """Address of a float32 for each row; None for None."""
+    return None if x is None else _flat(x, name, ("float32",), rows)[0]
+
+
+def LayerNorm(x, weight, bias, y, mean=None, rstd=None, eps=1e-5, stream=None):
+    """y = (x - mean) * rstd * weight + bias for every row of x, with its mean and
+    rstd = 1 / sqrt(its variance + eps). weight and bias are vectors of x's columns, or None
+    (ones, zeros); mean and rstd (float32, one a row) receive what LayerNormGrad needs. All
+    types may differ."""
+    if _several is not False:
+        _check_devices(x, weight, bias, y, mean, rstd)
+    src = _rows(x, "x")
+    _call(_hip.ps_layer_norm(
+        src, _vector(weight, "weight"), _vector(bias, "bias"), eps, _rows(y, "y"),
+        _per_row(mean, "mean", src.rows), _per_row(rstd, "rstd", src.rows), _stream(stream)))
+
+
+def layer_norm_grad_workspace_bytes(rows, cols):
+    """Workspace of LayerNormGrad for `rows` rows of `cols`, or for fewer of either."""
+    n = _hip.ps_layer_norm_grad_workspace_bytes(_fit(rows, _LONG), _fit(cols, _LONG))
+    if not n:
+        raise ValueError("layer_norm_grad_workspace_bytes: sizes out of range")
+    return n
+
+
+def LayerNormGrad(dy, x, weight, mean, rstd, dx, dweight, dbias, workspace, accumulate=False,
+                  stream=None):
+    """The gradients of LayerNorm: dx (of x's type), and dweight and dbias, vectors summed over
+    the rows (accumulate=True: added to them; None: not wanted, and workspace may be None where
+    both are). The sums' order is fixed: the same bits every time."""
+    if _several is not False:
+        _check_devices(dy, x, weight, mean, rstd, dx, dweight, dbias, workspace)
+    src = _rows(x, "x")
+    ptr, nbytes = (None, 0) if workspace is None else _space(workspace)
+    _call(_hip.ps_layer_norm_grad(
+        _rows(dy, "dy"), src, _vector(weight, "weight"), _per_row(mean, "mean", src.rows),
+        _per_row(rstd, "rstd", src.rows), bool(accumulate), _rows(dx, "dx"),
+        _vector(dweight, "dweight"), _vector(dbias, "dbias"), ptr, nbytes, _stream(stream)))
+
+
 # --------------------------------------------------------------- gradients
 
 def _spans(arrays, what):
@@ -463,3 +576,116 @@ def ClipGradNorm(grads, max_norm, norm, grad_scale=1.0, stream=None):
         _check_devices(grads, norm)
     _call(_hip.ps_clip_grad_norm(grads.handle, max_norm, grad_scale,
                                  _flat(norm, "norm", ("float32",), 1)[0], _stream(stream)))
+
+
+# ------------------------------------------------------------------- AdamW
+
+STATE_BLOCK = 256  # elements of an 8-bit state that share a pair of scales
+
+
+def state_blocks(elements):
+    """Pairs of scales of an 8-bit state of so many elements."""
+    return -(-int(elements) // STATE_BLOCK)
+
+
+class AdamWList:
+    """The tensors that AdamWStep updates, all contiguous: `params` (float32, float16 or
+    bfloat16), their `grads` of the same sizes (only read, any of these types), and the moments
+    `exp_avgs` and `exp_avg_sqs`, either float32, or of one byte an element (uint8, or a tensor
+    library's float8_e4m3fn) with `scales`: two float32 for every STATE_BLOCK elements of a
+    tensor, (state_blocks(elements), 2). Moments and scales begin with zeros. `copies`, a tensor
+    or None for each, receive the new parameters rounded to their type; `weight_decay` is a number
+    or one for each. Made once while the tensors stay where they are, as making it uploads and
+    waits for the device; steps of one list must not overlap. Keeps the tensors alive. Closing it,
+    or losing it, waits for nothing."""
+
+    def __init__(self, params, grads, exp_avgs, exp_avg_sqs, scales=None, copies=None,
+                 weight_decay=0.01):
+        self._h = None
+        n = len(params)
+        decay = list(weight_decay) if hasattr(weight_decay, "__len__") else [weight_decay] * n
+        given = dict(grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs, scales=scales,
+                     copies=copies, weight_decay=decay)
+        for name, x in given.items():
+            if x is not None and len(x) != n:
+                raise ValueError(f"{name}: one for each parameter")
+        self._keep = [list(x) for x in (params, grads, exp_avgs, exp_avg_sqs, scales or (),
+                                        copies or ())]
+        params, grads, exp_avgs, exp_avg_sqs, scales, copies = self._keep
+        if _several is not False:
+            _check_devices(*(x for xs in self._keep for x in xs))
+        state = ("uint8", "float8_e4m3fn") if scales else ("float32",)
+        table = (AdamWTensor * max(n, 1))()
+        for i in range(n):
+            t = table[i]
+            t.param, t.count, said = _flat(params[i], f"parameter {i}", _DTYPES)
+            t.param_dtype = _DTYPES[said]
+            t.grad, _, said = _flat(grads[i], f"gradient {i}", _DTYPES, t.count)
+            t.grad_dtype = _DTYPES[said]
+            t.exp_avg = _flat(exp_avgs[i], f"exp_avg {i}", state, t.count)[0]
+            t.exp_avg_sq = _flat(exp_avg_sqs[i], f"exp_avg_sq {i}", state, t.count)[0]
+            if scales:
+                t.scales = _flat(scales[i], f"scales {i}", ("float32",),
+                                 2 * state_blocks(t.count))[0]
+            if copies and copies[i] is not None:
+                t.copy, _, said = _flat(copies[i], f"copy {i}", _DTYPES, t.count)
+                t.copy_dtype = _DTYPES[said]
+            t.weight_decay = decay[i]
+        h = ctypes.c_void_p()
+        _call(_hip.ps_adamw_list_create(n, table, _E4M3 if scales else 0, ctypes.byref(h)))
+        self._h = h.value
+        self._device = _current_device()
+
+    def get_device(self):
+        """The device it was made on."""
+        return self._device
+
+    @property
+    def handle(self):
+        if not self._h:
+            raise ValueError("the AdamW list is closed")
+        return self._h
+
+    def close(self):
+        if self._h:
+            _hip.ps_adamw_list_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+_E4M3 = 3
+
+
+def AdamWStep(tensors, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, norm=None, max_norm=None,
+              grad_scale=1.0, stream=None):
+    """One update of an AdamWList with g = grad_scale * grad:
+
+        m = beta1 * m + (1 - beta1) * g,  v = beta2 * v + (1 - beta2) * g^2
+        p -= lr * (decay * p + (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps))
+
+    `step` counts from 1. lr and step are numbers, or one float32 and one int32 on the device,
+    read when the step runs. With `norm` (one float32 on the device, GradNorm's of grad_scale *
+    grad) g is also multiplied by min(1, max_norm / (norm + 1e-6)) on the way, max_norm None: not,
+    and a norm that is not finite leaves everything as it is."""
+    if _several is not False:
+        _check_devices(tensors, lr, step, norm)
+    o = AdamWOptions(beta1=beta1, beta2=beta2, eps=eps, grad_scale=grad_scale,
+                     max_norm=float("inf") if max_norm is None else max_norm)
+    if type(lr) is DeviceArray or hasattr(lr, "data_ptr"):
+        o.device_lr = _flat(lr, "lr", ("float32",), 1)[0]
+    else:
+        o.lr = lr
+    if type(step) is DeviceArray or hasattr(step, "data_ptr"):
+        o.device_step = _flat(step, "step", ("int32",), 1)[0]
+    else:
+        o.step = _fit(step, _LONG)
+    if norm is not None:
+        o.norm = _flat(norm, "norm", ("float32",), 1)[0]
+    elif max_norm is not None:
+        raise ValueError("max_norm needs the norm")
+    _call(_hip.ps_adamw_step(tensors.handle, ctypes.byref(o), _stream(stream)))
