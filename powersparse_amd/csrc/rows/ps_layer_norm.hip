@@ -1,7 +1,14 @@
 // Layer norm of rows, and its gradients.
 //
 // A row's mean is taken first and its squared deviations from it second: sums of
-// squares alone would cancel where the mean is large against the deviations.
+// squares alone would cancel where the mean is large against the deviations. A row
+// of up to 4,096 pieces stays in the registers of kLanes threads, kPieces each, and
+// is read once; these threads go from row to row, so weight and bias are loaded
+// once, and in the gradient a thread's columns stay the same: it adds up their
+// dweight and dbias in registers and leaves one sum a workgroup, which a second
+// launch adds up in order. No atomics: the same bits every time.
+#include <algorithm>
+
 #include "ps_rows.hpp"
 
 namespace ps {
@@ -45,6 +52,191 @@ __device__ __forceinline__ void each_new(const Pieces& p, int q, F&& f) {
 #pragma unroll
   for (int e = 0; e < N; ++e)
     if (e >= seen) f(e);
+}
+
+// Sums over the kLanes threads of a row, in every one of them. part: room for
+// them where these are a workgroup; two rooms are used in turn, so that one
+// barrier does: a thread that writes a room again has passed the other's.
+template <int kLanes>
+struct RowParts {
+  float of[2][2][kLanes > kWave ? kLanes / kWave : 1];
+};
+template <int kLanes, int kSums>
+__device__ __forceinline__ void row_sums(float (&v)[kSums], RowParts<kLanes>& part, int turn) {
+#pragma unroll
+  for (int d = (kLanes < kWave ? kLanes : kWave) / 2; d; d >>= 1)
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) v[k] += __shfl_xor(v[k], d, kWave);
+  if constexpr (kLanes > kWave) {
+    if (lane_id() == 0)
+#pragma unroll
+      for (int k = 0; k < kSums; ++k) part.of[turn][k][threadIdx.x / kWave] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kLanes / kWave; ++w) v[k] += part.of[turn][k][w];
+    }
+  }
+}
+
+constexpr int threads_of(int lanes) { return lanes > kRowThreads ? lanes : kRowThreads; }
+
+template <typename T, typename O, int N, int kLanes, int kPieces>
+__global__ __launch_bounds__(threads_of(kLanes)) void norm_kernel(Mat<const T> x, Vec weight,
+                                                                  Vec bias, float eps, Mat<O> y,
+                                                                  float* __restrict__ mean_out,
+                                                                  float* __restrict__ rstd_out,
+                                                                  Pieces p) {
+  constexpr int kRows = threads_of(kLanes) / kLanes;
+  __shared__ RowParts<kLanes> part;
+  const int lane = threadIdx.x % kLanes, pieces = int(p.per_row.d);
+  using V = typename PieceOf<T, N>::type;
+  Floats<N> w[kPieces], b[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int q = i * kLanes + lane;
+    if (q >= pieces) continue;
+    w[i] = weight.at<N>(p.begin(q));
+    b[i] = bias.at<N>(p.begin(q));
+  }
+  // threads without a row go along: the sums take every lane
+  for (long long r0 = (long long)blockIdx.x * kRows; r0 < x.rows; r0 += (long long)gridDim.x * kRows) {
+    const long long mine = r0 + threadIdx.x / kLanes, r = min(mine, x.rows - 1);
+    V v[kPieces];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int q = i * kLanes + lane;
+      if (q < pieces) v[i] = *reinterpret_cast<const V*>(x.at(r, p.begin(q)));
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int q = i * kLanes + lane;
+      const Floats<N> f = __builtin_convertvector(v[i], Floats<N>);
+      if (q < pieces) each_new<N>(p, q, [&](int e) { s[0] += f[e]; });
+    }
+    row_sums(s, part, 0);
+    const float mean = s[0] / float(p.cols);
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int q = i * kLanes + lane;
+      const Floats<N> f = __builtin_convertvector(v[i], Floats<N>) - mean;
+      if (q < pieces) each_new<N>(p, q, [&](int e) { s[0] += f[e] * f[e]; });
+    }
+    row_sums(s, part, 1);
+    const float rstd = 1.f / sqrtf(s[0] / float(p.cols) + eps);
+    if (mine >= x.rows) continue;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int q = i * kLanes + lane;
+      if (q >= pieces) continue;
+      const Floats<N> f = (__builtin_convertvector(v[i], Floats<N>) - mean) * rstd;
+      store_piece<N>(y.at(r, p.begin(q)), f * w[i] + b[i]);
+    }
+    if (lane == 0) {
+      if (mean_out) mean_out[r] = mean;
+      if (rstd_out) rstd_out[r] = rstd;
+    }
+  }
+}
+
+// parts: see grad_columns_kernel; null: not wanted.
+template <typename T, typename O, int N, int kLanes, int kPieces>
+__global__ __launch_bounds__(threads_of(kLanes)) void grad_kernel(
+    Mat<const O> dy, Mat<const T> x, Vec weight, const float* __restrict__ mean_in,
+    const float* __restrict__ rstd_in, Mat<T> dx, float* __restrict__ parts, Pieces p) {
+  constexpr int kThreads = threads_of(kLanes), kRows = kThreads / kLanes;
+  __shared__ RowParts<kLanes> part;
+  const int lane = threadIdx.x % kLanes, pieces = int(p.per_row.d);
+  using V = typename PieceOf<T, N>::type;
+  using G = typename PieceOf<O, N>::type;
+  Floats<N> w[kPieces], dw[kPieces], db[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int q = i * kLanes + lane;
+    dw[i] = db[i] = 0.f;
+    if (q < pieces) w[i] = weight.at<N>(p.begin(q));
+  }
+  int turn = 0;
+  for (long long r0 = (long long)blockIdx.x * kRows; r0 < x.rows; r0 += (long long)gridDim.x * kRows) {
+    const long long mine = r0 + threadIdx.x / kLanes, r = min(mine, x.rows - 1);
+    const float mean = mean_in[r], rstd = rstd_in[r];
+    V v[kPieces];
+    G g[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int q = i * kLanes + lane;
+      if (q >= pieces) continue;
+      v[i] = *reinterpret_cast<const V*>(x.at(r, p.begin(q)));
+      g[i] = *reinterpret_cast<const G*>(dy.at(r, p.begin(q)));
+    }
+    float s[2] = {0.f, 0.f};  // of g and of g * xh
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int q = i * kLanes + lane;
+      if (q >= pieces || mine >= x.rows) continue;
+      const Floats<N> xh = (__builtin_convertvector(v[i], Floats<N>) - mean) * rstd;
+      const Floats<N> f = __builtin_convertvector(g[i], Floats<N>), gw = f * w[i];
+      dw[i] += f * xh;
+      db[i] += f;
+      each_new<N>(p, q, [&](int e) {
+        s[0] += gw[e];
+        s[1] += gw[e] * xh[e];
+      });
+    }
+    row_sums(s, part, turn);
+    turn ^= 1;
+    const float mean_g = s[0] / float(p.cols), mean_gx = s[1] / float(p.cols);
+    if (mine >= x.rows) continue;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int q = i * kLanes + lane;
+      if (q >= pieces) continue;
+      const Floats<N> xh = (__builtin_convertvector(v[i], Floats<N>) - mean) * rstd;
+      const Floats<N> gw = __builtin_convertvector(g[i], Floats<N>) * w[i];
+      store_piece<N>(dx.at(r, p.begin(q)), rstd * (gw - mean_g - xh * mean_gx));
+    }
+  }
+  if (!parts) return;
+  float* const to = parts + size_t(blockIdx.x) * 2 * p.cols;
+  if constexpr (kRows == 1) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int q = i * kLanes + lane;
+      if (q >= pieces) continue;
+      const int c = p.begin(q);
+      each_new<N>(p, q, [&](int e) {
+        to[c + e] = dw[i][e];
+        to[p.cols + c + e] = db[i][e];
+      });
+    }
+  } else {
+    // The rows of the workgroup, in order: element by element through shared memory.
+    __shared__ float rows[kThreads * N];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < N; ++e) rows[threadIdx.x * N + e] = half ? db[i][e] : dw[i][e];
+        __syncthreads();
+        for (int at = threadIdx.x; at < kLanes * N; at += kThreads) {
+          const int q = i * kLanes + at / N;
+          if (q >= pieces) continue;
+          const int c = p.begin(q) + at % N;
+          if (c < q * N) continue;  // the piece before has it
+          float sum = 0.f;
+#pragma unroll
+          for (int m = 0; m < kRows; ++m) sum += rows[m * kLanes * N + at];
+          to[half * p.cols + c] = sum;
+        }
+      }
+    }
+  }
 }
 
 // Rows of any width: a workgroup a row, which is read three times.
@@ -194,6 +386,36 @@ Region per_row(const float* p, const ps_rows* m) {
 
 uint32_t wide_blocks(long long rows) { return uint32_t(rows < 4096 ? rows : 4096); }
 
+// Workgroups of the forward pass: as many as the device holds at once.
+constexpr long long kNormBlocks = 2048;
+uint32_t norm_blocks(long long rows, int per_block) {
+  const long long n = (rows + per_block - 1) / per_block;
+  return uint32_t(n < kNormBlocks ? n : kNormBlocks);
+}
+
+// Calls f(lanes, pieces of a lane) for rows of p's pieces, or f(0, 0) for wider ones.
+template <int N, typename F>
+int with_lanes(const Pieces& p, F&& f) {
+  const uint32_t n = p.per_row.d;
+  const auto call = [&](auto lanes, auto per) { return f(lanes, per); };
+  using std::integral_constant;
+  if (n <= 8) return call(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+  if constexpr (N == 1) {
+    return call(integral_constant<int, 0>{}, integral_constant<int, 0>{});  // (fewer than 8)
+  } else {
+    if (n <= 16) return call(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    if (n <= 32) return call(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+    if (n <= 64) return call(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    if (n <= 128) return call(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    if (n <= 256) return call(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    if (n <= 512) return call(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    if (n <= 1024) return call(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    if (n <= 2048) return call(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+    if (n <= 4096) return call(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+    return call(integral_constant<int, 0>{}, integral_constant<int, 0>{});
+  }
+}
+
 }  // namespace
 }  // namespace ps
 
@@ -233,12 +455,22 @@ int ps_layer_norm(const ps_rows* x, const ps_rows* weight, const ps_rows* bias, 
       constexpr int kSize = sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O);
       return ps::with_width<kSize>(x->cols, [&](auto n) {
         const ps::Pieces p(x->cols, n);
-        ps::norm_wide_kernel<T, O, n>
-            <<<ps::wide_blocks(x->rows), ps::kWideThreads, 0, ps::to_hip(stream)>>>(
+        return ps::with_lanes<n>(p, [&](auto lanes, auto per) {
+          const auto run = [&](auto kernel, uint32_t blocks, int threads) {
+            kernel<<<blocks, threads, 0, ps::to_hip(stream)>>>(
                 ps::mat<const T>(x), ps::vec(weight, 1.f), ps::vec(bias, 0.f), eps, ps::mat<O>(y),
                 mean, rstd, p);
-        PS_LAUNCHED();
-        return int(PS_OK);
+          };
+          if constexpr (lanes == 0) {
+            run(ps::norm_wide_kernel<T, O, n>, ps::wide_blocks(x->rows), ps::kWideThreads);
+          } else {
+            constexpr int kThreads = ps::threads_of(lanes);
+            run(ps::norm_kernel<T, O, n, lanes, per>, ps::norm_blocks(x->rows, kThreads / lanes),
+                kThreads);
+          }
+          PS_LAUNCHED();
+          return int(PS_OK);
+        });
       });
     });
   });
@@ -286,7 +518,7 @@ int ps_layer_norm_grad(const ps_rows* dy, const ps_rows* x, const ps_rows* weigh
   }
   const hipStream_t st = ps::to_hip(stream);
   float* const parts = static_cast<float*>(workspace);
-  const uint32_t part_count = uint32_t(ps::part_count(x->rows, x->cols));
+  uint32_t part_count = uint32_t(ps::part_count(x->rows, x->cols));
   if (x->rows) {
     const int rc = ps::with_dtype(x->dtype, [&](auto t) {
       return ps::with_dtype(dy->dtype, [&](auto o) {
@@ -295,18 +527,27 @@ int ps_layer_norm_grad(const ps_rows* dy, const ps_rows* x, const ps_rows* weigh
         constexpr int kSize = sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O);
         return ps::with_width<kSize>(x->cols, [&](auto n) {
           const ps::Pieces p(x->cols, n);
-          ps::grad_wide_kernel<T, O, n>
-              <<<ps::wide_blocks(x->rows), ps::kWideThreads, 0, st>>>(
+          return ps::with_lanes<n>(p, [&](auto lanes, auto per) {
+            if constexpr (lanes == 0) {
+              ps::grad_wide_kernel<T, O, n>
+                  <<<ps::wide_blocks(x->rows), ps::kWideThreads, 0, st>>>(
+                      ps::mat<const O>(dy), ps::mat<const T>(x), ps::vec(weight, 1.f), mean, rstd,
+                      ps::mat<T>(dx), p);
+              PS_LAUNCHED();
+              if (!sums) return int(PS_OK);
+              const dim3 grid((p.per_row.d + ps::kRowThreads - 1) / ps::kRowThreads, part_count);
+              ps::grad_columns_kernel<T, O, n><<<grid, ps::kRowThreads, 0, st>>>(
+                  ps::mat<const O>(dy), ps::mat<const T>(x), mean, rstd, parts, p);
+            } else {
+              constexpr int kThreads = ps::threads_of(lanes), kRows = kThreads / lanes;
+              part_count = std::min(part_count, uint32_t((x->rows + kRows - 1) / kRows));
+              ps::grad_kernel<T, O, n, lanes, per><<<part_count, kThreads, 0, st>>>(
                   ps::mat<const O>(dy), ps::mat<const T>(x), ps::vec(weight, 1.f), mean, rstd,
-                  ps::mat<T>(dx), p);
-          PS_LAUNCHED();
-          if (sums) {
-            const dim3 grid((p.per_row.d + ps::kRowThreads - 1) / ps::kRowThreads, part_count);
-            ps::grad_columns_kernel<T, O, n><<<grid, ps::kRowThreads, 0, st>>>(
-                ps::mat<const O>(dy), ps::mat<const T>(x), mean, rstd, parts, p);
+                  ps::mat<T>(dx), sums ? parts : nullptr, p);
+            }
             PS_LAUNCHED();
-          }
-          return int(PS_OK);
+            return int(PS_OK);
+          });
         });
       });
     });
