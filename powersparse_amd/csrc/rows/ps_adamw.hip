@@ -52,7 +52,7 @@ struct AdamCall {
   const float* device_lr;
   const int* device_step;
   const float* norm;
-  double max_norm, grad_scale;
+  float max_norm, grad_scale;
 };
 // The same as an element needs it.
 struct AdamStep {
@@ -63,25 +63,33 @@ struct AdamStep {
 
 // False: the norm is not finite, nothing is to change.
 __device__ __forceinline__ bool make_step(const AdamCall& c, AdamStep* s) {
-  double scale = c.grad_scale;
+  float scale = c.grad_scale;
   if (c.norm) {
-    const double n = *c.norm;
-    if (!(fabs(n) < INFINITY)) return false;
-    const double ratio = c.max_norm / (n + 1e-6);
-    if (ratio < 1.0) scale *= ratio;
+    const float n = *c.norm;
+    if (!(fabsf(n) < INFINITY)) return false;
+    scale *= fminf(c.max_norm * (1.f / (n + 1e-6f)), 1.f);
   }
   const long long t = c.device_step ? max(*c.device_step, 1) : c.step;
   *s = {c.beta1, c.one_beta1, c.beta2, c.one_beta2, c.eps, c.device_lr ? *c.device_lr : c.lr,
-        float(scale), float(-1.0 / expm1(double(t) * c.log_beta1)),
+        scale, float(-1.0 / expm1(double(t) * c.log_beta1)),
         float(1.0 / sqrt(-expm1(double(t) * c.log_beta2))), uint32_t(t) * kByStep};
   return true;
 }
 
-// m and v after the gradient g.
+// m and v after the gradient g. Every product and sum is rounded by itself, in the
+// order of the formulas: what decides between two codes of an 8-bit moment is then
+// the same wherever the formulas are computed in FP32, and so are the codes.
 __device__ __forceinline__ void advance(const AdamStep& s, float g, float* m, float* v) {
-  g *= s.grad_scale;
-  *m = fmaf(s.beta1, *m, s.one_beta1 * g);
-  *v = fmaf(s.beta2, *v, s.one_beta2 * g * g);
+#pragma clang fp contract(off)
+  g = g * s.grad_scale;
+  *m = s.beta1 * *m + s.one_beta1 * g;
+  *v = s.beta2 * *v + s.one_beta2 * g * g;
+}
+// x / d, correctly rounded but for the rarest cases, with by = 1 / d: one step of
+// Newton's iteration on the quotient (Markstein 1990).
+__device__ __forceinline__ float quotient(float x, float d, float by) {
+  const float q = x * by;
+  return fmaf(fmaf(-q, d, x), by, q);
 }
 // The parameter after a step by m and the root of v. The reciprocal is the
 // hardware's, off by a unit in the last place: of the update, which is smaller
@@ -134,9 +142,7 @@ __device__ void chunk_f32(const AdamTensor& t, const AdamStep& s, long long from
 }
 
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = kWave / 2; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
-  return v;
+  return lanes_all<kWave>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // The magnitude `a` (up to 448) on the grid of E4M3, rounded by u (32 bits). The
@@ -212,7 +218,7 @@ __device__ void block_f8(const AdamTensor& t, const AdamStep& s, long long from)
   for (int e = 0; e < 4; ++e) {
     float me = m[e], ve = r[e] * r[e];
     advance(s, g[e], &me, &ve);
-    const float root = __builtin_amdgcn_sqrtf(ve);
+    const float root = sqrtf(ve);
     p[e] = updated(s, t.decay, p[e], me, root);
     m[e] = me;
     r[e] = root;
@@ -221,13 +227,14 @@ __device__ void block_f8(const AdamTensor& t, const AdamStep& s, long long from)
   }
   m_most = wave_max(m_most);
   r_most = wave_max(r_most);
-  const float m_scale = fmaxf(m_most / 448.f, 0x1p-126f), r_scale = fmaxf(r_most / 448.f, 0x1p-126f);
+  const float m_scale = fmaxf(m_most * (1.f / 448.f), 0x1p-126f);
+  const float r_scale = fmaxf(r_most * (1.f / 448.f), 0x1p-126f);
   const float by_m = 1.f / m_scale, by_r = 1.f / r_scale;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const uint32_t u = uint32_t(i + e) * kByElement + s.weyl;
-    m[e] = copysignf(on_grid(fabsf(m[e]) * by_m, u), m[e]);
-    const float code = on_grid(r[e] * by_r, u);
+    m[e] = copysignf(on_grid(quotient(fabsf(m[e]), m_scale, by_m), u), m[e]);
+    const float code = on_grid(quotient(r[e], r_scale, by_r), u);
     r[e] = r[e] > 0.f ? fmaxf(code, 0x1p-9f) : code;
   }
   store_some(param, p, n);
@@ -406,8 +413,8 @@ int ps_adamw_step(ps_adamw_list* list, const ps_adamw_options* o, ps_stream_t st
                           o->device_lr,
                           o->device_step,
                           o->norm,
-                          double(o->max_norm),
-                          double(o->grad_scale)};
+                          o->max_norm,
+                          o->grad_scale};
   const uint32_t blocks = std::min(list->adam.chunk_count, ps::kAdamBlocks);
   const hipStream_t st = ps::to_hip(stream);
   if (list->in_8_bits)

@@ -29,22 +29,12 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 
 // Over the kLanes lanes of a token, in every one of them.
 template <int kLanes>
-__device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int d = kLanes / 2; d; d >>= 1) v += __shfl_xor(v, d, kWave);
-  return v;
-}
-template <int kLanes>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-#pragma unroll
-  for (int d = kLanes / 2; d; d >>= 1) v = max(v, uint32_t(__shfl_xor(int(v), d, kWave)));
-  return v;
+  return lanes_all<kLanes>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 template <int kLanes>
 __device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
-#pragma unroll
-  for (int d = kLanes / 2; d; d >>= 1) v = min(v, uint32_t(__shfl_xor(int(v), d, kWave)));
-  return v;
+  return lanes_all<kLanes>(v, [](uint32_t a, uint32_t b) { return min(a, b); });
 }
 
 // What the workgroups leave of the loss: sums of probabilities, and choices of
@@ -243,8 +233,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_grad_kernel(
       top = fmaxf(top, p[r]);
       h[r] = by_loss[r];
     }
-#pragma unroll
-    for (int d = kLanes / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
+    top = lanes_all<kLanes>(top, [](float a, float b) { return fmaxf(a, b); });
     if (top == -INFINITY) top = 0.f;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {

@@ -34,8 +34,7 @@ constexpr int kWideThreads = 1024;
 template <int kThreads>
 __device__ __forceinline__ float block_sum(float v) {
   __shared__ float part[kThreads / kWave];
-#pragma unroll
-  for (int d = kWave / 2; d; d >>= 1) v += __shfl_xor(v, d, kWave);
+  v = lanes_sum<kWave>(v);
   __syncthreads();
   if (lane_id() == 0) part[threadIdx.x / kWave] = v;
   __syncthreads();
@@ -64,9 +63,7 @@ struct RowParts {
 template <int kLanes, int kSums>
 __device__ __forceinline__ void row_sums(float (&v)[kSums], RowParts<kLanes>& part, int turn) {
 #pragma unroll
-  for (int d = (kLanes < kWave ? kLanes : kWave) / 2; d; d >>= 1)
-#pragma unroll
-    for (int k = 0; k < kSums; ++k) v[k] += __shfl_xor(v[k], d, kWave);
+  for (int k = 0; k < kSums; ++k) v[k] = lanes_sum<(kLanes < kWave ? kLanes : kWave)>(v[k]);
   if constexpr (kLanes > kWave) {
     if (lane_id() == 0)
 #pragma unroll

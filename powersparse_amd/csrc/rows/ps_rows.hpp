@@ -56,6 +56,35 @@ __device__ __forceinline__ void store_piece(T* p, const Floats<N>& f) {
   }
 }
 
+// op over groups of kLanes neighbouring lanes (8 to 64), in every one of them; all
+// lanes of the wave are active. Vector instructions alone, without the shared
+// memory's latency: inside 16 lanes by permuted reads (quads, then mirrored halves
+// and rows, which meet groups that already agree), beyond by swapping rows of 16
+// and halves of 32.
+template <int kLanes, typename T, typename Op>
+__device__ __forceinline__ T lanes_all(T v, Op op) {
+  static_assert(sizeof(T) == 4 && kLanes >= 1 && kLanes <= kWave, "");
+  const auto bits = [](T x) { return __builtin_bit_cast(int, x); };
+  const auto of = [](int x) { return __builtin_bit_cast(T, x); };
+  if constexpr (kLanes > 1) v = op(v, of(__builtin_amdgcn_update_dpp(0, bits(v), 0xB1, 0xF, 0xF, true)));
+  if constexpr (kLanes > 2) v = op(v, of(__builtin_amdgcn_update_dpp(0, bits(v), 0x4E, 0xF, 0xF, true)));
+  if constexpr (kLanes > 4) v = op(v, of(__builtin_amdgcn_update_dpp(0, bits(v), 0x141, 0xF, 0xF, true)));
+  if constexpr (kLanes > 8) v = op(v, of(__builtin_amdgcn_update_dpp(0, bits(v), 0x140, 0xF, 0xF, true)));
+  if constexpr (kLanes > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
+    v = op(of(int(r[0])), of(int(r[1])));
+  }
+  if constexpr (kLanes > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(bits(v), bits(v), false, false);
+    v = op(of(int(r[0])), of(int(r[1])));
+  }
+  return v;
+}
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v) {
+  return lanes_all<kLanes>(v, [](float a, float b) { return a + b; });
+}
+
 // A matrix as the kernels read it.
 template <typename T>
 struct Mat {

@@ -327,7 +327,15 @@ def test_large():
     s = torch.zeros((ps.state_blocks(n), 2), device="cuda")
     ps.AdamWStep(ps.AdamWList([p], [g], [m], [v], scales=[s], weight_decay=0.0), 0.5, 1)
     assert bool((p == -0.5).all())
-    assert bool((m == 0x7E).all()) and bool((v == 0x7E).all())  # 448
+    # All are their blocks' largest: 448 (code 0x7E). The scale is their FP32 product with FP32's
+    # 1 / 448, so their quotient is 448 (1 - 3 * 2^-24) at least, 14 (1 - 3 * 2^-24) steps of the
+    # grid: where u is below 14 * 3 * 2^-24 < 3 * 2^-20 the code below, 416, is right too.
+    for codes in (m, v):
+        for k, part in enumerate(codes.split(1 << 30)):
+            i = torch.nonzero(part != 0x7E).view(-1) + (k << 30)
+            assert bool((codes[i] == 0x7D).all())
+            u = (((i * 0x6A09E667) + 0x9E3779B9) & 0xFFFFFFFF) >> 12
+            assert bool((u < 3).all())
     assert float((s[-2:, 0] / (0.1 / 448) - 1).abs().max()) <= 8 * ref.U32
 
 
