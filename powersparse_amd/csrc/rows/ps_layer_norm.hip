@@ -104,11 +104,15 @@ __global__ __launch_bounds__(threads_of(kLanes)) void norm_kernel(Mat<const T> x
   __shared__ RowParts<kLanes> part;
   const int lane = threadIdx.x % kLanes, pieces = int(p.per_row.d);
   using V = typename PieceOf<T, N>::type;
+  // What does not fit the registers that are left (1,024 threads have half of 512's)
+  // is loaded again for every row: 2,048 x 32,768 BF16 136 and 73 us, but 4,096 x
+  // 16,384 FP32, which fit, 105 and 120.
+  constexpr bool kHeld = kPieces * N <= (kLanes > 256 ? 16 : 32);
   Floats<N> w[kPieces], b[kPieces];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
     const int q = i * kLanes + lane;
-    if (q >= pieces) continue;
+    if (!kHeld || q >= pieces) continue;
     w[i] = weight.at<N>(p.begin(q));
     b[i] = bias.at<N>(p.begin(q));
   }
@@ -145,6 +149,10 @@ __global__ __launch_bounds__(threads_of(kLanes)) void norm_kernel(Mat<const T> x
       const int q = i * kLanes + lane;
       if (q >= pieces) continue;
       const Floats<N> f = (__builtin_convertvector(v[i], Floats<N>) - mean) * rstd;
+      if constexpr (!kHeld) {
+        w[i] = weight.at<N>(p.begin(q));
+        b[i] = bias.at<N>(p.begin(q));
+      }
       store_piece<N>(y.at(r, p.begin(q)), f * w[i] + b[i]);
     }
     if (lane == 0) {
@@ -219,6 +227,11 @@ __global__ __launch_bounds__(threads_of(kLanes)) void grad_kernel(
       const int q = i * kLanes + lane;
       if (q >= pieces) continue;
       const int c = p.begin(q);
+      if (!repeats<N>(p)) {
+        store_piece<N>(to + c, dw[i]);
+        store_piece<N>(to + p.cols + c, db[i]);
+        continue;
+      }
       each_new<N, kPieces>(p, q, [&](int e) {
         to[c + e] = dw[i][e];
         to[p.cols + c + e] = db[i][e];
@@ -400,6 +413,13 @@ long long part_count(long long rows, long long cols) {
   return n < rows ? n : rows;
 }
 
+// Of them, the workgroups that take `turns` turns in all, eight each where 512 fill
+// the device (512 and 1,024, us: 4,096 x 2,048 BF16 21 and 25, 4,096 x 512 8.6 and
+// 10.3; with more turns 16,384 x 2,048 47 and 45, 65,536 x 512 FP32 88 and 80).
+uint32_t fewer_parts(uint32_t parts, long long turns) {
+  return uint32_t(std::min({(long long)parts, turns, std::max(turns / 8, 512LL)}));
+}
+
 Vec vec(const ps_rows* m, float otherwise) {
   return m ? Vec{m->data, m->dtype, otherwise} : Vec{nullptr, PS_F32, otherwise};
 }
@@ -422,27 +442,36 @@ uint32_t norm_blocks(long long rows, int per_block) {
   return uint32_t(std::min(std::max(n / 4, kNormBlocks), kMostNormBlocks));
 }
 
-// Calls f(lanes, pieces of a lane) for rows of p's pieces, or f(0, 0) for wider ones.
-template <int N, typename F>
-int with_lanes(const Pieces& p, F&& f) {
+// Calls f(lanes, pieces of a lane) for rows of p's pieces, or f(0, 0) for wider
+// ones (beyond kMost pieces: the gradient's four of 8 elements would not fit
+// 1,024 threads' registers, 472 us for 2,048 x 32,768 BF16, and 172 without).
+// `apart`: whether 65 to 256 pieces get a workgroup a row. Forward that is faster
+// where few rows leave most of the device idle (8 x 2,048 BF16 3.9 -> 2.9 us, but
+// 16,384 x 1,024 12 -> 19), in the gradient, with twice the registers, from 129
+// pieces on (16,384 x 2,048 BF16 47.5 -> 44.6; x 1,024 24.5 -> 31). 513 to 1,024
+// pieces of 8 elements, 512 threads for 256: 16,384 x 8,192 gradients 168 -> 157;
+// of 4 the other way: 16,384 x 4,096 137 -> 129.
+template <int N, int kMost, typename F>
+int with_lanes(const Pieces& p, bool apart, F&& f) {
   const uint32_t n = p.per_row.d;
   const auto call = [&](auto lanes, auto per) { return f(lanes, per); };
   using std::integral_constant;
   if (n <= 8) return call(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-  if constexpr (N == 1) {
-    return call(integral_constant<int, 0>{}, integral_constant<int, 0>{});  // (fewer than 8)
-  } else {
+  if constexpr (N > 1) {  // (else fewer than 8)
     if (n <= 16) return call(integral_constant<int, 16>{}, integral_constant<int, 1>{});
     if (n <= 32) return call(integral_constant<int, 32>{}, integral_constant<int, 1>{});
     if (n <= 64) return call(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    if (n <= 256 && apart) return call(integral_constant<int, 256>{}, integral_constant<int, 1>{});
     if (n <= 128) return call(integral_constant<int, 64>{}, integral_constant<int, 2>{});
     if (n <= 256) return call(integral_constant<int, 64>{}, integral_constant<int, 4>{});
     if (n <= 512) return call(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    if (n <= 1024) return call(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    if (n <= 1024)
+      return call(integral_constant<int, N == 8 ? 512 : 256>{}, integral_constant<int, N == 8 ? 2 : 4>{});
     if (n <= 2048) return call(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
-    if (n <= 4096) return call(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
-    return call(integral_constant<int, 0>{}, integral_constant<int, 0>{});
+    if constexpr (kMost >= 4096)
+      if (n <= 4096) return call(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
   }
+  return call(integral_constant<int, 0>{}, integral_constant<int, 0>{});
 }
 
 }  // namespace
@@ -484,7 +513,7 @@ int ps_layer_norm(const ps_rows* x, const ps_rows* weight, const ps_rows* bias, 
       constexpr int kSize = sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O);
       return ps::with_width<kSize>(x->cols, [&](auto n) {
         const ps::Pieces p(x->cols, n);
-        return ps::with_lanes<n>(p, [&](auto lanes, auto per) {
+        return ps::with_lanes<n, 4096>(p, x->rows <= 1024, [&](auto lanes, auto per) {
           const auto run = [&](auto kernel, uint32_t blocks, int threads) {
             kernel<<<blocks, threads, 0, ps::to_hip(stream)>>>(
                 ps::mat<const T>(x), ps::vec(weight, 1.f), ps::vec(bias, 0.f), eps, ps::mat<O>(y),
@@ -556,7 +585,7 @@ int ps_layer_norm_grad(const ps_rows* dy, const ps_rows* x, const ps_rows* weigh
         constexpr int kSize = sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O);
         return ps::with_width<kSize>(x->cols, [&](auto n) {
           const ps::Pieces p(x->cols, n);
-          return ps::with_lanes<n>(p, [&](auto lanes, auto per) {
+          return ps::with_lanes<n, n == 8 ? 2048 : 4096>(p, p.per_row.d > 128, [&](auto lanes, auto per) {
             if constexpr (lanes == 0) {
               ps::grad_wide_kernel<T, O, n>
                   <<<ps::wide_blocks(x->rows), ps::kWideThreads, 0, st>>>(
@@ -569,7 +598,7 @@ int ps_layer_norm_grad(const ps_rows* dy, const ps_rows* x, const ps_rows* weigh
                   ps::mat<const O>(dy), ps::mat<const T>(x), mean, rstd, parts, p);
             } else {
               constexpr int kThreads = ps::threads_of(lanes), kRows = kThreads / lanes;
-              part_count = std::min(part_count, uint32_t((x->rows + kRows - 1) / kRows));
+              part_count = ps::fewer_parts(part_count, (x->rows + kRows - 1) / kRows);
               ps::grad_kernel<T, O, n, lanes, per><<<part_count, kThreads, 0, st>>>(
                   ps::mat<const O>(dy), ps::mat<const T>(x), ps::vec(weight, 1.f), mean, rstd,
                   ps::mat<T>(dx), sums ? parts : nullptr, p);
