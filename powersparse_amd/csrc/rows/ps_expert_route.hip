@@ -11,7 +11,6 @@
 namespace ps {
 namespace {
 
-constexpr int kRouteThreads = 256;
 constexpr int kMostExperts = 1024;
 
 // Unsigned numbers that order as logits do, 0 for barred ones (-inf), the most
@@ -44,17 +43,17 @@ struct RouteParts {
   int* counts;  // blocks x (experts + 1)
 };
 
-template <typename T, int kLanes, int kPer>
-__global__ __launch_bounds__(kRouteThreads) void route_kernel(
+template <typename T, int kLanes, int kPer, int kThreads>
+__global__ __launch_bounds__(kThreads) void route_kernel(
     Mat<const T> logits, int experts, int top_k, bool normalize,
     const unsigned char* __restrict__ mask, int* __restrict__ ids, float* __restrict__ weights,
     RouteParts parts) {
-  constexpr int kTokens = kRouteThreads / kLanes;
+  constexpr int kTokens = kThreads / kLanes;
   __shared__ int chosen[kMostExperts + 1];
   __shared__ float sums[kMostExperts];
   const int lane = threadIdx.x % kLanes;
   if (parts.sums) {
-    for (int e = threadIdx.x; e <= experts; e += kRouteThreads) {
+    for (int e = threadIdx.x; e <= experts; e += kThreads) {
       chosen[e] = 0;
       if (e < experts) sums[e] = 0.f;
     }
@@ -93,7 +92,8 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(
     }
     int* const ids_t = ids + t * top_k;
     float* const weights_t = weights + t * top_k;
-    float total = 0.f;
+    float total = 0.f, my_w = 0.f;
+    int my_id = -1;  // slot k's are kept by lane k % kLanes
     for (int k = 0; k < top_k; ++k) {
       uint32_t best = 0, at = ~0u;
 #pragma unroll
@@ -110,14 +110,28 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(
         if (at == uint32_t(r * kLanes + lane)) key[r] = 0;
       const float w = best ? expf(value_of(best) - top) : 0.f;
       total += w;
-      if (lane == k % kLanes && mine) {
-        ids_t[k] = int(at);
-        weights_t[k] = normalize ? w : w * scale;
-        if (parts.sums && best) atomicAdd(&chosen[at], 1);
+      if (lane == k % kLanes) {
+        my_id = int(at);
+        my_w = normalize ? w : w * scale;
+      }
+      if (top_k > kLanes && (k % kLanes == kLanes - 1 || k + 1 == top_k)) {
+        const int slot = k - k % kLanes + lane;
+        if (slot <= k && mine) {
+          if (parts.sums && my_id >= 0) atomicAdd(&chosen[my_id], 1);
+          ids_t[slot] = my_id;
+          weights_t[slot] = my_w;
+        }
       }
     }
-    if (normalize && mine)
+    if (top_k <= kLanes) {
+      if (lane < top_k && mine) {
+        if (parts.sums && my_id >= 0) atomicAdd(&chosen[my_id], 1);
+        ids_t[lane] = my_id;
+        weights_t[lane] = normalize && most ? my_w / total : my_w;
+      }
+    } else if (normalize && mine) {
       for (int k = lane; k < top_k; k += kLanes) weights_t[k] = most ? weights_t[k] / total : 0.f;
+    }
   }
   if (!parts.sums) return;
   // The tokens of a wave, then the waves in order.
@@ -125,7 +139,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(
   for (int r = 0; r < kPer; ++r)
 #pragma unroll
     for (int d = kLanes; d < kWave; d <<= 1) acc[r] += __shfl_xor(acc[r], d, kWave);
-  for (int w = 0; w < kRouteThreads / kWave; ++w) {
+  for (int w = 0; w < kThreads / kWave; ++w) {
     __syncthreads();
     if (int(threadIdx.x / kWave) == w && lane_id() < kLanes)
 #pragma unroll
@@ -133,7 +147,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(
         if (r * kLanes + lane < experts) sums[r * kLanes + lane] += acc[r];
   }
   __syncthreads();
-  for (int e = threadIdx.x; e <= experts; e += kRouteThreads) {
+  for (int e = threadIdx.x; e <= experts; e += kThreads) {
     parts.counts[size_t(blockIdx.x) * (experts + 1) + e] = chosen[e];
     if (e < experts) parts.sums[size_t(blockIdx.x) * experts + e] = sums[e];
   }
@@ -141,7 +155,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(
 
 // The workgroups' parts added up, and the loss: one workgroup, a thread an
 // expert, the parts dealt to as many threads of the same expert as there are.
-constexpr int kJoinThreads = 1024;
+constexpr int kJoinThreads = 1024, kJoinAhead = 8;
 __global__ __launch_bounds__(kJoinThreads) void route_join_kernel(RouteParts parts, int part_count,
                                                                   int experts, int groups,
                                                                   int* __restrict__ counts,
@@ -154,10 +168,21 @@ __global__ __launch_bounds__(kJoinThreads) void route_join_kernel(RouteParts par
   const int e = threadIdx.x % per, group = threadIdx.x / per;
   int c = 0, tokens = 0;
   double s = 0;
-  for (int b = group; b < part_count; b += groups) {
-    if (e < experts) {
-      c += parts.counts[size_t(b) * (experts + 1) + e];
-      s += double(parts.sums[size_t(b) * experts + e]);
+  if (e < experts) {
+    for (int b0 = group; b0 < part_count; b0 += groups * kJoinAhead) {
+      int counts_of[kJoinAhead];
+      float sums_of[kJoinAhead];
+#pragma unroll
+      for (int j = 0; j < kJoinAhead; ++j) {
+        const int b = b0 + j * groups;
+        counts_of[j] = b < part_count ? parts.counts[size_t(b) * (experts + 1) + e] : 0;
+        sums_of[j] = b < part_count ? parts.sums[size_t(b) * experts + e] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < kJoinAhead; ++j) {
+        c += counts_of[j];
+        s += double(sums_of[j]);
+      }
     }
   }
   if (threadIdx.x < kWave)
@@ -195,12 +220,13 @@ __global__ __launch_bounds__(kJoinThreads) void route_join_kernel(RouteParts par
   }
 }
 
+constexpr int kRouteGradThreads = 256;
 template <typename T, int kLanes, int kPer>
-__global__ __launch_bounds__(kRouteThreads) void route_grad_kernel(
+__global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
     Mat<const T> logits, int experts, int top_k, bool normalize, const int* __restrict__ ids,
     const float* __restrict__ dweights, const int* __restrict__ counts,
     const float* __restrict__ dloss, Mat<T> dlogits) {
-  constexpr int kTokens = kRouteThreads / kLanes;
+  constexpr int kTokens = kRouteGradThreads / kLanes;
   const int lane = threadIdx.x % kLanes;
   // The loss's gradient by an expert's probability.
   float by_loss[kPer];
@@ -298,22 +324,27 @@ __global__ __launch_bounds__(kRouteThreads) void route_grad_kernel(
 
 // ----------------------------------------------------------------- host side
 
-// Workgroups of the forward pass: what they leave is added up by one workgroup.
-constexpr long long kRouteBlocks = 512;
-long long route_blocks(long long tokens, int per_block) {
+// Workgroups of the forward pass where the loss is wanted: what they leave is
+// added up by one workgroup.
+constexpr long long kRouteBlocks = 256;
+long long route_blocks(long long tokens, int per_block, long long most) {
   const long long n = (tokens + per_block - 1) / per_block;
-  return n < kRouteBlocks ? n : kRouteBlocks;
+  return n < most ? n : most;
 }
 
 // Calls f(lanes, logits per lane).
 template <typename F>
 int with_lanes(int experts, F&& f) {
-  const auto lanes = std::integral_constant<int, kWave>{};
-  if (experts <= kWave) return f(lanes, std::integral_constant<int, 1>{});
-  if (experts <= 2 * kWave) return f(lanes, std::integral_constant<int, 2>{});
-  if (experts <= 4 * kWave) return f(lanes, std::integral_constant<int, 4>{});
-  if (experts <= 8 * kWave) return f(lanes, std::integral_constant<int, 8>{});
-  return f(lanes, std::integral_constant<int, 16>{});
+  const auto call = [&](auto lanes, auto per) { return f(lanes, per); };
+  using std::integral_constant;
+  if (experts <= 8) return call(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+  if (experts <= 16) return call(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+  if (experts <= 32) return call(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+  if (experts <= 64) return call(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+  if (experts <= 128) return call(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+  if (experts <= 256) return call(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+  if (experts <= 512) return call(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+  return call(integral_constant<int, 64>{}, integral_constant<int, 16>{});
 }
 
 // What is wrong with logits and top_k, or null.
@@ -370,14 +401,23 @@ int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsig
   const int rc = ps::with_dtype(logits->dtype, [&](auto t) {
     return ps::with_lanes(experts, [&](auto lanes, auto per) {
       using T = decltype(t);
-      blocks = ps::route_blocks(logits->rows, ps::kRouteThreads / lanes);
+      // Large workgroups where there is work for them: the join's parts are few.
+      const bool large = logits->rows > ps::kRouteBlocks * (256 / lanes);
+      const int threads = large ? 1024 : 256;
+      blocks = ps::route_blocks(logits->rows, threads / lanes, loss ? ps::kRouteBlocks : 1 << 20);
       if (loss) {
         parts.sums = static_cast<float*>(workspace);
         parts.counts = reinterpret_cast<int*>(parts.sums + blocks * experts);
       }
       if (!blocks) return int(PS_OK);
-      ps::route_kernel<T, lanes, per><<<uint32_t(blocks), ps::kRouteThreads, 0, st>>>(
-          ps::mat<const T>(logits), experts, top_k, normalize != 0, mask, ids, weights, parts);
+      const auto run = [&](auto kernel) {
+        kernel<<<uint32_t(blocks), threads, 0, st>>>(ps::mat<const T>(logits), experts, top_k,
+                                                     normalize != 0, mask, ids, weights, parts);
+      };
+      if (large)
+        run(ps::route_kernel<T, lanes, per, 1024>);
+      else
+        run(ps::route_kernel<T, lanes, per, 256>);
       PS_LAUNCHED();
       return int(PS_OK);
     });
@@ -416,10 +456,9 @@ int ps_expert_route_grad(const ps_rows* logits, int top_k, int normalize, const 
   return ps::with_dtype(logits->dtype, [&](auto t) {
     return ps::with_lanes(experts, [&](auto lanes, auto per) {
       using T = decltype(t);
-      const long long per_block = ps::kRouteThreads / lanes;
-      const long long blocks = (logits->rows + per_block - 1) / per_block;
+      const long long blocks = ps::route_blocks(logits->rows, ps::kRouteGradThreads / lanes, 4096);
       ps::route_grad_kernel<T, lanes, per>
-          <<<uint32_t(blocks < 4096 ? blocks : 4096), ps::kRouteThreads, 0, ps::to_hip(stream)>>>(
+          <<<uint32_t(blocks), ps::kRouteGradThreads, 0, ps::to_hip(stream)>>>(
               ps::mat<const T>(logits), experts, top_k, normalize != 0, ids, dweights, counts,
               dloss, ps::mat<T>(dlogits));
       PS_LAUNCHED();
