@@ -2,10 +2,9 @@
 // experts and their weights, how often each expert was chosen, the loss that
 // asks for balance among them, and the gradient.
 //
-// kLanes threads share a token, each with kPer of its logits in registers:
-// expert e is element e / kLanes of lane e % kLanes. The largest logits are
-// found one after another, by keys that order as the logits do; equal ones go to
-// the lowest expert.
+// kLanes threads share a token, each with kPer of its logits in registers, kWide
+// neighbours at a time. The largest logits are found one after another, by keys
+// that order as the logits do; equal ones go to the lowest expert.
 #include "ps_rows.hpp"
 
 namespace ps {
@@ -36,27 +35,78 @@ __device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
   return lanes_all<kLanes>(v, [](uint32_t a, uint32_t b) { return min(a, b); });
 }
 
+// Which experts a lane of a token has: element r is expert of(r), ascending in r.
+template <int kLanes, int kPer, int kWide>
+struct Share {
+  static_assert(kPer % kWide == 0, "");
+  int first;
+  __device__ __forceinline__ explicit Share(int lane) : first(lane * kWide) {}
+  __device__ __forceinline__ int of(int r) const {
+    return first + r / kWide * kLanes * kWide + r % kWide;
+  }
+  // f(r, logit) of row t, absent where the expert does not exist.
+  template <typename T, typename F>
+  __device__ __forceinline__ void load(const Mat<const T>& m, long long t, int experts, bool on,
+                                       float absent, F&& f) const {
+    using V = typename PieceOf<T, kWide>::type;
+    V v[kPer / kWide];
+#pragma unroll
+    for (int c = 0; c < kPer / kWide; ++c) {
+      v[c] = V(T(absent));
+      if (on && of(c * kWide) < experts) v[c] = *reinterpret_cast<const V*>(m.at(t, of(c * kWide)));
+    }
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) f(r, float(v[r / kWide][r % kWide]));
+  }
+};
+
 // What the workgroups leave of the loss: sums of probabilities, and choices of
 // every expert with the tokens that take part behind them.
 struct RouteParts {
-  float* sums;  // blocks x experts
+  float* sums;  // blocks x experts; null: no loss is wanted
   int* counts;  // blocks x (experts + 1)
+  // their totals: experts sums, experts + 1 counts
+  double* all_sums;
+  int* all_counts;
 };
 
-template <typename T, int kLanes, int kPer, int kThreads>
+// The counts and the loss from the totals of every expert, by a wave.
+template <typename Sum, typename Count>
+__device__ __forceinline__ void finish(int experts, Sum&& sum_of, Count&& count_of,
+                                       int* __restrict__ counts, float* __restrict__ loss) {
+  long long total = 0;
+  double sum = 0;
+  for (int e = lane_id(); e < experts; e += kWave) {
+    const int c = count_of(e);
+    counts[e] = c;
+    total += c;
+    sum += double(c) * double(sum_of(e));
+  }
+#pragma unroll
+  for (int d = kWave / 2; d; d >>= 1) {
+    total += __shfl_xor(total, d, kWave);
+    sum += __shfl_xor(sum, d, kWave);
+  }
+  if (lane_id()) return;
+  const int tokens = count_of(experts);
+  counts[experts] = tokens;
+  *loss = tokens ? float(sum * experts / (double(tokens) * double(total))) : 0.f;
+}
+
+template <typename T, int kLanes, int kPer, int kWide, int kThreads>
 __global__ __launch_bounds__(kThreads) void route_kernel(
     Mat<const T> logits, int experts, int top_k, bool normalize,
     const unsigned char* __restrict__ mask, int* __restrict__ ids, float* __restrict__ weights,
-    RouteParts parts) {
+    RouteParts parts, int* __restrict__ counts, float* __restrict__ loss) {
   constexpr int kTokens = kThreads / kLanes;
-  __shared__ int chosen[kMostExperts + 1];
-  __shared__ float sums[kMostExperts];
+  constexpr int kMost = kLanes * kPer;
+  __shared__ int chosen[kMost + 1];
+  __shared__ float sums[kThreads / kWave][kMost];
   const int lane = threadIdx.x % kLanes;
+  const Share<kLanes, kPer, kWide> share(lane);
+  int tokens = 0;
   if (parts.sums) {
-    for (int e = threadIdx.x; e <= experts; e += kThreads) {
-      chosen[e] = 0;
-      if (e < experts) sums[e] = 0.f;
-    }
+    for (int e = threadIdx.x; e <= experts; e += kThreads) chosen[e] = 0;
     __syncthreads();
   }
   float acc[kPer];
@@ -69,12 +119,10 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
     const bool mine = t < logits.rows, on = mine && (!mask || mask[t]);
     uint32_t key[kPer];
     uint32_t most = 0;
-#pragma unroll
-    for (int r = 0; r < kPer; ++r) {
-      const int e = r * kLanes + lane;
-      key[r] = on && e < experts ? key_of(float(*logits.at(t, e))) : 0;
+    share.load(logits, t, experts, on, -INFINITY, [&](int r, float v) {
+      key[r] = key_of(v);
       most = max(most, key[r]);
-    }
+    });
     most = lanes_max<kLanes>(most);
     const float top = most ? value_of(most) : 0.f;  // nothing to choose: no probabilities either
     float p[kPer], s = 0.f;
@@ -88,7 +136,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
     if (parts.sums) {
 #pragma unroll
       for (int r = 0; r < kPer; ++r) acc[r] += p[r] * scale;
-      if (lane == 0 && most) atomicAdd(&chosen[experts], 1);
+      tokens += lane == 0 && most;
     }
     int* const ids_t = ids + t * top_k;
     float* const weights_t = weights + t * top_k;
@@ -102,12 +150,12 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
       if (best) {
 #pragma unroll
         for (int r = kPer - 1; r >= 0; --r)
-          if (key[r] == best) at = uint32_t(r * kLanes + lane);
+          if (key[r] == best) at = uint32_t(share.of(r));
       }
       at = lanes_min<kLanes>(at);
 #pragma unroll
       for (int r = 0; r < kPer; ++r)
-        if (at == uint32_t(r * kLanes + lane)) key[r] = 0;
+        if (at == uint32_t(share.of(r))) key[r] = 0;
       const float w = best ? expf(value_of(best) - top) : 0.f;
       total += w;
       if (lane == k % kLanes) {
@@ -139,95 +187,114 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
   for (int r = 0; r < kPer; ++r)
 #pragma unroll
     for (int d = kLanes; d < kWave; d <<= 1) acc[r] += __shfl_xor(acc[r], d, kWave);
-  for (int w = 0; w < kThreads / kWave; ++w) {
-    __syncthreads();
-    if (int(threadIdx.x / kWave) == w && lane_id() < kLanes)
+  if (lane_id() < kLanes)
 #pragma unroll
-      for (int r = 0; r < kPer; ++r)
-        if (r * kLanes + lane < experts) sums[r * kLanes + lane] += acc[r];
-  }
+    for (int r = 0; r < kPer; ++r) sums[threadIdx.x / kWave][share.of(r)] = acc[r];
+  tokens = lanes_all<kWave>(tokens, [](int a, int b) { return a + b; });
+  if (lane_id() == 0) atomicAdd(&chosen[experts], tokens);
   __syncthreads();
+  const auto sum_of = [&](int e) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) s += sums[w][e];
+    return s;
+  };
+  if (gridDim.x == 1) {  // nothing to join
+    if (threadIdx.x < kWave)
+      finish(experts, sum_of, [&](int e) { return chosen[e]; }, counts, loss);
+    return;
+  }
   for (int e = threadIdx.x; e <= experts; e += kThreads) {
     parts.counts[size_t(blockIdx.x) * (experts + 1) + e] = chosen[e];
-    if (e < experts) parts.sums[size_t(blockIdx.x) * experts + e] = sums[e];
+    if (e < experts) parts.sums[size_t(blockIdx.x) * experts + e] = sum_of(e);
   }
 }
 
-// The workgroups' parts added up, and the loss: one workgroup, a thread an
-// expert, the parts dealt to as many threads of the same expert as there are.
-constexpr int kJoinThreads = 1024, kJoinAhead = 8;
-__global__ __launch_bounds__(kJoinThreads) void route_join_kernel(RouteParts parts, int part_count,
-                                                                  int experts, int groups,
-                                                                  int* __restrict__ counts,
-                                                                  float* __restrict__ loss) {
-  __shared__ int count_of[kJoinThreads];
-  __shared__ double sum_of[kJoinThreads];
-  __shared__ int all_counts[kMostExperts];
-  __shared__ double products[kMostExperts];
-  const int per = kJoinThreads / groups;  // threads of a group, one an expert
-  const int e = threadIdx.x % per, group = threadIdx.x / per;
-  int c = 0, tokens = 0;
-  double s = 0;
-  if (e < experts) {
-    for (int b0 = group; b0 < part_count; b0 += groups * kJoinAhead) {
-      int counts_of[kJoinAhead];
-      float sums_of[kJoinAhead];
+// The workgroups' parts added up: 32 columns a workgroup, the experts' sums first,
+// the counts and the tokens behind them, 32 threads each with up to 16 parts under
+// way at once.
+constexpr int kJoinCols = 32, kJoinLanes = 32, kJoinAhead = 16;
+__global__ __launch_bounds__(kJoinCols* kJoinLanes) void route_join_kernel(RouteParts parts,
+                                                                           int part_count,
+                                                                           int experts) {
+  __shared__ double sums[kJoinLanes][kJoinCols];
+  const int lane = threadIdx.x / kJoinCols, i = threadIdx.x % kJoinCols;
+  const int c = blockIdx.x * kJoinCols + i, all = 2 * experts + 1;
+  double s = 0;  // (counts stay exact in it)
+  for (int k0 = lane; c < all && k0 < part_count; k0 += kJoinLanes * kJoinAhead) {
+    uint32_t v[kJoinAhead];
 #pragma unroll
-      for (int j = 0; j < kJoinAhead; ++j) {
-        const int b = b0 + j * groups;
-        counts_of[j] = b < part_count ? parts.counts[size_t(b) * (experts + 1) + e] : 0;
-        sums_of[j] = b < part_count ? parts.sums[size_t(b) * experts + e] : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < kJoinAhead; ++j) {
-        c += counts_of[j];
-        s += double(sums_of[j]);
-      }
+    for (int j = 0; j < kJoinAhead; ++j) {
+      const size_t k = k0 + j * kJoinLanes;
+      v[j] = 0;
+      if (k < size_t(part_count))
+        v[j] = c < experts ? __float_as_uint(parts.sums[k * experts + c])
+                           : uint32_t(parts.counts[k * (experts + 1) + c - experts]);
     }
+#pragma unroll
+    for (int j = 0; j < kJoinAhead; ++j) s += c < experts ? double(__uint_as_float(v[j])) : double(v[j]);
   }
+  sums[lane][i] = s;
+  __syncthreads();
+  if (lane || c >= all) return;
+#pragma unroll
+  for (int k = 1; k < kJoinLanes; ++k) s += sums[k][i];
+  if (c < experts)
+    parts.all_sums[c] = s;
+  else
+    parts.all_counts[c - experts] = int(s);
+}
+__global__ __launch_bounds__(kWave) void route_finish_kernel(RouteParts parts, int experts,
+                                                             int* __restrict__ counts,
+                                                             float* __restrict__ loss) {
+  finish(experts, [&](int e) { return parts.all_sums[e]; },
+         [&](int e) { return parts.all_counts[e]; }, counts, loss);
+}
+// Both for few parts, in one launch: all parts of a column under way at once.
+constexpr int kFewParts = 16, kFewThreads = 1024;
+__global__ __launch_bounds__(kFewThreads) void route_join_few_kernel(RouteParts parts,
+                                                                     int part_count, int experts,
+                                                                     int* __restrict__ counts,
+                                                                     float* __restrict__ loss) {
+  __shared__ double sums[kMostExperts];
+  __shared__ int chosen[kMostExperts + 1];
+  for (int e = threadIdx.x; e <= experts; e += kFewThreads) {
+    float s_of[kFewParts];
+    int c_of[kFewParts];
+#pragma unroll
+    for (int k = 0; k < kFewParts; ++k) {
+      c_of[k] = k < part_count ? parts.counts[k * (experts + 1) + e] : 0;
+      s_of[k] = k < part_count && e < experts ? parts.sums[k * experts + e] : 0.f;
+    }
+    int c = 0;
+    double s = 0;
+#pragma unroll
+    for (int k = 0; k < kFewParts; ++k) {
+      c += c_of[k];
+      s += double(s_of[k]);
+    }
+    chosen[e] = c;
+    if (e < experts) sums[e] = s;
+  }
+  __syncthreads();
   if (threadIdx.x < kWave)
-    for (int b = threadIdx.x; b < part_count; b += kWave)
-      tokens += parts.counts[size_t(b) * (experts + 1) + experts];
-  count_of[threadIdx.x] = c;
-  sum_of[threadIdx.x] = s;
-  __syncthreads();
-  if (group == 0) {
-    for (int g = 1; g < groups; ++g) {
-      c += count_of[g * per + e];
-      s += sum_of[g * per + e];
-    }
-    if (e < experts) counts[e] = c;
-    all_counts[e] = c;
-    products[e] = double(c) * s;
-  }
-  __syncthreads();
-  if (threadIdx.x >= kWave) return;
-  long long total = 0;
-  double sum = 0;
-  for (int i = threadIdx.x; i < per; i += kWave) {
-    total += all_counts[i];
-    sum += products[i];
-  }
-#pragma unroll
-  for (int d = kWave / 2; d; d >>= 1) {
-    tokens += __shfl_xor(tokens, d, kWave);
-    total += __shfl_xor(total, d, kWave);
-    sum += __shfl_xor(sum, d, kWave);
-  }
-  if (threadIdx.x == 0) {
-    counts[experts] = tokens;
-    *loss = tokens ? float(sum * experts / (double(tokens) * double(total))) : 0.f;
-  }
+    finish(experts, [&](int e) { return sums[e]; }, [&](int e) { return chosen[e]; }, counts, loss);
+}
+// Without tokens.
+__global__ __launch_bounds__(kWave) void route_nothing_kernel(int experts, int* __restrict__ counts,
+                                                              float* __restrict__ loss) {
+  finish(experts, [](int) { return 0.0; }, [](int) { return 0; }, counts, loss);
 }
 
 constexpr int kRouteGradThreads = 256;
-template <typename T, int kLanes, int kPer>
+template <typename T, int kLanes, int kPer, int kWide>
 __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
     Mat<const T> logits, int experts, int top_k, bool normalize, const int* __restrict__ ids,
     const float* __restrict__ dweights, const int* __restrict__ counts,
     const float* __restrict__ dloss, Mat<T> dlogits) {
   constexpr int kTokens = kRouteGradThreads / kLanes;
   const int lane = threadIdx.x % kLanes;
+  const Share<kLanes, kPer, kWide> share(lane);
   // The loss's gradient by an expert's probability.
   float by_loss[kPer];
 #pragma unroll
@@ -236,7 +303,7 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
     float total = 0.f;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      const int e = r * kLanes + lane;
+      const int e = share.of(r);
       by_loss[r] = e < experts ? float(counts[e]) : 0.f;
       total += by_loss[r];
     }
@@ -250,12 +317,29 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
     const long long t = t0 + threadIdx.x / kLanes;
     const bool mine = t < logits.rows;
     const int* const ids_t = ids + t * top_k;
-    const bool on = mine && ids_t[0] >= 0;
+    struct Choice {
+      int id;
+      float logit, dw;
+    };
+    const auto choice = [&](int k) {
+      Choice c{-1, 0.f, 0.f};
+      if (!mine || k >= top_k) return c;
+      const int id = ids_t[k];
+      if (id < 0 || id >= experts) return c;
+      c.id = id;
+      c.logit = float(*logits.at(t, id));
+      if (dweights) c.dw = dweights[t * top_k + k];
+      return c;
+    };
+    // All loads are under way before the first is waited for, but the chosen logits'.
+    const int id_0 = mine ? ids_t[0] : -1;
     float p[kPer], h[kPer], top = -INFINITY, s = 0.f;
+    share.load(logits, t, experts, mine, -INFINITY, [&](int r, float v) { p[r] = v; });
+    const Choice first = choice(lane);
+    const bool on = id_0 >= 0;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      const int e = r * kLanes + lane;
-      p[r] = on && e < experts ? float(*logits.at(t, e)) : -INFINITY;
+      p[r] = on ? p[r] : -INFINITY;
       top = fmaxf(top, p[r]);
       h[r] = by_loss[r];
     }
@@ -270,39 +354,35 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
     const float scale = on ? 1.f / s : 0.f;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) p[r] = on ? p[r] * scale : 0.f;
-    // The chosen experts, kLanes at a time: what their weights' gradients add.
+    float extra[kPer];
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) extra[r] = 0.f;
+    // What the chosen experts' weights' gradients add, kLanes of them at a time: the
+    // first ones have been loaded.
     float chosen = 0.f, dot = 0.f;
-    const auto choice = [&](int k, float& w, float& dw) {
-      const int id = on && k < top_k ? ids_t[k] : -1;
-      const bool taken = id >= 0 && id < experts;
-      w = taken ? expf(float(*logits.at(t, id)) - top) : 0.f;
-      dw = taken && dweights ? dweights[t * top_k + k] : 0.f;
-      return taken ? id : -1;
-    };
     if (normalize) {
+      Choice c = first;
       for (int k = 0; k < top_k; k += kLanes) {
-        float w, dw;
-        choice(k + lane, w, dw);
+        if (k) c = choice(k + lane);
+        const float w = c.id >= 0 ? expf(c.logit - top) : 0.f;
         chosen += w;
-        dot += w * dw;
+        dot += w * c.dw;
       }
       chosen = lanes_sum<kLanes>(chosen);
       dot = lanes_sum<kLanes>(dot) / chosen;
     }
-    float extra[kPer];
-#pragma unroll
-    for (int r = 0; r < kPer; ++r) extra[r] = 0.f;
+    Choice c = first;
     for (int k0 = 0; k0 < top_k; k0 += kLanes) {
-      float w, dw;
-      const int id = choice(k0 + lane, w, dw);
-      const float add = normalize ? w / chosen * (dw - dot) : dw;
+      if (k0) c = choice(k0 + lane);
+      float add = c.dw;
+      if (normalize) add = (c.id >= 0 ? expf(c.logit - top) : 0.f) / chosen * (c.dw - dot);
       const int n = min(kLanes, top_k - k0);
       for (int j = 0; j < n; ++j) {
-        const int id_j = __shfl(id, j, kLanes);
+        const int id_j = __shfl(c.id, j, kLanes);
         const float add_j = __shfl(add, j, kLanes);
 #pragma unroll
         for (int r = 0; r < kPer; ++r)
-          if (id_j == r * kLanes + lane) extra[r] += add_j;
+          if (id_j == share.of(r)) extra[r] += add_j;
       }
     }
     float sum = 0.f;
@@ -314,28 +394,35 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
     sum = lanes_sum<kLanes>(sum);
     if (!mine) continue;
 #pragma unroll
-    for (int r = 0; r < kPer; ++r) {
-      const int e = r * kLanes + lane;
-      const float g = p[r] * (h[r] - sum) + (normalize ? extra[r] : 0.f);
-      if (e < experts) *dlogits.at(t, e) = T(on ? g : 0.f);
+    for (int r = 0; r < kPer; r += kWide) {
+      if (share.of(r) >= experts) continue;
+      Floats<kWide> g;
+#pragma unroll
+      for (int j = 0; j < kWide; ++j)
+        g[j] = on ? p[r + j] * (h[r + j] - sum) + (normalize ? extra[r + j] : 0.f) : 0.f;
+      store_piece<kWide>(dlogits.at(t, share.of(r)), g);
     }
   }
 }
 
 // ----------------------------------------------------------------- host side
 
-// Workgroups of the forward pass where the loss is wanted: what they leave is
-// added up by one workgroup.
-constexpr long long kRouteBlocks = 256;
+// Workgroups of the forward pass where the loss is wanted: as many large ones as
+// the device holds at once; what they leave is added up.
+constexpr long long kRouteBlocks = 512;
 long long route_blocks(long long tokens, int per_block, long long most) {
   const long long n = (tokens + per_block - 1) / per_block;
   return n < most ? n : most;
 }
 
-// Calls f(lanes, logits per lane).
+// Calls f(lanes, logits per lane, logits at a time).
 template <typename F>
 int with_lanes(int experts, F&& f) {
-  const auto call = [&](auto lanes, auto per) { return f(lanes, per); };
+  const auto call = [&](auto lanes, auto per) {
+    constexpr int kWide = per < 4 ? per : 4;
+    if (experts % kWide == 0) return f(lanes, per, std::integral_constant<int, kWide>{});
+    return f(lanes, per, std::integral_constant<int, 1>{});
+  };
   using std::integral_constant;
   if (experts <= 8) return call(integral_constant<int, 4>{}, integral_constant<int, 2>{});
   if (experts <= 16) return call(integral_constant<int, 8>{}, integral_constant<int, 2>{});
@@ -367,7 +454,8 @@ extern "C" {
 size_t ps_expert_route_workspace_bytes(long long tokens, int experts) {
   if (tokens < 0 || tokens > (1LL << 30) || experts < 1 || experts > ps::kMostExperts) return 0;
   const size_t blocks = tokens < ps::kRouteBlocks ? size_t(tokens) : size_t(ps::kRouteBlocks);
-  return (blocks ? blocks : 1) * (2 * size_t(experts) + 1) * 4;
+  // the totals, then the workgroups' parts
+  return size_t(experts) * 8 + (blocks + 1) * (2 * size_t(experts) + 1) * 4;
 }
 
 int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsigned char* mask,
@@ -396,37 +484,54 @@ int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsig
       PS_CHECK_ARG(!ps::overlap(to[i], to[k]), "ps_expert_route: outputs and workspace overlap");
   }
   const hipStream_t st = ps::to_hip(stream);
-  ps::RouteParts parts{nullptr, nullptr};
+  if (!logits->rows) {
+    if (!loss) return PS_OK;
+    ps::route_nothing_kernel<<<1, ps::kWave, 0, st>>>(experts, counts, loss);
+    PS_LAUNCHED();
+    return PS_OK;
+  }
+  ps::RouteParts parts{};
   long long blocks = 0;
   const int rc = ps::with_dtype(logits->dtype, [&](auto t) {
-    return ps::with_lanes(experts, [&](auto lanes, auto per) {
+    return ps::with_lanes(experts, [&](auto lanes, auto per, auto wide) {
       using T = decltype(t);
-      // Large workgroups where there is work for them: the join's parts are few.
-      const bool large = logits->rows > ps::kRouteBlocks * (256 / lanes);
-      const int threads = large ? 1024 : 256;
+      // Large workgroups where there is work for them, so that the parts are few, and
+      // shared memory for a sum of each expert and wave.
+      constexpr int kLarge = lanes * per <= 512 ? 1024 : 512;
+      const bool large = logits->rows > 256 * (256 / lanes);
+      const int threads = large ? kLarge : 256;
       blocks = ps::route_blocks(logits->rows, threads / lanes, loss ? ps::kRouteBlocks : 1 << 20);
       if (loss) {
-        parts.sums = static_cast<float*>(workspace);
-        parts.counts = reinterpret_cast<int*>(parts.sums + blocks * experts);
+        parts.all_sums = static_cast<double*>(workspace);
+        parts.all_counts = reinterpret_cast<int*>(parts.all_sums + experts);
+        parts.counts = parts.all_counts + experts + 1;
+        parts.sums = reinterpret_cast<float*>(parts.counts + blocks * (experts + 1));
       }
-      if (!blocks) return int(PS_OK);
       const auto run = [&](auto kernel) {
         kernel<<<uint32_t(blocks), threads, 0, st>>>(ps::mat<const T>(logits), experts, top_k,
-                                                     normalize != 0, mask, ids, weights, parts);
+                                                     normalize != 0, mask, ids, weights, parts,
+                                                     counts, loss);
       };
       if (large)
-        run(ps::route_kernel<T, lanes, per, 1024>);
+        run(ps::route_kernel<T, lanes, per, wide, kLarge>);
       else
-        run(ps::route_kernel<T, lanes, per, 256>);
+        run(ps::route_kernel<T, lanes, per, wide, 256>);
       PS_LAUNCHED();
       return int(PS_OK);
     });
   });
-  if (rc != PS_OK || !loss) return rc;
-  int groups = ps::kJoinThreads;
-  while (ps::kJoinThreads / groups < experts) groups /= 2;
-  ps::route_join_kernel<<<1, ps::kJoinThreads, 0, st>>>(parts, int(blocks), experts, groups, counts,
-                                                        loss);
+  if (rc != PS_OK || !loss || blocks == 1) return rc;
+  if (blocks <= ps::kFewParts) {
+    ps::route_join_few_kernel<<<1, ps::kFewThreads, 0, st>>>(parts, int(blocks), experts, counts,
+                                                             loss);
+    PS_LAUNCHED();
+    return PS_OK;
+  }
+  const uint32_t columns = 2 * uint32_t(experts) + 1;
+  ps::route_join_kernel<<<(columns + ps::kJoinCols - 1) / ps::kJoinCols,
+                          ps::kJoinCols * ps::kJoinLanes, 0, st>>>(parts, int(blocks), experts);
+  PS_LAUNCHED();
+  ps::route_finish_kernel<<<1, ps::kWave, 0, st>>>(parts, experts, counts, loss);
   PS_LAUNCHED();
   return PS_OK;
 }
@@ -454,10 +559,10 @@ int ps_expert_route_grad(const ps_rows* logits, int top_k, int normalize, const 
                "ps_expert_route_grad: dlogits overlaps an input");
   if (!logits->rows) return PS_OK;
   return ps::with_dtype(logits->dtype, [&](auto t) {
-    return ps::with_lanes(experts, [&](auto lanes, auto per) {
+    return ps::with_lanes(experts, [&](auto lanes, auto per, auto wide) {
       using T = decltype(t);
       const long long blocks = ps::route_blocks(logits->rows, ps::kRouteGradThreads / lanes, 4096);
-      ps::route_grad_kernel<T, lanes, per>
+      ps::route_grad_kernel<T, lanes, per, wide>
           <<<uint32_t(blocks), ps::kRouteGradThreads, 0, ps::to_hip(stream)>>>(
               ps::mat<const T>(logits), experts, top_k, normalize != 0, ids, dweights, counts,
               dloss, ps::mat<T>(dlogits));
