@@ -126,10 +126,11 @@ int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsig
                     size_t workspace_bytes, ps_stream_t stream);
 
 /* dlogits = the gradient of sum(dweights * weights) + *dloss * loss by the logits,
- * the choices as they are: ids and counts are what ps_expert_route gave (counts may
- * be summed over the ranks of a job: the gradient is of the loss over all their
- * tokens then). dweights NULL: zeros; dloss (device) NULL: no loss, and counts may
- * be NULL too. A token whose first id is negative gets zeros. */
+ * the choices as they are: ids (a token's all different where they are not negative)
+ * and counts are what ps_expert_route gave. Counts may be summed over the ranks of
+ * a job: the gradient is of the loss over all their tokens then. dweights NULL:
+ * zeros; dloss (device) NULL: no loss, and counts may be NULL too. A token whose
+ * first id is negative gets zeros. */
 int ps_expert_route_grad(const ps_rows* logits, int top_k, int normalize, const int* ids,
                          const float* dweights, const int* counts, const float* dloss,
                          const ps_rows* dlogits, ps_stream_t stream);

@@ -12,17 +12,23 @@ namespace {
 
 constexpr int kMostExperts = 1024;
 
-// Unsigned numbers that order as logits do, 0 for barred ones (-inf), the most
-// for NaN; -0 and 0 are equal.
+// Unsigned numbers that order as logits do, NaN above all; -0 and 0 are equal.
+// Barred experts (-inf) and taken ones (0) are at kBarred or below.
+constexpr uint32_t kBarred = 0x007fffffu;
 __device__ __forceinline__ uint32_t key_of(float v) {
-  if (v != v) return ~0u;
-  if (v == -INFINITY) return 0;
-  const uint32_t b = __float_as_uint(v + 0.f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const int b = __float_as_int(v + 0.f);
+  const uint32_t key = uint32_t(b ^ ((b >> 31) | int(0x80000000u)));
+  return v != v ? ~0u : key;
 }
 // (~0 comes back as a NaN)
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+// e^x for x <= 0 by the hardware's power of two, off by 2^-24 (2 + 1.3 |x|)
+// relative: as much again as the logits' difference x itself.
+__device__ __forceinline__ float exp_of(float x) {
+  return __builtin_amdgcn_exp2f(x * 1.44269504f);
 }
 
 // Over the kLanes lanes of a token, in every one of them.
@@ -118,21 +124,23 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
     const long long t = t0 + threadIdx.x / kLanes;
     const bool mine = t < logits.rows, on = mine && (!mask || mask[t]);
     uint32_t key[kPer];
-    uint32_t most = 0;
-    share.load(logits, t, experts, on, -INFINITY, [&](int r, float v) {
-      key[r] = key_of(v);
-      most = max(most, key[r]);
-    });
-    most = lanes_max<kLanes>(most);
-    const float top = most ? value_of(most) : 0.f;  // nothing to choose: no probabilities either
+    uint32_t best = 0;
     float p[kPer], s = 0.f;
+    share.load(logits, t, experts, on, -INFINITY, [&](int r, float v) {
+      p[r] = v;
+      key[r] = key_of(v);
+      best = max(best, key[r]);
+    });
+    best = lanes_max<kLanes>(best);
+    const bool most = best > kBarred;
+    const float top = most ? value_of(best) : 0.f;  // nothing to choose: no probabilities either
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      p[r] = key[r] ? expf(value_of(key[r]) - top) : 0.f;
+      p[r] = exp_of(p[r] - top);
       s += p[r];
     }
     s = lanes_sum<kLanes>(s);
-    const float scale = most ? 1.f / s : 0.f;
+    const float scale = most ? __builtin_amdgcn_rcpf(s) : 0.f;
     if (parts.sums) {
 #pragma unroll
       for (int r = 0; r < kPer; ++r) acc[r] += p[r] * scale;
@@ -143,20 +151,28 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
     float total = 0.f, my_w = 0.f;
     int my_id = -1;  // slot k's are kept by lane k % kLanes
     for (int k = 0; k < top_k; ++k) {
-      uint32_t best = 0, at = ~0u;
+      if (k) {
+        best = key[0];
 #pragma unroll
-      for (int r = 0; r < kPer; ++r) best = max(best, key[r]);
-      best = lanes_max<kLanes>(best);
-      if (best) {
-#pragma unroll
-        for (int r = kPer - 1; r >= 0; --r)
-          if (key[r] == best) at = uint32_t(share.of(r));
+        for (int r = 1; r < kPer; ++r) best = max(best, key[r]);
+        best = lanes_max<kLanes>(best);
       }
-      at = lanes_min<kLanes>(at);
+      // The first of this lane's that are the best one, and of all lanes'.
+      const bool any = best > kBarred;
+      bool found = !any, is[kPer];
+      uint32_t mine_at = ~0u;
+#pragma unroll
+      for (int r = 0; r < kPer; ++r) {
+        is[r] = !found && key[r] == best;
+        found = found || is[r];
+        if (is[r]) mine_at = uint32_t(share.of(r));
+      }
+      const uint32_t at = lanes_min<kLanes>(mine_at);
+      const bool taken = mine_at == at;
 #pragma unroll
       for (int r = 0; r < kPer; ++r)
-        if (at == uint32_t(share.of(r))) key[r] = 0;
-      const float w = best ? expf(value_of(best) - top) : 0.f;
+        if (is[r] && taken) key[r] = 0;
+      const float w = any ? exp_of(value_of(best) - top) : 0.f;
       total += w;
       if (lane == k % kLanes) {
         my_id = int(at);
@@ -175,7 +191,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
       if (lane < top_k && mine) {
         if (parts.sums && my_id >= 0) atomicAdd(&chosen[my_id], 1);
         ids_t[lane] = my_id;
-        weights_t[lane] = normalize && most ? my_w / total : my_w;
+        weights_t[lane] = normalize && most ? my_w * __builtin_amdgcn_rcpf(total) : my_w;
       }
     } else if (normalize && mine) {
       for (int k = lane; k < top_k; k += kLanes) weights_t[k] = most ? weights_t[k] / total : 0.f;
@@ -293,8 +309,15 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
     const float* __restrict__ dweights, const int* __restrict__ counts,
     const float* __restrict__ dloss, Mat<T> dlogits) {
   constexpr int kTokens = kRouteGradThreads / kLanes;
+  // What the choices add to a token's logits, put in place by the lanes that know it
+  // and read by those that have the logits, all in one wave.
+  __shared__ float rows[kTokens][kLanes * kPer];
+  float* const row = rows[threadIdx.x / kLanes];
   const int lane = threadIdx.x % kLanes;
   const Share<kLanes, kPer, kWide> share(lane);
+#pragma unroll
+  for (int r = 0; r < kPer; ++r) row[share.of(r)] = 0.f;
+  wave_lds_sync();
   // The loss's gradient by an expert's probability.
   float by_loss[kPer];
 #pragma unroll
@@ -338,25 +361,15 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
     const Choice first = choice(lane);
     const bool on = id_0 >= 0;
 #pragma unroll
-    for (int r = 0; r < kPer; ++r) {
-      p[r] = on ? p[r] : -INFINITY;
-      top = fmaxf(top, p[r]);
-      h[r] = by_loss[r];
-    }
+    for (int r = 0; r < kPer; ++r) top = fmaxf(top, p[r]);
     top = lanes_all<kLanes>(top, [](float a, float b) { return fmaxf(a, b); });
     if (top == -INFINITY) top = 0.f;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      p[r] = expf(p[r] - top);
+      p[r] = exp_of(p[r] - top);
       s += p[r];
     }
-    s = lanes_sum<kLanes>(s);
-    const float scale = on ? 1.f / s : 0.f;
-#pragma unroll
-    for (int r = 0; r < kPer; ++r) p[r] = on ? p[r] * scale : 0.f;
-    float extra[kPer];
-#pragma unroll
-    for (int r = 0; r < kPer; ++r) extra[r] = 0.f;
+    const float scale = __builtin_amdgcn_rcpf(lanes_sum<kLanes>(s));
     // What the chosen experts' weights' gradients add, kLanes of them at a time: the
     // first ones have been loaded.
     float chosen = 0.f, dot = 0.f;
@@ -364,33 +377,32 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
       Choice c = first;
       for (int k = 0; k < top_k; k += kLanes) {
         if (k) c = choice(k + lane);
-        const float w = c.id >= 0 ? expf(c.logit - top) : 0.f;
+        const float w = c.id >= 0 ? exp_of(c.logit - top) : 0.f;
         chosen += w;
         dot += w * c.dw;
       }
-      chosen = lanes_sum<kLanes>(chosen);
-      dot = lanes_sum<kLanes>(dot) / chosen;
+      chosen = __builtin_amdgcn_rcpf(lanes_sum<kLanes>(chosen));
+      dot = lanes_sum<kLanes>(dot) * chosen;
     }
     Choice c = first;
     for (int k0 = 0; k0 < top_k; k0 += kLanes) {
       if (k0) c = choice(k0 + lane);
-      float add = c.dw;
-      if (normalize) add = (c.id >= 0 ? expf(c.logit - top) : 0.f) / chosen * (c.dw - dot);
-      const int n = min(kLanes, top_k - k0);
-      for (int j = 0; j < n; ++j) {
-        const int id_j = __shfl(c.id, j, kLanes);
-        const float add_j = __shfl(add, j, kLanes);
-#pragma unroll
-        for (int r = 0; r < kPer; ++r)
-          if (id_j == share.of(r)) extra[r] += add_j;
-      }
+      if (c.id < 0) continue;
+      atomicAdd(&row[c.id], normalize ? exp_of(c.logit - top) * chosen * (c.dw - dot) : c.dw);
     }
-    float sum = 0.f;
+    wave_lds_sync();
+    float extra[kPer], sum = 0.f;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      if (!normalize) h[r] += extra[r];
+      extra[r] = row[share.of(r)];
+      p[r] *= scale;
+      h[r] = by_loss[r] + (normalize ? 0.f : extra[r]);
       sum += p[r] * h[r];
     }
+    wave_lds_sync();
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) row[share.of(r)] = 0.f;
+    wave_lds_sync();
     sum = lanes_sum<kLanes>(sum);
     if (!mine) continue;
 #pragma unroll
@@ -398,8 +410,10 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
       if (share.of(r) >= experts) continue;
       Floats<kWide> g;
 #pragma unroll
-      for (int j = 0; j < kWide; ++j)
-        g[j] = on ? p[r + j] * (h[r + j] - sum) + (normalize ? extra[r + j] : 0.f) : 0.f;
+      for (int j = 0; j < kWide; ++j) {
+        const float d = p[r + j] * (h[r + j] - sum);
+        g[j] = on ? normalize ? d + extra[r + j] : d : 0.f;
+      }
       store_piece<kWide>(dlogits.at(t, share.of(r)), g);
     }
   }
@@ -415,9 +429,12 @@ long long route_blocks(long long tokens, int per_block, long long most) {
   return n < most ? n : most;
 }
 
-// Calls f(lanes, logits per lane, logits at a time).
+// Calls f(lanes, logits per lane, logits at a time). `many`: half as many lanes for
+// 65 to 512 experts: less work in all, as a lane's part of finding the next expert
+// hardly grows, and longer for a token alone (65,536 x 128 top 8 18 -> 16 us, 16,384
+// x 512 20 -> 16; but 512 x 64 4.3 -> 5.9, and the gradient 19.3 -> 20.2).
 template <typename F>
-int with_lanes(int experts, F&& f) {
+int with_lanes(int experts, bool many, F&& f) {
   const auto call = [&](auto lanes, auto per) {
     constexpr int kWide = per < 4 ? per : 4;
     if (experts % kWide == 0) return f(lanes, per, std::integral_constant<int, kWide>{});
@@ -428,6 +445,12 @@ int with_lanes(int experts, F&& f) {
   if (experts <= 16) return call(integral_constant<int, 8>{}, integral_constant<int, 2>{});
   if (experts <= 32) return call(integral_constant<int, 8>{}, integral_constant<int, 4>{});
   if (experts <= 64) return call(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+  if (many && experts <= 512) {
+    const auto per = integral_constant<int, 16>{};
+    if (experts <= 128) return call(integral_constant<int, 8>{}, per);
+    if (experts <= 256) return call(integral_constant<int, 16>{}, per);
+    return call(integral_constant<int, 32>{}, per);
+  }
   if (experts <= 128) return call(integral_constant<int, 16>{}, integral_constant<int, 8>{});
   if (experts <= 256) return call(integral_constant<int, 32>{}, integral_constant<int, 8>{});
   if (experts <= 512) return call(integral_constant<int, 64>{}, integral_constant<int, 8>{});
@@ -493,7 +516,7 @@ int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsig
   ps::RouteParts parts{};
   long long blocks = 0;
   const int rc = ps::with_dtype(logits->dtype, [&](auto t) {
-    return ps::with_lanes(experts, [&](auto lanes, auto per, auto wide) {
+    return ps::with_lanes(experts, logits->rows >= 8192, [&](auto lanes, auto per, auto wide) {
       using T = decltype(t);
       // Large workgroups where there is work for them, so that the parts are few, and
       // shared memory for a sum of each expert and wave.
@@ -559,7 +582,7 @@ int ps_expert_route_grad(const ps_rows* logits, int top_k, int normalize, const 
                "ps_expert_route_grad: dlogits overlaps an input");
   if (!logits->rows) return PS_OK;
   return ps::with_dtype(logits->dtype, [&](auto t) {
-    return ps::with_lanes(experts, [&](auto lanes, auto per, auto wide) {
+    return ps::with_lanes(experts, false, [&](auto lanes, auto per, auto wide) {
       using T = decltype(t);
       const long long blocks = ps::route_blocks(logits->rows, ps::kRouteGradThreads / lanes, 4096);
       ps::route_grad_kernel<T, lanes, per, wide>
