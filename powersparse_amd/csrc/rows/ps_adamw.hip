@@ -100,45 +100,87 @@ __device__ __forceinline__ float updated(const AdamStep& s, float decay, float p
   return fmaf(-s.lr, fmaf(decay, p, up), p);
 }
 
+// Addresses from the table, as global memory: the compiler would otherwise take
+// them for any kind and wait for shared memory too.
+template <typename T>
+using Global = __attribute__((address_space(1))) T*;
+template <int N, typename T>
+__device__ __forceinline__ typename PieceOf<T, N>::type raw(const T* p) {
+  return *(Global<const typename PieceOf<T, N>::type>)p;
+}
+template <int N, typename V>
+__device__ __forceinline__ Floats<N> floats(V v) {
+  return __builtin_convertvector(v, Floats<N>);
+}
+template <int N, typename T>
+__device__ __forceinline__ void put(T* p, const Floats<N>& f) {
+  using V = typename PieceOf<T, N>::type;
+  *(Global<V>)p = __builtin_convertvector(f, V);
+}
+
 template <int N>
 __device__ __forceinline__ void store_copy(const AdamTensor& t, long long i, const Floats<N>& f) {
   if (!t.copy) return;
   if (t.copy_dtype == PS_F32)
-    store_piece<N>(static_cast<f32*>(t.copy) + i, f);
+    put<N>(static_cast<f32*>(t.copy) + i, f);
   else if (t.copy_dtype == PS_F16)
-    store_piece<N>(static_cast<f16*>(t.copy) + i, f);
+    put<N>(static_cast<f16*>(t.copy) + i, f);
   else
-    store_piece<N>(static_cast<bf16*>(t.copy) + i, f);
+    put<N>(static_cast<bf16*>(t.copy) + i, f);
 }
 
-// N elements at i of a tensor with moments in 32 bits.
+// N elements of a tensor with moments in 32 bits.
 template <int N, typename P, typename G>
-__device__ __forceinline__ void step_f32(const AdamTensor& t, const AdamStep& s, long long i) {
-  P* const param = static_cast<P*>(t.param) + i;
-  float* const exp_avg = static_cast<float*>(t.exp_avg) + i;
-  float* const exp_avg_sq = static_cast<float*>(t.exp_avg_sq) + i;
-  Floats<N> p = load_piece<N>(param), m = load_piece<N>(exp_avg), v = load_piece<N>(exp_avg_sq);
-  const Floats<N> g = load_piece<N>(static_cast<const G*>(t.grad) + i);
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    float me = m[e], ve = v[e];
-    advance(s, g[e], &me, &ve);
-    p[e] = updated(s, t.decay, p[e], me, __builtin_amdgcn_sqrtf(ve));
-    m[e] = me;
-    v[e] = ve;
+struct Elements {
+  typename PieceOf<P, N>::type p;
+  typename PieceOf<G, N>::type g;
+  Floats<N> m, v;
+  __device__ __forceinline__ void load(const AdamTensor& t, long long i) {
+    p = raw<N>(static_cast<const P*>(t.param) + i);
+    g = raw<N>(static_cast<const G*>(t.grad) + i);
+    m = raw<N>(static_cast<const float*>(t.exp_avg) + i);
+    v = raw<N>(static_cast<const float*>(t.exp_avg_sq) + i);
   }
-  store_piece<N>(param, p);
-  store_piece<N>(exp_avg, m);
-  store_piece<N>(exp_avg_sq, v);
-  store_copy<N>(t, i, p);
-}
+  __device__ __forceinline__ void step(const AdamTensor& t, const AdamStep& s, long long i) {
+    Floats<N> pf = floats<N>(p);
+    const Floats<N> gf = floats<N>(g);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      float me = m[e], ve = v[e];
+      advance(s, gf[e], &me, &ve);
+      pf[e] = updated(s, t.decay, pf[e], me, __builtin_amdgcn_sqrtf(ve));
+      m[e] = me;
+      v[e] = ve;
+    }
+    put<N>(static_cast<P*>(t.param) + i, pf);
+    put<N>(static_cast<float*>(t.exp_avg) + i, m);
+    put<N>(static_cast<float*>(t.exp_avg_sq) + i, v);
+    store_copy<N>(t, i, pf);
+  }
+};
 
 template <typename P, typename G>
 __device__ void chunk_f32(const AdamTensor& t, const AdamStep& s, long long from, uint32_t count) {
-  constexpr int N = 4;
+  constexpr int N = 4, kTurn = kListThreads * N, kTurns = int(kChunk / kTurn);
   uint32_t i = threadIdx.x * N;
-  for (; i + N <= count; i += kListThreads * N) step_f32<N, P, G>(t, s, from + i);
-  for (; i < count; ++i) step_f32<1, P, G>(t, s, from + i);
+  if (count == kChunk) {  // all loads before the first store, which might be to any of them
+    Elements<N, P, G> all[kTurns];
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) all[k].load(t, from + i + k * kTurn);
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) all[k].step(t, s, from + i + k * kTurn);
+    return;
+  }
+  for (; i + N <= count; i += kTurn) {
+    Elements<N, P, G> some;
+    some.load(t, from + i);
+    some.step(t, s, from + i);
+  }
+  for (; i < count; ++i) {
+    Elements<1, P, G> one;
+    one.load(t, from + i);
+    one.step(t, s, from + i);
+  }
 }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -155,110 +197,126 @@ __device__ __forceinline__ float on_grid(float a, uint32_t u) {
   return f > 448.f ? 448.f : f;  // (a NaN stays one)
 }
 
-// N elements of four at i, zeros behind them.
-template <typename T>
-__device__ __forceinline__ Floats<4> load_some(const T* p, int n) {
-  if (n >= 4) return load_piece<4>(p);
-  Floats<4> f = 0.f;
+// Four elements, or n of them in a tensor's last block (zeros behind them).
+template <bool kWhole, typename T>
+__device__ __forceinline__ typename PieceOf<T, 4>::type some(const T* p, int n) {
+  if (kWhole || n >= 4) return raw<4>(p);
+  typename PieceOf<T, 4>::type v = T(0);
 #pragma unroll
   for (int e = 0; e < 3; ++e)
-    if (e < n) f[e] = float(p[e]);
-  return f;
-}
-template <typename T>
-__device__ __forceinline__ void store_some(T* p, const Floats<4>& f, int n) {
-  if (n >= 4) return store_piece<4>(p, f);
-#pragma unroll
-  for (int e = 0; e < 3; ++e)
-    if (e < n) p[e] = T(f[e]);
-}
-using Codes = PieceOf<uint8_t, 4>::type;
-__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int n) {
-  if (n >= 4) return __builtin_bit_cast(uint32_t, *reinterpret_cast<const Codes*>(p));
-  uint32_t v = 0;
-#pragma unroll
-  for (int e = 0; e < 3; ++e)
-    if (e < n) v |= uint32_t(p[e]) << 8 * e;
+    if (e < n) v[e] = *(Global<const T>)(p + e);
   return v;
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, uint32_t v, int n) {
-  if (n >= 4) {
-    *reinterpret_cast<Codes*>(p) = __builtin_bit_cast(Codes, v);
+template <bool kWhole, typename T>
+__device__ __forceinline__ void put_some(T* p, typename PieceOf<T, 4>::type v, int n) {
+  if (kWhole || n >= 4) {
+    *(Global<typename PieceOf<T, 4>::type>)p = v;
     return;
   }
 #pragma unroll
   for (int e = 0; e < 3; ++e)
-    if (e < n) p[e] = uint8_t(v >> 8 * e);
+    if (e < n) *(Global<T>)(p + e) = v[e];
 }
-__device__ __forceinline__ Floats<4> from_codes(uint32_t v) {
-  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(int(v), false);
-  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(int(v), true);
+template <bool kWhole, typename T>
+__device__ __forceinline__ void put_as(T* p, const Floats<4>& f, int n) {
+  put_some<kWhole>(p, __builtin_convertvector(f, typename PieceOf<T, 4>::type), n);
+}
+using Codes = PieceOf<uint8_t, 4>::type;
+__device__ __forceinline__ Floats<4> from_codes(Codes c) {
+  const int v = __builtin_bit_cast(int, c);
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(v, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
   return Floats<4>{lo[0], lo[1], hi[0], hi[1]};
 }
-__device__ __forceinline__ uint32_t to_codes(const Floats<4>& f) {
+__device__ __forceinline__ Codes to_codes(const Floats<4>& f) {
   const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-  return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], lo, true));
+  return __builtin_bit_cast(Codes, __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], lo, true));
 }
 
 // A block of a tensor with moments in 8 bits: a wave, four elements a lane.
-template <typename P, typename G>
-__device__ void block_f8(const AdamTensor& t, const AdamStep& s, long long from) {
-  const long long i = from + lane_id() * 4;
-  const int n = int(max(0LL, min(4LL, t.count - i)));
-  P* const param = static_cast<P*>(t.param) + i;
-  uint8_t* const exp_avg = static_cast<uint8_t*>(t.exp_avg) + i;
-  uint8_t* const exp_avg_sq = static_cast<uint8_t*>(t.exp_avg_sq) + i;
-  float* const scales = t.scales + from / kStateBlock * 2;
-  Floats<4> p = load_some(param, n);
-  const Floats<4> g = load_some(static_cast<const G*>(t.grad) + i, n);
-  Floats<4> m = from_codes(load_codes(exp_avg, n)) * scales[0];
-  Floats<4> r = from_codes(load_codes(exp_avg_sq, n)) * scales[1];
-  float m_most = 0.f, r_most = 0.f;
+template <typename P, typename G, bool kWhole>
+struct Block {
+  typename PieceOf<P, 4>::type p;
+  typename PieceOf<G, 4>::type g;
+  Codes m, r;
+  Floats<2> scales;
+
+  // `from`: the block's first element.
+  __device__ __forceinline__ void load(const AdamTensor& t, long long from) {
+    const long long i = from + lane_id() * 4;
+    const int n = left(t, i);
+    p = some<kWhole>(static_cast<const P*>(t.param) + i, n);
+    g = some<kWhole>(static_cast<const G*>(t.grad) + i, n);
+    m = some<kWhole>(static_cast<const uint8_t*>(t.exp_avg) + i, n);
+    r = some<kWhole>(static_cast<const uint8_t*>(t.exp_avg_sq) + i, n);
+    scales = raw<2>(t.scales + from / kStateBlock * 2);
+  }
+  __device__ __forceinline__ void step(const AdamTensor& t, const AdamStep& s, long long from) {
+    const long long i = from + lane_id() * 4;
+    const int n = left(t, i);
+    Floats<4> pf = floats<4>(p), mf = from_codes(m) * scales[0], rf = from_codes(r) * scales[1];
+    const Floats<4> gf = floats<4>(g);
+    float m_most = 0.f, r_most = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float me = m[e], ve = r[e] * r[e];
-    advance(s, g[e], &me, &ve);
-    const float root = sqrtf(ve);
-    p[e] = updated(s, t.decay, p[e], me, root);
-    m[e] = me;
-    r[e] = root;
-    m_most = fmaxf(m_most, fabsf(me));
-    r_most = fmaxf(r_most, root);
-  }
-  m_most = wave_max(m_most);
-  r_most = wave_max(r_most);
-  const float m_scale = fmaxf(m_most * (1.f / 448.f), 0x1p-126f);
-  const float r_scale = fmaxf(r_most * (1.f / 448.f), 0x1p-126f);
-  const float by_m = 1.f / m_scale, by_r = 1.f / r_scale;
+    for (int e = 0; e < 4; ++e) {
+      float me = mf[e], ve = rf[e] * rf[e];
+      advance(s, gf[e], &me, &ve);
+      const float root = sqrtf(ve);
+      pf[e] = updated(s, t.decay, pf[e], me, root);
+      mf[e] = me;
+      rf[e] = root;
+      m_most = fmaxf(m_most, fabsf(me));
+      r_most = fmaxf(r_most, root);
+    }
+    put_as<kWhole>(static_cast<P*>(t.param) + i, pf, n);
+    if (t.copy) {
+      if (t.copy_dtype == PS_F32)
+        put_as<kWhole>(static_cast<f32*>(t.copy) + i, pf, n);
+      else if (t.copy_dtype == PS_F16)
+        put_as<kWhole>(static_cast<f16*>(t.copy) + i, pf, n);
+      else
+        put_as<kWhole>(static_cast<bf16*>(t.copy) + i, pf, n);
+    }
+    m_most = wave_max(m_most);
+    r_most = wave_max(r_most);
+    const float m_scale = fmaxf(m_most * (1.f / 448.f), 0x1p-126f);
+    const float r_scale = fmaxf(r_most * (1.f / 448.f), 0x1p-126f);
+    const float by_m = 1.f / m_scale, by_r = 1.f / r_scale;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t u = uint32_t(i + e) * kByElement + s.weyl;
-    m[e] = copysignf(on_grid(quotient(fabsf(m[e]), m_scale, by_m), u), m[e]);
-    const float code = on_grid(quotient(r[e], r_scale, by_r), u);
-    r[e] = r[e] > 0.f ? fmaxf(code, 0x1p-9f) : code;
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t u = uint32_t(i + e) * kByElement + s.weyl;
+      mf[e] = copysignf(on_grid(quotient(fabsf(mf[e]), m_scale, by_m), u), mf[e]);
+      const float code = on_grid(quotient(rf[e], r_scale, by_r), u);
+      rf[e] = rf[e] > 0.f ? fmaxf(code, 0x1p-9f) : code;
+    }
+    put_some<kWhole>(static_cast<uint8_t*>(t.exp_avg) + i, to_codes(mf), n);
+    put_some<kWhole>(static_cast<uint8_t*>(t.exp_avg_sq) + i, to_codes(rf), n);
+    if (lane_id() == 0) put<2>(t.scales + from / kStateBlock * 2, Floats<2>{m_scale, r_scale});
   }
-  store_some(param, p, n);
-  store_codes(exp_avg, to_codes(m), n);
-  store_codes(exp_avg_sq, to_codes(r), n);
-  if (t.copy) {
-    if (t.copy_dtype == PS_F32)
-      store_some(static_cast<f32*>(t.copy) + i, p, n);
-    else if (t.copy_dtype == PS_F16)
-      store_some(static_cast<f16*>(t.copy) + i, p, n);
-    else
-      store_some(static_cast<bf16*>(t.copy) + i, p, n);
+
+ private:
+  static __device__ __forceinline__ int left(const AdamTensor& t, long long i) {
+    return kWhole ? 4 : int(max(0LL, min(4LL, t.count - i)));
   }
-  if (lane_id() == 0) {
-    scales[0] = m_scale;
-    scales[1] = r_scale;
-  }
-}
+};
 
 template <typename P, typename G>
 __device__ void chunk_f8(const AdamTensor& t, const AdamStep& s, long long from, uint32_t count) {
-  for (uint32_t i = threadIdx.x / kWave * kStateBlock; i < count;
-       i += kListThreads / kWave * kStateBlock)
-    block_f8<P, G>(t, s, from + i);
+  constexpr int kTurn = kListThreads / kWave * kStateBlock, kTurns = int(kChunk / kTurn);
+  uint32_t i = threadIdx.x / kWave * kStateBlock;
+  if (count == kChunk) {
+    Block<P, G, true> all[kTurns];
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) all[k].load(t, from + i + k * kTurn);
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) all[k].step(t, s, from + i + k * kTurn);
+    return;
+  }
+  for (; i < count; i += kTurn) {
+    Block<P, G, false> one;
+    one.load(t, from + i);
+    one.step(t, s, from + i);
+  }
 }
 
 template <bool k8, typename P, typename G>
