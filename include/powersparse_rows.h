@@ -232,8 +232,8 @@ typedef struct ps_adamw_options {
  * changes. The parameter moves by the moments before they are rounded to 8 bits;
  * there they go to either neighbouring code, by a rule of step and place that
  * keeps their mean over the steps, and a second moment that is not zero stays so.
- * A gradient that is not finite makes its element's moments NaN, in 8 bits perhaps
- * its block's. */
+ * A gradient that is not finite makes its element's moments so, in 8 bits its
+ * block's. */
 int ps_adamw_step(ps_adamw_list* list, const ps_adamw_options* options, ps_stream_t stream);
 
 #ifdef __cplusplus
