@@ -1,6 +1,6 @@
 // The row operators (powersparse_rows.h) for C++ callers: the same entry points
 // with errors as exceptions (PS_ERR_INVALID -> std::invalid_argument, else
-// std::runtime_error), and the gradient list as an owner. No reference
+// std::runtime_error), and the lists of tensors as owners. No reference
 // counterpart. Matrices and ids are the C ABI's ps_rows and ps_ids; every call is
 // enqueued on `stream` and returns.
 #ifndef POWERSPARSE_ROWS_HOST_H
@@ -64,6 +64,46 @@ inline void ExpertCombineGrad(const ps_rows& dy, const ps_rows& ys, const int* p
   ThrowOnError(ps_expert_combine_grad(&dy, &ys, position, weights, top_k, &dys, dweights, stream));
 }
 
+// The router: ids and weights (logits.rows x top_k) of every token's experts, mask
+// (null: none) a byte a token. counts (experts + 1) and loss (one value), or null for
+// both and the workspace: ps_expert_route_workspace_bytes(logits.rows, logits.cols).
+inline void ExpertRoute(const ps_rows& logits, int top_k, int* ids, float* weights,
+                        int* counts = nullptr, float* loss = nullptr, void* workspace = nullptr,
+                        size_t workspace_bytes = 0, const unsigned char* mask = nullptr,
+                        bool normalize = true, ps_stream_t stream = nullptr) {
+  ThrowOnError(ps_expert_route(&logits, top_k, normalize, mask, ids, weights, counts, loss,
+                               workspace, workspace_bytes, stream));
+}
+
+// dlogits = the gradient of sum(dweights * weights) + *dloss * loss; dweights null:
+// zeros, dloss null: no loss.
+inline void ExpertRouteGrad(const ps_rows& logits, int top_k, const int* ids,
+                            const float* dweights, const int* counts, const float* dloss,
+                            const ps_rows& dlogits, bool normalize = true,
+                            ps_stream_t stream = nullptr) {
+  ThrowOnError(ps_expert_route_grad(&logits, top_k, normalize, ids, dweights, counts, dloss,
+                                    &dlogits, stream));
+}
+
+// y = (x - mean) * rstd * weight + bias for every row; weight and bias (one row
+// each) or null, mean and rstd (a value a row) or null.
+inline void LayerNorm(const ps_rows& x, const ps_rows* weight, const ps_rows* bias, float eps,
+                      const ps_rows& y, float* mean = nullptr, float* rstd = nullptr,
+                      ps_stream_t stream = nullptr) {
+  ThrowOnError(ps_layer_norm(&x, weight, bias, eps, &y, mean, rstd, stream));
+}
+
+// The gradients of LayerNorm; dweight and dbias null: not wanted, nor the workspace
+// then: ps_layer_norm_grad_workspace_bytes(x.rows, x.cols).
+inline void LayerNormGrad(const ps_rows& dy, const ps_rows& x, const ps_rows* weight,
+                          const float* mean, const float* rstd, const ps_rows& dx,
+                          const ps_rows* dweight, const ps_rows* dbias, void* workspace,
+                          size_t workspace_bytes, bool accumulate = false,
+                          ps_stream_t stream = nullptr) {
+  ThrowOnError(ps_layer_norm_grad(&dy, &x, weight, mean, rstd, accumulate, &dx, dweight, dbias,
+                                  workspace, workspace_bytes, stream));
+}
+
 // A gradient tensor: `count` contiguous elements of `dtype` (PS_F32, ...).
 struct Gradient {
   void* data;
@@ -117,6 +157,25 @@ class GradientList {
 
  private:
   ps_grad_list* list_ = nullptr;
+};
+
+// The tensors that AdamW updates (ps_adamw_tensor says what each holds).
+class AdamWList {
+ public:
+  // state_dtype: PS_F32, or PS_E4M3 for moments in 8 bits.
+  explicit AdamWList(const std::vector<ps_adamw_tensor>& tensors, int state_dtype = PS_F32) {
+    ThrowOnError(ps_adamw_list_create(int(tensors.size()), tensors.data(), state_dtype, &list_));
+  }
+  ~AdamWList() { ps_adamw_list_destroy(list_); }
+  AdamWList(const AdamWList&) = delete;
+  AdamWList& operator=(const AdamWList&) = delete;
+
+  void Step(const ps_adamw_options& options, ps_stream_t stream = nullptr) const {
+    ThrowOnError(ps_adamw_step(list_, &options, stream));
+  }
+
+ private:
+  ps_adamw_list* list_ = nullptr;
 };
 
 }  // namespace PowerSparse
