@@ -4,7 +4,13 @@
 //
 // kLanes threads share a token, each with kPer of its logits in registers, kWide
 // neighbours at a time. The largest logits are found one after another, by keys
-// that order as the logits do; equal ones go to the lowest expert.
+// that order as the logits do; equal ones go to the lowest expert. Finding them is
+// most of the work, so the keys are cut to leave room for the expert beside them: a
+// maximum then says which, and as no two are equal the next one is the largest of
+// the differences from it that are below zero, two operations an element. What was
+// cut off decides where two keys agree in what is left: FP16 and BF16 lose nothing,
+// FP32 the last 8 bits for 128 experts (11 for 1,024), and a wave that meets two
+// such logits in a row takes the longer way, which finds the expert behind its key.
 #include "ps_rows.hpp"
 
 namespace ps {
@@ -105,7 +111,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
     const unsigned char* __restrict__ mask, int* __restrict__ ids, float* __restrict__ weights,
     RouteParts parts, int* __restrict__ counts, float* __restrict__ loss) {
   constexpr int kTokens = kThreads / kLanes;
-  constexpr int kMost = kLanes * kPer;
+  constexpr int kMost = kLanes * kPer, kBits = __builtin_ctz(kMost);
   __shared__ int chosen[kMost + 1];
   __shared__ float sums[kThreads / kWave][kMost];
   const int lane = threadIdx.x % kLanes;
@@ -123,78 +129,100 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
        t0 += (long long)gridDim.x * kTokens) {
     const long long t = t0 + threadIdx.x / kLanes;
     const bool mine = t < logits.rows, on = mine && (!mask || mask[t]);
-    uint32_t key[kPer];
-    uint32_t best = 0;
+    uint32_t key[kPer], most = 0;  // cut, with the expert
     float p[kPer], s = 0.f;
     share.load(logits, t, experts, on, -INFINITY, [&](int r, float v) {
       p[r] = v;
-      key[r] = key_of(v);
-      best = max(best, key[r]);
+      const uint32_t whole = key_of(v);
+      most = max(most, whole);
+      key[r] = (whole >> (kBits + 1) << kBits) + uint32_t(kMost - 1 - share.of(r));
     });
-    best = lanes_max<kLanes>(best);
-    const bool most = best > kBarred;
-    const float top = most ? value_of(best) : 0.f;  // nothing to choose: no probabilities either
+    most = lanes_max<kLanes>(most);
+    // nothing to choose: no probabilities either
+    const float top = most > kBarred ? value_of(most) : 0.f;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
       p[r] = exp_of(p[r] - top);
       s += p[r];
     }
     s = lanes_sum<kLanes>(s);
-    const float scale = most ? __builtin_amdgcn_rcpf(s) : 0.f;
+    const float scale = most > kBarred ? __builtin_amdgcn_rcpf(s) : 0.f;
     if (parts.sums) {
 #pragma unroll
       for (int r = 0; r < kPer; ++r) acc[r] += p[r] * scale;
-      tokens += lane == 0 && most;
+      tokens += lane == 0 && most > kBarred;
     }
-    int* const ids_t = ids + t * top_k;
-    float* const weights_t = weights + t * top_k;
-    float total = 0.f, my_w = 0.f;
-    int my_id = -1;  // slot k's are kept by lane k % kLanes
-    for (int k = 0; k < top_k; ++k) {
-      if (k) {
-        best = key[0];
+    // Slot k's expert is found by all lanes and kept by lane k % kLanes.
+    int my_id = -1;
+    bool found = top_k <= kLanes;
+    if (found) {
+      uint32_t best = key[0];
+#pragma unroll
+      for (int r = 1; r < kPer; ++r) best = max(best, key[r]);
+      best = lanes_max<kLanes>(best);
+      bool equal = false;
+      for (int k = 0; k < top_k; ++k) {
+        const bool any = best >> kBits > kBarred >> (kBits + 1);
+        if (lane == k && any) my_id = kMost - 1 - int(best & (kMost - 1));
+        uint32_t down = key[0] - best;  // from 2^31 up for those below it
+#pragma unroll
+        for (int r = 1; r < kPer; ++r) down = max(down, key[r] - best);
+        down = lanes_max<kLanes>(down);
+        equal = equal || (any && int(down) < 0 && (best + down) >> kBits == best >> kBits);
+        best += down;
+      }
+      if constexpr (sizeof(T) == 4) found = !__any(equal);
+    }
+    float total = 0.f;
+    const auto put = [&](int k, float& w) {  // slot k, this lane's
+      w = my_id >= 0 ? exp_of(float(*logits.at(t, my_id)) - top) : 0.f;
+      total += w;
+      ids[t * top_k + k] = my_id;
+      if (parts.sums && my_id >= 0) atomicAdd(&chosen[my_id], 1);
+    };
+    if (!found) {
+      my_id = -1;
+      share.load(logits, t, experts, on, -INFINITY, [&](int r, float v) { key[r] = key_of(v); });
+    }
+    for (int k0 = 0; k0 < top_k; k0 += kLanes) {
+      const int n = min(kLanes, top_k - k0);
+      for (int k = 0; !found && k < n; ++k) {
+        uint32_t best = key[0], mine_at = ~0u;
 #pragma unroll
         for (int r = 1; r < kPer; ++r) best = max(best, key[r]);
         best = lanes_max<kLanes>(best);
-      }
-      // The first of this lane's that are the best one, and of all lanes'.
-      const bool any = best > kBarred;
-      bool found = !any, is[kPer];
-      uint32_t mine_at = ~0u;
+        // The first of this lane's that are the best one, and of all lanes'.
+        bool past = best <= kBarred, is[kPer];
+        if (lane == k) my_id = -1;
 #pragma unroll
-      for (int r = 0; r < kPer; ++r) {
-        is[r] = !found && key[r] == best;
-        found = found || is[r];
-        if (is[r]) mine_at = uint32_t(share.of(r));
-      }
-      const uint32_t at = lanes_min<kLanes>(mine_at);
-      const bool taken = mine_at == at;
-#pragma unroll
-      for (int r = 0; r < kPer; ++r)
-        if (is[r] && taken) key[r] = 0;
-      const float w = any ? exp_of(value_of(best) - top) : 0.f;
-      total += w;
-      if (lane == k % kLanes) {
-        my_id = int(at);
-        my_w = normalize ? w : w * scale;
-      }
-      if (top_k > kLanes && (k % kLanes == kLanes - 1 || k + 1 == top_k)) {
-        const int slot = k - k % kLanes + lane;
-        if (slot <= k && mine) {
-          if (parts.sums && my_id >= 0) atomicAdd(&chosen[my_id], 1);
-          ids_t[slot] = my_id;
-          weights_t[slot] = my_w;
+        for (int r = 0; r < kPer; ++r) {
+          is[r] = !past && key[r] == best;
+          past = past || is[r];
+          if (is[r]) mine_at = uint32_t(share.of(r));
         }
+        const uint32_t at = lanes_min<kLanes>(mine_at);
+        const bool taken = mine_at == at;
+#pragma unroll
+        for (int r = 0; r < kPer; ++r)
+          if (is[r] && taken) key[r] = 0;
+        if (lane == k) my_id = int(at);
+      }
+      float w = 0.f;
+      if (lane < n && mine) put(k0 + lane, w);
+      if (top_k <= kLanes) {
+        const float sum = lanes_sum<kLanes>(total);
+        if (lane < n && mine)
+          weights[t * top_k + lane] =
+              normalize ? (sum > 0.f || sum != sum ? w * __builtin_amdgcn_rcpf(sum) : 0.f) : w * scale;
+      } else if (lane < n && mine) {
+        weights[t * top_k + k0 + lane] = normalize ? w : w * scale;
       }
     }
-    if (top_k <= kLanes) {
-      if (lane < top_k && mine) {
-        if (parts.sums && my_id >= 0) atomicAdd(&chosen[my_id], 1);
-        ids_t[lane] = my_id;
-        weights_t[lane] = normalize && most ? my_w * __builtin_amdgcn_rcpf(total) : my_w;
-      }
-    } else if (normalize && mine) {
-      for (int k = lane; k < top_k; k += kLanes) weights_t[k] = most ? weights_t[k] / total : 0.f;
+    if (top_k > kLanes && normalize) {
+      total = lanes_sum<kLanes>(total);
+      if (mine)
+        for (int k = lane; k < top_k; k += kLanes)
+          weights[t * top_k + k] = total > 0.f || total != total ? weights[t * top_k + k] / total : 0.f;
     }
   }
   if (!parts.sums) return;
