@@ -10,7 +10,10 @@
 // the differences from it that are below zero, two operations an element. What was
 // cut off decides where two keys agree in what is left: FP16 and BF16 lose nothing,
 // FP32 the last 8 bits for 128 experts (11 for 1,024), and a wave that meets two
-// such logits in a row takes the longer way, which finds the expert behind its key.
+// such logits in a row, or a NaN, takes the longer way, which finds the expert
+// behind its key.
+#include <algorithm>
+
 #include "ps_rows.hpp"
 
 namespace ps {
@@ -21,11 +24,11 @@ constexpr int kMostExperts = 1024;
 // Unsigned numbers that order as logits do, NaN above all; -0 and 0 are equal.
 // Barred experts (-inf) and taken ones (0) are at kBarred or below.
 constexpr uint32_t kBarred = 0x007fffffu;
-__device__ __forceinline__ uint32_t key_of(float v) {
+__device__ __forceinline__ uint32_t key_of_number(float v) {
   const int b = __float_as_int(v + 0.f);
-  const uint32_t key = uint32_t(b ^ ((b >> 31) | int(0x80000000u)));
-  return v != v ? ~0u : key;
+  return uint32_t(b ^ ((b >> 31) | int(0x80000000u)));
 }
+__device__ __forceinline__ uint32_t key_of(float v) { return v != v ? ~0u : key_of_number(v); }
 // (~0 comes back as a NaN)
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
@@ -80,6 +83,7 @@ struct RouteParts {
   // their totals: experts sums, experts + 1 counts
   double* all_sums;
   int* all_counts;
+  int* joined;  // workgroups of the join that are done; the first kernel clears it
 };
 
 // The counts and the loss from the totals of every expert, by a wave.
@@ -119,6 +123,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
   int tokens = 0;
   if (parts.sums) {
     for (int e = threadIdx.x; e <= experts; e += kThreads) chosen[e] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *parts.joined = 0;
     __syncthreads();
   }
   float acc[kPer];
@@ -133,24 +138,27 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
     float p[kPer], s = 0.f;
     share.load(logits, t, experts, on, -INFINITY, [&](int r, float v) {
       p[r] = v;
-      const uint32_t whole = key_of(v);
+      const uint32_t whole = key_of_number(v);  // (a NaN shows in the sum below)
       most = max(most, whole);
       key[r] = (whole >> (kBits + 1) << kBits) + uint32_t(kMost - 1 - share.of(r));
     });
     most = lanes_max<kLanes>(most);
     // nothing to choose: no probabilities either
-    const float top = most > kBarred ? value_of(most) : 0.f;
+    float top = most > kBarred ? value_of(most) : 0.f;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
       p[r] = exp_of(p[r] - top);
       s += p[r];
     }
     s = lanes_sum<kLanes>(s);
-    const float scale = most > kBarred ? __builtin_amdgcn_rcpf(s) : 0.f;
+    const bool nan = s != s;
+    if (nan) top = s;
+    const bool takes_part = most > kBarred || nan;
+    const float scale = takes_part ? __builtin_amdgcn_rcpf(s) : 0.f;
     if (parts.sums) {
 #pragma unroll
       for (int r = 0; r < kPer; ++r) acc[r] += p[r] * scale;
-      tokens += lane == 0 && most > kBarred;
+      tokens += lane == 0 && takes_part;
     }
     // Slot k's expert is found by all lanes and kept by lane k % kLanes.
     int my_id = -1;
@@ -171,7 +179,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
         equal = equal || (any && int(down) < 0 && (best + down) >> kBits == best >> kBits);
         best += down;
       }
-      if constexpr (sizeof(T) == 4) found = !__any(equal);
+      found = !__any((sizeof(T) == 4 && equal) || nan);
     }
     float total = 0.f;
     const auto put = [&](int k, float& w) {  // slot k, this lane's
@@ -228,9 +236,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
   if (!parts.sums) return;
   // The tokens of a wave, then the waves in order.
 #pragma unroll
-  for (int r = 0; r < kPer; ++r)
-#pragma unroll
-    for (int d = kLanes; d < kWave; d <<= 1) acc[r] += __shfl_xor(acc[r], d, kWave);
+  for (int r = 0; r < kPer; ++r) acc[r] = groups_sum<kLanes>(acc[r]);
   if (lane_id() < kLanes)
 #pragma unroll
     for (int r = 0; r < kPer; ++r) sums[threadIdx.x / kWave][share.of(r)] = acc[r];
@@ -256,12 +262,15 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
 
 // The workgroups' parts added up: 32 columns a workgroup, the experts' sums first,
 // the counts and the tokens behind them, 32 threads each with up to 16 parts under
-// way at once.
+// way at once. The last workgroup to be done has all totals and finishes.
 constexpr int kJoinCols = 32, kJoinLanes = 32, kJoinAhead = 16;
 __global__ __launch_bounds__(kJoinCols* kJoinLanes) void route_join_kernel(RouteParts parts,
                                                                            int part_count,
-                                                                           int experts) {
+                                                                           int experts,
+                                                                           int* __restrict__ counts,
+                                                                           float* __restrict__ loss) {
   __shared__ double sums[kJoinLanes][kJoinCols];
+  __shared__ bool last;
   const int lane = threadIdx.x / kJoinCols, i = threadIdx.x % kJoinCols;
   const int c = blockIdx.x * kJoinCols + i, all = 2 * experts + 1;
   double s = 0;  // (counts stay exact in it)
@@ -280,17 +289,21 @@ __global__ __launch_bounds__(kJoinCols* kJoinLanes) void route_join_kernel(Route
   }
   sums[lane][i] = s;
   __syncthreads();
-  if (lane || c >= all) return;
+  if (lane == 0 && c < all) {
 #pragma unroll
-  for (int k = 1; k < kJoinLanes; ++k) s += sums[k][i];
-  if (c < experts)
-    parts.all_sums[c] = s;
-  else
-    parts.all_counts[c - experts] = int(s);
-}
-__global__ __launch_bounds__(kWave) void route_finish_kernel(RouteParts parts, int experts,
-                                                             int* __restrict__ counts,
-                                                             float* __restrict__ loss) {
+    for (int k = 1; k < kJoinLanes; ++k) s += sums[k][i];
+    if (c < experts)
+      parts.all_sums[c] = s;
+    else
+      parts.all_counts[c - experts] = int(s);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)  // releases this workgroup's totals, acquires the others'
+    last = __hip_atomic_fetch_add(parts.joined, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+           int(gridDim.x) - 1;
+  __syncthreads();
+  if (!last || threadIdx.x >= kWave) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   finish(experts, [&](int e) { return parts.all_sums[e]; },
          [&](int e) { return parts.all_counts[e]; }, counts, loss);
 }
@@ -449,9 +462,11 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
 
 // ----------------------------------------------------------------- host side
 
-// Workgroups of the forward pass where the loss is wanted: as many large ones as
-// the device holds at once; what they leave is added up.
-constexpr long long kRouteBlocks = 512;
+// Workgroups of the forward pass where the loss is wanted, what they leave is added
+// up: at most kRouteThreads threads in all, half of what the device holds at once
+// (65,536 x 128 top 8: 24.6 us, 25.8 with all of it), and no more workgroups than
+// those of 512 threads.
+constexpr long long kRouteThreads = 1 << 18, kRouteBlocks = kRouteThreads / 512;
 long long route_blocks(long long tokens, int per_block, long long most) {
   const long long n = (tokens + per_block - 1) / per_block;
   return n < most ? n : most;
@@ -505,8 +520,8 @@ extern "C" {
 size_t ps_expert_route_workspace_bytes(long long tokens, int experts) {
   if (tokens < 0 || tokens > (1LL << 30) || experts < 1 || experts > ps::kMostExperts) return 0;
   const size_t blocks = tokens < ps::kRouteBlocks ? size_t(tokens) : size_t(ps::kRouteBlocks);
-  // the totals, then the workgroups' parts
-  return size_t(experts) * 8 + (blocks + 1) * (2 * size_t(experts) + 1) * 4;
+  // the totals and the join's counter, then the workgroups' parts
+  return size_t(experts) * 8 + (size_t(experts) + 2) * 4 + blocks * (2 * size_t(experts) + 1) * 4;
 }
 
 int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsigned char* mask,
@@ -551,11 +566,13 @@ int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsig
       constexpr int kLarge = lanes * per <= 512 ? 1024 : 512;
       const bool large = logits->rows > 256 * (256 / lanes);
       const int threads = large ? kLarge : 256;
-      blocks = ps::route_blocks(logits->rows, threads / lanes, loss ? ps::kRouteBlocks : 1 << 20);
+      blocks = ps::route_blocks(logits->rows, threads / lanes,
+                                loss ? std::min(ps::kRouteThreads / threads, ps::kRouteBlocks) : 1LL << 20);
       if (loss) {
         parts.all_sums = static_cast<double*>(workspace);
         parts.all_counts = reinterpret_cast<int*>(parts.all_sums + experts);
-        parts.counts = parts.all_counts + experts + 1;
+        parts.joined = parts.all_counts + experts + 1;
+        parts.counts = parts.joined + 1;
         parts.sums = reinterpret_cast<float*>(parts.counts + blocks * (experts + 1));
       }
       const auto run = [&](auto kernel) {
@@ -580,9 +597,8 @@ int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsig
   }
   const uint32_t columns = 2 * uint32_t(experts) + 1;
   ps::route_join_kernel<<<(columns + ps::kJoinCols - 1) / ps::kJoinCols,
-                          ps::kJoinCols * ps::kJoinLanes, 0, st>>>(parts, int(blocks), experts);
-  PS_LAUNCHED();
-  ps::route_finish_kernel<<<1, ps::kWave, 0, st>>>(parts, experts, counts, loss);
+                          ps::kJoinCols * ps::kJoinLanes, 0, st>>>(parts, int(blocks), experts,
+                                                                   counts, loss);
   PS_LAUNCHED();
   return PS_OK;
 }

@@ -85,6 +85,24 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return lanes_all<kLanes>(v, [](float a, float b) { return a + b; });
 }
 
+// The sum over the lanes of a wave that are in the same place of their group of
+// kLanes (4 to 64), in every lane.
+template <int kLanes>
+__device__ __forceinline__ float groups_sum(float v) {
+  static_assert(kLanes >= 4 && kLanes <= kWave, "");
+  if constexpr (kLanes <= 4) v += xor_shfl<4>(v);
+  if constexpr (kLanes <= 8) v += xor_shfl<8>(v);
+  if constexpr (kLanes <= 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    v = __int_as_float(r[0]) + __int_as_float(r[1]);
+  }
+  if constexpr (kLanes <= 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    v = __int_as_float(r[0]) + __int_as_float(r[1]);
+  }
+  return v;
+}
+
 // A matrix as the kernels read it.
 template <typename T>
 struct Mat {
