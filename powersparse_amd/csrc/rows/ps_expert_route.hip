@@ -380,27 +380,28 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
        t0 += (long long)gridDim.x * kTokens) {
     const long long t = t0 + threadIdx.x / kLanes;
     const bool mine = t < logits.rows;
-    const int* const ids_t = ids + t * top_k;
     struct Choice {
       int id;
       float logit, dw;
     };
+    // Slot k's; loads that are in range whatever k and the id are need no branches.
+    const long long tt = min(t, logits.rows - 1);
     const auto choice = [&](int k) {
+      const long long at = tt * top_k + min(k, top_k - 1);
+      const int id = ids[at];
+      const bool taken = mine && k < top_k && id >= 0 && id < experts;
       Choice c{-1, 0.f, 0.f};
-      if (!mine || k >= top_k) return c;
-      const int id = ids_t[k];
-      if (id < 0 || id >= experts) return c;
-      c.id = id;
-      c.logit = float(*logits.at(t, id));
-      if (dweights) c.dw = dweights[t * top_k + k];
+      const float logit = float(*logits.at(tt, taken ? id : 0));
+      const float dw = dweights ? dweights[at] : 0.f;
+      if (taken) c = {id, logit, dw};
       return c;
     };
     // All loads are under way before the first is waited for, but the chosen logits'.
-    const int id_0 = mine ? ids_t[0] : -1;
+    const int id_0 = ids[tt * top_k];
     float p[kPer], h[kPer], top = -INFINITY, s = 0.f;
-    share.load(logits, t, experts, mine, -INFINITY, [&](int r, float v) { p[r] = v; });
+    share.load(logits, tt, experts, true, -INFINITY, [&](int r, float v) { p[r] = v; });
     const Choice first = choice(lane);
-    const bool on = id_0 >= 0;
+    const bool on = mine && id_0 >= 0;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) top = fmaxf(top, p[r]);
     top = lanes_all<kLanes>(top, [](float a, float b) { return fmaxf(a, b); });
@@ -472,10 +473,11 @@ long long route_blocks(long long tokens, int per_block, long long most) {
   return n < most ? n : most;
 }
 
-// Calls f(lanes, logits per lane, logits at a time). `many`: half as many lanes for
-// 65 to 512 experts: less work in all, as a lane's part of finding the next expert
-// hardly grows, and longer for a token alone (65,536 x 128 top 8 18 -> 16 us, 16,384
-// x 512 20 -> 16; but 512 x 64 4.3 -> 5.9, and the gradient 19.3 -> 20.2).
+// Calls f(lanes, logits per lane, logits at a time). `many`: half as many lanes,
+// which is less work in all, as a lane's part of finding the next expert hardly
+// grows, and longer for a token alone (65,536 x 128 top 8 18 -> 16 us, 16,384 x 512
+// 20 -> 16, 300,007 x 17 FP16 20 -> 14; 512 x 64 4.3 -> 5.9; the gradient, which
+// finds none, 19.3 -> 20.2 and 16.6 -> 22.5). Not for 64 experts: 9.2 -> 10.1.
 template <typename F>
 int with_lanes(int experts, bool many, F&& f) {
   const auto call = [&](auto lanes, auto per) {
@@ -484,16 +486,18 @@ int with_lanes(int experts, bool many, F&& f) {
     return f(lanes, per, std::integral_constant<int, 1>{});
   };
   using std::integral_constant;
-  if (experts <= 8) return call(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-  if (experts <= 16) return call(integral_constant<int, 8>{}, integral_constant<int, 2>{});
-  if (experts <= 32) return call(integral_constant<int, 8>{}, integral_constant<int, 4>{});
-  if (experts <= 64) return call(integral_constant<int, 8>{}, integral_constant<int, 8>{});
-  if (many && experts <= 512) {
+  if (many && experts > 8 && experts <= 512 && (experts <= 32 || experts > 64)) {
+    if (experts <= 16) return call(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    if (experts <= 32) return call(integral_constant<int, 4>{}, integral_constant<int, 8>{});
     const auto per = integral_constant<int, 16>{};
     if (experts <= 128) return call(integral_constant<int, 8>{}, per);
     if (experts <= 256) return call(integral_constant<int, 16>{}, per);
     return call(integral_constant<int, 32>{}, per);
   }
+  if (experts <= 8) return call(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+  if (experts <= 16) return call(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+  if (experts <= 32) return call(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+  if (experts <= 64) return call(integral_constant<int, 8>{}, integral_constant<int, 8>{});
   if (experts <= 128) return call(integral_constant<int, 16>{}, integral_constant<int, 8>{});
   if (experts <= 256) return call(integral_constant<int, 32>{}, integral_constant<int, 8>{});
   if (experts <= 512) return call(integral_constant<int, 64>{}, integral_constant<int, 8>{});

@@ -95,7 +95,7 @@ __device__ __forceinline__ void row_sums(float (&v)[kSums], RowParts<kLanes>& pa
 constexpr int threads_of(int lanes) { return lanes > kRowThreads ? lanes : kRowThreads; }
 
 template <typename T, typename O, int N, int kLanes, int kPieces>
-__global__ __launch_bounds__(threads_of(kLanes)) void norm_kernel(Mat<const T> x, Vec weight,
+__global__ __launch_bounds__(threads_of(kLanes)) void layer_norm_kernel(Mat<const T> x, Vec weight,
                                                                   Vec bias, float eps, Mat<O> y,
                                                                   float* __restrict__ mean_out,
                                                                   float* __restrict__ rstd_out,
@@ -162,9 +162,9 @@ __global__ __launch_bounds__(threads_of(kLanes)) void norm_kernel(Mat<const T> x
   }
 }
 
-// parts: see grad_columns_kernel; null: not wanted.
+// parts: see layer_norm_columns_kernel; null: not wanted.
 template <typename T, typename O, int N, int kLanes, int kPieces>
-__global__ __launch_bounds__(threads_of(kLanes)) void grad_kernel(
+__global__ __launch_bounds__(threads_of(kLanes)) void layer_norm_grad_kernel(
     Mat<const O> dy, Mat<const T> x, Vec weight, const float* __restrict__ mean_in,
     const float* __restrict__ rstd_in, Mat<T> dx, float* __restrict__ parts, Pieces p) {
   constexpr int kThreads = threads_of(kLanes), kRows = kThreads / kLanes;
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(threads_of(kLanes)) void grad_kernel(
 
 // Rows of any width: a workgroup a row, which is read three times.
 template <typename T, typename O, int N>
-__global__ __launch_bounds__(kWideThreads) void norm_wide_kernel(Mat<const T> x, Vec weight,
+__global__ __launch_bounds__(kWideThreads) void layer_norm_wide_kernel(Mat<const T> x, Vec weight,
                                                                  Vec bias, float eps, Mat<O> y,
                                                                  float* __restrict__ mean_out,
                                                                  float* __restrict__ rstd_out,
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_wide_kernel(Mat<const T> x,
 
 // dx of rows of any width: a workgroup a row, which is read twice.
 template <typename T, typename O, int N>
-__global__ __launch_bounds__(kWideThreads) void grad_wide_kernel(Mat<const O> dy, Mat<const T> x,
+__global__ __launch_bounds__(kWideThreads) void layer_norm_grad_wide_kernel(Mat<const O> dy, Mat<const T> x,
                                                                  Vec weight,
                                                                  const float* __restrict__ mean_in,
                                                                  const float* __restrict__ rstd_in,
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(kWideThreads) void grad_wide_kernel(Mat<const O> dy
 // Parts of the sums over the rows: one piece of every row of a range a thread.
 // parts holds for each range dweight's sums and then dbias's.
 template <typename T, typename O, int N>
-__global__ __launch_bounds__(kRowThreads) void grad_columns_kernel(
+__global__ __launch_bounds__(kRowThreads) void layer_norm_columns_kernel(
     Mat<const O> dy, Mat<const T> x, const float* __restrict__ mean_in,
     const float* __restrict__ rstd_in, float* __restrict__ parts, Pieces p) {
   const int q = blockIdx.x * kRowThreads + threadIdx.x;
@@ -373,7 +373,7 @@ struct VecOut {
 // dweight first, then dbias's.
 constexpr int kJoinCols = 32, kJoinLanes = 32, kJoinAhead = 8;
 constexpr int kJoinThreads = kJoinCols * kJoinLanes;
-__global__ __launch_bounds__(kJoinThreads) void grad_join_kernel(const float* __restrict__ parts,
+__global__ __launch_bounds__(kJoinThreads) void layer_norm_join_kernel(const float* __restrict__ parts,
                                                                  int part_count, int cols,
                                                                  VecOut dweight, VecOut dbias,
                                                                  bool add) {
@@ -520,10 +520,10 @@ int ps_layer_norm(const ps_rows* x, const ps_rows* weight, const ps_rows* bias, 
                 mean, rstd, p);
           };
           if constexpr (lanes == 0) {
-            run(ps::norm_wide_kernel<T, O, n>, ps::wide_blocks(x->rows), ps::kWideThreads);
+            run(ps::layer_norm_wide_kernel<T, O, n>, ps::wide_blocks(x->rows), ps::kWideThreads);
           } else {
             constexpr int kThreads = ps::threads_of(lanes);
-            run(ps::norm_kernel<T, O, n, lanes, per>, ps::norm_blocks(x->rows, kThreads / lanes),
+            run(ps::layer_norm_kernel<T, O, n, lanes, per>, ps::norm_blocks(x->rows, kThreads / lanes),
                 kThreads);
           }
           PS_LAUNCHED();
@@ -587,19 +587,19 @@ int ps_layer_norm_grad(const ps_rows* dy, const ps_rows* x, const ps_rows* weigh
           const ps::Pieces p(x->cols, n);
           return ps::with_lanes<n, n == 8 ? 2048 : 4096>(p, p.per_row.d > 128, [&](auto lanes, auto per) {
             if constexpr (lanes == 0) {
-              ps::grad_wide_kernel<T, O, n>
+              ps::layer_norm_grad_wide_kernel<T, O, n>
                   <<<ps::wide_blocks(x->rows), ps::kWideThreads, 0, st>>>(
                       ps::mat<const O>(dy), ps::mat<const T>(x), ps::vec(weight, 1.f), mean, rstd,
                       ps::mat<T>(dx), p);
               PS_LAUNCHED();
               if (!sums) return int(PS_OK);
               const dim3 grid((p.per_row.d + ps::kRowThreads - 1) / ps::kRowThreads, part_count);
-              ps::grad_columns_kernel<T, O, n><<<grid, ps::kRowThreads, 0, st>>>(
+              ps::layer_norm_columns_kernel<T, O, n><<<grid, ps::kRowThreads, 0, st>>>(
                   ps::mat<const O>(dy), ps::mat<const T>(x), mean, rstd, parts, p);
             } else {
               constexpr int kThreads = ps::threads_of(lanes), kRows = kThreads / lanes;
               part_count = ps::fewer_parts(part_count, (x->rows + kRows - 1) / kRows);
-              ps::grad_kernel<T, O, n, lanes, per><<<part_count, kThreads, 0, st>>>(
+              ps::layer_norm_grad_kernel<T, O, n, lanes, per><<<part_count, kThreads, 0, st>>>(
                   ps::mat<const O>(dy), ps::mat<const T>(x), ps::vec(weight, 1.f), mean, rstd,
                   ps::mat<T>(dx), sums ? parts : nullptr, p);
             }
@@ -613,7 +613,7 @@ int ps_layer_norm_grad(const ps_rows* dy, const ps_rows* x, const ps_rows* weigh
   }
   if (sums) {
     const uint32_t blocks = uint32_t((2 * x->cols + ps::kJoinCols - 1) / ps::kJoinCols);
-    ps::grad_join_kernel<<<blocks, ps::kJoinThreads, 0, st>>>(
+    ps::layer_norm_join_kernel<<<blocks, ps::kJoinThreads, 0, st>>>(
         parts, int(part_count), int(x->cols), ps::vec_out(dweight), ps::vec_out(dbias),
         accumulate != 0);
     PS_LAUNCHED();

@@ -26,12 +26,13 @@
       active lanes per VALU instruction of the sparse launch; means over the
       operator's calls.
 
-  python -m powersparse_amd.perf rows [--passes 8]
+  python -m powersparse_amd.perf rows [--passes 8] [--cases more_operators]
   python -m powersparse_amd.perf rows-summarize --trace KT.db --fetch F.db --write W.db
       The same for the row operators: every listed workload of
-      perf/operators.py between two calibration copies, and per workload and
-      kernel the launches of a pass, their median time and traffic. The trace
-      and each counter come from a run of their own, all of as many passes.
+      perf/operators.py (or of perf/more_operators.py) between two calibration
+      copies, and per workload and kernel the launches of a pass, their median
+      time and traffic. The trace and each counter come from a run of their own,
+      all of as many passes.
 """
 import argparse
 import collections
@@ -545,21 +546,27 @@ def summarize(args):
 
 # The row operators' kernels, as plain or mangled names hold them.
 ROW_KERNEL = re.compile(r"(?:^|\W|\d)(id_sort_tile|id_count|id_place|id_clear|lookup|grad_runs|"
-                        r"grad_join|dispatch|combine_grad|combine|norm_join|norm|clip)_kernel")
+                        r"grad_join|dispatch|combine_grad|combine|norm_join|norm|clip|"
+                        r"layer_norm(?:_wide|_grad|_grad_wide|_columns|_join)?|"
+                        r"route(?:_grad|_join|_join_few|_nothing)?|adamw)_kernel")
 
 
-def row_cases():
-    """perf/operators.py as a module that makes the framework's calls."""
+def row_cases(name="operators"):
+    """perf/operators.py, or another file there, as a module that makes the framework's calls."""
     import importlib.util
     import os
 
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "perf",
-                        "operators.py")
+                        name + ".py")
     spec = importlib.util.spec_from_file_location("row_operators", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
     module.own = True
     return module
+
+
+def chosen_cases(args):
+    return row_cases() if args.cases == "operators" else row_cases(args.cases)
 
 
 def rows_workload(args):
@@ -576,7 +583,7 @@ def rows_workload(args):
         copy_f32(dst, src, CALIB_BYTES // 4)
         ps.synchronize()
 
-    module = row_cases()
+    module = chosen_cases(args)
     for case in module.listed():
         states = [module.prepare(case, k) for k in range(2)]  # inputs change from pass to pass
         for state in states:
@@ -608,7 +615,7 @@ def rows_summarize(args):
     def median(values):
         return sorted(values)[len(values) // 2]
 
-    names = [case["name"] for case in row_cases().listed()]
+    names = [case["name"] for case in chosen_cases(args).listed()]
     fetch, write = read_counters(args.fetch, "FETCH_SIZE"), read_counters(args.write, "WRITE_SIZE")
     kf, kw = calibration(fetch), calibration(write)
     parts = [row_passes(d) for d in (read_dispatches(args.trace), fetch, write)]
@@ -653,6 +660,8 @@ def main(argv=None):
     rs.add_argument("--fetch", required=True)
     rs.add_argument("--write", required=True)
     rs.add_argument("--passes", type=int, default=8)
+    for parser in (r, rs):
+        parser.add_argument("--cases", default="operators", choices=("operators", "more_operators"))
     s = sub.add_parser("summarize")
     s.add_argument("--trace", required=True)
     s.add_argument("--fetch")
