@@ -105,8 +105,10 @@ def route(logits, top_k, normalize, mask=None):
         far[t] = top - min(row[e] for e in open_to)
         counts[best] += 1
         counts[E] += 1
-    # exponential: its argument's rounding, its own; the sum over the experts; two divisions
-    rel = (2 * far + E + 12) * U32
+    # exponential by powers of two: the difference of logits is rounded, and its product with
+    # log2(e), whose FP32 value is 0.22 U32 off: 2.22 times the difference; its own error; the sum
+    # over the experts; two divisions
+    rel = (2.25 * far + E + 12) * U32
     off = weights * rel[:, None] + 2.0 ** -126
     chosen, tokens = counts[:E].double(), int(counts[E])
     loss, loss_off = 0.0, 0.0
@@ -134,7 +136,7 @@ def route_grad(logits, ids, dweights, counts, dloss, normalize):
             continue
         p = torch.softmax(l[t], 0)
         open_to = l[t][l[t] > -math.inf]
-        rel = float(2 * (open_to.max() - open_to.min()) + 2 * E + 24) * U32
+        rel = float(2.25 * (open_to.max() - open_to.min()) + 2 * E + 24) * U32
         chosen = ids[t][ids[t] >= 0]
         d = dw[t][ids[t] >= 0]
         h = by_loss.clone()
