@@ -417,16 +417,18 @@ int ps_adamw_list_create(int tensors, const ps_adamw_tensor* list, int state_dty
     long long total = 0, chunks = 0;
     for (int i = 0; i < tensors; ++i) {
       const ps_adamw_tensor& t = list[i];
-      const std::string name = "ps_adamw_list_create: tensor " + std::to_string(i);
+      const auto bad = [i](const char* what) {
+        return "ps_adamw_list_create: tensor " + std::to_string(i) + ": " + what;
+      };
       PS_CHECK_ARG(ps::dtype_valid(t.param_dtype) && ps::dtype_valid(t.grad_dtype) &&
                        (!t.copy || ps::dtype_valid(t.copy_dtype)),
-                   name + ": unknown element type");
+                   bad("unknown element type"));
       PS_CHECK_ARG(t.count >= 0 && t.count <= (1LL << 44) && total <= (1LL << 44),
-                   name + ": bad count");
-      PS_CHECK_ARG(std::isfinite(t.weight_decay), name + ": weight decay is not a number");
+                   bad("bad count"));
+      PS_CHECK_ARG(std::isfinite(t.weight_decay), bad("weight decay is not a number"));
       if (!t.count) continue;
       PS_CHECK_ARG(t.param && t.grad && t.exp_avg && t.exp_avg_sq && (!in_8_bits || t.scales),
-                   name + ": null data");
+                   bad("null data"));
       const size_t state = in_8_bits ? 1 : 4, n = size_t(t.count);
       const size_t blocks = (n + ps::kStateBlock - 1) / ps::kStateBlock;
       const auto misaligned = [](const void* p, size_t size) {
@@ -437,7 +439,7 @@ int ps_adamw_list_create(int tensors, const ps_adamw_tensor* list, int state_dty
                        !misaligned(t.exp_avg, state) && !misaligned(t.exp_avg_sq, state) &&
                        !(in_8_bits && misaligned(t.scales, 4)) &&
                        !(t.copy && misaligned(t.copy, ps::dtype_size(t.copy_dtype))),
-                   name + ": misaligned data");
+                   bad("misaligned data"));
       written.add(t.param, n * ps::dtype_size(t.param_dtype));
       written.add(t.exp_avg, n * state);
       written.add(t.exp_avg_sq, n * state);

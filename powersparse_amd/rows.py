@@ -12,6 +12,7 @@ synchronising: arrays and workspaces must stay alive, and be written by nothing 
 the stream has passed the call. Wrong arguments raise ValueError.
 """
 import ctypes
+import struct
 
 from . import _native
 from ._native import AdamWOptions, AdamWTensor, Ids, Rows
@@ -588,6 +589,23 @@ def state_blocks(elements):
     return -(-int(elements) // STATE_BLOCK)
 
 
+# An AdamWTensor's fields.
+_TENSOR = struct.Struct("@6Pq3if")
+
+
+def _some(x, what, i, dtypes, count):
+    """_flat of array i of a list, which is named only where it is refused."""
+    try:
+        if x.is_cuda and x.is_contiguous():
+            said, n = _names[x.dtype], x.numel()
+            if said in dtypes and (count is None or n == count):
+                return x.data_ptr(), n, said
+    except (AttributeError, KeyError, TypeError):
+        pass
+    ptr, n, said = _flat(x, f"{what} {i}", dtypes, count)
+    return ptr or 0, n, said
+
+
 class AdamWList:
     """The tensors that AdamWStep updates, all contiguous: `params` (float32, float16 or
     bfloat16), their `grads` of the same sizes (only read, any of these types), and the moments
@@ -615,22 +633,21 @@ class AdamWList:
         if _several is not False:
             _check_devices(*(x for xs in self._keep for x in xs))
         state = ("uint8", "float8_e4m3fn") if scales else ("float32",)
-        table = (AdamWTensor * max(n, 1))()
-        for i in range(n):
-            t = table[i]
-            t.param, t.count, said = _flat(params[i], f"parameter {i}", _DTYPES)
-            t.param_dtype = _DTYPES[said]
-            t.grad, _, said = _flat(grads[i], f"gradient {i}", _DTYPES, t.count)
-            t.grad_dtype = _DTYPES[said]
-            t.exp_avg = _flat(exp_avgs[i], f"exp_avg {i}", state, t.count)[0]
-            t.exp_avg_sq = _flat(exp_avg_sqs[i], f"exp_avg_sq {i}", state, t.count)[0]
+        table = ctypes.create_string_buffer(max(n, 1) * _TENSOR.size)
+        for i in range(n):  # some hundred at a time: the six arrays of each in one step
+            p, count, p_type = _some(params[i], "parameter", i, _DTYPES, None)
+            g, _, g_type = _some(grads[i], "gradient", i, _DTYPES, count)
+            m = _some(exp_avgs[i], "exp_avg", i, state, count)[0]
+            v = _some(exp_avg_sqs[i], "exp_avg_sq", i, state, count)[0]
+            s = c = c_type = 0
             if scales:
-                t.scales = _flat(scales[i], f"scales {i}", ("float32",),
-                                 2 * state_blocks(t.count))[0]
+                s = _some(scales[i], "scales", i, ("float32",), 2 * state_blocks(count))[0]
             if copies and copies[i] is not None:
-                t.copy, _, said = _flat(copies[i], f"copy {i}", _DTYPES, t.count)
-                t.copy_dtype = _DTYPES[said]
-            t.weight_decay = decay[i]
+                c, _, c_type = _some(copies[i], "copy", i, _DTYPES, count)
+                c_type = _DTYPES[c_type]
+            _TENSOR.pack_into(table, i * _TENSOR.size, p, g, m, v, s, c, count, _DTYPES[p_type],
+                              _DTYPES[g_type], c_type, decay[i])
+        table = ctypes.cast(table, ctypes.POINTER(AdamWTensor))
         h = ctypes.c_void_p()
         _call(_hip.ps_adamw_list_create(n, table, _E4M3 if scales else 0, ctypes.byref(h)))
         self._h = h.value
