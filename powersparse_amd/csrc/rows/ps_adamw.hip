@@ -370,6 +370,9 @@ __device__ __forceinline__ void chunk_of(const AdamTensor& t, const AdamStep& s,
     chunk_of<k8, P, bf16>(t, s, from, count);
 }
 
+// Bound by memory: 400 M FP32 parameters, BF16 gradients and copies, FP32 moments:
+// 11.2 GB in 2,138 us, 5.2 TB/s; moments in 8 bits 6.4 GB in 1,192 us, 5.4 TB/s, with
+// as much time's worth of instructions, some 100 an element, under it.
 template <bool k8>
 __global__ __launch_bounds__(kListThreads) void adamw_kernel(Adam a, AdamCall call) {
   AdamStep s;
