@@ -483,16 +483,18 @@ long long route_blocks(long long tokens, int per_block, long long most) {
 // which is less work in all, as a lane's part of finding the next expert hardly
 // grows, and longer for a token alone (65,536 x 128 top 8 18 -> 16 us, 16,384 x 512
 // 20 -> 16, 300,007 x 17 FP16 20 -> 14; 512 x 64 4.3 -> 5.9; the gradient, which
-// finds none, 19.3 -> 20.2 and 16.6 -> 22.5). Not for 64 experts: 9.2 -> 10.1.
+// finds none, 19.3 -> 20.2 and 16.6 -> 22.5). Not for 64 experts, 9.2 -> 10.1, nor
+// for more slots than lanes, which the shorter way does not take.
 template <typename F>
-int with_lanes(int experts, bool many, F&& f) {
+int with_lanes(int experts, int top_k, bool many, F&& f) {
   const auto call = [&](auto lanes, auto per) {
     constexpr int kWide = per < 4 ? per : 4;
     if (experts % kWide == 0) return f(lanes, per, std::integral_constant<int, kWide>{});
     return f(lanes, per, std::integral_constant<int, 1>{});
   };
   using std::integral_constant;
-  if (many && experts > 8 && experts <= 512 && (experts <= 32 || experts > 64)) {
+  const int half = experts <= 32 ? 4 : experts <= 128 ? 8 : experts <= 256 ? 16 : 32;
+  if (many && top_k <= half && experts > 8 && experts <= 512 && (experts <= 32 || experts > 64)) {
     if (experts <= 16) return call(integral_constant<int, 4>{}, integral_constant<int, 4>{});
     if (experts <= 32) return call(integral_constant<int, 4>{}, integral_constant<int, 8>{});
     const auto per = integral_constant<int, 16>{};
@@ -569,7 +571,7 @@ int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsig
   ps::RouteParts parts{};
   long long blocks = 0;
   const int rc = ps::with_dtype(logits->dtype, [&](auto t) {
-    return ps::with_lanes(experts, logits->rows >= 8192, [&](auto lanes, auto per, auto wide) {
+    return ps::with_lanes(experts, top_k, logits->rows >= 8192, [&](auto lanes, auto per, auto wide) {
       using T = decltype(t);
       // Large workgroups where there is work for them, so that the parts are few, and
       // shared memory for a sum of each expert and wave.
@@ -636,7 +638,7 @@ int ps_expert_route_grad(const ps_rows* logits, int top_k, int normalize, const 
                "ps_expert_route_grad: dlogits overlaps an input");
   if (!logits->rows) return PS_OK;
   return ps::with_dtype(logits->dtype, [&](auto t) {
-    return ps::with_lanes(experts, false, [&](auto lanes, auto per, auto wide) {
+    return ps::with_lanes(experts, top_k, false, [&](auto lanes, auto per, auto wide) {
       using T = decltype(t);
       const long long blocks = ps::route_blocks(logits->rows, ps::kRouteGradThreads / lanes, 4096);
       ps::route_grad_kernel<T, lanes, per, wide>
