@@ -576,10 +576,14 @@ int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsig
       // Large workgroups where there is work for them, so that the parts are few, and
       // shared memory for a sum of each expert and wave.
       constexpr int kLarge = lanes * per <= 512 ? 1024 : 512;
-      const bool large = logits->rows > 256 * (256 / lanes);
+      // One alone for what it takes in a turn: nothing is left to join (128 x 64 7.1 ->
+      // 5.7 us; with two turns 8.0 -> 8.6).
+      const bool alone = loss && logits->rows > 256 / lanes && logits->rows <= kLarge / lanes;
+      const bool large = alone || logits->rows > 256 * (256 / lanes);
       const int threads = large ? kLarge : 256;
-      blocks = ps::route_blocks(logits->rows, threads / lanes,
-                                loss ? std::min(ps::kRouteThreads / threads, ps::kRouteBlocks) : 1LL << 20);
+      const long long most =
+          loss ? std::min(ps::kRouteThreads / threads, ps::kRouteBlocks) : 1LL << 20;
+      blocks = ps::route_blocks(logits->rows, threads / lanes, most);
       if (loss) {
         parts.all_sums = static_cast<double*>(workspace);
         parts.all_counts = reinterpret_cast<int*>(parts.all_sums + experts);
