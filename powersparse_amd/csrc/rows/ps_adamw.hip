@@ -496,16 +496,18 @@ int ps_adamw_step(ps_adamw_list* list, const ps_adamw_options* o, ps_stream_t st
     PS_CHECK_ARG(!p || !list->written.meets(p, 4),
                  "ps_adamw_step: the rate, step or norm lies in what the step writes");
   if (!list->adam.chunk_count) return PS_OK;
+  const double log_beta1 = std::log(o->beta1), log_beta2 = std::log(o->beta2);
+  const double step = o->device_step ? 1.0 : double(o->step);
   const ps::AdamCall call{float(o->beta1),
                           float(1.0 - o->beta1),
                           float(o->beta2),
                           float(1.0 - o->beta2),
                           float(o->eps),
                           float(o->lr),
-                          std::log(o->beta1),
-                          std::log(o->beta2),
-                          o->device_step ? 1.f : ps::mean_factor(double(o->step), std::log(o->beta1)),
-                          o->device_step ? 1.f : ps::root_factor(double(o->step), std::log(o->beta2)),
+                          log_beta1,
+                          log_beta2,
+                          ps::mean_factor(step, log_beta1),
+                          ps::root_factor(step, log_beta2),
                           uint32_t(o->step),
                           o->device_lr,
                           o->device_step,

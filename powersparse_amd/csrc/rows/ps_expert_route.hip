@@ -222,18 +222,17 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
       if (lane < n && mine) put(k0 + lane, w);
       if (top_k <= kLanes) {
         const float sum = lanes_sum<kLanes>(total);
-        if (lane < n && mine)
-          weights[t * top_k + lane] =
-              normalize ? (sum > 0.f || sum != sum ? w * __builtin_amdgcn_rcpf(sum) : 0.f) : w * scale;
+        const float by = normalize ? (sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum)) : scale;
+        if (lane < n && mine) weights[t * top_k + lane] = w * by;
       } else if (lane < n && mine) {
         weights[t * top_k + k0 + lane] = normalize ? w : w * scale;
       }
     }
     if (top_k > kLanes && normalize) {
       total = lanes_sum<kLanes>(total);
+      const float by = total == 0.f ? 0.f : __builtin_amdgcn_rcpf(total);
       if (mine)
-        for (int k = lane; k < top_k; k += kLanes)
-          weights[t * top_k + k] = total > 0.f || total != total ? weights[t * top_k + k] / total : 0.f;
+        for (int k = lane; k < top_k; k += kLanes) weights[t * top_k + k] *= by;
     }
   }
   if (!parts.sums) return;
@@ -267,11 +266,9 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
 // the counts and the tokens behind them, 32 threads each with up to 16 parts under
 // way at once. The last workgroup to be done has all totals and finishes.
 constexpr int kJoinCols = 32, kJoinLanes = 32, kJoinAhead = 16;
-__global__ __launch_bounds__(kJoinCols* kJoinLanes) void route_join_kernel(RouteParts parts,
-                                                                           int part_count,
-                                                                           int experts,
-                                                                           int* __restrict__ counts,
-                                                                           float* __restrict__ loss) {
+__global__ __launch_bounds__(kJoinCols* kJoinLanes) void route_join_kernel(
+    RouteParts parts, int part_count, int experts, int* __restrict__ counts,
+    float* __restrict__ loss) {
   __shared__ double sums[kJoinLanes][kJoinCols];
   __shared__ bool last;
   const int lane = threadIdx.x / kJoinCols, i = threadIdx.x % kJoinCols;
@@ -288,7 +285,8 @@ __global__ __launch_bounds__(kJoinCols* kJoinLanes) void route_join_kernel(Route
                            : uint32_t(parts.counts[k * (experts + 1) + c - experts]);
     }
 #pragma unroll
-    for (int j = 0; j < kJoinAhead; ++j) s += c < experts ? double(__uint_as_float(v[j])) : double(v[j]);
+    for (int j = 0; j < kJoinAhead; ++j)
+      s += c < experts ? double(__uint_as_float(v[j])) : double(v[j]);
   }
   sums[lane][i] = s;
   __syncthreads();
@@ -479,13 +477,14 @@ long long route_blocks(long long tokens, int per_block, long long most) {
   return n < most ? n : most;
 }
 
-// Calls f(lanes, logits per lane, logits at a time). `many`: half as many lanes,
-// which is less work in all, as a lane's part of finding the next expert hardly
-// grows, and longer for a token alone (65,536 x 128 top 8 18 -> 16 us, 16,384 x 512
-// 20 -> 16, 300,007 x 17 FP16 20 -> 14; 512 x 64 4.3 -> 5.9; the gradient, which
-// finds none, 19.3 -> 20.2 and 16.6 -> 22.5). Not for 64 experts, 9.2 -> 10.1, nor
-// for more slots than lanes, which the shorter way does not take.
-template <typename F>
+// Calls f(lanes, logits per lane, logits at a time). `many` (kFind: where experts
+// are found): half as many lanes, which is less work in all, as a lane's part of
+// finding the next expert hardly grows, and longer for a token alone (65,536 x 128
+// top 8 18 -> 16 us, 16,384 x 512 20 -> 16, 300,007 x 17 FP16 20 -> 14; 512 x 64 4.3 ->
+// 5.9; the gradient, which finds none, 19.3 -> 20.2 and 16.6 -> 22.5). Not for 64
+// experts, 9.2 -> 10.1, nor for more slots than lanes, which the shorter way does
+// not take.
+template <bool kFind, typename F>
 int with_lanes(int experts, int top_k, bool many, F&& f) {
   const auto call = [&](auto lanes, auto per) {
     constexpr int kWide = per < 4 ? per : 4;
@@ -493,14 +492,16 @@ int with_lanes(int experts, int top_k, bool many, F&& f) {
     return f(lanes, per, std::integral_constant<int, 1>{});
   };
   using std::integral_constant;
-  const int half = experts <= 32 ? 4 : experts <= 128 ? 8 : experts <= 256 ? 16 : 32;
-  if (many && top_k <= half && experts > 8 && experts <= 512 && (experts <= 32 || experts > 64)) {
-    if (experts <= 16) return call(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-    if (experts <= 32) return call(integral_constant<int, 4>{}, integral_constant<int, 8>{});
-    const auto per = integral_constant<int, 16>{};
-    if (experts <= 128) return call(integral_constant<int, 8>{}, per);
-    if (experts <= 256) return call(integral_constant<int, 16>{}, per);
-    return call(integral_constant<int, 32>{}, per);
+  if constexpr (kFind) {
+    const int half = experts <= 32 ? 4 : experts <= 128 ? 8 : experts <= 256 ? 16 : 32;
+    if (many && top_k <= half && experts > 8 && experts <= 512 && (experts <= 32 || experts > 64)) {
+      if (experts <= 16) return call(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+      if (experts <= 32) return call(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+      const auto per = integral_constant<int, 16>{};
+      if (experts <= 128) return call(integral_constant<int, 8>{}, per);
+      if (experts <= 256) return call(integral_constant<int, 16>{}, per);
+      return call(integral_constant<int, 32>{}, per);
+    }
   }
   if (experts <= 8) return call(integral_constant<int, 4>{}, integral_constant<int, 2>{});
   if (experts <= 16) return call(integral_constant<int, 8>{}, integral_constant<int, 2>{});
@@ -571,7 +572,8 @@ int ps_expert_route(const ps_rows* logits, int top_k, int normalize, const unsig
   ps::RouteParts parts{};
   long long blocks = 0;
   const int rc = ps::with_dtype(logits->dtype, [&](auto t) {
-    return ps::with_lanes(experts, top_k, logits->rows >= 8192, [&](auto lanes, auto per, auto wide) {
+    const bool many = logits->rows >= 8192;
+    return ps::with_lanes<true>(experts, top_k, many, [&](auto lanes, auto per, auto wide) {
       using T = decltype(t);
       // Large workgroups where there is work for them, so that the parts are few, and
       // shared memory for a sum of each expert and wave.
@@ -642,7 +644,7 @@ int ps_expert_route_grad(const ps_rows* logits, int top_k, int normalize, const 
                "ps_expert_route_grad: dlogits overlaps an input");
   if (!logits->rows) return PS_OK;
   return ps::with_dtype(logits->dtype, [&](auto t) {
-    return ps::with_lanes(experts, top_k, false, [&](auto lanes, auto per, auto wide) {
+    return ps::with_lanes<false>(experts, top_k, false, [&](auto lanes, auto per, auto wide) {
       using T = decltype(t);
       const long long blocks = ps::route_blocks(logits->rows, ps::kRouteGradThreads / lanes, 4096);
       ps::route_grad_kernel<T, lanes, per, wide>

@@ -98,11 +98,9 @@ constexpr int threads_of(int lanes) { return lanes > kRowThreads ? lanes : kRowT
 // 1,000,000 x 128 FP32: 1.03 GB in 183 us, 5.6 TB/s; 32,768 x 4,096 BF16: 0.54 GB in
 // 102 us, 5.3 TB/s. Non-temporal stores gave 1.5%.
 template <typename T, typename O, int N, int kLanes, int kPieces>
-__global__ __launch_bounds__(threads_of(kLanes)) void layer_norm_kernel(Mat<const T> x, Vec weight,
-                                                                  Vec bias, float eps, Mat<O> y,
-                                                                  float* __restrict__ mean_out,
-                                                                  float* __restrict__ rstd_out,
-                                                                  Pieces p) {
+__global__ __launch_bounds__(threads_of(kLanes)) void layer_norm_kernel(
+    Mat<const T> x, Vec weight, Vec bias, float eps, Mat<O> y, float* __restrict__ mean_out,
+    float* __restrict__ rstd_out, Pieces p) {
   constexpr int kRows = threads_of(kLanes) / kLanes;
   __shared__ RowParts<kLanes> part;
   const int lane = threadIdx.x % kLanes, pieces = int(p.per_row.d);
@@ -120,7 +118,8 @@ __global__ __launch_bounds__(threads_of(kLanes)) void layer_norm_kernel(Mat<cons
     b[i] = bias.at<N>(p.begin(q));
   }
   // threads without a row go along: the sums take every lane
-  for (long long r0 = (long long)blockIdx.x * kRows; r0 < x.rows; r0 += (long long)gridDim.x * kRows) {
+  for (long long r0 = (long long)blockIdx.x * kRows; r0 < x.rows;
+       r0 += (long long)gridDim.x * kRows) {
     const long long mine = r0 + threadIdx.x / kLanes, r = min(mine, x.rows - 1);
     V v[kPieces];
     float s[1] = {0.f};
@@ -186,7 +185,8 @@ __global__ __launch_bounds__(threads_of(kLanes)) void layer_norm_grad_kernel(
     if (q < pieces) w[i] = weight.at<N>(p.begin(q));
   }
   int turn = 0;
-  for (long long r0 = (long long)blockIdx.x * kRows; r0 < x.rows; r0 += (long long)gridDim.x * kRows) {
+  for (long long r0 = (long long)blockIdx.x * kRows; r0 < x.rows;
+       r0 += (long long)gridDim.x * kRows) {
     const long long mine = r0 + threadIdx.x / kLanes, r = min(mine, x.rows - 1);
     const float mean = mean_in[r], rstd = rstd_in[r];
     V v[kPieces];
@@ -271,11 +271,9 @@ __global__ __launch_bounds__(threads_of(kLanes)) void layer_norm_grad_kernel(
 
 // Rows of any width: a workgroup a row, which is read three times.
 template <typename T, typename O, int N>
-__global__ __launch_bounds__(kWideThreads) void layer_norm_wide_kernel(Mat<const T> x, Vec weight,
-                                                                 Vec bias, float eps, Mat<O> y,
-                                                                 float* __restrict__ mean_out,
-                                                                 float* __restrict__ rstd_out,
-                                                                 Pieces p) {
+__global__ __launch_bounds__(kWideThreads) void layer_norm_wide_kernel(
+    Mat<const T> x, Vec weight, Vec bias, float eps, Mat<O> y, float* __restrict__ mean_out,
+    float* __restrict__ rstd_out, Pieces p) {
   const int pieces = int(p.per_row.d);
   for (long long r = blockIdx.x; r < x.rows; r += gridDim.x) {
     float s = 0.f;
@@ -304,11 +302,9 @@ __global__ __launch_bounds__(kWideThreads) void layer_norm_wide_kernel(Mat<const
 
 // dx of rows of any width: a workgroup a row, which is read twice.
 template <typename T, typename O, int N>
-__global__ __launch_bounds__(kWideThreads) void layer_norm_grad_wide_kernel(Mat<const O> dy, Mat<const T> x,
-                                                                 Vec weight,
-                                                                 const float* __restrict__ mean_in,
-                                                                 const float* __restrict__ rstd_in,
-                                                                 Mat<T> dx, Pieces p) {
+__global__ __launch_bounds__(kWideThreads) void layer_norm_grad_wide_kernel(
+    Mat<const O> dy, Mat<const T> x, Vec weight, const float* __restrict__ mean_in,
+    const float* __restrict__ rstd_in, Mat<T> dx, Pieces p) {
   const int pieces = int(p.per_row.d);
   for (long long r = blockIdx.x; r < x.rows; r += gridDim.x) {
     const float mean = mean_in[r], rstd = rstd_in[r];
@@ -379,10 +375,9 @@ struct VecOut {
 // dweight first, then dbias's.
 constexpr int kJoinCols = 32, kJoinLanes = 32, kJoinAhead = 8;
 constexpr int kJoinThreads = kJoinCols * kJoinLanes;
-__global__ __launch_bounds__(kJoinThreads) void layer_norm_join_kernel(const float* __restrict__ parts,
-                                                                 int part_count, int cols,
-                                                                 VecOut dweight, VecOut dbias,
-                                                                 bool add) {
+__global__ __launch_bounds__(kJoinThreads) void layer_norm_join_kernel(
+    const float* __restrict__ parts, int part_count, int cols, VecOut dweight, VecOut dbias,
+    bool add) {
   __shared__ float sums[kJoinLanes][kJoinCols];
   const int lane = threadIdx.x / kJoinCols, i = threadIdx.x % kJoinCols;
   const long long c = (long long)blockIdx.x * kJoinCols + i;
@@ -457,7 +452,7 @@ uint32_t norm_blocks(long long rows, int per_block) {
 // pieces on (16,384 x 2,048 BF16 47.5 -> 44.6; x 1,024 24.5 -> 31). 513 to 1,024
 // pieces of 8 elements, 512 threads for 256: 16,384 x 8,192 gradients 168 -> 157;
 // of 4 the other way: 16,384 x 4,096 137 -> 129.
-template <int N, int kMost, typename F>
+template <int N, int kMost, bool kForward, typename F>
 int with_lanes(const Pieces& p, bool apart, F&& f) {
   const uint32_t n = p.per_row.d;
   const auto call = [&](auto lanes, auto per) { return f(lanes, per); };
@@ -469,10 +464,12 @@ int with_lanes(const Pieces& p, bool apart, F&& f) {
     if (n <= 64) return call(integral_constant<int, 64>{}, integral_constant<int, 1>{});
     if (n <= 256 && apart) return call(integral_constant<int, 256>{}, integral_constant<int, 1>{});
     if (n <= 128) return call(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-    if (n <= 256) return call(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    if constexpr (kForward)  // (there the gradient's are apart)
+      if (n <= 256) return call(integral_constant<int, 64>{}, integral_constant<int, 4>{});
     if (n <= 512) return call(integral_constant<int, 256>{}, integral_constant<int, 2>{});
     if (n <= 1024)
-      return call(integral_constant<int, N == 8 ? 512 : 256>{}, integral_constant<int, N == 8 ? 2 : 4>{});
+      return call(integral_constant<int, N == 8 ? 512 : 256>{},
+                  integral_constant<int, N == 8 ? 2 : 4>{});
     if (n <= 2048) return call(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
     if constexpr (kMost >= 4096)
       if (n <= 4096) return call(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
@@ -519,7 +516,7 @@ int ps_layer_norm(const ps_rows* x, const ps_rows* weight, const ps_rows* bias, 
       constexpr int kSize = sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O);
       return ps::with_width<kSize>(x->cols, [&](auto n) {
         const ps::Pieces p(x->cols, n);
-        return ps::with_lanes<n, 4096>(p, x->rows <= 1024, [&](auto lanes, auto per) {
+        return ps::with_lanes<n, 4096, true>(p, x->rows <= 1024, [&](auto lanes, auto per) {
           const auto run = [&](auto kernel, uint32_t blocks, int threads) {
             kernel<<<blocks, threads, 0, ps::to_hip(stream)>>>(
                 ps::mat<const T>(x), ps::vec(weight, 1.f), ps::vec(bias, 0.f), eps, ps::mat<O>(y),
@@ -529,8 +526,8 @@ int ps_layer_norm(const ps_rows* x, const ps_rows* weight, const ps_rows* bias, 
             run(ps::layer_norm_wide_kernel<T, O, n>, ps::wide_blocks(x->rows), ps::kWideThreads);
           } else {
             constexpr int kThreads = ps::threads_of(lanes);
-            run(ps::layer_norm_kernel<T, O, n, lanes, per>, ps::norm_blocks(x->rows, kThreads / lanes),
-                kThreads);
+            run(ps::layer_norm_kernel<T, O, n, lanes, per>,
+                ps::norm_blocks(x->rows, kThreads / lanes), kThreads);
           }
           PS_LAUNCHED();
           return int(PS_OK);
@@ -591,7 +588,9 @@ int ps_layer_norm_grad(const ps_rows* dy, const ps_rows* x, const ps_rows* weigh
         constexpr int kSize = sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O);
         return ps::with_width<kSize>(x->cols, [&](auto n) {
           const ps::Pieces p(x->cols, n);
-          return ps::with_lanes<n, n == 8 ? 2048 : 4096>(p, p.per_row.d > 128, [&](auto lanes, auto per) {
+          constexpr int kMost = n == 8 ? 2048 : 4096;
+          const bool apart = p.per_row.d > 128;
+          return ps::with_lanes<n, kMost, false>(p, apart, [&](auto lanes, auto per) {
             if constexpr (lanes == 0) {
               ps::layer_norm_grad_wide_kernel<T, O, n>
                   <<<ps::wide_blocks(x->rows), ps::kWideThreads, 0, st>>>(

@@ -66,10 +66,12 @@ __device__ __forceinline__ T lanes_all(T v, Op op) {
   static_assert(sizeof(T) == 4 && kLanes >= 1 && kLanes <= kWave, "");
   const auto bits = [](T x) { return __builtin_bit_cast(int, x); };
   const auto of = [](int x) { return __builtin_bit_cast(T, x); };
-  if constexpr (kLanes > 1) v = op(v, of(__builtin_amdgcn_update_dpp(0, bits(v), 0xB1, 0xF, 0xF, true)));
-  if constexpr (kLanes > 2) v = op(v, of(__builtin_amdgcn_update_dpp(0, bits(v), 0x4E, 0xF, 0xF, true)));
-  if constexpr (kLanes > 4) v = op(v, of(__builtin_amdgcn_update_dpp(0, bits(v), 0x141, 0xF, 0xF, true)));
-  if constexpr (kLanes > 8) v = op(v, of(__builtin_amdgcn_update_dpp(0, bits(v), 0x140, 0xF, 0xF, true)));
+#define PS_FROM(pattern) of(__builtin_amdgcn_update_dpp(0, bits(v), pattern, 0xF, 0xF, true))
+  if constexpr (kLanes > 1) v = op(v, PS_FROM(0xB1));
+  if constexpr (kLanes > 2) v = op(v, PS_FROM(0x4E));
+  if constexpr (kLanes > 4) v = op(v, PS_FROM(0x141));
+  if constexpr (kLanes > 8) v = op(v, PS_FROM(0x140));
+#undef PS_FROM
   if constexpr (kLanes > 16) {
     const auto r = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
     v = op(of(int(r[0])), of(int(r[1])));
@@ -93,11 +95,13 @@ __device__ __forceinline__ float groups_sum(float v) {
   if constexpr (kLanes <= 4) v += xor_shfl<4>(v);
   if constexpr (kLanes <= 8) v += xor_shfl<8>(v);
   if constexpr (kLanes <= 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    const int b = __float_as_int(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
     v = __int_as_float(r[0]) + __int_as_float(r[1]);
   }
   if constexpr (kLanes <= 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    const int b = __float_as_int(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
     v = __int_as_float(r[0]) + __int_as_float(r[1]);
   }
   return v;

@@ -1,5 +1,6 @@
 """AdamW over many tensors against 64-bit forms: types, sizes from nothing to several chunks, odd
-alignments, moments in 32 and in 8 bits, clipping on the way, rates and steps on the device, graphs."""
+alignments, moments in 32 and in 8 bits, clipping on the way, rates and steps on the device,
+graphs."""
 import math
 import zlib
 
@@ -56,7 +57,8 @@ class Model:
             put = lambda x, dtype: Place(x, dtype, i % 5)  # noqa: E731
             self.p.append(put(0.02 * torch.randn(n, generator=gen), F[param]))
             self.g.append(put(torch.randn(n, generator=gen) * size, F[grad]))
-            m, v = 0.3 * torch.randn(n, generator=gen) * size, (size * torch.rand(n, generator=gen)) ** 2
+            m = 0.3 * torch.randn(n, generator=gen) * size
+            v = (size * torch.rand(n, generator=gen)) ** 2
             if f8:
                 m, v = m.double(), v.double().sqrt()
                 mc, ms, _, _ = ref.to_8_bits(m, 1, False)
@@ -149,7 +151,8 @@ def test_types(param, grad, f8):
 def test_options(f8):
     gen = generator("options", f8)
     for beta1, beta2, eps, lr, step in ((0.0, 0.9, 1e-3, 0.1, 1), (0.95, 0.0, 1e-6, 1e-2, 7),
-                                        (0.99, 0.9999, 0.1, 1e-5, 10 ** 9), (0.5, 0.5, 1e-8, 0.0, 3)):
+                                        (0.99, 0.9999, 0.1, 1e-5, 10 ** 9),
+                                        (0.5, 0.5, 1e-8, 0.0, 3)):
         model = Model(gen, SIZES, "f32", "f32", None, f8)
         before = model.exact()
         ps.AdamWStep(model.list(), lr, step, beta1=beta1, beta2=beta2, eps=eps, grad_scale=0.25)
