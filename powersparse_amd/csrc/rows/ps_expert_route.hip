@@ -109,9 +109,9 @@ __device__ __forceinline__ void finish(int experts, Sum&& sum_of, Count&& count_
   *loss = tokens ? float(sum * experts / (double(tokens) * double(total))) : 0.f;
 }
 
-// Bound by its instructions, some 900 for the eight tokens of a wave with 128
-// experts, 55 of them for each expert that is found: 65,536 x 128 FP32, 38 MB, top 8
-// 14 us and top 1 7.4; with the sums for the loss 17.7 and the join 5.8.
+// Bound by its instructions, some 750 for the eight tokens of a wave with 128
+// experts, 35 of them for each expert that is found: 65,536 x 128 FP32, 38 MB, top 8
+// 13.3 us and top 1 7.3; with the sums for the loss 17.3 and the join 6.
 template <typename T, int kLanes, int kPer, int kWide, int kThreads>
 __global__ __launch_bounds__(kThreads) void route_kernel(
     Mat<const T> logits, int experts, int top_k, bool normalize,
@@ -171,17 +171,22 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
 #pragma unroll
       for (int r = 1; r < kPer; ++r) best = max(best, key[r]);
       best = lanes_max<kLanes>(best);
-      bool equal = false;
+      uint32_t my_best = 0, down = 0;
       for (int k = 0; k < top_k; ++k) {
-        const bool any = best >> kBits > kBarred >> (kBits + 1);
-        if (lane == k && any) my_id = kMost - 1 - int(best & (kMost - 1));
-        uint32_t down = key[0] - best;  // from 2^31 up for those below it
+        if (lane == k) my_best = best;
+        down = key[0] - best;  // from 2^31 up for those below it
 #pragma unroll
         for (int r = 1; r < kPer; ++r) down = max(down, key[r] - best);
         down = lanes_max<kLanes>(down);
-        equal = equal || (any && int(down) < 0 && (best + down) >> kBits == best >> kBits);
         best += down;
       }
+      // Whether a slot's key agrees with the next one's, the last slot's with that of
+      // the expert after it (if there is one).
+      const bool any = lane < top_k && my_best >> kBits > kBarred >> (kBits + 1);
+      if (any) my_id = kMost - 1 - int(my_best & (kMost - 1));
+      uint32_t next = uint32_t(__shfl_down(int(my_best), 1, kLanes));
+      if (lane == top_k - 1) next = int(down) < 0 ? best : 0;
+      const bool equal = any && next >> kBits == my_best >> kBits;
       found = !__any((sizeof(T) == 4 && equal) || nan);
     }
     float total = 0.f;
