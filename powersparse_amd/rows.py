@@ -645,8 +645,11 @@ class AdamWList:
             if copies and copies[i] is not None:
                 c, _, c_type = _some(copies[i], "copy", i, _DTYPES, count)
                 c_type = _DTYPES[c_type]
-            _TENSOR.pack_into(table, i * _TENSOR.size, p, g, m, v, s, c, count, _DTYPES[p_type],
-                              _DTYPES[g_type], c_type, decay[i])
+            try:
+                _TENSOR.pack_into(table, i * _TENSOR.size, p, g, m, v, s, c, count,
+                                  _DTYPES[p_type], _DTYPES[g_type], c_type, decay[i])
+            except (struct.error, OverflowError, TypeError):
+                raise ValueError(f"weight_decay {i} is not a number in float32's range") from None
         table = ctypes.cast(table, ctypes.POINTER(AdamWTensor))
         h = ctypes.c_void_p()
         _call(_hip.ps_adamw_list_create(n, table, _E4M3 if scales else 0, ctypes.byref(h)))

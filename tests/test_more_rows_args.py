@@ -160,6 +160,8 @@ def test_adamw_list():
     refused("tensor 0: null data", call, grads=[vec(0, 1000)])
     refused("tensor 0: misaligned", call, exp_avgs=[vec(C + 2, 1000)])
     refused("tensor 0: weight decay is not", call, weight_decay=float("nan"))
+    for decay in (1e300, [1e300], ["0.1"], [None]):
+        refused("weight.decay (0 )?is not a number", call, weight_decay=decay)
     codes = dict(exp_avgs=[vec(C, 1000, "uint8")], exp_avg_sqs=[vec(D, 1000, "uint8")])
     refused("scales 0 has 7 elements where 8", call, scales=[vec(G, 7)], **codes)
     refused("exp_avg 0: element type float32", call, scales=[vec(G, 8)])
