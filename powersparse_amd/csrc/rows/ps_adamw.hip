@@ -106,6 +106,18 @@ __device__ __forceinline__ float quotient(float x, float d, float by) {
   const float q = x * by;
   return fmaf(fmaf(-q, d, x), by, q);
 }
+// sqrt(v), correctly rounded but for the rarest cases: the hardware's reciprocal
+// root and one step of Newton's iteration on the root (Markstein 1990), numbers
+// whose residual would be lost scaled by 2^64.
+__device__ __forceinline__ float root_of(float v) {
+  const bool small = v < 0x1p-96f;
+  const float x = small ? v * 0x1p64f : v;
+  const float y = __builtin_amdgcn_rsqf(x);
+  const float q = x * y;
+  const float r = fmaf(fmaf(-q, q, x), 0.5f * y, q);
+  return x > 0.f && x < INFINITY ? (small ? r * 0x1p-32f : r) : v;  // (0, infinity and NaN)
+}
+
 // The parameter after a step by m and the root of v. The reciprocal is the
 // hardware's, off by a unit in the last place: of the update, which is smaller
 // than the parameter it is rounded into.
@@ -163,7 +175,7 @@ struct Elements {
     for (int e = 0; e < N; ++e) {
       float me = m[e], ve = v[e];
       advance(s, gf[e], &me, &ve);
-      pf[e] = updated(s, t.decay, pf[e], me, __builtin_amdgcn_sqrtf(ve));
+      pf[e] = updated(s, t.decay, pf[e], me, root_of(ve));
       m[e] = me;
       v[e] = ve;
     }
@@ -208,18 +220,6 @@ __device__ __forceinline__ float wave_most(uint32_t v) {
 __device__ __forceinline__ float scale_of(float most) {
   const float s = most * (1.f / 448.f);
   return s < 0x1p-126f ? 0x1p-126f : s;
-}
-
-// sqrt(v), correctly rounded but for the rarest cases: the hardware's reciprocal
-// root and one step of Newton's iteration on the root (Markstein 1990), numbers
-// whose residual would be lost scaled by 2^64.
-__device__ __forceinline__ float root_of(float v) {
-  const bool small = v < 0x1p-96f;
-  const float x = small ? v * 0x1p64f : v;
-  const float y = __builtin_amdgcn_rsqf(x);
-  const float q = x * y;
-  const float r = fmaf(fmaf(-q, q, x), 0.5f * y, q);
-  return x > 0.f && x < INFINITY ? (small ? r * 0x1p-32f : r) : v;  // (0, infinity and NaN)
 }
 
 // The magnitude `a` (up to 448) on the grid of E4M3, rounded by u (32 bits). The

@@ -287,6 +287,23 @@ def test_zeros_stay_zeros_and_nothing_becomes_zero():
     assert float((p - 1).abs().max()) <= 3 * 1.1e-3  # m / sqrt(v) is 1 at most for equal gradients
 
 
+@pytest.mark.parametrize("f8", [False, True])
+def test_second_moments_below_the_normal_numbers(f8):
+    """Gradients of 1e-18 and no eps: the first step goes by one. (1 - beta2) g^2 is 1e-39, where
+    FP32 numbers are 2^-149 apart, 1.4e-6 of it: the root is off by 0.7e-6, and some forty FP32
+    roundings come to 2.4e-6."""
+    n = 1000
+    p, g = torch.zeros(n, device="cuda"), torch.full((n,), 1e-18, device="cuda")
+    g[::2] *= -1
+    if f8:
+        m, v = (torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2))
+        scales = [torch.zeros((ps.state_blocks(n), 2), device="cuda")]
+    else:
+        m, v, scales = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda"), None
+    ps.AdamWStep(ps.AdamWList([p], [g], [m], [v], scales=scales), 1.0, 1, eps=0.0)
+    assert float((p + g.sign()).abs().max()) <= 4e-6
+
+
 def test_moments_in_8_bits_follow_the_gradients():
     """A second moment that gains a part in 1000 a step gains it in its codes too, which rounding to
     nearest would leave at 4.5. 2000 steps of gradients twice as large take the exact root from 1 to
