@@ -621,7 +621,10 @@ class AdamWList:
                  weight_decay=0.01):
         self._h = None
         n = len(params)
-        decay = list(weight_decay) if hasattr(weight_decay, "__len__") else [weight_decay] * n
+        try:
+            decay = list(weight_decay)
+        except TypeError:  # a number, an array without dimensions too
+            decay = [weight_decay] * n
         given = dict(grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs, scales=scales,
                      copies=copies, weight_decay=decay)
         for name, x in given.items():

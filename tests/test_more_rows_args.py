@@ -1,8 +1,11 @@
 """What layer norm, the router and AdamW refuse, on the host and before any device call, through
 Python and through the C ABI, and their workspace sizes. The addresses are never followed."""
 import ctypes
+import math
 
+import numpy as np
 import pytest
+import torch
 
 import powersparse_amd as ps
 from powersparse_amd import _native
@@ -237,3 +240,15 @@ def test_workspaces_grow_with_every_argument():
 
 def test_state_blocks():
     assert [ps.state_blocks(n) for n in (0, 1, 256, 257, 1 << 33)] == [0, 1, 1, 2, 1 << 25]
+
+
+def test_adamw_weight_decay_of_no_dimension():
+    """A number in an array without dimensions is a number."""
+    two = {k: v + [ps.DeviceArray(v[0].ptr + (1 << 20), 1000, v[0].dtype)]
+           for k, v in good_list().items()}
+    for value in (math.nan, 1e300):
+        for number in (np.array(value), torch.tensor(value, dtype=torch.float64)):
+            refused("weight.decay (0 )?is not a number", ps.AdamWList, weight_decay=number, **two)
+    refused("weight_decay: one for each parameter", ps.AdamWList, weight_decay=np.zeros(3), **two)
+    refused("tensor 1: weight decay is not", ps.AdamWList,
+            weight_decay=torch.tensor([0.1, float("nan")]), **two)
