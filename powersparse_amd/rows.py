@@ -620,18 +620,19 @@ class AdamWList:
     def __init__(self, params, grads, exp_avgs, exp_avg_sqs, scales=None, copies=None,
                  weight_decay=0.01):
         self._h = None
-        n = len(params)
+        self._keep = [list(x) for x in (params, grads, exp_avgs, exp_avg_sqs,
+                                        () if scales is None else scales,
+                                        () if copies is None else copies)]
+        n = len(self._keep[0])
         try:
             decay = list(weight_decay)
         except TypeError:  # a number, an array without dimensions too
             decay = [weight_decay] * n
-        given = dict(grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs, scales=scales,
-                     copies=copies, weight_decay=decay)
-        for name, x in given.items():
-            if x is not None and len(x) != n:
+        for name, x, items in zip(
+                ("grads", "exp_avgs", "exp_avg_sqs", "scales", "copies", "weight_decay"),
+                (grads, exp_avgs, exp_avg_sqs, scales, copies, decay), self._keep[1:] + [decay]):
+            if x is not None and len(items) != n:
                 raise ValueError(f"{name}: one for each parameter")
-        self._keep = [list(x) for x in (params, grads, exp_avgs, exp_avg_sqs, scales or (),
-                                        copies or ())]
         params, grads, exp_avgs, exp_avg_sqs, scales, copies = self._keep
         if _several is not False:
             _check_devices(*(x for xs in self._keep for x in xs))

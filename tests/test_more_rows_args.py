@@ -252,3 +252,18 @@ def test_adamw_weight_decay_of_no_dimension():
     refused("weight_decay: one for each parameter", ps.AdamWList, weight_decay=np.zeros(3), **two)
     refused("tensor 1: weight decay is not", ps.AdamWList,
             weight_decay=torch.tensor([0.1, float("nan")]), **two)
+
+
+def test_adamw_list_of_iterators():
+    """What may be gone through once is taken like a list, as for gradient lists."""
+    def call(**other):
+        given = good_list(**other)
+        ps.AdamWList(**{k: iter(v) for k, v in given.items()})
+
+    refused("gradient 0 has 999 elements", call, grads=[vec(B, 999)])
+    refused("grads: one for each parameter", call, grads=[])
+    refused("copies: one for each parameter", call, copies=[None, None])
+    refused("weight_decay: one for each parameter", call, weight_decay=[0.1, 0.2])
+    codes = dict(exp_avgs=[vec(C, 1000, "uint8")], exp_avg_sqs=[vec(D, 1000, "uint8")])
+    refused("scales 0 has 7 elements where 8", call, scales=[vec(G, 7)], **codes)
+    refused("scales: one for each parameter", call, scales=[], **codes)
