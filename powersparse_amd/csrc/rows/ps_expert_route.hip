@@ -189,6 +189,8 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
       const bool equal = any && next >> kBits == my_best >> kBits;
       found = !__any((sizeof(T) == 4 && equal) || nan);
     }
+    // A place left over weighs 0 whatever the others are divided by, NaN too.
+    const auto times = [](float w, float by) { return w == 0.f ? 0.f : w * by; };
     float total = 0.f;
     const auto put = [&](int k, float& w) {  // slot k, this lane's
       w = my_id >= 0 ? exp_of(float(*logits.at(t, my_id)) - top) : 0.f;
@@ -228,16 +230,17 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
       if (top_k <= kLanes) {
         const float sum = lanes_sum<kLanes>(total);
         const float by = normalize ? (sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum)) : scale;
-        if (lane < n && mine) weights[t * top_k + lane] = w * by;
+        if (lane < n && mine) weights[t * top_k + lane] = times(w, by);
       } else if (lane < n && mine) {
-        weights[t * top_k + k0 + lane] = normalize ? w : w * scale;
+        weights[t * top_k + k0 + lane] = normalize ? w : times(w, scale);
       }
     }
     if (top_k > kLanes && normalize) {
       total = lanes_sum<kLanes>(total);
       const float by = total == 0.f ? 0.f : __builtin_amdgcn_rcpf(total);
       if (mine)
-        for (int k = lane; k < top_k; k += kLanes) weights[t * top_k + k] *= by;
+        for (int k = lane; k < top_k; k += kLanes)
+          weights[t * top_k + k] = times(weights[t * top_k + k], by);
     }
   }
   if (!parts.sums) return;

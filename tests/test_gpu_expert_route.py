@@ -333,3 +333,26 @@ def test_in_a_graph_on_into_the_sort(tokens):
         on = mask[:, None].float()
         assert float((y - x * on).abs().max()) <= 8 * ref.U32 * float(x.abs().max())
         assert torch.equal(position < 0, ~mask[:, None].expand(-1, K))
+
+
+@pytest.mark.parametrize("tokens,experts,top_k", [(4, 70, 5), (9004, 20, 3), (12, 300, 100)])
+def test_places_left_over_beside_a_nan(tokens, experts, top_k):
+    """A NaN makes its token's weights NaN, but of the experts that were chosen: places left over
+    have id -1 and weight 0 whatever the logits."""
+    logits = torch.full((tokens, experts), -math.inf, device="cuda")
+    logits[0::4, 2] = 0.5
+    logits[1::4, 9], logits[1::4, 4] = float("nan"), 1.0
+    logits[2::4, 11] = -float("nan")
+    logits[3::4, 1] = math.inf
+    for normalize in (True, False):
+        for losses in (True, False):
+            ids, weights = route(logits, top_k, normalize, losses=losses)[:2]
+            want = torch.full_like(ids, -1)
+            want[0::4, 0], want[1::4, 0], want[1::4, 1] = 2, 9, 4
+            want[2::4, 0], want[3::4, 0] = 11, 1
+            assert torch.equal(ids, want)
+            assert bool((weights[0::4, 0] == 1).all())
+            for k in (1, 2, 3):
+                taken = want[k::4] >= 0
+                assert bool(torch.isnan(weights[k::4][taken]).all())
+            assert not weights[want < 0].any()
