@@ -148,3 +148,30 @@ def test_nan_among_many(dtype):
     rest[rows, at[rows]] = -math.inf
     order = torch.sort(rest, dim=1, descending=True, stable=True).indices[:, :K - 1]
     assert torch.equal(ids[rows, 1:].long(), order[rows])
+
+
+@pytest.mark.parametrize("experts", [5, 16, 17, 64, 128, 200, 300, 1024])
+def test_the_loss_takes_every_token_once(experts):
+    """The loss to less than a token's part of it. A probability is off by the exponential, 2 + 2.3
+    times the logits' difference of up to 12, the sum of the experts, at most 15 + 6 additions, a
+    reciprocal and a product, 3: 54 units; a sum over the tokens has 10 turns of a lane at most, 4
+    steps in a wave and 16 waves, then 64-bit sums and one rounding: 86 units together, 5.2e-6. A
+    token's part is some 1 / 40,007, 2.5e-5."""
+    T, K = 40007, min(experts, 4)
+    gen = generator("every token", experts)
+    logits = torch.randn((T, experts), generator=gen, device="cuda")
+    ids, w = torch.empty((T, K), dtype=torch.int32, device="cuda"), torch.empty((T, K), device="cuda")
+    counts = torch.empty(experts + 1, dtype=torch.int32, device="cuda")
+    loss = torch.empty(1, device="cuda")
+    work = torch.empty(ps.expert_route_workspace_bytes(T, experts), dtype=torch.uint8, device="cuda")
+    ps.ExpertRoute(logits, ids, w, counts, loss, work)
+    l = logits.double()
+    assert float((l.amax(1) - l.amin(1)).max()) <= 12
+    p = torch.softmax(l, 1)
+    freq = torch.bincount(torch.sort(l, dim=1, descending=True, stable=True).indices[:, :K]
+                          .reshape(-1), minlength=experts)
+    assert torch.equal(counts.long(), torch.cat([freq, torch.tensor([T], device="cuda")]))
+    each = experts * (p * freq.double()).sum(1) / (T * freq.sum())  # a token's part of the loss
+    exact = float(each.sum())
+    off = 86 * ref.U32 * exact
+    assert float(each.min()) > 4 * off and abs(float(loss) - exact) <= off
