@@ -213,7 +213,8 @@ void ps_adamw_list_destroy(ps_adamw_list* list);
 
 /* step: the number of this update, from 1. device_lr, device_step and norm (device,
  * one value each): NULL, or read when the step runs, lr and step ignored then (a
- * device step below 1 counts as 1); none may lie in what the step writes. */
+ * device step below 1 counts as 1); none may lie in what the step writes. lr and eps
+ * are numbers within FP32's range, eps from 0 up (PS_ERR_INVALID otherwise). */
 typedef struct ps_adamw_options {
   double lr, beta1, beta2, eps;
   long long step;

@@ -16,6 +16,7 @@
 // it over the elements. A second moment that is not zero never becomes zero: the
 // step divides by it.
 #include <cmath>
+#include <limits>
 
 #include "ps_tensor_list.hpp"
 
@@ -483,8 +484,10 @@ int ps_adamw_step(ps_adamw_list* list, const ps_adamw_options* o, ps_stream_t st
   PS_CHECK_ARG(list && o, "ps_adamw_step: null argument");
   PS_CHECK_ARG(o->beta1 >= 0 && o->beta1 < 1 && o->beta2 >= 0 && o->beta2 < 1,
                "ps_adamw_step: betas are from 0 up to below 1");
-  PS_CHECK_ARG(o->eps >= 0, "ps_adamw_step: eps is not a number from 0 up");
-  PS_CHECK_ARG(o->device_lr || std::isfinite(o->lr), "ps_adamw_step: the rate is not a number");
+  constexpr double kLargest = std::numeric_limits<float>::max();  // the kernel computes in FP32
+  PS_CHECK_ARG(o->eps >= 0 && o->eps <= kLargest, "ps_adamw_step: eps is not a number from 0 up");
+  PS_CHECK_ARG(o->device_lr || std::fabs(o->lr) <= kLargest,
+               "ps_adamw_step: the rate is not a number");
   PS_CHECK_ARG(o->device_step || o->step >= 1, "ps_adamw_step: steps are counted from 1");
   PS_CHECK_ARG(!o->norm || o->max_norm >= 0.f,
                "ps_adamw_step: the bound is not a number from 0 up");

@@ -385,3 +385,33 @@ def test_a_list_may_go_at_any_time():
     torch.cuda.synchronize()
     model.check(before, 1e-3, 1)
     another.close()
+
+
+def test_steps_that_are_refused():
+    """Numbers on the host that FP32 does not hold, and other options out of range."""
+    p, g, m, v = (torch.ones(100, device="cuda") for _ in range(4))
+    tensors = ps.AdamWList([p], [g], [m], [v])
+
+    def refused(text, lr=1e-3, step=1, **more):
+        with pytest.raises(ValueError, match=text):
+            ps.AdamWStep(tensors, lr, step, **more)
+
+    for rate in (math.nan, math.inf, 1e39, -1e39, 1e300):
+        refused("the rate is not a number", lr=rate)
+    for eps in (math.nan, -1e-8, math.inf, 1e39):
+        refused("eps is not a number", eps=eps)
+    for beta in (math.nan, -0.1, 1.0):
+        refused("betas", beta1=beta)
+        refused("betas", beta2=beta)
+    for step in (0, -1):
+        refused("counted from 1", step=step)
+    norm = torch.ones(1, device="cuda")
+    for bound in (math.nan, -1.0):
+        refused("the bound is not a number", norm=norm, max_norm=bound)
+    refused("max_norm needs the norm", max_norm=1.0)
+    assert all(bool((x == 1).all()) for x in (p, g, m, v))
+    largest = torch.finfo(torch.float32).max
+    ps.AdamWStep(tensors, 0.0, 1, eps=largest)
+    assert bool((p == 1).all())
+    ps.AdamWStep(tensors, largest, 1, eps=largest)
+    assert bool(torch.isfinite(p).all())
