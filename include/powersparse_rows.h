@@ -230,8 +230,10 @@ typedef struct ps_adamw_options {
  * exp_avg_sq = beta2 * exp_avg_sq + (1 - beta2) * g^2,
  * param -= lr * (weight_decay * param + (exp_avg / (1 - beta1^step)) /
  * (sqrt(exp_avg_sq / (1 - beta2^step)) + eps)). A norm that is not finite: nothing
- * changes. The parameter moves by the moments before they are rounded to 8 bits;
- * there they go to either neighbouring code, by a rule of step and place that
+ * changes, and `step` is not to count such a call (with four counted before it the
+ * first update is 0.55 of its size); a step on the device can be advanced by whether
+ * the norm is finite. The parameter moves by the moments before they are rounded to 8
+ * bits; there they go to either neighbouring code, by a rule of step and place that
  * keeps their mean over the steps, and a second moment that is not zero stays so.
  * A gradient that is not finite makes its element's moments so, in 8 bits its
  * block's. */

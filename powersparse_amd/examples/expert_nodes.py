@@ -223,7 +223,8 @@ def problem(nodes, classes=16, tokens=2000, seed=0):
 
 
 class AdamW:
-    """AdamW over parameters whose gradients stay where they are: those of matrices decay."""
+    """AdamW over parameters whose gradients stay where they are: those of matrices decay. Updates
+    are counted on the device, where they are made or, by a norm that is not finite, skipped."""
 
     def __init__(self, params, bits=32):
         state = torch.float32 if bits == 32 else torch.uint8
@@ -235,10 +236,10 @@ class AdamW:
         self.tensors = ps.AdamWList([p.detach() for p in params], [p.grad for p in params], m, v,
                                     scales=scales,
                                     weight_decay=[0.01 if p.dim() > 1 else 0.0 for p in params])
-        self.steps = 0
+        self.steps = torch.zeros(1, dtype=torch.int32, device=params[0].device)
 
     def step(self, rate, norm, max_norm):
-        self.steps += 1
+        self.steps += torch.isfinite(norm)
         ps.AdamWStep(self.tensors, rate, self.steps, norm=norm, max_norm=max_norm, stream=_stream())
 
 

@@ -695,7 +695,9 @@ def AdamWStep(tensors, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, norm=None, ma
     `step` counts from 1. lr and step are numbers, or one float32 and one int32 on the device,
     read when the step runs. With `norm` (one float32 on the device, GradNorm's of grad_scale *
     grad) g is also multiplied by min(1, max_norm / (norm + 1e-6)) on the way, max_norm None: not,
-    and a norm that is not finite leaves everything as it is."""
+    and a norm that is not finite leaves everything as it is. Such a call is not to be counted by
+    the next ones' `step`: a step on the device can be advanced by whether the norm is finite
+    (step += torch.isfinite(norm))."""
     if _several is not False:
         _check_devices(tensors, lr, step, norm)
     o = AdamWOptions(beta1=beta1, beta2=beta2, eps=eps, grad_scale=grad_scale,

@@ -85,3 +85,30 @@ def test_runs(adamw):
                              balance=0.01, adamw=adamw)
     assert all(math.isfinite(v) for v in losses) and all(n > 0 for n in norms)
     assert len(lines) == 3
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_skipped_update_is_not_counted(bits):
+    """Updates whose norm is not finite change nothing, and the first one after them is the first
+    of the formula: counted as the third, it would be 0.58 of that."""
+    setup()
+    model = ex.Model(200, 8, seed=1, norm=True)
+    params = model.parameters()
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for p in params:
+        p.grad = torch.randn(p.shape, generator=gen, device="cuda")
+    optimizer = ex.AdamW(params, bits)
+    before = [p.detach().clone() for p in params]
+    size = torch.empty(1, device="cuda")
+    for bad in (math.inf, math.nan):
+        optimizer.step(0.01, size.fill_(bad), 1.0)
+        assert all(torch.equal(p.detach(), old) for p, old in zip(params, before))
+    ps.GradNorm(ps.GradientList([p.grad for p in params]), size)
+    optimizer.step(0.01, size, 1.0)
+    norm = math.sqrt(sum(float(p.grad.double().square().sum()) for p in params))
+    for p, old in zip(params, before):
+        g, old = p.grad.double() / (norm + 1e-6), old.double()
+        decay = 0.01 if p.dim() > 1 else 0.0
+        want = old - 0.01 * (decay * old + g / (g.abs() + 1e-8))
+        # as in test_update
+        assert bool(((p.detach().double() - want).abs() <= 2.0 ** -24 * (0.4 + 2 * old.abs())).all())
