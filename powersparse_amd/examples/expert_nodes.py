@@ -264,6 +264,7 @@ def train(nodes=8192, steps=60, seed=0, max_norm=0.1, rate=None, say=print, norm
             for p in params:
                 p.grad.zero_()
         (loss + balance * model.balance.sum()).backward()
+        model.balance = model.balance.detach()  # the value alone: its graph goes with the step's
         if optimizer:
             ps.GradNorm(grads, size, stream=_stream())
             optimizer.step(rate, size, max_norm)

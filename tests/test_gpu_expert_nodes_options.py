@@ -112,3 +112,19 @@ def test_a_skipped_update_is_not_counted(bits):
         want = old - 0.01 * (decay * old + g / (g.abs() + 1e-8))
         # as in test_update
         assert bool(((p.detach().double() - want).abs() <= 2.0 ** -24 * (0.4 + 2 * old.abs())).all())
+
+
+def test_a_step_leaves_no_graph(monkeypatch):
+    """What the model keeps of a pass holds none of its graph once the step is done."""
+    setup()
+    made = []
+
+    class Kept(ex.Model):
+        def __init__(self, *args, **kwargs):
+            super().__init__(*args, **kwargs)
+            made.append(self)
+
+    monkeypatch.setattr(ex, "Model", Kept)
+    ex.train(nodes=512, steps=1, seed=1, say=lambda line: None, norm=True, balance=0.01)
+    assert made[0].balance.grad_fn is None and not made[0].balance.requires_grad
+    assert math.isfinite(float(made[0].balance))
