@@ -13,7 +13,12 @@
 // is the golden ratio's fraction, so an element's u is spread evenly over the
 // steps (Weyl's equidistribution), and its code goes up as often as its moment
 // gains a step of the grid; a / 2^32 (the square root of two's fraction) spreads
-// it over the elements. A second moment that is not zero never becomes zero: the
+// it over the elements. Under constant gradients that keeps an element within a step
+// of the grid. Under random ones its moves and u have nothing in common, and it walks:
+// after 2,000 steps of N(0, 1) gradients with beta2 = 0.999 the roots are off by 15%
+// rms, 1.5 steps of the grid and at most 4.6, their mean by 0.6%. What is unbiased in
+// the root adds its variance to the square, which is 3.4% too large then and up to
+// 3.8% later (10,000 steps); the first moment (beta1 = 0.9) is off by 7% of its size. A second moment that is not zero never becomes zero: the
 // step divides by it.
 #include <cmath>
 #include <limits>

@@ -415,3 +415,40 @@ def test_steps_that_are_refused():
     assert bool((p == 1).all())
     ps.AdamWStep(tensors, largest, 1, eps=largest)
     assert bool(torch.isfinite(p).all())
+
+
+def test_moments_in_8_bits_under_random_gradients():
+    """2000 steps of N(0, 1) gradients from a root of 1, beside the exact course and the rule in 64
+    bits. A step moves a root r by d = 0.0005 (g^2 - r^2) / r, 0.00048 r on average, and a code goes
+    up with the probability d / q, q its step of the grid, r / 8 at most: the variance of a rounding
+    is at most q |d| = 6.1e-5 r^2. What it leaves decays by 0.999 a step: 500 of them are in the
+    root, 0.030, whose root is 0.174. They add up in the square, 1000 of them, 0.061, and so the
+    root's mean may rise by 0.03. Means of 16,384 elements that walk by themselves are off by
+    0.174 / 128 and their spread by 1 / 181."""
+    n, beta1, beta2 = 16384, 0.9, 0.999
+    gen = generator("walk")
+    p, g = torch.zeros(n, device="cuda"), torch.empty(n, device="cuda")
+    code, scale, _, _ = ref.to_8_bits(torch.ones(n, dtype=torch.float64), 1, True)
+    m, v = torch.zeros(n, device="cuda").to(F8), code.float().cuda().to(F8)
+    s = torch.stack([torch.zeros_like(scale), scale], 1).float().cuda()
+    tensors = ps.AdamWList([p], [g], [m], [v], scales=[s], weight_decay=0.0)
+    exact = torch.ones(n, dtype=torch.float64)
+    rule = exact.clone()
+    for t in range(1, 2001):
+        fresh = torch.randn(n, generator=gen)
+        g.copy_(fresh)
+        ps.AdamWStep(tensors, 0.0, t, beta1=beta1, beta2=beta2)
+        square = fresh.double().square_()
+        exact = beta2 * exact + (1 - beta2) * square
+        code, scale, _, _ = ref.to_8_bits((beta2 * rule * rule + (1 - beta2) * square).sqrt(), t, True)
+        rule = code * scale.repeat_interleave(256)
+    got = (v.float().view(-1, 256) * s[:, 1:]).view(-1).cpu().double()
+    means, spreads = [], []
+    for root in (got, rule):
+        off = root / exact.sqrt() - 1
+        means.append(float(off.mean()))
+        spreads.append(float(off.square().mean().sqrt()))
+        assert abs(means[-1]) <= 0.03 and spreads[-1] <= 0.18
+        assert -0.01 <= float((root * root / exact).mean()) - 1 <= 0.065
+    assert abs(means[0] - means[1]) <= 6 * 0.174 / 128 * math.sqrt(2)
+    assert abs(spreads[0] / spreads[1] - 1) <= 6 / 181 * math.sqrt(2)
