@@ -34,10 +34,26 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// e^x for x <= 0 by the hardware's power of two, off by 2^-24 (2 + 1.3 |x|)
-// relative: as much again as the logits' difference x itself.
-__device__ __forceinline__ float exp_of(float x) {
+// e^x for x <= 0 by the hardware's power of two: off by 2^-24 (2 + 1.3 |x|) relative,
+// as the exponent is rounded. For sums, where that averages out: the terms far below
+// the largest count little.
+__device__ __forceinline__ float rough_exp(float x) {
   return __builtin_amdgcn_exp2f(x * 1.44269504f);
+}
+// The same with what the rounding lost of x, x - t ln(2), put back by the first terms
+// of the series: off by 2^-24 (3 + 0.05 |x|). (The bounds are for x = -inf, whose
+// difference is no number, and whose power is 0.) For what a call gives back: weights,
+// of which a token has top_k, and the gradient. 65,536 x 128 FP32 top 8 13.5 -> 13.6 us,
+// with it in the sums too 14.4; the gradient of 16,384 x 512 BF16 15.4 -> 15.7.
+__device__ __forceinline__ float exp_of(float x) {
+  const float t = x * 1.44269504f, r = __builtin_amdgcn_exp2f(t);
+  const float lost = __builtin_amdgcn_fmed3f(fmaf(t, -0.693147182f, x), -1.f, 1.f);
+  return fmaf(r, lost, r);
+}
+// 1 / s for s from 1 up, or NaN: the hardware's and one step of Newton's iteration.
+__device__ __forceinline__ float reciprocal(float s) {
+  const float r = __builtin_amdgcn_rcpf(s);
+  return fmaf(fmaf(-s, r, 1.f), r, r);
 }
 
 // Over the kLanes lanes of a token, in every one of them.
@@ -150,14 +166,14 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
     float top = most > kBarred ? value_of(most) : 0.f;
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      p[r] = exp_of(p[r] - top);
+      p[r] = rough_exp(p[r] - top);
       s += p[r];
     }
     s = lanes_sum<kLanes>(s);
     const bool nan = s != s;
     if (nan) top = s;
     const bool takes_part = most > kBarred || nan;
-    const float scale = takes_part ? __builtin_amdgcn_rcpf(s) : 0.f;
+    const float scale = takes_part ? reciprocal(s) : 0.f;
     if (parts.sums) {
 #pragma unroll
       for (int r = 0; r < kPer; ++r) acc[r] += p[r] * scale;
@@ -229,7 +245,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
       if (lane < n && mine) put(k0 + lane, w);
       if (top_k <= kLanes) {
         const float sum = lanes_sum<kLanes>(total);
-        const float by = normalize ? (sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum)) : scale;
+        const float by = normalize ? (sum == 0.f ? 0.f : reciprocal(sum)) : scale;
         if (lane < n && mine) weights[t * top_k + lane] = times(w, by);
       } else if (lane < n && mine) {
         weights[t * top_k + k0 + lane] = normalize ? w : times(w, scale);
@@ -237,7 +253,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(
     }
     if (top_k > kLanes && normalize) {
       total = lanes_sum<kLanes>(total);
-      const float by = total == 0.f ? 0.f : __builtin_amdgcn_rcpf(total);
+      const float by = total == 0.f ? 0.f : reciprocal(total);
       if (mine)
         for (int k = lane; k < top_k; k += kLanes)
           weights[t * top_k + k] = times(weights[t * top_k + k], by);
@@ -423,7 +439,7 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
       p[r] = exp_of(p[r] - top);
       s += p[r];
     }
-    const float scale = __builtin_amdgcn_rcpf(lanes_sum<kLanes>(s));
+    const float scale = reciprocal(lanes_sum<kLanes>(s));
     // What the chosen experts' weights' gradients add, kLanes of them at a time: the
     // first ones have been loaded.
     float chosen = 0.f, dot = 0.f;
@@ -435,7 +451,7 @@ __global__ __launch_bounds__(kRouteGradThreads) void route_grad_kernel(
         chosen += w;
         dot += w * c.dw;
       }
-      chosen = __builtin_amdgcn_rcpf(lanes_sum<kLanes>(chosen));
+      chosen = reciprocal(lanes_sum<kLanes>(chosen));
       dot = lanes_sum<kLanes>(dot) * chosen;
     }
     Choice c = first;

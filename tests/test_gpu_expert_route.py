@@ -356,3 +356,23 @@ def test_places_left_over_beside_a_nan(tokens, experts, top_k):
                 taken = want[k::4] >= 0
                 assert bool(torch.isnan(weights[k::4][taken]).all())
             assert not weights[want < 0].any()
+
+
+@pytest.mark.parametrize("tokens,experts", [(400, 8), (9000, 8), (400, 16), (9000, 20), (400, 64),
+                                            (100, 128)])
+@pytest.mark.parametrize("std", [1, 8])
+def test_weights_of_far_logits(tokens, experts, std):
+    """All experts chosen, weights over a hundred powers of two: logits whose differences FP32
+    holds, so that what is off is the exponentials, 2^-24 (3 + 0.05 |x|) of a weight's own and 4 of
+    the sum's, whose terms are near the largest, additions one behind another, experts / 4 of a lane
+    and 6 joins at most, the reciprocal, 2, and a product."""
+    gen = generator("far", tokens, experts, std)
+    logits = torch.round(std * 64 * torch.randn((tokens, experts), generator=gen)) / 64
+    assert float(logits.abs().max()) < 64
+    ids, weights = route(logits.cuda(), experts, True, losses=False)
+    want = torch.sort(logits.double(), dim=1, descending=True, stable=True)
+    assert torch.equal(ids.cpu().long(), want.indices)
+    exact = torch.softmax(want.values, 1)
+    x = want.values[:, :1] - want.values
+    units = 3 + 0.05 * x + 4 + experts / 4 + 6 + 2 + 1
+    assert bool(((weights.cpu().double() - exact).abs() <= units * ref.U32 * exact + 2.0 ** -126).all())
