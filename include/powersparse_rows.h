@@ -148,7 +148,8 @@ int ps_layer_norm(const ps_rows* x, const ps_rows* weight, const ps_rows* bias, 
  * rows of dy * xh, dbias = sum over the rows of dy. weight NULL: ones; dweight and
  * dbias, one row each, NULL: not wanted; accumulate != 0: the sums are added to
  * them. dx has x's type; dy, weight, dweight and dbias may have others. Where the
- * rows' sums are cut follows from the sizes. */
+ * rows' sums are cut follows from the sizes. The workspace is 32 MB at most up to
+ * 262,144 columns and 128 bytes a column beyond. */
 size_t ps_layer_norm_grad_workspace_bytes(long long rows, long long cols);
 int ps_layer_norm_grad(const ps_rows* dy, const ps_rows* x, const ps_rows* weight,
                        const float* mean, const float* rstd, int accumulate, const ps_rows* dx,

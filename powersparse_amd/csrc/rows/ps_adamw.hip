@@ -18,8 +18,8 @@
 // after 2,000 steps of N(0, 1) gradients with beta2 = 0.999 the roots are off by 15%
 // rms, 1.5 steps of the grid and at most 4.6, their mean by 0.6%. What is unbiased in
 // the root adds its variance to the square, which is 3.4% too large then and up to
-// 3.8% later (10,000 steps); the first moment (beta1 = 0.9) is off by 7% of its size. A second moment that is not zero never becomes zero: the
-// step divides by it.
+// 3.8% later (10,000 steps); the first moment (beta1 = 0.9) is off by 7% of its size.
+// A second moment that is not zero never becomes zero: the step divides by it.
 #include <cmath>
 #include <limits>
 
@@ -378,7 +378,9 @@ __device__ __forceinline__ void chunk_of(const AdamTensor& t, const AdamStep& s,
 
 // Bound by memory: 400 M FP32 parameters, BF16 gradients and copies, FP32 moments:
 // 11.2 GB in 2,138 us, 5.2 TB/s; moments in 8 bits 6.4 GB in 1,192 us, 5.4 TB/s, with
-// as much time's worth of instructions, some 100 an element, under it.
+// as much time's worth of instructions, some 100 an element, under it. With rate and
+// step on the device, whose factors every thread computes in 64 bits, 0.4% and 1.5%
+// more (captured: 2,087 -> 2,095 and 1,152 -> 1,170).
 template <bool k8>
 __global__ __launch_bounds__(kListThreads) void adamw_kernel(Adam a, AdamCall call) {
   AdamStep s;

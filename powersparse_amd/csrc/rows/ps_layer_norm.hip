@@ -2,11 +2,12 @@
 //
 // A row's mean is taken first and its squared deviations from it second: sums of
 // squares alone would cancel where the mean is large against the deviations. A row
-// of up to 4,096 pieces stays in the registers of kLanes threads, kPieces each, and
-// is read once; these threads go from row to row, so weight and bias are loaded
-// once, and in the gradient a thread's columns stay the same: it adds up their
-// dweight and dbias in registers and leaves one sum a workgroup, which a second
-// launch adds up in order. No atomics: the same bits every time.
+// of up to 4,096 pieces (in the gradient 2,048 of 8 elements) stays in the registers
+// of kLanes threads, kPieces each, and is read once; these threads go from row to row,
+// so weight and bias are loaded once, and in the gradient a thread's columns stay the
+// same: it adds up their dweight and dbias in registers and leaves one sum a
+// workgroup, which a second launch adds up in order. No atomics: the same bits every
+// time.
 #include <algorithm>
 
 #include "ps_rows.hpp"
@@ -269,7 +270,9 @@ __global__ __launch_bounds__(threads_of(kLanes)) void layer_norm_grad_kernel(
   }
 }
 
-// Rows of any width: a workgroup a row, which is read three times.
+// Rows of any width: a workgroup a row, which is read three times. 2,048 x 50,000 BF16,
+// 0.41 GB to be read and written once, in 144 us, FP32 249: the caches have the row for
+// its later reads.
 template <typename T, typename O, int N>
 __global__ __launch_bounds__(kWideThreads) void layer_norm_wide_kernel(
     Mat<const T> x, Vec weight, Vec bias, float eps, Mat<O> y, float* __restrict__ mean_out,
@@ -300,7 +303,9 @@ __global__ __launch_bounds__(kWideThreads) void layer_norm_wide_kernel(
   }
 }
 
-// dx of rows of any width: a workgroup a row, which is read twice.
+// dx of rows of any width: a workgroup a row, which is read twice; the sums over the
+// rows read all a third time. 2,048 x 50,000 BF16 with them, 0.61 GB to be read and
+// written once, 287 us, FP32 513.
 template <typename T, typename O, int N>
 __global__ __launch_bounds__(kWideThreads) void layer_norm_grad_wide_kernel(
     Mat<const O> dy, Mat<const T> x, Vec weight, const float* __restrict__ mean_in,
@@ -406,7 +411,8 @@ __global__ __launch_bounds__(kJoinThreads) void layer_norm_join_kernel(
 // ----------------------------------------------------------------- host side
 
 // Ranges of rows that the sums over them are cut into: enough to fill the
-// device, and no more than some 32 MB of parts.
+// device, and no more than 32 MB of parts up to 262,144 columns; beyond, 128 bytes a
+// column (sixteen ranges), 2 GB for the widest rows.
 constexpr long long kParts = 1024, kFewParts = 16, kPartCells = 1 << 22;
 long long part_count(long long rows, long long cols) {
   long long n = kPartCells / cols;

@@ -56,7 +56,7 @@ __device__ __forceinline__ void store_piece(T* p, const Floats<N>& f) {
   }
 }
 
-// op over groups of kLanes neighbouring lanes (8 to 64), in every one of them; all
+// op over groups of kLanes neighbouring lanes (up to 64), in every one of them; all
 // lanes of the wave are active. Vector instructions alone, without the shared
 // memory's latency: inside 16 lanes by permuted reads (quads, then mirrored halves
 // and rows, which meet groups that already agree), beyond by swapping rows of 16

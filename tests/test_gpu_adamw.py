@@ -440,7 +440,8 @@ def test_moments_in_8_bits_under_random_gradients():
         ps.AdamWStep(tensors, 0.0, t, beta1=beta1, beta2=beta2)
         square = fresh.double().square_()
         exact = beta2 * exact + (1 - beta2) * square
-        code, scale, _, _ = ref.to_8_bits((beta2 * rule * rule + (1 - beta2) * square).sqrt(), t, True)
+        new = (beta2 * rule * rule + (1 - beta2) * square).sqrt()
+        code, scale, _, _ = ref.to_8_bits(new, t, True)
         rule = code * scale.repeat_interleave(256)
     got = (v.float().view(-1, 256) * s[:, 1:]).view(-1).cpu().double()
     means, spreads = [], []

@@ -110,8 +110,8 @@ def test_a_skipped_update_is_not_counted(bits):
         g, old = p.grad.double() / (norm + 1e-6), old.double()
         decay = 0.01 if p.dim() > 1 else 0.0
         want = old - 0.01 * (decay * old + g / (g.abs() + 1e-8))
-        # as in test_update
-        assert bool(((p.detach().double() - want).abs() <= 2.0 ** -24 * (0.4 + 2 * old.abs())).all())
+        off = (p.detach().double() - want).abs()
+        assert bool((off <= 2.0 ** -24 * (0.4 + 2 * old.abs())).all())  # as in test_update
 
 
 def test_a_step_leaves_no_graph(monkeypatch):

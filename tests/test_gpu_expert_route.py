@@ -375,4 +375,5 @@ def test_weights_of_far_logits(tokens, experts, std):
     exact = torch.softmax(want.values, 1)
     x = want.values[:, :1] - want.values
     units = 3 + 0.05 * x + 4 + experts / 4 + 6 + 2 + 1
-    assert bool(((weights.cpu().double() - exact).abs() <= units * ref.U32 * exact + 2.0 ** -126).all())
+    off = (weights.cpu().double() - exact).abs()
+    assert bool((off <= units * ref.U32 * exact + 2.0 ** -126).all())

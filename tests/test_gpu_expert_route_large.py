@@ -160,10 +160,11 @@ def test_the_loss_takes_every_token_once(experts):
     T, K = 40007, min(experts, 4)
     gen = generator("every token", experts)
     logits = torch.randn((T, experts), generator=gen, device="cuda")
-    ids, w = torch.empty((T, K), dtype=torch.int32, device="cuda"), torch.empty((T, K), device="cuda")
+    ids = torch.empty((T, K), dtype=torch.int32, device="cuda")
+    w, loss = torch.empty((T, K), device="cuda"), torch.empty(1, device="cuda")
     counts = torch.empty(experts + 1, dtype=torch.int32, device="cuda")
-    loss = torch.empty(1, device="cuda")
-    work = torch.empty(ps.expert_route_workspace_bytes(T, experts), dtype=torch.uint8, device="cuda")
+    work = torch.empty(ps.expert_route_workspace_bytes(T, experts), dtype=torch.uint8,
+                       device="cuda")
     ps.ExpertRoute(logits, ids, w, counts, loss, work)
     l = logits.double()
     assert float((l.amax(1) - l.amin(1)).max()) <= 12
