@@ -453,3 +453,52 @@ def test_moments_in_8_bits_under_random_gradients():
         assert -0.01 <= float((root * root / exact).mean()) - 1 <= 0.065
     assert abs(means[0] - means[1]) <= 6 * 0.174 / 128 * math.sqrt(2)
     assert abs(spreads[0] / spreads[1] - 1) <= 6 / 181 * math.sqrt(2)
+
+
+@pytest.mark.parametrize("f8", [False, True])
+def test_skipped_updates_in_a_graph(f8):
+    """A step on the device that goes up by whether the norm is finite, captured with the norm and
+    the update: replays whose gradients overflow change nothing and are not counted, and those after
+    them are the first, second and third updates."""
+    a, b = (Model(generator("skipped"), SIZES, "f32", "f16", "bf16", f8) for _ in range(2))
+    la, lb = a.list(), b.list()
+    grads = ps.GradientList([g.t for g in a.g])
+    norm, step = torch.empty(1, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def run():
+        s = torch.cuda.current_stream()
+        ps.GradNorm(grads, norm, stream=s)
+        step.add_(torch.isfinite(norm))
+        ps.AdamWStep(la, 1e-2, step, norm=norm, max_norm=0.01, stream=s)
+
+    model_state = [x.whole.clone() for x in a.p + a.m + a.v + a.s]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for x, was in zip(a.p + a.m + a.v + a.s, model_state):
+        x.whole.copy_(was)
+    step.zero_()
+    gen = generator("skipped gradients")
+    done = 0
+    for bad in (True, True, False, True, False, False):
+        for k, (x, y) in enumerate(zip(a.g, b.g)):
+            x.t.copy_(torch.randn(x.t.shape, generator=gen) * 1e-2)
+            if bad and k == 13:
+                x.t[50000] = math.inf
+            y.t.copy_(x.t)
+        graph.replay()
+        torch.cuda.synchronize()
+        if not bad:
+            done += 1
+            ps.AdamWStep(lb, 1e-2, done, norm=norm, max_norm=0.01)
+        torch.cuda.synchronize()
+        assert int(step) == done and bool(torch.isfinite(norm)) != bad
+        for x, y in zip(a.p + a.m + a.v + a.s, b.p + b.m + b.v + b.s):
+            assert torch.equal(x.whole, y.whole)
+        for x, y in zip(a.c, b.c):
+            assert x is None or done == 0 or torch.equal(x.whole, y.whole)
