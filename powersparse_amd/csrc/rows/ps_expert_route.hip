@@ -50,7 +50,8 @@ __device__ __forceinline__ float exp_of(float x) {
   const float lost = __builtin_amdgcn_fmed3f(fmaf(t, -0.693147182f, x), -1.f, 1.f);
   return fmaf(r, lost, r);
 }
-// 1 / s for s from 1 up, or NaN: the hardware's and one step of Newton's iteration.
+// 1 / s for s from 1 up, or NaN: the hardware's and one step of Newton's iteration
+// (0, a padding token's in the gradient, gives NaN, and that token zeros anyway).
 __device__ __forceinline__ float reciprocal(float s) {
   const float r = __builtin_amdgcn_rcpf(s);
   return fmaf(fmaf(-s, r, 1.f), r, r);
